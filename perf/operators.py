@@ -163,43 +163,47 @@ def prepare(case, seed):
 
 # ---- the framework's calls ------------------------------------------------------------------------------------
 
-def dtypes():
+def bind(s):
+    """What a program sets up once and keeps with its buffers: the function, its arguments, the workspace and the stream.  Every
+    pass then makes the call itself."""
     from clpeak_b200 import native as N
-    return {"bf16": N.DT_BF16, "f16": N.DT_F16, "f32": N.DT_F32, "i8": N.DT_I8}
-
-
-def run_own(s):
-    from clpeak_b200 import native as N
-    K, stream, DT = N.kernels(), torch.cuda.current_stream().cuda_stream, dtypes()
-    path, ptr = s["path"], lambda name: s[name].data_ptr()
+    K, stream = N.kernels(), torch.cuda.current_stream().cuda_stream
+    DT = {"bf16": N.DT_BF16, "f16": N.DT_F16, "f32": N.DT_F32, "i8": N.DT_I8}
+    path, ptr, step = s["path"], lambda name: s[name].data_ptr(), lambda name: s[name].stride(0)
     if path == "quantize":
-        K.clpk_quantize_rows_i8(ptr("q"), ptr("scale"), ptr("x"), s["rows"], s["cols"], s["q"].stride(0), s["x"].stride(0), DT[s["dtype"]], stream)
-        return s["q"], s["scale"]
+        return K.clpk_quantize_rows_i8, (ptr("q"), ptr("scale"), ptr("x"), s["rows"], s["cols"], step("q"), step("x"), DT[s["dtype"]], stream)
     if path == "linear":
         args = N.GemmI8ScaledArgs(m=s["m"], n=s["n"], k=s["k"], out_dtype=DT[s["out"]], d_a=ptr("a"), d_b=ptr("b"), d_c=ptr("c"),
-                                  lda=s["a"].stride(0), ldb=s["b"].stride(0), ldc=s["c"].stride(0), d_a_scale=ptr("a_scale"),
-                                  d_b_scale=ptr("b_scale"), d_bias=ptr("bias") if s["bias"] is not None else None, d_status=ptr("status"))
-        K.clpk_gemm_i8_scaled(C.byref(args), stream)
-        return s["c"]
+                                  lda=step("a"), ldb=step("b"), ldc=step("c"), d_a_scale=ptr("a_scale"), d_b_scale=ptr("b_scale"),
+                                  d_bias=ptr("bias") if s["bias"] is not None else None, d_status=ptr("status"))
+        return K.clpk_gemm_i8_scaled, (C.byref(args), stream)
     act = ACTS.index(s["act"])
     if path == "ffn":
         args = N.GatedFfnArgs(dtype=DT[s["dtype"]], out_dtype=DT[s["out"]], activation=act, m=s["m"], d=s["d"], f=s["f"],
-                              d_x=ptr("x"), d_wg=ptr("wg"), d_wu=ptr("wu"), d_h=ptr("h"), ldx=s["x"].stride(0),
-                              ldw=s["wg"].stride(0), ldh=s["h"].stride(0), d_status=ptr("status"))
+                              d_x=ptr("x"), d_wg=ptr("wg"), d_wu=ptr("wu"), d_h=ptr("h"), ldx=step("x"), ldw=step("wg"), ldh=step("h"),
+                              d_status=ptr("status"))
         if s["dtype"] == "i8":
             args.d_x_scale, args.d_wg_scale, args.d_wu_scale = ptr("x_scale"), ptr("wg_scale"), ptr("wu_scale")
-        K.clpk_gated_ffn(C.byref(args), stream)
-        return s["h"]
-    if "workspace" not in s:                                    # a training program keeps it from step to step
-        need = C.c_size_t(0)
-        K.clpk_gated_ffn_backward_workspace_bytes(DT[s["dtype"]], s["m"], s["d"], s["f"], C.byref(need))
-        s["workspace"] = torch.empty(max(need.value, 16), dtype=torch.uint8, device="cuda")
+        return K.clpk_gated_ffn, (C.byref(args), stream)
+    need = C.c_size_t(0)
+    K.clpk_gated_ffn_backward_workspace_bytes(DT[s["dtype"]], s["m"], s["d"], s["f"], C.byref(need))
+    s["workspace"] = torch.empty(max(need.value, 16), dtype=torch.uint8, device="cuda")
     args = N.GatedFfnBackwardArgs(dtype=DT[s["dtype"]], activation=act, m=s["m"], d=s["d"], f=s["f"], d_x=ptr("x"), d_wg=ptr("wg"),
                                   d_wu=ptr("wu"), d_dh=ptr("dh"), d_g=ptr("g"), d_u=ptr("u"), d_dx=ptr("dx"), d_dwg=ptr("dwg"),
-                                  d_dwu=ptr("dwu"), ldx=s["x"].stride(0), ldw=s["wg"].stride(0), ldh=s["dh"].stride(0),
-                                  d_workspace=ptr("workspace"), workspace_bytes=s["workspace"].numel(), d_status=ptr("status"))
-    K.clpk_gated_ffn_backward(C.byref(args), stream)
-    return s["dx"], s["dwg"], s["dwu"]
+                                  d_dwu=ptr("dwu"), ldx=step("x"), ldw=step("wg"), ldh=step("dh"), d_workspace=ptr("workspace"),
+                                  workspace_bytes=need.value, d_status=ptr("status"))
+    return K.clpk_gated_ffn_backward, (C.byref(args), stream)
+
+
+OUTPUTS = {"quantize": ("q", "scale"), "linear": ("c",), "ffn": ("h",), "backward": ("dx", "dwg", "dwu")}
+
+
+def run_own(s):
+    if "call" not in s:
+        s["call"] = bind(s)
+    function, args = s["call"]
+    function(*args)
+    return [s[name] for name in OUTPUTS[s["path"]]]
 
 
 # ---- plain forms ------------------------------------------------------------------------------------------------
@@ -230,23 +234,23 @@ def run_plain(s):
         scale = top / torch.full((), 127.0, device=x.device)
         scale = torch.where(scale >= 2.0 ** -126, scale, torch.zeros_like(scale))           # below: taken as zeros
         inverse = torch.where(scale > 0, torch.reciprocal(scale), torch.zeros_like(scale))
-        return torch.round(x * inverse[:, None]).to(torch.int8), scale
+        return [torch.round(x * inverse[:, None]).to(torch.int8), scale]
     if path == "linear":
         c = (s["a"].float() @ s["b"].float().T) * s["a_scale"][:, None] * s["b_scale"]
         if s["bias"] is not None:
             c = c + s["bias"].float()
-        return c.to(TORCH[s["out"]])
+        return [c.to(TORCH[s["out"]])]
     x, wg, wu = s["x"].float(), s["wg"].float(), s["wu"].float()
     if path == "ffn":
         g, u = x @ wg.T, x @ wu.T
         if s["dtype"] == "i8":
             g, u = g * s["x_scale"][:, None] * s["wg_scale"], u * s["x_scale"][:, None] * s["wu_scale"]
-        return (activation(s["act"], g)[0] * u).to(TORCH[s["out"]])
+        return [(activation(s["act"], g)[0] * u).to(TORCH[s["out"]])]
     dh, g, u = s["dh"].float(), s["g"].float(), s["u"].float()
     a, da = activation(s["act"], g)
     dg, du = dh * u * da, dh * a
     out = dg @ wg + du @ wu, dg.T @ x, du.T @ x
-    return tuple(t.to(TORCH[s["dtype"]]) for t in out)
+    return [t.to(TORCH[s["dtype"]]) for t in out]
 
 
 def run(state):
@@ -277,10 +281,10 @@ def exact(case, seed):
     s = prepare(case, seed)
     w = {n: t.to(torch.float64) for n, t in s.items() if isinstance(t, torch.Tensor) and n not in ("q", "scale", "c", "h", "dx", "dwg", "dwu", "workspace")}
     if case["path"] == "quantize":
-        return None, w["x"].abs().max(dim=1).values / 127
+        return [None, w["x"].abs().max(dim=1).values / 127]
     if case["path"] == "linear":
         c = torch.matmul(w["a"] * w["a_scale"].unsqueeze(1), (w["b"] * w["b_scale"].unsqueeze(1)).t())
-        return c + w["bias"] if case["bias"] else c
+        return [c + w["bias"] if case["bias"] else c]
     act = case["act"]
 
     def phi(z):                                                 # the activation alone, as its textbook form has it
@@ -297,8 +301,8 @@ def exact(case, seed):
             for n in ("x", "wg", "wu"):
                 w[n] = w[n] * w[n + "_scale"].unsqueeze(1)
         gate = phi(torch.matmul(w["x"], w["wg"].t()))
-        return gate * torch.matmul(w["x"], w["wu"].t())
+        return [gate * torch.matmul(w["x"], w["wu"].t())]
     g = w["g"].requires_grad_()
     u = w["u"].requires_grad_()
     dg, du = torch.autograd.grad(phi(g) * u, (g, u), w["dh"])   # through the two products by hand, from their definition
-    return torch.matmul(dg, w["wg"]) + torch.matmul(du, w["wu"]), torch.matmul(dg.t(), w["x"]), torch.matmul(du.t(), w["x"])
+    return [torch.matmul(dg, w["wg"]) + torch.matmul(du, w["wu"]), torch.matmul(dg.t(), w["x"]), torch.matmul(du.t(), w["x"])]
