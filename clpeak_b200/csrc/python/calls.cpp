@@ -2,7 +2,7 @@
 // call with five arguments and 1.3 for seven, as much as half of the launch behind it (2.2 us in the driver), and small calls wait for
 // nothing else.  The two launches of a small operand (513 x 1040 to fp8) 7.4 -> 5.7 us, a bandwidth step over short arrays 31 -> 29.
 //
-// A call takes plain int, float and None arguments, and byref() of a clpk_gemm_args_t.  Whatever else ctypes would accept, convert
+// A call takes plain int, float and None arguments, and byref() of a structure of arguments.  Whatever else ctypes would accept, convert
 // or refuse goes to the ctypes wrapper, which is handed over when the call is bound.  The GIL is released meanwhile, as ctypes does.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -23,7 +23,7 @@ struct Call {
     void *fn;
     PyObject *slow;              // the ctypes wrapper
     PyObject *failed;            // raises for a status
-    PyTypeObject *byref_type, *gemm_args_type;
+    PyTypeObject *byref_type, *args_type;      // args_type: of the structure that the call takes by reference
     Py_ssize_t address_at;       // see where_the_address_lies
 };
 
@@ -96,7 +96,11 @@ template <> struct Arg<float> {
     void done() {}
 };
 
-template <typename P> struct Arg<P *, std::enable_if_t<!std::is_same<P, const clpk_gemm_args_t>::value>> {
+// structures that a call takes by reference
+template <typename P> constexpr bool is_args = std::is_same<P, const clpk_gemm_args_t>::value || std::is_same<P, const clpk_gemm_i8_scaled_args_t>::value ||
+                                               std::is_same<P, const clpk_gated_ffn_args_t>::value || std::is_same<P, const clpk_gated_ffn_backward_args_t>::value;
+
+template <typename P> struct Arg<P *, std::enable_if_t<!is_args<P>>> {
     P *v;
     bool from(const Call *, PyObject *o)
     {
@@ -119,8 +123,8 @@ template <typename P> struct Arg<P *, std::enable_if_t<!std::is_same<P, const cl
 
 // byref(args): the structure lies in the buffer of the object that it refers to, unless byref was given an offset: only where the
 // address that it carries is the buffer's.
-template <> struct Arg<const clpk_gemm_args_t *> {
-    const clpk_gemm_args_t *v = nullptr;
+template <typename P> struct Arg<P *, std::enable_if_t<is_args<P>>> {
+    P *v = nullptr;
     Py_buffer buffer = {};
     bool from(const Call *call, PyObject *o)
     {
@@ -132,18 +136,18 @@ template <> struct Arg<const clpk_gemm_args_t *> {
             PyErr_Clear();
             return false;
         }
-        bool ok = Py_TYPE(args) == call->gemm_args_type;
+        bool ok = Py_TYPE(args) == call->args_type;
         if (ok && PyObject_GetBuffer(args, &buffer, PyBUF_SIMPLE) != 0) {
             PyErr_Clear();
             ok = false;
         }
         Py_DECREF(args);                                     // the buffer holds the object
-        if (ok && (buffer.len != (Py_ssize_t)sizeof(clpk_gemm_args_t) || address_in(o, call->address_at) != buffer.buf)) {
+        if (ok && (buffer.len != (Py_ssize_t)sizeof(P) || address_in(o, call->address_at) != buffer.buf)) {
             done();
             ok = false;
         }
         if (ok)
-            v = static_cast<const clpk_gemm_args_t *>(buffer.buf);
+            v = static_cast<P *>(buffer.buf);
         return ok;
     }
     void done() { PyBuffer_Release(&buffer); }
@@ -186,7 +190,8 @@ const struct {
     const char *name;
     vectorcallfunc invoke;
 } kCalls[] = {CALL(clpk_fill_f32), CALL(clpk_fill_i8), CALL(clpk_convert_f32), CALL(clpk_absmax_f32), CALL(clpk_quantize_fp4), CALL(clpk_stream_read),
-              CALL(clpk_stream_copy), CALL(clpk_stream_triad), CALL(clpk_gemm), CALL(clpk_gemm_pack_scales)};
+              CALL(clpk_stream_copy), CALL(clpk_stream_triad), CALL(clpk_gemm), CALL(clpk_gemm_pack_scales), CALL(clpk_quantize_rows_i8), CALL(clpk_gemm_i8_scaled),
+              CALL(clpk_gated_ffn), CALL(clpk_gated_ffn_backward)};
 
 int call_traverse(PyObject *self, visitproc visit, void *arg)
 {
@@ -194,7 +199,7 @@ int call_traverse(PyObject *self, visitproc visit, void *arg)
     Py_VISIT(c->slow);
     Py_VISIT(c->failed);
     Py_VISIT(c->byref_type);
-    Py_VISIT(c->gemm_args_type);
+    Py_VISIT(c->args_type);
     return 0;
 }
 int call_clear(PyObject *self)
@@ -203,7 +208,7 @@ int call_clear(PyObject *self)
     Py_CLEAR(c->slow);
     Py_CLEAR(c->failed);
     Py_CLEAR(c->byref_type);
-    Py_CLEAR(c->gemm_args_type);
+    Py_CLEAR(c->args_type);
     return 0;
 }
 void call_dealloc(PyObject *self)
@@ -233,7 +238,7 @@ PyObject *bind(PyObject *, PyObject *args)
             call->slow = Py_NewRef(slow);
             call->failed = Py_NewRef(failed);
             call->byref_type = reinterpret_cast<PyTypeObject *>(Py_NewRef(byref_type));
-            call->gemm_args_type = reinterpret_cast<PyTypeObject *>(Py_NewRef(args_type));
+            call->args_type = reinterpret_cast<PyTypeObject *>(Py_NewRef(args_type));
             call->address_at = where_the_address_lies(byref, args_type);
             PyObject_GC_Track(reinterpret_cast<PyObject *>(call));
             return reinterpret_cast<PyObject *>(call);

@@ -33,6 +33,8 @@ CHAIN_NAMES = {CHAIN_HALF: "half", CHAIN_HALF2: "half2", CHAIN_DOUBLE: "double",
                CHAIN_INT32: "int", CHAIN_INT8_DOT1: "int8_dp", CHAIN_INT8_DOT2: "int8_dp2", CHAIN_INT8_DOT4: "int8_dp4",
                CHAIN_INT8_DOT8: "int8_dp8"}
 
+(ACT_SILU, ACT_GELU_TANH, ACT_GELU, ACT_RELU, ACT_SIGMOID) = range(5)
+
 MMA_KIND_NAMES = {
     MMA_F16: "fp16", MMA_BF16: "bf16", MMA_E4M3: "fp8_e4m3", MMA_E5M2: "fp8_e5m2", MMA_I8: "int8",
     MMA_MXF4: "mxf4_e2m1", MMA_NVF4: "nvf4_e2m1", MMA_E4M3_SP: "fp8_e4m3_sparse",
@@ -78,6 +80,42 @@ class GemmArgs(C.Structure):
         ("d_a", C.c_void_p), ("d_b", C.c_void_p), ("d_c", C.c_void_p),
         ("d_sfa", C.c_void_p), ("d_sfb", C.c_void_p),
         ("alpha", C.c_float),
+        ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("d_status", C.c_void_p),
+    ]
+
+
+class GemmI8ScaledArgs(C.Structure):
+    _fields_ = [
+        ("m", C.c_uint32), ("n", C.c_uint32), ("k", C.c_uint32),
+        ("out_dtype", C.c_int),
+        ("d_a", C.c_void_p), ("d_b", C.c_void_p), ("d_c", C.c_void_p),
+        ("lda", C.c_uint64), ("ldb", C.c_uint64), ("ldc", C.c_uint64),
+        ("d_a_scale", C.c_void_p), ("d_b_scale", C.c_void_p), ("d_bias", C.c_void_p),
+        ("d_status", C.c_void_p),
+    ]
+
+
+class GatedFfnArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("out_dtype", C.c_int), ("activation", C.c_int),
+        ("m", C.c_uint32), ("d", C.c_uint32), ("f", C.c_uint32),
+        ("d_x", C.c_void_p), ("d_wg", C.c_void_p), ("d_wu", C.c_void_p),
+        ("d_x_scale", C.c_void_p), ("d_wg_scale", C.c_void_p), ("d_wu_scale", C.c_void_p),
+        ("d_h", C.c_void_p), ("d_g", C.c_void_p), ("d_u", C.c_void_p),
+        ("ldx", C.c_uint64), ("ldw", C.c_uint64), ("ldh", C.c_uint64),
+        ("d_status", C.c_void_p),
+    ]
+
+
+class GatedFfnBackwardArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("activation", C.c_int),
+        ("m", C.c_uint32), ("d", C.c_uint32), ("f", C.c_uint32),
+        ("d_x", C.c_void_p), ("d_wg", C.c_void_p), ("d_wu", C.c_void_p),
+        ("d_dh", C.c_void_p), ("d_g", C.c_void_p), ("d_u", C.c_void_p),
+        ("d_dx", C.c_void_p), ("d_dwg", C.c_void_p), ("d_dwu", C.c_void_p),
+        ("ldx", C.c_uint64), ("ldw", C.c_uint64), ("ldh", C.c_uint64),
         ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("d_status", C.c_void_p),
     ]
@@ -146,9 +184,16 @@ KERNEL_API = {
     "clpk_gemm_last_launch_aligned": [],
     "clpk_gemm_wave_state": [C.POINTER(_u32), C.POINTER(_u32), _vp],
     "clpk_gemm_last_clock": [C.POINTER(C.c_ulonglong), C.POINTER(C.c_ulonglong), _vp],
+    "clpk_quantize_rows_i8": [_vp, _vp, _vp, _u64, _u64, _u64, _u64, _i, _vp],
+    "clpk_gemm_i8_scaled": [C.POINTER(GemmI8ScaledArgs), _vp],
+    "clpk_gated_ffn": [C.POINTER(GatedFfnArgs), _vp],
+    "clpk_gated_ffn_backward_workspace_bytes": [_i, _u32, _u32, _u32, C.POINTER(C.c_size_t)],
+    "clpk_gated_ffn_backward": [C.POINTER(GatedFfnBackwardArgs), _vp],
     "clpk_set_tuning": [_i, _i],
     "clpk_get_tuning": [_i, C.POINTER(_i)],
 }
+# the structure that a call of the extension takes by reference, where it is not GemmArgs
+_ARGUMENTS = {"clpk_gemm_i8_scaled": GemmI8ScaledArgs, "clpk_gated_ffn": GatedFfnArgs, "clpk_gated_ffn_backward": GatedFfnBackwardArgs}
 _RESTYPES = {
     "clpk_last_error": C.c_char_p,
     "clpk_version": C.c_char_p,
@@ -207,7 +252,8 @@ class Kernels:
                 failed(rc)
         if _calls() is None:
             return call
-        return _calls().bind(name, C.cast(fn, C.c_void_p).value, call, failed, C.byref, type(C.byref(C.c_int())), GemmArgs) or call
+        return _calls().bind(name, C.cast(fn, C.c_void_p).value, call, failed, C.byref, type(C.byref(C.c_int())),
+                             _ARGUMENTS.get(name, GemmArgs)) or call
 
     def last_error(self) -> str:
         return (self.lib.clpk_last_error() or b"").decode()

@@ -474,6 +474,99 @@ CLPK_API int clpk_gemm_wave_state(uint32_t *h_counters_set, uint32_t *h_dropouts
  * do not write it. */
 CLPK_API int clpk_gemm_last_clock(unsigned long long *h_cycles, unsigned long long *h_ns, void *stream);
 
+/* ---- feed-forward layers ------------------------------------------------------------------------
+ * What a gated feed-forward layer  y = (act(x Wg^T) * (x Wu^T)) Wd^T  needs next to clpk_gemm: its first half as one
+ * kernel, that half's gradients, and the same layer in 8-bit integers.  No counterpart in the reference.
+ *
+ * Every matrix is row-major with a pitch ld* in elements from one row to the next; 0 means rows that lie one behind
+ * another.  A pitch is a multiple of 16 bytes and not shorter than a row, and matrices start on 16 bytes; row lengths are
+ * free.  What lies between the end of a row and the next one is neither read into a result nor written.  Outputs do not
+ * overlap inputs.  A call with no tokens (m = 0) succeeds: it writes no activations, and zeros as gradients of weights.
+ * *d_status is cleared by the call and set where a device-side wait expired. */
+
+/* One scale for each row of a matrix and 8-bit integers: scale = max |x| / 127, q = rint(x * (1 / scale)), ties to even,
+ * in fp32.  dtype: CLPK_DT_F32, F16 or BF16.  A row whose scale would be below 2^-126 has the scale 0 and zeros; one with an
+ * infinity or a NaN has the scale NaN and zeros, so that products with it are NaN.  ld_q and ld_src as above, except that
+ * any alignment, pitch and length will do here (aligned rows are faster). */
+CLPK_API int clpk_quantize_rows_i8(int8_t *d_q, float *d_scales, const void *d_src, uint64_t rows, uint64_t cols, uint64_t ld_q,
+                                   uint64_t ld_src, int dtype, void *stream);
+
+/* C[M][N] = A[M][K] * B[N][K]^T in 8-bit integers with scales:
+ *   c_mn = round(float(sum_k a_mk b_nk) * a_scale_m * b_scale_n + bias_n)
+ * with the sum exact (K <= 131071, so that it fits 32 bits) and the rest in fp32.  A holds tokens, B a weight's output
+ * channels; their scales are those of clpk_quantize_rows_i8.  M, N and K are free, M = 0 included. */
+typedef struct clpk_gemm_i8_scaled_args {
+    uint32_t      m, n, k;
+    int           out_dtype;      /* CLPK_DT_F32, F16 or BF16: of C and of the bias  */
+    const int8_t *d_a;            /* [M][K]                                          */
+    const int8_t *d_b;            /* [N][K]                                          */
+    void         *d_c;            /* [M][N]                                          */
+    uint64_t      lda, ldb, ldc;
+    const float  *d_a_scale;      /* [M]                                             */
+    const float  *d_b_scale;      /* [N]                                             */
+    const void   *d_bias;         /* [N], or NULL                                    */
+    uint32_t     *d_status;       /* one word, cleared by the call                   */
+} clpk_gemm_i8_scaled_args_t;
+
+CLPK_API int clpk_gemm_i8_scaled(const clpk_gemm_i8_scaled_args_t *args, void *stream);
+
+/* Activations of the gate. */
+#define CLPK_ACT_SILU      0   /* g / (1 + exp(-g))                                                      */
+#define CLPK_ACT_GELU_TANH 1   /* g / 2 * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3)))                  */
+#define CLPK_ACT_GELU      2   /* g / 2 * (1 + erf(g / sqrt(2)))                                         */
+#define CLPK_ACT_RELU      3   /* max(g, 0); its derivative at 0 is 0                                    */
+#define CLPK_ACT_SIGMOID   4   /* 1 / (1 + exp(-g))                                                      */
+#define CLPK_ACT_COUNT     5
+
+/* h = act(g) * u with g = x Wg^T and u = x Wu^T: both products, the activation and the product in one kernel.
+ *   dtype            x, Wg, Wu    sums    h, g, u
+ *   CLPK_DT_BF16     bf16         fp32    bf16
+ *   CLPK_DT_F16      fp16         fp32    fp16
+ *   CLPK_DT_I8       int8         int32   out_dtype (F32, F16 or BF16); g = float(sum) * x_scale_m * wg_scale_f, u likewise
+ * Activation and product are in fp32 and rounded once.  With d_g and d_u (both or neither; not CLPK_DT_I8) the call also
+ * keeps g and u for the backward pass. */
+typedef struct clpk_gated_ffn_args {
+    int           dtype;
+    int           out_dtype;      /* CLPK_DT_I8 only; otherwise h is of `dtype`      */
+    int           activation;     /* CLPK_ACT_*                                      */
+    uint32_t      m, d, f;        /* tokens, model width, hidden width               */
+    const void   *d_x;            /* [m][d], pitch ldx                               */
+    const void   *d_wg, *d_wu;    /* [f][d], pitch ldw                               */
+    const float  *d_x_scale;      /* [m]; CLPK_DT_I8 only, as the next two           */
+    const float  *d_wg_scale;     /* [f]                                             */
+    const float  *d_wu_scale;     /* [f]                                             */
+    void         *d_h;            /* [m][f], pitch ldh                               */
+    void         *d_g, *d_u;      /* as h, or NULL                                   */
+    uint64_t      ldx, ldw, ldh;
+    uint32_t     *d_status;
+} clpk_gated_ffn_args_t;
+
+CLPK_API int clpk_gated_ffn(const clpk_gated_ffn_args_t *args, void *stream);
+
+/* Gradients of clpk_gated_ffn in CLPK_DT_BF16 or F16, from that of h and the g and u that it kept:
+ *   dg = dh * u * act'(g),  du = dh * act(g)      in fp32, rounded to `dtype` (the workspace holds them)
+ *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x      sums in fp32, rounded once
+ * d_dx may be NULL, and so may d_dwg and d_dwu (both or neither): what is not asked for is not computed.  Sums are formed
+ * in the same order in every call. */
+typedef struct clpk_gated_ffn_backward_args {
+    int           dtype;
+    int           activation;
+    uint32_t      m, d, f;
+    const void   *d_x;            /* [m][d], pitch ldx                               */
+    const void   *d_wg, *d_wu;    /* [f][d], pitch ldw                               */
+    const void   *d_dh;           /* [m][f], pitch ldh                               */
+    const void   *d_g, *d_u;      /* [m][f], pitch ldh                               */
+    void         *d_dx;           /* [m][d], pitch ldx                               */
+    void         *d_dwg, *d_dwu;  /* [f][d], pitch ldw                               */
+    uint64_t      ldx, ldw, ldh;
+    void         *d_workspace;    /* 16-byte aligned                                 */
+    size_t        workspace_bytes;
+    uint32_t     *d_status;
+} clpk_gated_ffn_backward_args_t;
+
+CLPK_API int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, uint32_t f, size_t *bytes);
+CLPK_API int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
