@@ -32,7 +32,7 @@
 constexpr int kTilesMaxStages = 16;
 constexpr uint32_t kTilesChunk = 32;                               // columns of C per tcgen05.ld and per TMA store box
 constexpr uint32_t kTilesM = 256;
-constexpr uint32_t kTilesSmemMax = 227 * 1024;
+constexpr uint32_t kTilesSmemMax = kSmemMax;
 
 struct TilesSmem {
     uint64_t full[kTilesMaxStages];
@@ -165,18 +165,6 @@ __device__ __forceinline__ void tiles_store_chunk(uint32_t (&r)[32], float alpha
 // Partial sums of a 32-column chunk in the owner's shared memory: [8 groups of 4 columns][128 rows][4 words], so that
 // a warp's 32 rows are 512 consecutive bytes per group on both sides.
 constexpr uint32_t kTilesChunkBytes = kTilesChunk * 128 * 4;
-
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
-{
-    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
-__device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t cta)
-{
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(cta));
-    return a;
-}
 
 // 3-D tile load whose completion bytes go to the leader's barrier
 __device__ __forceinline__ void tma_load_pair_3d_at(void *smem_dst, const CUtensorMap *tmap, int32_t x, int32_t y, int32_t z, uint32_t leader_bar)

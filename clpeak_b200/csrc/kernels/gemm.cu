@@ -31,12 +31,11 @@
 #include <type_traits>
 
 #include "../clpk_internal.h"
+#include "../clpk_pair.cuh"
 #include "../clpk_ptx.cuh"
 
 namespace clpk {
 
-constexpr uint32_t kRowBytesK = 128;                        // K bytes per row per stage
-constexpr uint32_t kHalfTileBytes = 128 * kRowBytesK;       // 16 KiB: 128 rows x 128 B
 constexpr uint32_t kTileMN = 256;
 constexpr int kGemmThreads = 320;                          // dense kernel: producer, MMA, 8 epilogue warps
 
@@ -70,36 +69,6 @@ __device__ __forceinline__ void join_previous_launch(const GemmParams &p)
 // Output element of a GEMM dtype: fp32 for TF32, int32 for I8, bf16 for everything else.
 template <int DT> struct OutBytes { static constexpr uint32_t value = (DT == CLPK_DT_TF32 || DT == CLPK_DT_I8) ? 4u : 2u; };
 
-// 2-D tile load whose completion bytes go to the pair's leader CTA: leader_bar is its barrier's address (leader_addr).
-__device__ __forceinline__ void tma_load_pair_at(void *smem_dst, const CUtensorMap *tmap, int32_t x, int32_t y,
-                                                 uint32_t leader_bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
-        "l"(tmap), "r"(leader_bar), "r"(x), "r"(y)
-        : "memory");
-}
-
-__device__ __forceinline__ uint32_t leader_addr(const void *p)
-{
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
-    return a;
-}
-
-// Roles that issue TMA or tcgen05 instructions run their loops with the whole warp and let
-// one elected lane issue.  Addresses and descriptors are then warp-uniform values, which is
-// what those instructions take.  With the loop inside `if (lane == 0)` each instruction cost
-// its thread 110-130 cycles (measured with clock64 around it: four MMAs 460 cycles, against
-// 115 this way), and a thread that must issue four MMAs and a commit per 512 tensor-core
-// cycles, or eight and a commit per 1024, was the slowest stage of the pipeline.
-// warp_wait: every lane waits; the verdict is made uniform so that the warp stays together.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity)
-{
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity) ? 1 : 0) != 0;
-}
-
 // DT: BF16 / F16 -> kind::f16 (K = 16 per instruction); E4M3 / E5M2 -> kind::f8f6f4 (K = 32);
 // TF32 -> kind::tf32 (K = 8, fp32 out); I8 -> kind::i8 (K = 32, int32 out).  Always 128 bytes of K per stage.
 //
@@ -118,9 +87,6 @@ constexpr int kDenseStages = 4;
 constexpr uint32_t kDenseStageBytes = 3 * kHalfTileBytes;          // A half 0, A half 1, B half
 constexpr uint32_t kDenseTileM = 512;
 
-constexpr int kEpilogueWarps = 8;
-constexpr uint32_t kStagingBytes = 32 * 128;                       // 32 rows x 128 bytes of C
-
 struct DenseSmem {
     uint64_t full[kDenseStages];
     uint64_t empty[kDenseStages];
@@ -128,19 +94,6 @@ struct DenseSmem {
     uint64_t tmem_empty;
     uint32_t tmem_base;
 };
-
-// Tiles are walked in groups of `group` tile columns, M fastest inside a group.
-__device__ __forceinline__ void dense_tile_coords(uint32_t tile, uint32_t tiles_m, uint32_t tiles_n, uint32_t group,
-                                                  uint32_t &mb, uint32_t &nb)
-{
-    const uint32_t per_group = group * tiles_m;
-    const uint32_t g = tile / per_group;
-    const uint32_t within = tile - g * per_group;
-    const uint32_t first_n = g * group;
-    const uint32_t width = (tiles_n - first_n) < group ? (tiles_n - first_n) : group;
-    mb = within / width;
-    nb = first_n + within % width;
-}
 
 // Epilogue of one warp for one tile of the dense kernel: the warp's 32 rows (TMEM lanes) x 128 columns of each
 // of the two row blocks, moved in boxes of 128 bytes per row (64 bf16 or 32 fp32/int32 columns): tcgen05.ld ->
@@ -162,26 +115,6 @@ __device__ __forceinline__ void dense_tile_coords(uint32_t tile, uint32_t tiles_
 // and an mbarrier.arrive.release.cluster that took 1 650 cycles to retire because a release waits for the warp's
 // earlier shared-memory and bulk stores.  Now every column is read and converted before anything is stored and
 // the arrive is relaxed (the hand-over carries no memory): 2 200 cycles, 8192^3 fp8 3.9 % and NVFP4 5.5 % fewer.
-
-// one staging box out: wait until the previous store has read the box, fill it, hand it to TMA
-__device__ __forceinline__ void store_staged_box(const uint32_t (&w)[32], uint8_t *box, const CUtensorMap *tmap_c, uint32_t col,
-                                                 uint32_t row, int lane)
-{
-    uint8_t *my_row = box + lane * 128;
-    const uint32_t sw = (uint32_t)(lane & 7);
-    if (lane == 0)
-        bulk_wait_read<0>();
-    __syncwarp();
-#pragma unroll
-    for (uint32_t j = 0; j < 8; j++)
-        *reinterpret_cast<uint4 *>(my_row + ((j ^ sw) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-        tma_store_2d(tmap_c, box, (int32_t)col, (int32_t)row);
-        bulk_commit();
-    }
-}
 
 __device__ __forceinline__ void pack_bf16x64(uint32_t (&w)[32], const uint32_t (&r0)[32], const uint32_t (&r1)[32], float alpha)
 {
@@ -915,28 +848,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNvGemmThreads)
 
 // ---- host side -----------------------------------------------------------------------------
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-static int get_encode_fn(EncodeTiledFn *out)
-{
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void *sym = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        CLPK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres));
-        if (qres != cudaDriverEntryPointSuccess || !sym) {
-            set_error("cuTensorMapEncodeTiled is not available from this driver");
-            return CLPK_ERR_CUDA;
-        }
-        fn = reinterpret_cast<EncodeTiledFn>(sym);
-    }
-    *out = fn;
-    return CLPK_OK;
-}
-
 // Row-major [rows][row_bytes] operand, box = box_rows (128 unless said otherwise) x 128 bytes, 128-byte swizzle.
 static int make_operand_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows = 128)
 {
@@ -1223,30 +1134,6 @@ static TilesPlan raw_scales_plan(const clpk_gemm_args_t *a, const PackOperand &s
     return plan;
 }
 
-// CTAs in clusters of `cluster`, behind the kernel before them
-template <typename Maps, typename Params>
-static int launch_clusters(void (*kernel)(Maps, Params), const char *what, uint32_t ctas, int threads, size_t smem, uint32_t cluster, cudaStream_t s,
-                           const Maps &maps, const Params &p)
-{
-    CLPK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTilesSmemMax));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = tuning(CLPK_TUNE_GEMM_NO_PDL) == 1 ? 0 : 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    g_last_aligned = 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p);
-    return e == cudaSuccess ? CLPK_OK : cuda_fail(e, what);
-}
-
 // sa, sb: where the arranged scale factors lie (block-scaled kinds), and kRaw: where they come from
 template <int DT, uint32_t kRowBlocks = 1, bool kRaw = false>
 static int launch_tiles(const clpk_gemm_args_t *a, const CUtensorMap &ta, uint64_t row_bytes, uint32_t k_blocks, TilesPlan plan, cudaStream_t s,
@@ -1300,6 +1187,7 @@ static int launch_tiles(const clpk_gemm_args_t *a, const CUtensorMap &ta, uint64
         p.tmem_cols *= 2;
     CLPK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void **>(&p.clock), g_gemm_clock));
     const size_t smem = p.stages * stage_bytes + fixed;
+    g_last_aligned = 0;
     return launch_clusters(gemm_tiles_kernel<DT, kRowBlocks, kRaw>, "gemm_tiles", clusters * 2 * plan.splits, tiles_threads(kRaw), smem, 2 * plan.splits, s, maps, p);
 }
 
@@ -1375,6 +1263,7 @@ static int launch_f32(const clpk_gemm_args_t *a, uint32_t splits, cudaStream_t s
     p.status = a->d_status;
     const uint32_t n_tiles = p.tiles_m * p.tiles_n, pairs = (uint32_t)num_sms() / 2;
     const uint32_t clusters = splits > 1 ? n_tiles : (n_tiles < pairs ? n_tiles : pairs);
+    g_last_aligned = 0;
     return launch_clusters(gemm_f32_kernel<TN>, "gemm_f32", clusters * 2 * splits, kF32Threads, T::smem_bytes, 2 * splits, s, maps, p);
 }
 
