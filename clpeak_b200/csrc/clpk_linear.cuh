@@ -1,0 +1,540 @@
+// Products of a feed-forward layer with many tokens, on CTA pairs (included by feed_forward.cu).
+//
+// Same pieces as gemm_tiles_kernel -- TMA ring, M = 256 instructions of a pair, two accumulators, K over the pairs of a cluster
+// -- with three things that clpk_gemm does not have:
+//
+//  * Two products that share A in one pass (kGated).  In a pair's instruction each CTA brings half of the tile's columns of B, so
+//    the leader loads Wg's rows and its peer Wu's: columns [0, tn / 2) of the accumulator are g and [tn / 2, tn) are u of the same
+//    features, a thread of the epilogue holds both, and h = act(g) * u leaves without g or u having been anywhere.
+//  * Operands that are contiguous along M or N instead of K (kAMn, kBMn): what the gradients need, dx = dg Wg with Wg as it lies
+//    and dW = dg^T x with neither transposed.  A stage is then boxes of 64 elements along M or N times 64 of K, in the same
+//    128-byte swizzle; the descriptors' leading offset is the distance between two boxes, their stride that of eight rows of K.
+//  * A sum over two pairs of operands (dx = dg Wg + du Wu) as one K range, and two products of the same shape (dWg and dWu) as
+//    one set of tiles.
+#pragma once
+
+enum LinearForm { kPlain = 0, kGated = 1, kScaled = 2 };
+
+constexpr int kLinearMaxStages = 12;
+constexpr uint32_t kLinearM = 256;
+constexpr uint32_t kLinearK = 64;                                   // of 16-bit elements: 128 bytes; 128 of the 8-bit ones
+constexpr uint32_t kLinearChunk = 32;                               // columns per tcgen05.ld and per box of C
+constexpr int kLinearThreads = 64 + 32 * kEpilogueWarps;
+
+struct LinearSmem {
+    uint64_t full[kLinearMaxStages];
+    uint64_t empty[kLinearMaxStages];
+    uint64_t tmem_full[2];
+    uint64_t tmem_empty[2];
+    uint32_t tmem_base;
+};
+// 8-bit integers: the scales of the columns that a warp works on, behind the rest
+struct LinearSmemScaled : LinearSmem {
+    __align__(16) float scales[kEpilogueWarps][2][kLinearChunk];
+};
+template <int DT> using LinearSmemOf = std::conditional_t<DT == CLPK_DT_I8, LinearSmemScaled, LinearSmem>;
+
+struct LinearMaps {
+    CUtensorMap a[2], b[2], c[3];
+};
+
+struct LinearParams {
+    uint32_t m, n;
+    uint32_t tiles_m, tiles_n, group, products;     // products: sets of tiles, 1 or 2
+    uint32_t k_blocks, k_segment;                   // K blocks of a tile; those of its first pair of operands
+    uint32_t tn, splits, stages, kps, tmem_cols;
+    int out, activation;                            // CLPK_DT_* of c, CLPK_ACT_*
+    uint32_t keep;                                  // kGated: g and u are stored too
+    uint32_t ragged;                                // rows of c end inside 16 bytes
+    void *c[3];
+    uint64_t ldc;
+    const float *a_scale, *b_scale, *u_scale;
+    const void *bias;
+    uint32_t *status;
+};
+
+// bytes of one K block in a CTA: its 128 rows of each row block of A and its half of the tile's columns of B
+__host__ __device__ constexpr uint32_t linear_block_bytes(uint32_t tn, uint32_t row_blocks) { return row_blocks * kHalfTileBytes + tn / 2 * kRowBytesK; }
+
+// an operand's part of a K block: `rows` of M or N at `row`
+template <bool kMn>
+__device__ __forceinline__ void linear_load(uint8_t *dst, const CUtensorMap *map, uint32_t kb, uint32_t row, uint32_t rows, uint32_t bar)
+{
+    if constexpr (kMn) {
+        for (uint32_t i = 0; i < rows; i += 64)
+            tma_load_pair_at(dst + i * kRowBytesK, map, (int32_t)((row + i) * 2), (int32_t)(kb * kLinearK), bar);
+    } else {
+        tma_load_pair_at(dst, map, (int32_t)(kb * kRowBytesK), (int32_t)row, bar);
+    }
+}
+
+template <bool kMn> __device__ __forceinline__ uint64_t linear_desc(uint32_t addr) { return make_smem_desc(addr, kMn ? 64 * kRowBytesK : 16, 1024, kSwizzle128B); }
+// from one instruction's K to the next, in the descriptor's 16-byte units: 32 bytes of a row, or 16 rows
+template <bool kMn> constexpr uint32_t linear_step = kMn ? 16 * kRowBytesK / 16 : 2;
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int type)
+{
+    if (type == CLPK_DT_F16) {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// 32 columns of one row per lane -> the warp's staging box (rows of 64 or 128 bytes in the swizzle of that width) -> one TMA
+// store, which clips what lies beyond C -- in units of 16 bytes: where a row of C ends inside one, the box that holds its end is
+// written element by element, so that what lies behind the row stays as it is.
+__device__ __forceinline__ void linear_store(const float (&v)[32], const LinearParams &p, uint32_t which, uint8_t *boxes, uint32_t &n_stored,
+                                             const CUtensorMap *map, uint32_t col, uint32_t row, int lane)
+{
+    const bool wide = p.out == CLPK_DT_F32;
+    // 16 bits: two 2 KiB boxes in turn: the one filled now was handed to TMA two stores ago
+    uint8_t *box = wide ? boxes : boxes + (n_stored & 1) * 2048;
+    if (lane == 0) {
+        if (wide)
+            bulk_wait_read<0>();
+        else
+            bulk_wait_read<1>();
+    }
+    __syncwarp();
+    if (wide) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++)
+            *reinterpret_cast<float4 *>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const float *x = v + 8 * j;
+            *reinterpret_cast<uint4 *>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(pack16(x[0], x[1], p.out), pack16(x[2], x[3], p.out), pack16(x[4], x[5], p.out), pack16(x[6], x[7], p.out));
+        }
+    }
+    if (p.ragged && col < p.n && p.n - col < kLinearChunk) {
+        __syncwarp();
+        const uint32_t left = p.n - col, j = lane * (wide ? 4 : 2), piece = j >> 4, in_piece = j & 15;
+        for (uint32_t i = 0; i < 32 && row + i < p.m; i++) {
+            const uint64_t at = (uint64_t)(row + i) * p.ldc + col + lane;
+            if (lane < left) {
+                if (wide)
+                    static_cast<float *>(p.c[which])[at] = *reinterpret_cast<const float *>(box + i * 128 + ((piece ^ (i & 7)) << 4) + in_piece);
+                else
+                    static_cast<uint16_t *>(p.c[which])[at] = *reinterpret_cast<const uint16_t *>(box + i * 64 + ((piece ^ ((i >> 1) & 3)) << 4) + in_piece);
+            }
+        }
+        __syncwarp();
+        if (lane == 0)
+            bulk_commit();                              // an empty group: the boxes' turns are counted in groups
+    } else {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, box, (int32_t)col, (int32_t)row);
+            bulk_commit();
+        }
+    }
+    n_stored++;
+}
+
+template <int ACT>
+__device__ __forceinline__ void gate32(float (&h)[32], const float (&u)[32])
+{
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+        h[i] = activate<ACT>(h[i]) * u[i];
+}
+
+__device__ __forceinline__ void gate32_by(int act, float (&h)[32], const float (&u)[32])
+{
+    switch (act) {
+    case CLPK_ACT_SILU:      gate32<CLPK_ACT_SILU>(h, u); break;
+    case CLPK_ACT_GELU_TANH: gate32<CLPK_ACT_GELU_TANH>(h, u); break;
+    case CLPK_ACT_GELU:      gate32<CLPK_ACT_GELU>(h, u); break;
+    case CLPK_ACT_RELU:      gate32<CLPK_ACT_RELU>(h, u); break;
+    default:                 gate32<CLPK_ACT_SIGMOID>(h, u); break;
+    }
+}
+
+// the sums of a chunk in fp32; those of 8-bit integers with their scales
+template <int DT>
+__device__ __forceinline__ void scaled32(float (&v)[32], const uint32_t (&sum)[32], float row_scale, const float *col_scales)
+{
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+        if constexpr (DT == CLPK_DT_I8) {
+            const float4 s = *reinterpret_cast<const float4 *>(col_scales + i);
+            v[i] = (float)(int32_t)sum[i] * row_scale * s.x;
+            v[i + 1] = (float)(int32_t)sum[i + 1] * row_scale * s.y;
+            v[i + 2] = (float)(int32_t)sum[i + 2] * row_scale * s.z;
+            v[i + 3] = (float)(int32_t)sum[i + 3] * row_scale * s.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                v[i + j] = __uint_as_float(sum[i + j]);
+        }
+    }
+}
+
+__device__ __forceinline__ float bias_at(const void *bias, int type, uint32_t col)
+{
+    if (type == CLPK_DT_F32)
+        return static_cast<const float *>(bias)[col];
+    return type == CLPK_DT_F16 ? __half2float(static_cast<const __half *>(bias)[col]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(bias)[col]);
+}
+
+// What becomes of a unit of sums: one chunk of 32 columns, or with kGated the chunk of g and that of u.
+template <int DT, LinearForm FORM>
+__device__ __forceinline__ void linear_finish(const LinearMaps &maps, const LinearParams &p, LinearSmemOf<DT> *sh, const uint32_t (&s0)[32], const uint32_t (&s1)[32],
+                                              uint32_t product, uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int ew, int lane)
+{
+    float row_scale = 1.0f;
+    const float *scales0 = nullptr, *scales1 = nullptr;
+    if constexpr (DT == CLPK_DT_I8) {
+        float(*scales)[kLinearChunk] = sh->scales[ew];
+        scales0 = scales[0];
+        scales1 = scales[1];
+        const uint32_t c = col + lane;
+        __syncwarp();
+        scales[0][lane] = c < p.n ? p.b_scale[c] : 0.0f;
+        if constexpr (FORM == kGated)
+            scales[1][lane] = c < p.n ? p.u_scale[c] : 0.0f;
+        else
+            scales[1][lane] = p.bias && c < p.n ? bias_at(p.bias, p.out, c) : 0.0f;
+        row_scale = row + lane < p.m ? p.a_scale[row + lane] : 0.0f;
+        __syncwarp();
+    }
+    float v[32];
+    scaled32<DT>(v, s0, row_scale, scales0);
+    if constexpr (FORM == kGated) {
+        float u[32];
+        scaled32<DT>(u, s1, row_scale, scales1);
+        if (p.keep) {
+            linear_store(v, p, 1, boxes, n_stored, &maps.c[1], col, row, lane);
+            linear_store(u, p, 2, boxes, n_stored, &maps.c[2], col, row, lane);
+        }
+        gate32_by(p.activation, v, u);
+    } else if constexpr (FORM == kScaled) {
+        if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 b = *reinterpret_cast<const float4 *>(scales1 + i);
+                v[i] += b.x; v[i + 1] += b.y; v[i + 2] += b.z; v[i + 3] += b.w;
+            }
+        }
+    }
+    const uint32_t which = FORM == kPlain ? product : 0;
+    linear_store(v, p, which, boxes, n_stored, &maps.c[which], col, row, lane);
+}
+
+template <int DT, LinearForm FORM, bool kAMn, bool kBMn, uint32_t kRowBlocks>
+__global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_constant__ LinearMaps maps, LinearParams p)
+{
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    constexpr uint32_t b_at = kRowBlocks * kHalfTileBytes;
+    const uint32_t block_bytes = linear_block_bytes(p.tn, kRowBlocks), stage_bytes = p.kps * block_bytes;
+    uint8_t *staging = smem + (size_t)p.stages * stage_bytes;
+    LinearSmemOf<DT> *sh = reinterpret_cast<LinearSmemOf<DT> *>(staging + kEpilogueWarps * kStagingBytes);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank(), r = rank & 1, leader = rank & ~1u, split = rank >> 1;
+    const uint32_t cluster_id = blockIdx.x / (2 * p.splits), n_clusters = gridDim.x / (2 * p.splits);
+    const uint32_t tiles = p.tiles_m * p.tiles_n, n_tiles = p.products * tiles;
+    const bool two_accs = kRowBlocks * p.tn <= 256;
+    const uint32_t kb0 = split * p.k_blocks / p.splits, kb1 = (split + 1) * p.k_blocks / p.splits;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.stages; s++) {
+            mbar_init(&sh->full[s], 1);
+            mbar_init(&sh->empty[s], 1);
+        }
+        for (int acc = 0; acc < 2; acc++) {
+            mbar_init(&sh->tmem_full[acc], 1);
+            mbar_init(&sh->tmem_empty[acc], 2 * kEpilogueWarps);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&maps.a[0]);
+        tma_prefetch_desc(&maps.b[FORM == kGated ? r : 0]);
+        tma_prefetch_desc(&maps.c[0]);
+    }
+    if (warp == 1)
+        tmem_alloc<2>(&sh->tmem_base, p.tmem_cols);
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh->tmem_base;
+    griddep_wait();
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *p.status = 0u;
+    griddep_launch_dependents();
+
+    const uint32_t q = (uint32_t)(warp & 3), half = (uint32_t)(warp - 2) >> 2;     // epilogue warps
+    const uint32_t units = (FORM == kGated ? p.tn / 2 : p.tn) / kLinearChunk, unit_cols = FORM == kGated ? p.tn / 2 : p.tn;
+    constexpr uint32_t kSubs = FORM == kGated ? 2 : 1;                             // chunks per unit, tn / 2 columns apart
+    uint8_t *boxes = staging + (size_t)(warp - 2) * kStagingBytes;
+    uint32_t n_stored = 0;
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        const uint32_t full0 = cluster_addr(&sh->full[0], leader);
+        uint32_t s = 0, parity = 1;                            // parity of the empty barrier's previous phase
+        bool ok = true;
+        for (uint32_t tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
+            const uint32_t product = tile >= tiles ? 1 : 0;
+            uint32_t mb, nb;
+            dense_tile_coords(tile - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
+            const uint32_t row_a = mb * kRowBlocks * kLinearM + r * 128;
+            const uint32_t row_b = FORM == kGated ? nb * (p.tn / 2) : nb * p.tn + r * (p.tn / 2);
+            for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
+                if (!warp_wait(&sh->empty[s], parity)) {       // a fresh barrier's preceding phase counts as complete
+                    if (lane == 0)
+                        atomicCAS(p.status, 0u, 0x301u);
+                    ok = false;
+                    break;
+                }
+                uint8_t *st = smem + (size_t)s * stage_bytes;
+                const uint32_t nk = kb1 - kb < p.kps ? kb1 - kb : p.kps;
+                if (elect_one()) {
+                    if (r == 0)
+                        mbar_expect_tx(&sh->full[s], nk * 2 * block_bytes);
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; h++)
+                        if (h < nk) {
+                            uint8_t *blk = st + h * block_bytes;
+                            const uint32_t segment = kb + h >= p.k_segment ? 1 : 0, k = kb + h - segment * p.k_segment;
+                            const CUtensorMap *a = &maps.a[product | segment], *b = &maps.b[FORM == kGated ? r : segment];
+                            linear_load<kAMn>(blk, a, k, row_a, 128, full0 + 8 * s);
+                            if constexpr (kRowBlocks == 2)
+                                linear_load<kAMn>(blk + kHalfTileBytes, a, k, row_a + kLinearM, 128, full0 + 8 * s);
+                            linear_load<kBMn>(blk + b_at, b, k, row_b, p.tn / 2, full0 + 8 * s);
+                        }
+                }
+                __syncwarp();
+                if (++s == p.stages) {
+                    s = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (the pair's leader) ----------------
+        if (r == 0) {
+            constexpr uint32_t kFmt = DT == CLPK_DT_BF16 ? kFmtBF16 : DT == CLPK_DT_F16 ? kFmtF16 : kFmtS8;
+            const uint32_t idesc = make_idesc(256, p.tn, kFmt, kFmt, DT == CLPK_DT_I8 ? kAccS32 : kAccF32) | (kAMn ? kMajorA : 0u) | (kBMn ? kMajorB : 0u);
+            const uint16_t pair_mask = (uint16_t)(3u << leader);
+            uint32_t s = 0, parity = 0, tcount = 0;
+            bool ok = true;
+            for (uint32_t tile = cluster_id; tile < n_tiles && ok; tile += n_clusters, tcount++) {
+                const uint32_t acc = two_accs ? tcount & 1 : 0, use = two_accs ? tcount >> 1 : tcount;
+                if (use > 0 && !warp_wait(&sh->tmem_empty[acc], (use - 1) & 1)) {
+                    if (lane == 0)
+                        atomicCAS(p.status, 0u, 0x302u);
+                    break;
+                }
+                tc_fence_after_sync();
+                const uint32_t d = tmem + acc * kRowBlocks * p.tn;
+                for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
+                    if (!warp_wait(&sh->full[s], parity)) {
+                        if (lane == 0)
+                            atomicCAS(p.status, 0u, 0x303u);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t base = smem_u32(smem + (size_t)s * stage_bytes);
+                    const uint32_t nk = kb1 - kb < p.kps ? kb1 - kb : p.kps;
+                    const uint32_t s_now = s;
+                    if (++s == p.stages) {
+                        s = 0;
+                        parity ^= 1;
+                    }
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; h++) {
+                            if (h >= nk)
+                                break;
+                            const uint32_t blk = base + h * block_bytes;
+                            const uint64_t bd = linear_desc<kBMn>(blk + b_at);
+#pragma unroll
+                            for (uint32_t rb = 0; rb < kRowBlocks; rb++) {
+                                const uint64_t ad = linear_desc<kAMn>(blk + rb * kHalfTileBytes);
+#pragma unroll
+                                for (uint32_t kk = 0; kk < 4; kk++) {
+                                    const uint32_t accumulate = (kb != kb0 || h != 0 || kk != 0) ? 1u : 0u;
+                                    const uint64_t ak = ad + kk * linear_step<kAMn>, bk = bd + kk * linear_step<kBMn>;
+                                    if constexpr (DT == CLPK_DT_I8)
+                                        mma2_i8_ss(d + rb * p.tn, ak, bk, idesc, accumulate);
+                                    else
+                                        mma2_f16_ss(d + rb * p.tn, ak, bk, idesc, accumulate);
+                                }
+                            }
+                        }
+                        tc_commit_pair(&sh->empty[s_now], pair_mask);
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one())
+                    tc_commit_pair(&sh->tmem_full[acc], pair_mask);
+                __syncwarp();
+            }
+        }
+    } else if (p.splits == 1) {
+        // ---------------- epilogue, K not split: the two warps of a lane quarter take every other unit ----------------
+        uint32_t tcount = 0;
+        for (uint32_t tile = cluster_id; tile < n_tiles; tile += n_clusters, tcount++) {
+            const uint32_t product = tile >= tiles ? 1 : 0;
+            uint32_t mb, nb;
+            dense_tile_coords(tile - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
+            const uint32_t acc = two_accs ? tcount & 1 : 0, use = two_accs ? tcount >> 1 : tcount;
+            if (!warp_wait(&sh->tmem_full[acc], use & 1)) {
+                if (lane == 0)
+                    atomicCAS(p.status, 0u, 0x304u);
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t taddr = tmem + acc * kRowBlocks * p.tn + ((q * 32) << 16);
+            const uint32_t row = mb * kRowBlocks * kLinearM + r * 128 + q * 32;
+            auto release = [&]() {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], leader);
+            };
+            if (half >= kRowBlocks * units)
+                release();
+            for (uint32_t c = half; c < kRowBlocks * units; c += 2) {
+                const uint32_t rb = c / units, unit = c - rb * units;
+                uint32_t s0[32], s1[32];
+                tmem_ld_32x32b_x32(taddr + rb * p.tn + unit * kLinearChunk, s0);
+                if constexpr (kSubs == 2)
+                    tmem_ld_32x32b_x32(taddr + rb * p.tn + p.tn / 2 + unit * kLinearChunk, s1);
+                tmem_ld_wait();
+                if (c + 2 >= kRowBlocks * units)
+                    release();
+                linear_finish<DT, FORM>(maps, p, sh, s0, s1, product, row + rb * kLinearM, nb * unit_cols + unit * kLinearChunk, boxes, n_stored, warp - 2, lane);
+            }
+        }
+    } else if (!warp_wait(&sh->tmem_full[0], 0)) {
+        if (lane == 0)
+            atomicCAS(p.status, 0u, 0x305u);
+    }
+
+    if (p.splits > 1) {
+        // ---------------- K split over the cluster's pairs (one tile per cluster, one row block) ----------------
+        // Every pair's instructions have retired, so the stages of the ring are free to take partial sums: slot (src, j) of CTA
+        // (owner, r) holds pair src's sums of the owner's j-th unit, src counted without the owner.  They are added in the order
+        // of the pairs, whoever owns the unit.
+        constexpr uint32_t kUnitBytes = kSubs * kLinearChunk * 128 * 4;
+        tc_fence_before_sync();
+        __syncwarp();
+        cluster_sync();
+        tc_fence_after_sync();
+        const uint32_t slots = (units + p.splits - 1) / p.splits;
+        const uint32_t taddr = tmem + ((q * 32) << 16), my_row = q * 32 + lane;
+        const bool epilogue = warp >= 2;
+        if (epilogue) {
+            for (uint32_t i = half; i < kSubs * units; i += 2) {
+                const uint32_t c = i / kSubs, sub = i % kSubs, owner = c % p.splits;
+                if (owner == split)
+                    continue;
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(taddr + sub * (p.tn / 2) + c * kLinearChunk, v);
+                tmem_ld_wait();
+                const uint32_t src = split < owner ? split : split - 1;
+                const uint32_t dst = cluster_addr(smem + (size_t)(src * slots + c / p.splits) * kUnitBytes + sub * (kUnitBytes / kSubs) + my_row * 16, owner * 2 + r);
+#pragma unroll
+                for (uint32_t g = 0; g < 8; g++)
+                    st_cluster_v4(dst + g * 2048, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (epilogue) {
+            const uint32_t product = cluster_id >= tiles ? 1 : 0;
+            uint32_t mb, nb;
+            dense_tile_coords(cluster_id - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
+            const uint32_t row = mb * kLinearM + r * 128 + q * 32;
+            for (uint32_t j = half; split + j * p.splits < units; j += 2) {
+                const uint32_t c = split + j * p.splits;
+                uint32_t sum[2][32];
+#pragma unroll
+                for (uint32_t sub = 0; sub < kSubs; sub++) {
+                    uint32_t own[32];
+                    tmem_ld_32x32b_x32(taddr + sub * (p.tn / 2) + c * kLinearChunk, own);
+                    tmem_ld_wait();
+                    for (uint32_t src = 0; src < p.splits; src++) {
+                        const uint8_t *slot = smem + (size_t)((src < split ? src : src - 1) * slots + j) * kUnitBytes + sub * (kUnitBytes / kSubs) + my_row * 16;
+#pragma unroll
+                        for (uint32_t g = 0; g < 8; g++) {
+                            uint4 v = make_uint4(own[4 * g], own[4 * g + 1], own[4 * g + 2], own[4 * g + 3]);
+                            if (src != split)
+                                v = *reinterpret_cast<const uint4 *>(slot + g * 2048);
+                            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (uint32_t t = 0; t < 4; t++) {
+                                uint32_t &x = sum[sub][4 * g + t];
+                                if (src == 0)
+                                    x = e[t];
+                                else if constexpr (DT == CLPK_DT_I8)
+                                    x += e[t];
+                                else
+                                    x = __float_as_uint(__uint_as_float(x) + __uint_as_float(e[t]));
+                            }
+                        }
+                    }
+                }
+                linear_finish<DT, FORM>(maps, p, sh, sum[0], sum[kSubs - 1], product, row, nb * unit_cols + c * kLinearChunk, boxes, n_stored, warp - 2, lane);
+            }
+        }
+    }
+    // the staging boxes must have been read before this CTA's shared memory goes away
+    if (warp >= 2 && lane == 0)
+        bulk_wait_read<0>();
+
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1)
+        tmem_dealloc<2>(tmem, p.tmem_cols);
+}
+
+// ---- host side -----------------------------------------------------------------------------
+
+// a row-major matrix, in boxes of 128 bytes of a row times box_rows rows
+static int make_matrix_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t row_bytes, uint64_t pitch_bytes, uint32_t box_rows)
+{
+    EncodeTiledFn enc = nullptr;
+    const int rc = get_encode_fn(&enc);
+    if (rc != CLPK_OK)
+        return rc;
+    const cuuint64_t dims[2] = {row_bytes, rows}, strides[1] = {pitch_bytes};
+    const cuuint32_t box[2] = {kRowBytesK, box_rows}, estr[2] = {1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+        return CLPK_ERR_CUDA;
+    }
+    return CLPK_OK;
+}
+
+// a result, in boxes of 32 x 32
+static int make_result_map(CUtensorMap *map, void *base, uint64_t rows, uint64_t cols, uint64_t ld, int type)
+{
+    EncodeTiledFn enc = nullptr;
+    const int rc = get_encode_fn(&enc);
+    if (rc != CLPK_OK)
+        return rc;
+    const uint32_t elem = type == CLPK_DT_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * elem};
+    const cuuint32_t box[2] = {kLinearChunk, 32}, estr[2] = {1, 1};
+    const CUresult r = enc(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, elem == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled (result) failed with CUresult %d", (int)r);
+        return CLPK_ERR_CUDA;
+    }
+    return CLPK_OK;
+}

@@ -23,6 +23,15 @@ __device__ __forceinline__ void tma_load_pair_at(void *smem_dst, const CUtensorM
         : "memory");
 }
 
+// 2-D tile load into this CTA's shared memory, its bytes counted by this CTA's barrier
+__device__ __forceinline__ void tma_load_own(void *smem_dst, const CUtensorMap *tmap, int32_t x, int32_t y, uint64_t *bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y)
+        : "memory");
+}
+
 __device__ __forceinline__ uint32_t leader_addr(const void *p)
 {
     uint32_t a;

@@ -277,6 +277,17 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
         : "memory");
 }
 
+// 32 lanes x 16 columns
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 __device__ __forceinline__ void tmem_ld_wait()
 {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -404,6 +415,8 @@ __host__ __device__ __forceinline__ uint32_t make_idesc(uint32_t m, uint32_t n, 
 }
 
 constexpr uint32_t kNegateA = 1u << 13;         // floating kinds: A's elements with the other sign
+constexpr uint32_t kMajorA = 1u << 15;          // A is contiguous along M: its descriptor's leading offset is the distance between
+constexpr uint32_t kMajorB = 1u << 16;          // blocks of one swizzled row (64 16-bit elements), its stride that of 8 rows of K; B along N
 
 // Block-scaled kinds (mxf8f6f4 / mxf4 / mxf4nvf4): same operand fields, plus
 //   [4,6) B scale-factor id   [23] scale format (0 ue4m3, 1 ue8m0)

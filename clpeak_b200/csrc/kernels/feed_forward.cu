@@ -8,172 +8,269 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../clpk_activation.cuh"
 #include "../clpk_internal.h"
+#include "../clpk_pair.cuh"
 #include "../clpk_ptx.cuh"
 
 namespace clpk {
 
-// a matrix whose element (i, k) lies at base[i * rows + k * cols]
-struct Strided {
-    const void *base;
-    uint64_t rows, cols;
-};
+#include "../clpk_linear.cuh"
+#include "../clpk_linear_few.cuh"
 
-struct ProductParams {
-    Strided a[2], b[2];
-    uint32_t m, n, k;
-    int segments;                       // products that are added: a[0] b[0]^T + a[1] b[1]^T
-    int activation;
-    void *c, *g, *u;
-    uint64_t ldc;
-    const float *a_scale, *b_scale, *u_scale;
-    const void *bias;
-};
-
-template <typename T> __device__ __forceinline__ float to_float(T v) { return (float)v; }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float activate_by(int act, float g)
-{
-    switch (act) {
-    case CLPK_ACT_SILU:      return activate<CLPK_ACT_SILU>(g);
-    case CLPK_ACT_GELU_TANH: return activate<CLPK_ACT_GELU_TANH>(g);
-    case CLPK_ACT_GELU:      return activate<CLPK_ACT_GELU>(g);
-    case CLPK_ACT_RELU:      return activate<CLPK_ACT_RELU>(g);
-    default:                 return activate<CLPK_ACT_SIGMOID>(g);
-    }
-}
-
-// 32 x 32 results a block, a thread four of a column, through 32 x 32 tiles in shared memory
-template <typename T, typename Acc, typename Out, bool kGated>
-__global__ void __launch_bounds__(256) product_kernel(ProductParams p)
-{
-    __shared__ Acc ta[32][33], tb[2][32][33];
-    const uint32_t tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-    const uint32_t row0 = blockIdx.y * 32, col0 = blockIdx.x * 32;
-    Acc acc[2][4] = {};
-    griddep_wait();
-    griddep_launch_dependents();
-    for (int s = 0; s < p.segments; s++) {
-        const Strided &a = p.a[s];
-        for (uint32_t k0 = 0; k0 < p.k; k0 += 32) {
-            for (uint32_t i = ty; i < 32; i += 8) {
-                const uint32_t k = k0 + tx;
-                ta[i][tx] = row0 + i < p.m && k < p.k ? (Acc)static_cast<const T *>(a.base)[(row0 + i) * a.rows + k * a.cols] : Acc(0);
-                for (int o = 0; o < (kGated ? 2 : 1); o++) {
-                    const Strided &b = p.b[kGated ? o : s];
-                    tb[o][i][tx] = col0 + i < p.n && k < p.k ? (Acc)static_cast<const T *>(b.base)[(col0 + i) * b.rows + k * b.cols] : Acc(0);
-                }
-            }
-            __syncthreads();
-            for (uint32_t k = 0; k < 32; k++)
-                for (uint32_t i = 0; i < 4; i++) {
-                    acc[0][i] += ta[ty + 8 * i][k] * tb[0][tx][k];
-                    if (kGated)
-                        acc[1][i] += ta[ty + 8 * i][k] * tb[1][tx][k];
-                }
-            __syncthreads();
-        }
-    }
-    const uint32_t col = col0 + tx;
-    for (uint32_t i = 0; i < 4; i++) {
-        const uint32_t row = row0 + ty + 8 * i;
-        if (row >= p.m || col >= p.n)
-            continue;
-        const uint64_t at = row * p.ldc + col;
-        float v = (float)acc[0][i];
-        if (p.a_scale)
-            v = v * p.a_scale[row] * p.b_scale[col];
-        if constexpr (kGated) {
-            float u = (float)acc[1][i];
-            if (p.a_scale)
-                u = u * p.a_scale[row] * p.u_scale[col];
-            if (p.g) {
-                static_cast<Out *>(p.g)[at] = from_float<Out>(v);
-                static_cast<Out *>(p.u)[at] = from_float<Out>(u);
-            }
-            v = activate_by(p.activation, v) * u;
-        } else if (p.bias) {
-            v += to_float(static_cast<const Out *>(p.bias)[col]);
-        }
-        static_cast<Out *>(p.c)[at] = from_float<Out>(v);
-    }
-}
-
+// ---- dg = dh * u * act'(g) and du = dh * act(g) -----------------------------------------------------------
+//
+// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements per step and thread.
 struct GradParams {
     const void *dh, *g, *u;
     void *dg, *du;
     uint64_t ldh, ldw;                  // of the first three, and of the two in the workspace
     uint32_t m, f;
+    uint32_t vectors;                   // of eight elements in a row
 };
 
-template <typename T, int ACT>
+template <int DT>
+__device__ __forceinline__ float2 widen(uint32_t w)
+{
+    if constexpr (DT == CLPK_DT_F16)
+        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+// eight elements of a row of `f`, zeros beyond it
+__device__ __forceinline__ uint4 load8(const void *base, uint64_t at, uint32_t left)
+{
+    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+    if (left >= 8)
+        return *reinterpret_cast<const uint4 *>(p);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; i++)
+        if (i < left)
+            w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int DT, int ACT>
 __global__ void __launch_bounds__(256) gate_gradients_kernel(GradParams p)
 {
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t col = blockIdx.x * 256 + threadIdx.x;
-    if (col >= p.f)
-        return;
-    for (uint32_t row = blockIdx.y; row < p.m; row += gridDim.y) {
-        const uint64_t at = row * p.ldh + col, to = row * p.ldw + col;
-        const float dh = to_float(static_cast<const T *>(p.dh)[at]), u = to_float(static_cast<const T *>(p.u)[at]);
-        float a, da;
-        activate_both<ACT>(to_float(static_cast<const T *>(p.g)[at]), a, da);
-        static_cast<T *>(p.dg)[to] = from_float<T>(dh * u * da);
-        static_cast<T *>(p.du)[to] = from_float<T>(dh * a);
+    const uint64_t all = (uint64_t)p.m * p.vectors;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = i / p.vectors;
+        const uint32_t col = (uint32_t)(i - row * p.vectors) * 8, left = p.f - col;
+        const uint64_t at = row * p.ldh + col;
+        const uint4 vdh = load8(p.dh, at, left), vg = load8(p.g, at, left), vu = load8(p.u, at, left);
+        const uint32_t dh[4] = {vdh.x, vdh.y, vdh.z, vdh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
+        uint32_t dg[4], du[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 h2 = widen<DT>(dh[j]), g2 = widen<DT>(g[j]), u2 = widen<DT>(u[j]);
+            float ax, dx, ay, dy;
+            activate_both<ACT>(g2.x, ax, dx);
+            activate_both<ACT>(g2.y, ay, dy);
+            dg[j] = pack16(h2.x * u2.x * dx, h2.y * u2.y * dy, DT);
+            du[j] = pack16(h2.x * ax, h2.y * ay, DT);
+        }
+        const uint64_t to = row * p.ldw + col;          // whole vectors: the workspace's pitch has room for them
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dg) + to) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.du) + to) = make_uint4(du[0], du[1], du[2], du[3]);
     }
 }
 
-template <typename T, typename Acc, typename Out, bool kGated>
-static int launch_product(const ProductParams &p, uint32_t *status, cudaStream_t s)
-{
-    CLPK_CUDA(cudaMemsetAsync(status, 0, sizeof(uint32_t), s));
-    product_kernel<T, Acc, Out, kGated><<<dim3((p.n + 31) / 32, (p.m + 31) / 32), 256, 0, s>>>(p);
-    CLPK_LAUNCH_CHECK("product");
-    return CLPK_OK;
-}
-
-template <bool kGated>
-static int launch_i8(const ProductParams &p, int out_dtype, uint32_t *status, cudaStream_t s)
-{
-    switch (out_dtype) {
-    case CLPK_DT_F32: return launch_product<int8_t, int32_t, float, kGated>(p, status, s);
-    case CLPK_DT_F16: return launch_product<int8_t, int32_t, __half, kGated>(p, status, s);
-    default:          return launch_product<int8_t, int32_t, __nv_bfloat16, kGated>(p, status, s);
-    }
-}
-
-template <bool kGated>
-static int launch_16(const ProductParams &p, int dtype, uint32_t *status, cudaStream_t s)
-{
-    return dtype == CLPK_DT_F16 ? launch_product<__half, float, __half, kGated>(p, status, s)
-                                : launch_product<__nv_bfloat16, float, __nv_bfloat16, kGated>(p, status, s);
-}
-
-template <typename T>
+template <int DT>
 static int launch_gradients(const GradParams &p, int act, cudaStream_t s)
 {
-    const dim3 grid((p.f + 255) / 256, std::min(p.m, 65535u));
+    const uint64_t blocks = ((uint64_t)p.m * p.vectors + 255) / 256;
+    const unsigned grid = (unsigned)std::min<uint64_t>(blocks, 1u << 30);
     switch (act) {
-    case CLPK_ACT_SILU:      gate_gradients_kernel<T, CLPK_ACT_SILU><<<grid, 256, 0, s>>>(p); break;
-    case CLPK_ACT_GELU_TANH: gate_gradients_kernel<T, CLPK_ACT_GELU_TANH><<<grid, 256, 0, s>>>(p); break;
-    case CLPK_ACT_GELU:      gate_gradients_kernel<T, CLPK_ACT_GELU><<<grid, 256, 0, s>>>(p); break;
-    case CLPK_ACT_RELU:      gate_gradients_kernel<T, CLPK_ACT_RELU><<<grid, 256, 0, s>>>(p); break;
-    default:                 gate_gradients_kernel<T, CLPK_ACT_SIGMOID><<<grid, 256, 0, s>>>(p); break;
+    case CLPK_ACT_SILU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SILU>, "gate_gradients", grid, 256, 0, s, p);
+    case CLPK_ACT_GELU_TANH: return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU_TANH>, "gate_gradients", grid, 256, 0, s, p);
+    case CLPK_ACT_GELU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU>, "gate_gradients", grid, 256, 0, s, p);
+    case CLPK_ACT_RELU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_RELU>, "gate_gradients", grid, 256, 0, s, p);
+    default:                 return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SIGMOID>, "gate_gradients", grid, 256, 0, s, p);
     }
-    CLPK_LAUNCH_CHECK("gate_gradients");
-    return CLPK_OK;
+}
+
+// ---- the products -------------------------------------------------------------------------------------------
+
+struct Matrix {
+    const void *base;
+    uint64_t ld;                        // elements
+};
+
+// One product of a layer: sums over `k` of an m x n result.
+struct Product {
+    uint32_t m, n, k;
+    Matrix a[2], b[2];                  // kGated: b[0] = Wg, b[1] = Wu
+    int segments, products;             // pairs of operands that are added; products of the same shape
+    void *c[3];                         // of each product; kGated: h, g, u
+    uint64_t ldc;
+    int out, activation;
+    const float *a_scale, *b_scale, *u_scale;
+    const void *bias;
+    uint32_t *status;
+};
+
+struct LinearPlan {
+    uint32_t tn, splits, row_blocks;
+};
+
+static uint64_t elem_bytes(int dtype) { return dtype == CLPK_DT_F32 ? 4 : dtype == CLPK_DT_I8 ? 1 : 2; }
+
+// K blocks of 128 bytes (64 of 16-bit elements, whichever way they lie)
+static uint32_t linear_k_blocks(const Product &w, int dtype) { return (uint32_t)(((uint64_t)w.k * elem_bytes(dtype) + kRowBytesK - 1) / kRowBytesK); }
+
+static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks, bool b_mn)
+{
+    const uint32_t pairs = (uint32_t)num_sms() / 2, cols = form == kGated ? 2 * w.n : w.n;
+    LinearPlan plan = {256, 1, 1};
+    float best = 1e30f;
+    for (uint32_t splits = 1; splits <= 4 && splits <= k_blocks; splits *= 2)
+        for (uint32_t tn = b_mn ? 128 : 64; tn <= 256; tn += b_mn ? 128 : 64) {
+            const uint32_t resident = splits == 1 ? pairs : splits == 2 ? pairs * 33 / 74 : pairs * 15 / 74;
+            const uint64_t tiles = (uint64_t)w.products * ((w.m - 1) / kLinearM + 1) * ((cols - 1) / tn + 1);
+            if (resident == 0)
+                continue;
+            const float waves = (float)((tiles - 1) / resident + 1), wide = (float)tn / 256.0f;
+            float t = 3.9f + waves * ((float)((k_blocks - 1) / splits + 1) * (0.118f + 0.265f * wide) + 1.2f * wide);
+            if (splits > 1)
+                t += waves * (1.0f + 4.3f * wide);
+            if (t < best) {
+                best = t;
+                plan = {tn, splits, 1};
+            }
+        }
+    return plan;
+}
+
+template <int DT, LinearForm FORM, bool kAMn, bool kBMn, uint32_t kRowBlocks>
+static int launch_linear(const Product &w, LinearPlan plan, uint32_t k_blocks, cudaStream_t s)
+{
+    const uint64_t elem = elem_bytes(DT);
+    LinearMaps maps = {};
+    int rc = CLPK_OK;
+    for (int i = 0; i < 2; i++) {
+        if (w.a[i].base) {
+            rc = kAMn ? make_matrix_map(&maps.a[i], w.a[i].base, w.k, w.m * elem, w.a[i].ld * elem, 64)
+                      : make_matrix_map(&maps.a[i], w.a[i].base, w.m, w.k * elem, w.a[i].ld * elem, 128);
+            if (rc != CLPK_OK)
+                return rc;
+        }
+        if (w.b[i].base) {
+            rc = kBMn ? make_matrix_map(&maps.b[i], w.b[i].base, w.k, w.n * elem, w.b[i].ld * elem, 64)
+                      : make_matrix_map(&maps.b[i], w.b[i].base, w.n, w.k * elem, w.b[i].ld * elem, plan.tn / 2);
+            if (rc != CLPK_OK)
+                return rc;
+        }
+    }
+    for (int i = 0; i < 3; i++)
+        if (w.c[i]) {
+            rc = make_result_map(&maps.c[i], w.c[i], w.m, w.n, w.ldc, w.out);
+            if (rc != CLPK_OK)
+                return rc;
+        }
+    LinearParams p = {};
+    p.m = w.m;
+    p.n = w.n;
+    p.products = (uint32_t)w.products;
+    p.tiles_m = (w.m - 1) / (kLinearM * kRowBlocks) + 1;
+    const uint32_t tile_cols = FORM == kGated ? plan.tn / 2 : plan.tn;
+    p.tiles_n = (w.n - 1) / tile_cols + 1;
+    p.group = 8;
+    p.k_segment = k_blocks;
+    p.k_blocks = k_blocks * (uint32_t)w.segments;
+    p.tn = plan.tn;
+    p.splits = plan.splits;
+    p.out = w.out;
+    p.activation = w.activation;
+    p.keep = FORM == kGated && w.c[1] ? 1 : 0;
+    p.ragged = w.n * elem_bytes(w.out) % 16 != 0;
+    std::copy(w.c, w.c + 3, p.c);
+    p.ldc = w.ldc;
+    p.a_scale = w.a_scale;
+    p.b_scale = w.b_scale;
+    p.u_scale = w.u_scale;
+    p.bias = w.bias;
+    p.status = w.status;
+    const uint32_t n_tiles = p.products * p.tiles_m * p.tiles_n, pairs = (uint32_t)num_sms() / 2;
+    const uint32_t clusters = plan.splits > 1 ? n_tiles : std::min(n_tiles, pairs);
+    constexpr size_t fixed = kEpilogueWarps * kStagingBytes + sizeof(LinearSmemOf<DT>) + 1024;
+    p.kps = plan.tn <= 128 && kRowBlocks == 1 ? 2 : 1;
+    const uint32_t stage_bytes = p.kps * linear_block_bytes(plan.tn, kRowBlocks);
+    p.stages = std::min<uint32_t>((uint32_t)((kSmemMax - fixed) / stage_bytes), kLinearMaxStages);
+    p.tmem_cols = 32;
+    while (p.tmem_cols < (n_tiles > clusters && kRowBlocks * plan.tn <= 256 ? 2 : 1) * kRowBlocks * plan.tn)
+        p.tmem_cols *= 2;
+    return launch_clusters(linear_kernel<DT, FORM, kAMn, kBMn, kRowBlocks>, "linear", clusters * 2 * plan.splits, kLinearThreads,
+                           p.stages * stage_bytes + fixed, 2 * plan.splits, s, maps, p);
+}
+
+constexpr uint32_t kFewTokens = 128;
+
+template <int DT, LinearForm FORM>
+static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
+{
+    constexpr uint32_t tile_cols = FORM == kGated ? 64 : 128;
+    const uint64_t elem = elem_bytes(DT);
+    FewParams p = {};
+    p.m = w.m;
+    p.n = w.n;
+    p.k_blocks = k_blocks;
+    p.tokens = (w.m + 15) / 16 * 16;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < p.tokens)
+        p.tmem_cols *= 2;
+    const uint32_t tiles = (w.n - 1) / tile_cols + 1, sms = (uint32_t)num_sms();
+    p.splits = 1;
+    while (p.splits < 8 && tiles * p.splits < 2 * sms && k_blocks >= 8 * p.splits)
+        p.splits *= 2;
+    const uint32_t stage_bytes = kHalfTileBytes + p.tokens * kRowBytesK;
+    p.stages = std::min<uint32_t>(72 * 1024 / stage_bytes, kFewMaxStages);
+    p.out = w.out;
+    p.activation = w.activation;
+    p.c = w.c[0];
+    p.g = w.c[1];
+    p.u = w.c[2];
+    p.ldc = w.ldc;
+    p.a_scale = w.a_scale;
+    p.b_scale = w.b_scale;
+    p.u_scale = w.u_scale;
+    p.bias = w.bias;
+    p.status = w.status;
+    FewMaps maps = {};
+    int rc = make_matrix_map(&maps.x, w.a[0].base, w.m, w.k * elem, w.a[0].ld * elem, p.tokens);
+    for (int i = 0; i < (FORM == kGated ? 2 : 1) && rc == CLPK_OK; i++)
+        rc = make_matrix_map(&maps.w[i], w.b[i].base, w.n, w.k * elem, w.b[i].ld * elem, tile_cols);
+    if (rc != CLPK_OK)
+        return rc;
+    return launch_clusters(linear_few_kernel<DT, FORM>, "linear_few", tiles * p.splits, kFewThreads, p.stages * stage_bytes + sizeof(FewSmem) + 1024, p.splits, s,
+                           maps, p);
+}
+
+// a product whose operands are contiguous along K, with few tokens or many
+template <int DT, LinearForm FORM>
+static int run_tokens(const Product &w, cudaStream_t s)
+{
+    const uint32_t k_blocks = linear_k_blocks(w, DT);
+    if (w.m <= kFewTokens)
+        return launch_few<DT, FORM>(w, k_blocks, s);
+    return launch_linear<DT, FORM, false, false, 1>(w, plan_linear(w, FORM, k_blocks, false), k_blocks, s);
+}
+
+// a product of the backward pass: B contiguous along N, A along K or M
+template <int DT, bool kAMn>
+static int run_gradient(const Product &w, cudaStream_t s)
+{
+    const uint32_t k_blocks = linear_k_blocks(w, DT);
+    return launch_linear<DT, kPlain, kAMn, true, 1>(w, plan_linear(w, kPlain, k_blocks * (uint32_t)w.segments, true), k_blocks, s);
 }
 
 // ---- what the calls ask of their arguments ------------------------------------------------------------
-
-static uint64_t elem_bytes(int dtype) { return dtype == CLPK_DT_F32 ? 4 : dtype == CLPK_DT_I8 ? 1 : 2; }
 
 // the pitch of a matrix with `cols` columns; 0 in *ld: rows one behind another
 static int check_matrix(const char *what, const char *name, const void *base, uint64_t cols, uint64_t *ld, int dtype)
@@ -248,19 +345,21 @@ int clpk_gemm_i8_scaled(const clpk_gemm_i8_scaled_args_t *args, void *stream)
     CLPK_TRY(check_scales(what, "d_a_scale", a.d_a_scale));
     CLPK_TRY(check_scales(what, "d_b_scale", a.d_b_scale));
     CLPK_REQUIRE((uintptr_t)a.d_bias % elem_bytes(a.out_dtype) == 0, "%s: d_bias is not aligned to its elements", what);
-    ProductParams p = {};
-    p.a[0] = {a.d_a, a.lda, 1};
-    p.b[0] = {a.d_b, a.ldb, 1};
-    p.m = a.m;
-    p.n = a.n;
-    p.k = a.k;
-    p.segments = 1;
-    p.c = a.d_c;
-    p.ldc = a.ldc;
-    p.a_scale = a.d_a_scale;
-    p.b_scale = a.d_b_scale;
-    p.bias = a.d_bias;
-    return launch_i8<false>(p, a.out_dtype, a.d_status, s);
+    Product w = {};
+    w.m = a.m;
+    w.n = a.n;
+    w.k = a.k;
+    w.a[0] = {a.d_a, a.lda};
+    w.b[0] = {a.d_b, a.ldb};
+    w.segments = w.products = 1;
+    w.c[0] = a.d_c;
+    w.ldc = a.ldc;
+    w.out = a.out_dtype;
+    w.a_scale = a.d_a_scale;
+    w.b_scale = a.d_b_scale;
+    w.bias = a.d_bias;
+    w.status = a.d_status;
+    return run_tokens<CLPK_DT_I8, kScaled>(w, s);
 }
 
 int clpk_gated_ffn(const clpk_gated_ffn_args_t *args, void *stream)
@@ -297,26 +396,28 @@ int clpk_gated_ffn(const clpk_gated_ffn_args_t *args, void *stream)
         CLPK_TRY(check_scales(what, "d_wg_scale", a.d_wg_scale));
         CLPK_TRY(check_scales(what, "d_wu_scale", a.d_wu_scale));
     }
-    ProductParams p = {};
-    p.a[0] = {a.d_x, a.ldx, 1};
-    p.b[0] = {a.d_wg, a.ldw, 1};
-    p.b[1] = {a.d_wu, a.ldw, 1};
-    p.m = a.m;
-    p.n = a.f;
-    p.k = a.d;
-    p.segments = 1;
-    p.activation = a.activation;
-    p.c = a.d_h;
-    p.g = a.d_g;
-    p.u = a.d_u;
-    p.ldc = a.ldh;
+    Product w = {};
+    w.m = a.m;
+    w.n = a.f;
+    w.k = a.d;
+    w.a[0] = {a.d_x, a.ldx};
+    w.b[0] = {a.d_wg, a.ldw};
+    w.b[1] = {a.d_wu, a.ldw};
+    w.segments = w.products = 1;
+    w.c[0] = a.d_h;
+    w.c[1] = a.d_g;
+    w.c[2] = a.d_u;
+    w.ldc = a.ldh;
+    w.out = out;
+    w.activation = a.activation;
+    w.status = a.d_status;
     if (i8) {
-        p.a_scale = a.d_x_scale;
-        p.b_scale = a.d_wg_scale;
-        p.u_scale = a.d_wu_scale;
-        return launch_i8<true>(p, out, a.d_status, s);
+        w.a_scale = a.d_x_scale;
+        w.b_scale = a.d_wg_scale;
+        w.u_scale = a.d_wu_scale;
+        return run_tokens<CLPK_DT_I8, kGated>(w, s);
     }
-    return launch_16<true>(p, out, a.d_status, s);
+    return a.dtype == CLPK_DT_F16 ? run_tokens<CLPK_DT_F16, kGated>(w, s) : run_tokens<CLPK_DT_BF16, kGated>(w, s);
 }
 
 int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, uint32_t f, size_t *bytes)
@@ -368,32 +469,41 @@ int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *st
 
     const uint64_t ld = gradient_pitch(a.f);
     uint8_t *dg = static_cast<uint8_t *>(a.d_workspace), *du = dg + a.m * ld * 2;
-    const GradParams gp = {a.d_dh, a.d_g, a.d_u, dg, du, a.ldh, ld, a.m, a.f};
-    CLPK_TRY(a.dtype == CLPK_DT_F16 ? launch_gradients<__half>(gp, a.activation, s) : launch_gradients<__nv_bfloat16>(gp, a.activation, s));
-    ProductParams p = {};
+    const GradParams gp = {a.d_dh, a.d_g, a.d_u, dg, du, a.ldh, ld, a.m, a.f, (uint32_t)(ld / 8)};
+    CLPK_TRY(a.dtype == CLPK_DT_F16 ? launch_gradients<CLPK_DT_F16>(gp, a.activation, s) : launch_gradients<CLPK_DT_BF16>(gp, a.activation, s));
     if (a.d_dx) {
-        p.a[0] = {dg, ld, 1};
-        p.a[1] = {du, ld, 1};
-        p.b[0] = {a.d_wg, 1, a.ldw};
-        p.b[1] = {a.d_wu, 1, a.ldw};
-        p.m = a.m;
-        p.n = a.d;
-        p.k = a.f;
-        p.segments = 2;
-        p.c = a.d_dx;
-        p.ldc = a.ldx;
-        CLPK_TRY(launch_16<false>(p, a.dtype, a.d_status, s));
+        Product w = {};
+        w.m = a.m;
+        w.n = a.d;
+        w.k = a.f;
+        w.a[0] = {dg, ld};
+        w.a[1] = {du, ld};
+        w.b[0] = {a.d_wg, a.ldw};
+        w.b[1] = {a.d_wu, a.ldw};
+        w.segments = 2;
+        w.products = 1;
+        w.c[0] = a.d_dx;
+        w.ldc = a.ldx;
+        w.out = a.dtype;
+        w.status = a.d_status;
+        CLPK_TRY((a.dtype == CLPK_DT_F16 ? run_gradient<CLPK_DT_F16, false>(w, s) : run_gradient<CLPK_DT_BF16, false>(w, s)));
     }
-    for (int o = 0; o < 2 && a.d_dwg; o++) {
-        p.a[0] = {o ? du : dg, 1, ld};
-        p.b[0] = {a.d_x, 1, a.ldx};
-        p.m = a.f;
-        p.n = a.d;
-        p.k = a.m;
-        p.segments = 1;
-        p.c = o ? a.d_dwu : a.d_dwg;
-        p.ldc = a.ldw;
-        CLPK_TRY(launch_16<false>(p, a.dtype, a.d_status, s));
+    if (a.d_dwg) {
+        Product w = {};
+        w.m = a.f;
+        w.n = a.d;
+        w.k = a.m;
+        w.a[0] = {dg, ld};
+        w.a[1] = {du, ld};
+        w.b[0] = {a.d_x, a.ldx};
+        w.segments = 1;
+        w.products = 2;
+        w.c[0] = a.d_dwg;
+        w.c[1] = a.d_dwu;
+        w.ldc = a.ldw;
+        w.out = a.dtype;
+        w.status = a.d_status;
+        CLPK_TRY((a.dtype == CLPK_DT_F16 ? run_gradient<CLPK_DT_F16, true>(w, s) : run_gradient<CLPK_DT_BF16, true>(w, s)));
     }
     return CLPK_OK;
 }
