@@ -210,12 +210,43 @@ static int launch_linear(const Product &w, LinearPlan plan, uint32_t k_blocks, c
                            p.stages * stage_bytes + fixed, 2 * plan.splits, s, maps, p);
 }
 
-constexpr uint32_t kFewTokens = 128;
+template <LinearForm FORM> constexpr uint32_t few_cols = FORM == kGated ? 64 : 128;      // features of a tile
+
+// K ranges of linear_few_kernel: as many as the chip holds CTAs for at once, as long as each has some blocks of K; with long sums
+// also where that loads the SMs more evenly.  Of 160 shapes (1 to 128 tokens) it is 1 % slower than the fastest in the geometric
+// mean.  What it decides: int8 1 x 4096 x 4096 in one range 9.2 us, in four 5.2; 8 x 30080 x 4096 (235 tiles) 26.7, in two 22.8.
+static uint32_t few_splits(uint32_t tokens, uint32_t tiles, uint32_t k_blocks, uint32_t sms)
+{
+    uint32_t splits = 1;
+    if (k_blocks >= 8 && tiles * 2 <= sms)
+        splits = 2;
+    if ((k_blocks >= 48 && tiles > sms && tiles * 5 <= sms * 6) || (k_blocks >= 16 && tiles * 2 > sms * 3 && tiles < sms * 2))
+        splits = 2;
+    if (k_blocks >= (tokens >= 64 ? 4u : 8u) && tiles * 4 <= sms * 9 / 7)
+        splits = 4;
+    if (k_blocks >= 32 && tokens <= 48 && tiles * 2 > sms && tiles * 10 <= sms * 7)
+        splits = 4;
+    if (k_blocks >= 14 && tiles * 8 <= (k_blocks >= 64 ? sms : sms * 6 / 7))
+        splits = 8;
+    return splits;
+}
+
+// Whether the tokens are few: up to 64 they are; then it depends on whether finishing them or filling the chip costs more (96
+// tokens: 15 tiles of 48 blocks 7.3 us here, 10.1 on pairs; 128 tokens: 12 of 50 9.4 and 13.4, 126 of 25 20.8 and 17.8, 4 of 4
+// 6.4 and 5.0).
+static bool few_tokens(uint32_t tokens, uint32_t tiles, uint32_t k_blocks, uint32_t sms)
+{
+    if (tokens <= 64)
+        return true;
+    if (tokens <= 96)
+        return k_blocks < 36 || tiles * 5 <= sms * 3;
+    return tokens <= 128 && k_blocks >= 20 && few_splits(tokens, tiles, k_blocks, sms) >= 4;
+}
 
 template <int DT, LinearForm FORM>
 static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
 {
-    constexpr uint32_t tile_cols = FORM == kGated ? 64 : 128;
+    constexpr uint32_t tile_cols = few_cols<FORM>;
     const uint64_t elem = elem_bytes(DT);
     FewParams p = {};
     p.m = w.m;
@@ -226,11 +257,24 @@ static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
     while (p.tmem_cols < p.tokens)
         p.tmem_cols *= 2;
     const uint32_t tiles = (w.n - 1) / tile_cols + 1, sms = (uint32_t)num_sms();
-    p.splits = 1;
-    while (p.splits < 8 && tiles * p.splits < 2 * sms && k_blocks >= 8 * p.splits)
-        p.splits *= 2;
-    const uint32_t stage_bytes = kHalfTileBytes + p.tokens * kRowBytesK;
-    p.stages = std::min<uint32_t>(72 * 1024 / stage_bytes, kFewMaxStages);
+    p.splits = few_splits(w.m, tiles, k_blocks, sms);
+    // as many CTAs as an SM gets share its memory; a ring has two stages at least, and is as large as the sums
+    const uint32_t stage_bytes = kHalfTileBytes + p.tokens * kRowBytesK, sums = p.splits * ((p.m + p.splits - 1) / p.splits) * kFewRows * 4;
+    uint32_t each = std::min((tiles * p.splits - 1) / sms + 1, (uint32_t)kFewResident), budget = 0;
+    if ((each == 2 || (each == 1 && k_blocks < 32 * p.splits)) && 227 * 1024 / (each + 1) >= 3 * stage_bytes + 4096)
+        each++;
+    for (;; each--) {
+        budget = 227 * 1024 / each - 1024 - 1024 - (uint32_t)sizeof(FewSmem);
+        if (each == 1 || budget >= std::max(2 * stage_bytes, p.tokens * kFewRows * 4))
+            break;
+    }
+    p.stages = std::min<uint32_t>(budget / stage_bytes, kFewMaxStages);
+    p.sums_at = 0;
+    if (p.splits > 1 && p.stages > 2 && sums + 2 * stage_bytes <= budget) {
+        p.stages = std::min((budget - sums) / stage_bytes, p.stages);
+        p.sums_at = p.stages * stage_bytes;
+    }
+    p.smem_bytes = p.sums_at ? p.sums_at + sums : std::max(p.stages * stage_bytes, std::max(sums, p.tokens * kFewRows * 4));
     p.out = w.out;
     p.activation = w.activation;
     p.c = w.c[0];
@@ -248,8 +292,7 @@ static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
         rc = make_matrix_map(&maps.w[i], w.b[i].base, w.n, w.k * elem, w.b[i].ld * elem, tile_cols);
     if (rc != CLPK_OK)
         return rc;
-    return launch_clusters(linear_few_kernel<DT, FORM>, "linear_few", tiles * p.splits, kFewThreads, p.stages * stage_bytes + sizeof(FewSmem) + 1024, p.splits, s,
-                           maps, p);
+    return launch_clusters(linear_few_kernel<DT, FORM>, "linear_few", tiles * p.splits, kFewThreads, p.smem_bytes + sizeof(FewSmem) + 1024, p.splits, s, maps, p);
 }
 
 // a product whose operands are contiguous along K, with few tokens or many
@@ -257,7 +300,7 @@ template <int DT, LinearForm FORM>
 static int run_tokens(const Product &w, cudaStream_t s)
 {
     const uint32_t k_blocks = linear_k_blocks(w, DT);
-    if (w.m <= kFewTokens)
+    if (few_tokens(w.m, (w.n - 1) / few_cols<FORM> + 1, k_blocks, (uint32_t)num_sms()))
         return launch_few<DT, FORM>(w, k_blocks, s);
     return launch_linear<DT, FORM, false, false, 1>(w, plan_linear(w, FORM, k_blocks, false), k_blocks, s);
 }
