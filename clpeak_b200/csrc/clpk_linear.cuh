@@ -28,12 +28,6 @@ struct LinearSmem {
     uint64_t tmem_empty[2];
     uint32_t tmem_base;
 };
-// 8-bit integers: the scales of the columns that a warp works on, behind the rest
-struct LinearSmemScaled : LinearSmem {
-    __align__(16) float scales[kEpilogueWarps][2][kLinearChunk];
-};
-template <int DT> using LinearSmemOf = std::conditional_t<DT == CLPK_DT_I8, LinearSmemScaled, LinearSmem>;
-
 struct LinearMaps {
     CUtensorMap a[2], b[2], c[3];
 };
@@ -53,8 +47,8 @@ struct LinearParams {
     uint32_t *status;
 };
 
-// bytes of one K block in a CTA: its 128 rows of each row block of A and its half of the tile's columns of B
-__host__ __device__ constexpr uint32_t linear_block_bytes(uint32_t tn, uint32_t row_blocks) { return row_blocks * kHalfTileBytes + tn / 2 * kRowBytesK; }
+// bytes of one K block in a CTA: its 128 rows of A and its half of the tile's columns of B
+__host__ __device__ constexpr uint32_t linear_block_bytes(uint32_t tn) { return kHalfTileBytes + tn / 2 * kRowBytesK; }
 
 // an operand's part of a K block: `rows` of M or N at `row`
 template <bool kMn>
@@ -155,23 +149,16 @@ __device__ __forceinline__ void gate32_by(int act, float (&h)[32], const float (
     }
 }
 
-// the sums of a chunk in fp32; those of 8-bit integers with their scales
+// the sums of a chunk in fp32; those of 8-bit integers with their scales, of which lane i has that of column i
 template <int DT>
-__device__ __forceinline__ void scaled32(float (&v)[32], const uint32_t (&sum)[32], float row_scale, const float *col_scales)
+__device__ __forceinline__ void scaled32(float (&v)[32], const uint32_t (&sum)[32], float row_scale, float col_scale)
 {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-        if constexpr (DT == CLPK_DT_I8) {
-            const float4 s = *reinterpret_cast<const float4 *>(col_scales + i);
-            v[i] = (float)(int32_t)sum[i] * row_scale * s.x;
-            v[i + 1] = (float)(int32_t)sum[i + 1] * row_scale * s.y;
-            v[i + 2] = (float)(int32_t)sum[i + 2] * row_scale * s.z;
-            v[i + 3] = (float)(int32_t)sum[i + 3] * row_scale * s.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                v[i + j] = __uint_as_float(sum[i + j]);
-        }
+    for (int i = 0; i < 32; i++) {
+        if constexpr (DT == CLPK_DT_I8)
+            v[i] = (float)(int32_t)sum[i] * row_scale * __shfl_sync(0xffffffffu, col_scale, i);
+        else
+            v[i] = __uint_as_float(sum[i]);
     }
 }
 
@@ -184,30 +171,24 @@ __device__ __forceinline__ float bias_at(const void *bias, int type, uint32_t co
 
 // What becomes of a unit of sums: one chunk of 32 columns, or with kGated the chunk of g and that of u.
 template <int DT, LinearForm FORM>
-__device__ __forceinline__ void linear_finish(const LinearMaps &maps, const LinearParams &p, LinearSmemOf<DT> *sh, const uint32_t (&s0)[32], const uint32_t (&s1)[32],
-                                              uint32_t product, uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int ew, int lane)
+__device__ __forceinline__ void linear_finish(const LinearMaps &maps, const LinearParams &p, const uint32_t (&s0)[32], const uint32_t (&s1)[32],
+                                              uint32_t product, uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int lane)
 {
-    float row_scale = 1.0f;
-    const float *scales0 = nullptr, *scales1 = nullptr;
+    float row_scale = 1.0f, scale0 = 1.0f, scale1 = 1.0f, bias = 0.0f;
     if constexpr (DT == CLPK_DT_I8) {
-        float(*scales)[kLinearChunk] = sh->scales[ew];
-        scales0 = scales[0];
-        scales1 = scales[1];
         const uint32_t c = col + lane;
-        __syncwarp();
-        scales[0][lane] = c < p.n ? p.b_scale[c] : 0.0f;
-        if constexpr (FORM == kGated)
-            scales[1][lane] = c < p.n ? p.u_scale[c] : 0.0f;
-        else
-            scales[1][lane] = p.bias && c < p.n ? bias_at(p.bias, p.out, c) : 0.0f;
         row_scale = row + lane < p.m ? p.a_scale[row + lane] : 0.0f;
-        __syncwarp();
+        scale0 = c < p.n ? p.b_scale[c] : 0.0f;
+        if constexpr (FORM == kGated)
+            scale1 = c < p.n ? p.u_scale[c] : 0.0f;
+        else
+            bias = p.bias && c < p.n ? bias_at(p.bias, p.out, c) : 0.0f;
     }
     float v[32];
-    scaled32<DT>(v, s0, row_scale, scales0);
+    scaled32<DT>(v, s0, row_scale, scale0);
     if constexpr (FORM == kGated) {
         float u[32];
-        scaled32<DT>(u, s1, row_scale, scales1);
+        scaled32<DT>(u, s1, row_scale, scale1);
         if (p.keep) {
             linear_store(v, p, 1, boxes, n_stored, &maps.c[1], col, row, lane);
             linear_store(u, p, 2, boxes, n_stored, &maps.c[2], col, row, lane);
@@ -216,31 +197,27 @@ __device__ __forceinline__ void linear_finish(const LinearMaps &maps, const Line
     } else if constexpr (FORM == kScaled) {
         if (p.bias) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 b = *reinterpret_cast<const float4 *>(scales1 + i);
-                v[i] += b.x; v[i + 1] += b.y; v[i + 2] += b.z; v[i + 3] += b.w;
-            }
+            for (int i = 0; i < 32; i++)
+                v[i] += __shfl_sync(0xffffffffu, bias, i);
         }
     }
     const uint32_t which = FORM == kPlain ? product : 0;
     linear_store(v, p, which, boxes, n_stored, &maps.c[which], col, row, lane);
 }
 
-template <int DT, LinearForm FORM, bool kAMn, bool kBMn, uint32_t kRowBlocks>
+template <int DT, LinearForm FORM, bool kAMn, bool kBMn>
 __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_constant__ LinearMaps maps, LinearParams p)
 {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    constexpr uint32_t b_at = kRowBlocks * kHalfTileBytes;
-    const uint32_t block_bytes = linear_block_bytes(p.tn, kRowBlocks), stage_bytes = p.kps * block_bytes;
+    const uint32_t block_bytes = linear_block_bytes(p.tn), stage_bytes = p.kps * block_bytes;
     uint8_t *staging = smem + (size_t)p.stages * stage_bytes;
-    LinearSmemOf<DT> *sh = reinterpret_cast<LinearSmemOf<DT> *>(staging + kEpilogueWarps * kStagingBytes);
+    LinearSmem *sh = reinterpret_cast<LinearSmem *>(staging + kEpilogueWarps * kStagingBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), r = rank & 1, leader = rank & ~1u, split = rank >> 1;
     const uint32_t cluster_id = blockIdx.x / (2 * p.splits), n_clusters = gridDim.x / (2 * p.splits);
     const uint32_t tiles = p.tiles_m * p.tiles_n, n_tiles = p.products * tiles;
-    const bool two_accs = kRowBlocks * p.tn <= 256;
     const uint32_t kb0 = split * p.k_blocks / p.splits, kb1 = (split + 1) * p.k_blocks / p.splits;
 
     if (threadIdx.x == 0) {
@@ -284,7 +261,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             const uint32_t product = tile >= tiles ? 1 : 0;
             uint32_t mb, nb;
             dense_tile_coords(tile - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
-            const uint32_t row_a = mb * kRowBlocks * kLinearM + r * 128;
+            const uint32_t row_a = mb * kLinearM + r * 128;
             const uint32_t row_b = FORM == kGated ? nb * (p.tn / 2) : nb * p.tn + r * (p.tn / 2);
             for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
                 if (!warp_wait(&sh->empty[s], parity)) {       // a fresh barrier's preceding phase counts as complete
@@ -305,9 +282,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                             const uint32_t segment = kb + h >= p.k_segment ? 1 : 0, k = kb + h - segment * p.k_segment;
                             const CUtensorMap *a = &maps.a[product | segment], *b = &maps.b[FORM == kGated ? r : segment];
                             linear_load<kAMn>(blk, a, k, row_a, 128, full0 + 8 * s);
-                            if constexpr (kRowBlocks == 2)
-                                linear_load<kAMn>(blk + kHalfTileBytes, a, k, row_a + kLinearM, 128, full0 + 8 * s);
-                            linear_load<kBMn>(blk + b_at, b, k, row_b, p.tn / 2, full0 + 8 * s);
+                            linear_load<kBMn>(blk + kHalfTileBytes, b, k, row_b, p.tn / 2, full0 + 8 * s);
                         }
                 }
                 __syncwarp();
@@ -326,14 +301,14 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             uint32_t s = 0, parity = 0, tcount = 0;
             bool ok = true;
             for (uint32_t tile = cluster_id; tile < n_tiles && ok; tile += n_clusters, tcount++) {
-                const uint32_t acc = two_accs ? tcount & 1 : 0, use = two_accs ? tcount >> 1 : tcount;
+                const uint32_t acc = tcount & 1, use = tcount >> 1;
                 if (use > 0 && !warp_wait(&sh->tmem_empty[acc], (use - 1) & 1)) {
                     if (lane == 0)
                         atomicCAS(p.status, 0u, 0x302u);
                     break;
                 }
                 tc_fence_after_sync();
-                const uint32_t d = tmem + acc * kRowBlocks * p.tn;
+                const uint32_t d = tmem + acc * p.tn;
                 for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
                     if (!warp_wait(&sh->full[s], parity)) {
                         if (lane == 0)
@@ -355,19 +330,16 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                             if (h >= nk)
                                 break;
                             const uint32_t blk = base + h * block_bytes;
-                            const uint64_t bd = linear_desc<kBMn>(blk + b_at);
+                            const uint64_t bd = linear_desc<kBMn>(blk + kHalfTileBytes);
+const uint64_t ad = linear_desc<kAMn>(blk);
 #pragma unroll
-                            for (uint32_t rb = 0; rb < kRowBlocks; rb++) {
-                                const uint64_t ad = linear_desc<kAMn>(blk + rb * kHalfTileBytes);
-#pragma unroll
-                                for (uint32_t kk = 0; kk < 4; kk++) {
-                                    const uint32_t accumulate = (kb != kb0 || h != 0 || kk != 0) ? 1u : 0u;
-                                    const uint64_t ak = ad + kk * linear_step<kAMn>, bk = bd + kk * linear_step<kBMn>;
-                                    if constexpr (DT == CLPK_DT_I8)
-                                        mma2_i8_ss(d + rb * p.tn, ak, bk, idesc, accumulate);
-                                    else
-                                        mma2_f16_ss(d + rb * p.tn, ak, bk, idesc, accumulate);
-                                }
+                            for (uint32_t kk = 0; kk < 4; kk++) {
+                                const uint32_t accumulate = (kb != kb0 || h != 0 || kk != 0) ? 1u : 0u;
+                                const uint64_t ak = ad + kk * linear_step<kAMn>, bk = bd + kk * linear_step<kBMn>;
+                                if constexpr (DT == CLPK_DT_I8)
+                                    mma2_i8_ss(d, ak, bk, idesc, accumulate);
+                                else
+                                    mma2_f16_ss(d, ak, bk, idesc, accumulate);
                             }
                         }
                         tc_commit_pair(&sh->empty[s_now], pair_mask);
@@ -386,33 +358,32 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             const uint32_t product = tile >= tiles ? 1 : 0;
             uint32_t mb, nb;
             dense_tile_coords(tile - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
-            const uint32_t acc = two_accs ? tcount & 1 : 0, use = two_accs ? tcount >> 1 : tcount;
+            const uint32_t acc = tcount & 1, use = tcount >> 1;
             if (!warp_wait(&sh->tmem_full[acc], use & 1)) {
                 if (lane == 0)
                     atomicCAS(p.status, 0u, 0x304u);
                 break;
             }
             tc_fence_after_sync();
-            const uint32_t taddr = tmem + acc * kRowBlocks * p.tn + ((q * 32) << 16);
-            const uint32_t row = mb * kRowBlocks * kLinearM + r * 128 + q * 32;
+            const uint32_t taddr = tmem + acc * p.tn + ((q * 32) << 16);
+            const uint32_t row = mb * kLinearM + r * 128 + q * 32;
             auto release = [&]() {
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], leader);
             };
-            if (half >= kRowBlocks * units)
+            if (half >= units)
                 release();
-            for (uint32_t c = half; c < kRowBlocks * units; c += 2) {
-                const uint32_t rb = c / units, unit = c - rb * units;
+            for (uint32_t c = half; c < units; c += 2) {
                 uint32_t s0[32], s1[32];
-                tmem_ld_32x32b_x32(taddr + rb * p.tn + unit * kLinearChunk, s0);
+                tmem_ld_32x32b_x32(taddr + c * kLinearChunk, s0);
                 if constexpr (kSubs == 2)
-                    tmem_ld_32x32b_x32(taddr + rb * p.tn + p.tn / 2 + unit * kLinearChunk, s1);
+                    tmem_ld_32x32b_x32(taddr + p.tn / 2 + c * kLinearChunk, s1);
                 tmem_ld_wait();
-                if (c + 2 >= kRowBlocks * units)
+                if (c + 2 >= units)
                     release();
-                linear_finish<DT, FORM>(maps, p, sh, s0, s1, product, row + rb * kLinearM, nb * unit_cols + unit * kLinearChunk, boxes, n_stored, warp - 2, lane);
+                linear_finish<DT, FORM>(maps, p, s0, s1, product, row, nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
             }
         }
     } else if (!warp_wait(&sh->tmem_full[0], 0)) {
@@ -421,7 +392,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
     }
 
     if (p.splits > 1) {
-        // ---------------- K split over the cluster's pairs (one tile per cluster, one row block) ----------------
+        // ---------------- K split over the cluster's pairs (one tile per cluster) ----------------
         // Every pair's instructions have retired, so the stages of the ring are free to take partial sums: slot (src, j) of CTA
         // (owner, r) holds pair src's sums of the owner's j-th unit, src counted without the owner.  They are added in the order
         // of the pairs, whoever owns the unit.
@@ -484,7 +455,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                         }
                     }
                 }
-                linear_finish<DT, FORM>(maps, p, sh, sum[0], sum[kSubs - 1], product, row, nb * unit_cols + c * kLinearChunk, boxes, n_stored, warp - 2, lane);
+                linear_finish<DT, FORM>(maps, p, sum[0], sum[kSubs - 1], product, row, nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
             }
         }
     }

@@ -117,7 +117,7 @@ struct Product {
 };
 
 struct LinearPlan {
-    uint32_t tn, splits, row_blocks;
+    uint32_t tn, splits;
 };
 
 static uint64_t elem_bytes(int dtype) { return dtype == CLPK_DT_F32 ? 4 : dtype == CLPK_DT_I8 ? 1 : 2; }
@@ -128,7 +128,7 @@ static uint32_t linear_k_blocks(const Product &w, int dtype) { return (uint32_t)
 static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks, bool b_mn)
 {
     const uint32_t pairs = (uint32_t)num_sms() / 2, cols = form == kGated ? 2 * w.n : w.n;
-    LinearPlan plan = {256, 1, 1};
+    LinearPlan plan = {256, 1};
     float best = 1e30f;
     for (uint32_t splits = 1; splits <= 4 && splits <= k_blocks; splits *= 2)
         for (uint32_t tn = b_mn ? 128 : 64; tn <= 256; tn += b_mn ? 128 : 64) {
@@ -142,13 +142,13 @@ static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_bloc
                 t += waves * (1.0f + 4.3f * wide);
             if (t < best) {
                 best = t;
-                plan = {tn, splits, 1};
+                plan = {tn, splits};
             }
         }
     return plan;
 }
 
-template <int DT, LinearForm FORM, bool kAMn, bool kBMn, uint32_t kRowBlocks>
+template <int DT, LinearForm FORM, bool kAMn, bool kBMn>
 static int launch_linear(const Product &w, LinearPlan plan, uint32_t k_blocks, cudaStream_t s)
 {
     const uint64_t elem = elem_bytes(DT);
@@ -178,7 +178,7 @@ static int launch_linear(const Product &w, LinearPlan plan, uint32_t k_blocks, c
     p.m = w.m;
     p.n = w.n;
     p.products = (uint32_t)w.products;
-    p.tiles_m = (w.m - 1) / (kLinearM * kRowBlocks) + 1;
+    p.tiles_m = (w.m - 1) / kLinearM + 1;
     const uint32_t tile_cols = FORM == kGated ? plan.tn / 2 : plan.tn;
     p.tiles_n = (w.n - 1) / tile_cols + 1;
     p.group = 8;
@@ -199,14 +199,14 @@ static int launch_linear(const Product &w, LinearPlan plan, uint32_t k_blocks, c
     p.status = w.status;
     const uint32_t n_tiles = p.products * p.tiles_m * p.tiles_n, pairs = (uint32_t)num_sms() / 2;
     const uint32_t clusters = plan.splits > 1 ? n_tiles : std::min(n_tiles, pairs);
-    constexpr size_t fixed = kEpilogueWarps * kStagingBytes + sizeof(LinearSmemOf<DT>) + 1024;
-    p.kps = plan.tn <= 128 && kRowBlocks == 1 ? 2 : 1;
-    const uint32_t stage_bytes = p.kps * linear_block_bytes(plan.tn, kRowBlocks);
+    constexpr size_t fixed = kEpilogueWarps * kStagingBytes + sizeof(LinearSmem) + 1024;
+    p.kps = plan.tn <= 128 ? 2 : 1;
+    const uint32_t stage_bytes = p.kps * linear_block_bytes(plan.tn);
     p.stages = std::min<uint32_t>((uint32_t)((kSmemMax - fixed) / stage_bytes), kLinearMaxStages);
     p.tmem_cols = 32;
-    while (p.tmem_cols < (n_tiles > clusters && kRowBlocks * plan.tn <= 256 ? 2 : 1) * kRowBlocks * plan.tn)
+    while (p.tmem_cols < (n_tiles > clusters ? 2 : 1) * plan.tn)
         p.tmem_cols *= 2;
-    return launch_clusters(linear_kernel<DT, FORM, kAMn, kBMn, kRowBlocks>, "linear", clusters * 2 * plan.splits, kLinearThreads,
+    return launch_clusters(linear_kernel<DT, FORM, kAMn, kBMn>, "linear", clusters * 2 * plan.splits, kLinearThreads,
                            p.stages * stage_bytes + fixed, 2 * plan.splits, s, maps, p);
 }
 
@@ -302,7 +302,7 @@ static int run_tokens(const Product &w, cudaStream_t s)
     const uint32_t k_blocks = linear_k_blocks(w, DT);
     if (few_tokens(w.m, (w.n - 1) / few_cols<FORM> + 1, k_blocks, (uint32_t)num_sms()))
         return launch_few<DT, FORM>(w, k_blocks, s);
-    return launch_linear<DT, FORM, false, false, 1>(w, plan_linear(w, FORM, k_blocks, false), k_blocks, s);
+    return launch_linear<DT, FORM, false, false>(w, plan_linear(w, FORM, k_blocks, false), k_blocks, s);
 }
 
 // a product of the backward pass: B contiguous along N, A along K or M
@@ -310,7 +310,7 @@ template <int DT, bool kAMn>
 static int run_gradient(const Product &w, cudaStream_t s)
 {
     const uint32_t k_blocks = linear_k_blocks(w, DT);
-    return launch_linear<DT, kPlain, kAMn, true, 1>(w, plan_linear(w, kPlain, k_blocks * (uint32_t)w.segments, true), k_blocks, s);
+    return launch_linear<DT, kPlain, kAMn, true>(w, plan_linear(w, kPlain, k_blocks * (uint32_t)w.segments, true), k_blocks, s);
 }
 
 // ---- what the calls ask of their arguments ------------------------------------------------------------

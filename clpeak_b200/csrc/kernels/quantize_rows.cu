@@ -2,7 +2,7 @@
 //
 //   scale = max |x| / 127,   q = rint(x * (1 / scale))
 //
-// Every element is read once: a row stays in the registers of the 32, 256 or 1024 threads that share it, as the vectors it was
+// Every element is read once: a row stays in the registers of the 32 or 256 threads that share it, as the vectors it was
 // loaded in, while they find its largest element.  That is a maximum over the bits of |x|, which order like the values and put
 // infinities and NaNs above them, so that one comparison tells a row that has any.  A rounded quotient is the low byte of
 // x * r + 1.5 * 2^23: one multiplication, one addition and three quarters of a byte permutation per element.
@@ -188,6 +188,8 @@ __global__ void __launch_bounds__(256) quantize_rows_plain_kernel(RowParams p)
         q[at] = none ? (int8_t)0 : (int8_t)quotient(E::get(word(at), 0), r);
 }
 
+constexpr uint64_t kMostVectors = 16;                // that a thread holds
+
 template <int DT, int THREADS>
 static int launch_rows(const RowParams &p, uint64_t vectors, cudaStream_t s)
 {
@@ -200,7 +202,11 @@ static int launch_rows(const RowParams &p, uint64_t vectors, cudaStream_t s)
         return launch_behind(quantize_rows_kernel<DT, THREADS, 2>, "quantize_rows", grid, threads, 0, s, p);
     if (each <= 4)
         return launch_behind(quantize_rows_kernel<DT, THREADS, 4>, "quantize_rows", grid, threads, 0, s, p);
-    return launch_behind(quantize_rows_kernel<DT, THREADS, 8>, "quantize_rows", grid, threads, 0, s, p);
+    if (each <= 8)
+        return launch_behind(quantize_rows_kernel<DT, THREADS, 8>, "quantize_rows", grid, threads, 0, s, p);
+    if (each <= 12)
+        return launch_behind(quantize_rows_kernel<DT, THREADS, 12>, "quantize_rows", grid, threads, 0, s, p);
+    return launch_behind(quantize_rows_kernel<DT, THREADS, 16>, "quantize_rows", grid, threads, 0, s, p);
 }
 
 template <int DT>
@@ -209,11 +215,9 @@ static int quantize_rows(const RowParams &p, cudaStream_t s)
     constexpr uint64_t elem = sizeof(typename RowElem<DT>::T), per_vector = 16 / elem;
     const uint64_t vectors = (p.cols + per_vector - 1) / per_vector;
     const bool aligned = (uintptr_t)p.src % 16 == 0 && p.ld_src % per_vector == 0 && (uintptr_t)p.q % per_vector == 0 && p.ld_q % per_vector == 0;
-    if (!aligned || vectors > 8 * 1024)
+    if (!aligned || vectors > kMostVectors * 256)
         return launch_behind(quantize_rows_plain_kernel<DT>, "quantize_rows_plain", (unsigned)p.rows, 256, 0, s, p);
-    if (vectors <= 4 * 32)
-        return launch_rows<DT, 32>(p, vectors, s);
-    return vectors <= 8 * 256 ? launch_rows<DT, 256>(p, vectors, s) : launch_rows<DT, 1024>(p, vectors, s);
+    return vectors <= 4 * 32 ? launch_rows<DT, 32>(p, vectors, s) : launch_rows<DT, 256>(p, vectors, s);
 }
 
 } // namespace clpk
