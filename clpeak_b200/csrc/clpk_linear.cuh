@@ -1,19 +1,16 @@
 // Products of a feed-forward layer with many tokens, on CTA pairs (included by feed_forward.cu).
 //
 // Same pieces as gemm_tiles_kernel -- TMA ring, M = 256 instructions of a pair, two accumulators, K over the pairs of a cluster
-// -- with three things that clpk_gemm does not have:
+// -- in three forms that clpk_gemm does not have:
 //
-//  * Two products that share A in one pass (kGated).  In a pair's instruction each CTA brings half of the tile's columns of B, so
+//  * kScaled: sums of 8-bit integers with scales for each token and channel and a bias in the epilogue.
+//  * kGated: two products that share A in one pass.  In a pair's instruction each CTA brings half of the tile's columns of B, so
 //    the leader loads Wg's rows and its peer Wu's: columns [0, tn / 2) of the accumulator are g and [tn / 2, tn) are u of the same
 //    features, a thread of the epilogue holds both, and h = act(g) * u leaves without g or u having been anywhere.
-//  * Operands that are contiguous along M or N instead of K (kAMn, kBMn): what the gradients need, dx = dg Wg with Wg as it lies
-//    and dW = dg^T x with neither transposed.  A stage is then boxes of 64 elements along M or N times 64 of K, in the same
-//    128-byte swizzle; the descriptors' leading offset is the distance between two boxes, their stride that of eight rows of K.
-//  * A sum over two pairs of operands (dx = dg Wg + du Wu) as one K range, and two products of the same shape (dWg and dWu) as
-//    one set of tiles.
+//  * kGradients: the products of the backward pass (clpk_linear_grad.cuh).
 #pragma once
 
-enum LinearForm { kPlain = 0, kGated = 1, kScaled = 2 };
+enum LinearForm { kGated = 0, kScaled = 1, kGradients = 2 };
 
 constexpr int kLinearMaxStages = 12;
 constexpr uint32_t kLinearM = 256;
@@ -28,20 +25,23 @@ struct LinearSmem {
     uint64_t tmem_empty[2];
     uint32_t tmem_base;
 };
-struct LinearMaps {
-    CUtensorMap a[2], b[2], c[3];
+
+// a result: h, g, u or c; dx, dWg, dWu
+struct LinearResult {
+    void *base;
+    uint64_t ld;
+    uint32_t m, n;
+    uint32_t ragged;                                // its rows end inside 16 bytes
+    int type;                                       // CLPK_DT_*
 };
 
 struct LinearParams {
-    uint32_t m, n;
-    uint32_t tiles_m, tiles_n, group, products;     // products: sets of tiles, 1 or 2
-    uint32_t k_blocks, k_segment;                   // K blocks of a tile; those of its first pair of operands
-    uint32_t tn, splits, stages, kps, tmem_cols;
-    int out, activation;                            // CLPK_DT_* of c, CLPK_ACT_*
+    uint32_t tiles_m, tiles_n, group;
+    uint32_t k_blocks;                              // of 128 bytes
+    uint32_t tn, splits, stages, kps, tmem_cols;    // kps: K blocks per stage
+    int activation;                                 // CLPK_ACT_*
     uint32_t keep;                                  // kGated: g and u are stored too
-    uint32_t ragged;                                // rows of c end inside 16 bytes
-    void *c[3];
-    uint64_t ldc;
+    LinearResult c[3];
     const float *a_scale, *b_scale, *u_scale;
     const void *bias;
     uint32_t *status;
@@ -49,22 +49,6 @@ struct LinearParams {
 
 // bytes of one K block in a CTA: its 128 rows of A and its half of the tile's columns of B
 __host__ __device__ constexpr uint32_t linear_block_bytes(uint32_t tn) { return kHalfTileBytes + tn / 2 * kRowBytesK; }
-
-// an operand's part of a K block: `rows` of M or N at `row`
-template <bool kMn>
-__device__ __forceinline__ void linear_load(uint8_t *dst, const CUtensorMap *map, uint32_t kb, uint32_t row, uint32_t rows, uint32_t bar)
-{
-    if constexpr (kMn) {
-        for (uint32_t i = 0; i < rows; i += 64)
-            tma_load_pair_at(dst + i * kRowBytesK, map, (int32_t)((row + i) * 2), (int32_t)(kb * kLinearK), bar);
-    } else {
-        tma_load_pair_at(dst, map, (int32_t)(kb * kRowBytesK), (int32_t)row, bar);
-    }
-}
-
-template <bool kMn> __device__ __forceinline__ uint64_t linear_desc(uint32_t addr) { return make_smem_desc(addr, kMn ? 64 * kRowBytesK : 16, 1024, kSwizzle128B); }
-// from one instruction's K to the next, in the descriptor's 16-byte units: 32 bytes of a row, or 16 rows
-template <bool kMn> constexpr uint32_t linear_step = kMn ? 16 * kRowBytesK / 16 : 2;
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, int type)
 {
@@ -79,10 +63,10 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type)
 // 32 columns of one row per lane -> the warp's staging box (rows of 64 or 128 bytes in the swizzle of that width) -> one TMA
 // store, which clips what lies beyond C -- in units of 16 bytes: where a row of C ends inside one, the box that holds its end is
 // written element by element, so that what lies behind the row stays as it is.
-__device__ __forceinline__ void linear_store(const float (&v)[32], const LinearParams &p, uint32_t which, uint8_t *boxes, uint32_t &n_stored,
-                                             const CUtensorMap *map, uint32_t col, uint32_t row, int lane)
+__device__ __forceinline__ void linear_store(const float (&v)[32], const LinearResult &c, uint8_t *boxes, uint32_t &n_stored, const CUtensorMap *map, uint32_t col,
+                                             uint32_t row, int lane)
 {
-    const bool wide = p.out == CLPK_DT_F32;
+    const bool wide = c.type == CLPK_DT_F32;
     // 16 bits: two 2 KiB boxes in turn: the one filled now was handed to TMA two stores ago
     uint8_t *box = wide ? boxes : boxes + (n_stored & 1) * 2048;
     if (lane == 0) {
@@ -101,19 +85,19 @@ __device__ __forceinline__ void linear_store(const float (&v)[32], const LinearP
         for (uint32_t j = 0; j < 4; j++) {
             const float *x = v + 8 * j;
             *reinterpret_cast<uint4 *>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(pack16(x[0], x[1], p.out), pack16(x[2], x[3], p.out), pack16(x[4], x[5], p.out), pack16(x[6], x[7], p.out));
+                make_uint4(pack16(x[0], x[1], c.type), pack16(x[2], x[3], c.type), pack16(x[4], x[5], c.type), pack16(x[6], x[7], c.type));
         }
     }
-    if (p.ragged && col < p.n && p.n - col < kLinearChunk) {
+    if (c.ragged && col < c.n && c.n - col < kLinearChunk) {
         __syncwarp();
-        const uint32_t left = p.n - col, j = lane * (wide ? 4 : 2), piece = j >> 4, in_piece = j & 15;
-        for (uint32_t i = 0; i < 32 && row + i < p.m; i++) {
-            const uint64_t at = (uint64_t)(row + i) * p.ldc + col + lane;
+        const uint32_t left = c.n - col, j = lane * (wide ? 4 : 2), piece = j >> 4, in_piece = j & 15;
+        for (uint32_t i = 0; i < 32 && row + i < c.m; i++) {
+            const uint64_t at = (uint64_t)(row + i) * c.ld + col + lane;
             if (lane < left) {
                 if (wide)
-                    static_cast<float *>(p.c[which])[at] = *reinterpret_cast<const float *>(box + i * 128 + ((piece ^ (i & 7)) << 4) + in_piece);
+                    static_cast<float *>(c.base)[at] = *reinterpret_cast<const float *>(box + i * 128 + ((piece ^ (i & 7)) << 4) + in_piece);
                 else
-                    static_cast<uint16_t *>(p.c[which])[at] = *reinterpret_cast<const uint16_t *>(box + i * 64 + ((piece ^ ((i >> 1) & 3)) << 4) + in_piece);
+                    static_cast<uint16_t *>(c.base)[at] = *reinterpret_cast<const uint16_t *>(box + i * 64 + ((piece ^ ((i >> 1) & 3)) << 4) + in_piece);
             }
         }
         __syncwarp();
@@ -169,20 +153,21 @@ __device__ __forceinline__ float bias_at(const void *bias, int type, uint32_t co
     return type == CLPK_DT_F16 ? __half2float(static_cast<const __half *>(bias)[col]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(bias)[col]);
 }
 
-// What becomes of a unit of sums: one chunk of 32 columns, or with kGated the chunk of g and that of u.
+// What becomes of a unit of sums: one chunk of 32 columns, or with kGated the chunk of g and that of u.  `which`: the result
+// that plain sums (kGradients) belong to.
 template <int DT, LinearForm FORM>
-__device__ __forceinline__ void linear_finish(const LinearMaps &maps, const LinearParams &p, const uint32_t (&s0)[32], const uint32_t (&s1)[32],
-                                              uint32_t product, uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int lane)
+__device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const LinearParams &p, const uint32_t (&s0)[32], const uint32_t (&s1)[32], uint32_t which,
+                                              uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int lane)
 {
     float row_scale = 1.0f, scale0 = 1.0f, scale1 = 1.0f, bias = 0.0f;
     if constexpr (DT == CLPK_DT_I8) {
         const uint32_t c = col + lane;
-        row_scale = row + lane < p.m ? p.a_scale[row + lane] : 0.0f;
-        scale0 = c < p.n ? p.b_scale[c] : 0.0f;
+        row_scale = row + lane < p.c[0].m ? p.a_scale[row + lane] : 0.0f;
+        scale0 = c < p.c[0].n ? p.b_scale[c] : 0.0f;
         if constexpr (FORM == kGated)
-            scale1 = c < p.n ? p.u_scale[c] : 0.0f;
+            scale1 = c < p.c[0].n ? p.u_scale[c] : 0.0f;
         else
-            bias = p.bias && c < p.n ? bias_at(p.bias, p.out, c) : 0.0f;
+            bias = p.bias && c < p.c[0].n ? bias_at(p.bias, p.c[0].type, c) : 0.0f;
     }
     float v[32];
     scaled32<DT>(v, s0, row_scale, scale0);
@@ -190,8 +175,8 @@ __device__ __forceinline__ void linear_finish(const LinearMaps &maps, const Line
         float u[32];
         scaled32<DT>(u, s1, row_scale, scale1);
         if (p.keep) {
-            linear_store(v, p, 1, boxes, n_stored, &maps.c[1], col, row, lane);
-            linear_store(u, p, 2, boxes, n_stored, &maps.c[2], col, row, lane);
+            linear_store(v, p.c[1], boxes, n_stored, maps + 1, col, row, lane);
+            linear_store(u, p.c[2], boxes, n_stored, maps + 2, col, row, lane);
         }
         gate32_by(p.activation, v, u);
     } else if constexpr (FORM == kScaled) {
@@ -201,12 +186,41 @@ __device__ __forceinline__ void linear_finish(const LinearMaps &maps, const Line
                 v[i] += __shfl_sync(0xffffffffu, bias, i);
         }
     }
-    const uint32_t which = FORM == kPlain ? product : 0;
-    linear_store(v, p, which, boxes, n_stored, &maps.c[which], col, row, lane);
+    linear_store(v, p.c[which], boxes, n_stored, maps + which, col, row, lane);
 }
 
-template <int DT, LinearForm FORM, bool kAMn, bool kBMn>
-__global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_constant__ LinearMaps maps, LinearParams p)
+#include "clpk_linear_grad.cuh"
+
+struct LinearMaps {
+    CUtensorMap a, b[2], c[3];
+};
+template <LinearForm FORM> using LinearMapsOf = std::conditional_t<FORM == kGradients, GradMaps, LinearMaps>;
+template <LinearForm FORM> using LinearParamsOf = std::conditional_t<FORM == kGradients, GradParams, LinearParams>;
+
+// a tile: which result, where in it, and over how many K blocks
+struct LinearTile {
+    uint32_t which, mb, nb, k_blocks;
+};
+
+// the i-th tile of a cluster; false: it has no more
+template <LinearForm FORM>
+__device__ __forceinline__ bool linear_tile(const LinearParamsOf<FORM> &p, uint32_t cluster, uint32_t clusters, uint32_t i, LinearTile &t)
+{
+    if constexpr (FORM == kGradients) {
+        return grad_tile(p, cluster, clusters, i, t.which, t.mb, t.nb, t.k_blocks);
+    } else {
+        const uint32_t tile = cluster + i * clusters;
+        t.which = 0;
+        t.k_blocks = p.k_blocks;
+        if (tile >= p.tiles_m * p.tiles_n)
+            return false;
+        dense_tile_coords(tile, p.tiles_m, p.tiles_n, p.group, t.mb, t.nb);
+        return true;
+    }
+}
+
+template <int DT, LinearForm FORM>
+__global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_constant__ LinearMapsOf<FORM> maps, const __grid_constant__ LinearParamsOf<FORM> p)
 {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -216,9 +230,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), r = rank & 1, leader = rank & ~1u, split = rank >> 1;
-    const uint32_t cluster_id = blockIdx.x / (2 * p.splits), n_clusters = gridDim.x / (2 * p.splits);
-    const uint32_t tiles = p.tiles_m * p.tiles_n, n_tiles = p.products * tiles;
-    const uint32_t kb0 = split * p.k_blocks / p.splits, kb1 = (split + 1) * p.k_blocks / p.splits;
+    const uint32_t cluster = blockIdx.x / (2 * p.splits), clusters = gridDim.x / (2 * p.splits);
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < p.stages; s++) {
@@ -230,9 +242,11 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             mbar_init(&sh->tmem_empty[acc], 2 * kEpilogueWarps);
         }
         mbar_fence_init();
-        tma_prefetch_desc(&maps.a[0]);
-        tma_prefetch_desc(&maps.b[FORM == kGated ? r : 0]);
-        tma_prefetch_desc(&maps.c[0]);
+        if constexpr (FORM != kGradients) {
+            tma_prefetch_desc(&maps.a);
+            tma_prefetch_desc(&maps.b[FORM == kGated ? r : 0]);
+            tma_prefetch_desc(&maps.c[0]);
+        }
     }
     if (warp == 1)
         tmem_alloc<2>(&sh->tmem_base, p.tmem_cols);
@@ -247,23 +261,23 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
     griddep_launch_dependents();
 
     const uint32_t q = (uint32_t)(warp & 3), half = (uint32_t)(warp - 2) >> 2;     // epilogue warps
-    const uint32_t units = (FORM == kGated ? p.tn / 2 : p.tn) / kLinearChunk, unit_cols = FORM == kGated ? p.tn / 2 : p.tn;
+    const uint32_t unit_cols = FORM == kGated ? p.tn / 2 : p.tn, units = unit_cols / kLinearChunk;
     constexpr uint32_t kSubs = FORM == kGated ? 2 : 1;                             // chunks per unit, tn / 2 columns apart
     uint8_t *boxes = staging + (size_t)(warp - 2) * kStagingBytes;
     uint32_t n_stored = 0;
+    LinearTile t;
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         const uint32_t full0 = cluster_addr(&sh->full[0], leader);
         uint32_t s = 0, parity = 1;                            // parity of the empty barrier's previous phase
         bool ok = true;
-        for (uint32_t tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
-            const uint32_t product = tile >= tiles ? 1 : 0;
-            uint32_t mb, nb;
-            dense_tile_coords(tile - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
-            const uint32_t row_a = mb * kLinearM + r * 128;
-            const uint32_t row_b = FORM == kGated ? nb * (p.tn / 2) : nb * p.tn + r * (p.tn / 2);
+        for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
+            const uint32_t row_a = t.mb * kLinearM + r * 128;
+            const uint32_t row_b = FORM == kGated ? t.nb * (p.tn / 2) : t.nb * p.tn + r * (p.tn / 2);
+            const uint32_t kb0 = split * t.k_blocks / p.splits, kb1 = (split + 1) * t.k_blocks / p.splits;
             for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
+                const uint32_t nk = kb1 - kb < p.kps ? kb1 - kb : p.kps;
                 if (!warp_wait(&sh->empty[s], parity)) {       // a fresh barrier's preceding phase counts as complete
                     if (lane == 0)
                         atomicCAS(p.status, 0u, 0x301u);
@@ -271,7 +285,6 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                     break;
                 }
                 uint8_t *st = smem + (size_t)s * stage_bytes;
-                const uint32_t nk = kb1 - kb < p.kps ? kb1 - kb : p.kps;
                 if (elect_one()) {
                     if (r == 0)
                         mbar_expect_tx(&sh->full[s], nk * 2 * block_bytes);
@@ -279,10 +292,12 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                     for (uint32_t h = 0; h < 2; h++)
                         if (h < nk) {
                             uint8_t *blk = st + h * block_bytes;
-                            const uint32_t segment = kb + h >= p.k_segment ? 1 : 0, k = kb + h - segment * p.k_segment;
-                            const CUtensorMap *a = &maps.a[product | segment], *b = &maps.b[FORM == kGated ? r : segment];
-                            linear_load<kAMn>(blk, a, k, row_a, 128, full0 + 8 * s);
-                            linear_load<kBMn>(blk + kHalfTileBytes, b, k, row_b, p.tn / 2, full0 + 8 * s);
+                            if constexpr (FORM == kGradients) {
+                                grad_load(maps, p, t.which, blk, kb + h, row_a, row_b, full0 + 8 * s);
+                            } else {
+                                tma_load_pair_at(blk, &maps.a, (int32_t)((kb + h) * kRowBytesK), (int32_t)row_a, full0 + 8 * s);
+                                tma_load_pair_at(blk + kHalfTileBytes, &maps.b[FORM == kGated ? r : 0], (int32_t)((kb + h) * kRowBytesK), (int32_t)row_b, full0 + 8 * s);
+                            }
                         }
                 }
                 __syncwarp();
@@ -296,12 +311,12 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         // ---------------- MMA issuer (the pair's leader) ----------------
         if (r == 0) {
             constexpr uint32_t kFmt = DT == CLPK_DT_BF16 ? kFmtBF16 : DT == CLPK_DT_F16 ? kFmtF16 : kFmtS8;
-            const uint32_t idesc = make_idesc(256, p.tn, kFmt, kFmt, DT == CLPK_DT_I8 ? kAccS32 : kAccF32) | (kAMn ? kMajorA : 0u) | (kBMn ? kMajorB : 0u);
             const uint16_t pair_mask = (uint16_t)(3u << leader);
-            uint32_t s = 0, parity = 0, tcount = 0;
+            uint32_t s = 0, parity = 0;
             bool ok = true;
-            for (uint32_t tile = cluster_id; tile < n_tiles && ok; tile += n_clusters, tcount++) {
-                const uint32_t acc = tcount & 1, use = tcount >> 1;
+            for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
+                const uint32_t acc = i & 1, use = i >> 1;
+                const uint32_t kb0 = split * t.k_blocks / p.splits, kb1 = (split + 1) * t.k_blocks / p.splits;
                 if (use > 0 && !warp_wait(&sh->tmem_empty[acc], (use - 1) & 1)) {
                     if (lane == 0)
                         atomicCAS(p.status, 0u, 0x302u);
@@ -309,6 +324,11 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                 }
                 tc_fence_after_sync();
                 const uint32_t d = tmem + acc * p.tn;
+                const bool a_mn = FORM == kGradients && t.which > 0;       // A contiguous along M
+                const uint32_t idesc = make_idesc(256, p.tn, kFmt, kFmt, DT == CLPK_DT_I8 ? kAccS32 : kAccF32) | (a_mn ? kMajorA : 0u) |
+                                       (FORM == kGradients ? kMajorB : 0u);
+                const uint32_t a_lbo = a_mn ? kMnLead : 16, a_step = a_mn ? kMnStep : 2;
+                constexpr uint32_t kBLbo = FORM == kGradients ? kMnLead : 16, kBStep = FORM == kGradients ? kMnStep : 2;
                 for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
                     if (!warp_wait(&sh->full[s], parity)) {
                         if (lane == 0)
@@ -330,16 +350,14 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                             if (h >= nk)
                                 break;
                             const uint32_t blk = base + h * block_bytes;
-                            const uint64_t bd = linear_desc<kBMn>(blk + kHalfTileBytes);
-const uint64_t ad = linear_desc<kAMn>(blk);
+                            const uint64_t ad = make_smem_desc(blk, a_lbo, 1024, kSwizzle128B), bd = make_smem_desc(blk + kHalfTileBytes, kBLbo, 1024, kSwizzle128B);
 #pragma unroll
                             for (uint32_t kk = 0; kk < 4; kk++) {
                                 const uint32_t accumulate = (kb != kb0 || h != 0 || kk != 0) ? 1u : 0u;
-                                const uint64_t ak = ad + kk * linear_step<kAMn>, bk = bd + kk * linear_step<kBMn>;
                                 if constexpr (DT == CLPK_DT_I8)
-                                    mma2_i8_ss(d, ak, bk, idesc, accumulate);
+                                    mma2_i8_ss(d, ad + kk * a_step, bd + kk * kBStep, idesc, accumulate);
                                 else
-                                    mma2_f16_ss(d, ak, bk, idesc, accumulate);
+                                    mma2_f16_ss(d, ad + kk * a_step, bd + kk * kBStep, idesc, accumulate);
                             }
                         }
                         tc_commit_pair(&sh->empty[s_now], pair_mask);
@@ -353,12 +371,8 @@ const uint64_t ad = linear_desc<kAMn>(blk);
         }
     } else if (p.splits == 1) {
         // ---------------- epilogue, K not split: the two warps of a lane quarter take every other unit ----------------
-        uint32_t tcount = 0;
-        for (uint32_t tile = cluster_id; tile < n_tiles; tile += n_clusters, tcount++) {
-            const uint32_t product = tile >= tiles ? 1 : 0;
-            uint32_t mb, nb;
-            dense_tile_coords(tile - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
-            const uint32_t acc = tcount & 1, use = tcount >> 1;
+        for (uint32_t i = 0; linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
+            const uint32_t acc = i & 1, use = i >> 1;
             if (!warp_wait(&sh->tmem_full[acc], use & 1)) {
                 if (lane == 0)
                     atomicCAS(p.status, 0u, 0x304u);
@@ -366,7 +380,7 @@ const uint64_t ad = linear_desc<kAMn>(blk);
             }
             tc_fence_after_sync();
             const uint32_t taddr = tmem + acc * p.tn + ((q * 32) << 16);
-            const uint32_t row = mb * kLinearM + r * 128 + q * 32;
+            const uint32_t row = t.mb * kLinearM + r * 128 + q * 32;
             auto release = [&]() {
                 tc_fence_before_sync();
                 __syncwarp();
@@ -383,7 +397,7 @@ const uint64_t ad = linear_desc<kAMn>(blk);
                 tmem_ld_wait();
                 if (c + 2 >= units)
                     release();
-                linear_finish<DT, FORM>(maps, p, s0, s1, product, row, nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
+                linear_finish<DT, FORM>(maps.c, p, s0, s1, t.which, row, t.nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
             }
         }
     } else if (!warp_wait(&sh->tmem_full[0], 0)) {
@@ -421,11 +435,8 @@ const uint64_t ad = linear_desc<kAMn>(blk);
         }
         __syncwarp();
         cluster_sync();
-        if (epilogue) {
-            const uint32_t product = cluster_id >= tiles ? 1 : 0;
-            uint32_t mb, nb;
-            dense_tile_coords(cluster_id - product * tiles, p.tiles_m, p.tiles_n, p.group, mb, nb);
-            const uint32_t row = mb * kLinearM + r * 128 + q * 32;
+        if (epilogue && linear_tile<FORM>(p, cluster, clusters, 0, t)) {
+            const uint32_t row = t.mb * kLinearM + r * 128 + q * 32;
             for (uint32_t j = half; split + j * p.splits < units; j += 2) {
                 const uint32_t c = split + j * p.splits;
                 uint32_t sum[2][32];
@@ -443,19 +454,19 @@ const uint64_t ad = linear_desc<kAMn>(blk);
                                 v = *reinterpret_cast<const uint4 *>(slot + g * 2048);
                             const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                            for (uint32_t t = 0; t < 4; t++) {
-                                uint32_t &x = sum[sub][4 * g + t];
+                            for (uint32_t l = 0; l < 4; l++) {
+                                uint32_t &x = sum[sub][4 * g + l];
                                 if (src == 0)
-                                    x = e[t];
+                                    x = e[l];
                                 else if constexpr (DT == CLPK_DT_I8)
-                                    x += e[t];
+                                    x += e[l];
                                 else
-                                    x = __float_as_uint(__uint_as_float(x) + __uint_as_float(e[t]));
+                                    x = __float_as_uint(__uint_as_float(x) + __uint_as_float(e[l]));
                             }
                         }
                     }
                 }
-                linear_finish<DT, FORM>(maps, p, sum[0], sum[kSubs - 1], product, row, nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
+                linear_finish<DT, FORM>(maps.c, p, sum[0], sum[kSubs - 1], t.which, row, t.nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
             }
         }
     }
@@ -491,16 +502,16 @@ static int make_matrix_map(CUtensorMap *map, const void *base, uint64_t rows, ui
 }
 
 // a result, in boxes of 32 x 32
-static int make_result_map(CUtensorMap *map, void *base, uint64_t rows, uint64_t cols, uint64_t ld, int type)
+static int make_result_map(CUtensorMap *map, const LinearResult &c)
 {
     EncodeTiledFn enc = nullptr;
     const int rc = get_encode_fn(&enc);
     if (rc != CLPK_OK)
         return rc;
-    const uint32_t elem = type == CLPK_DT_F32 ? 4 : 2;
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * elem};
+    const uint32_t elem = c.type == CLPK_DT_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {c.n, c.m}, strides[1] = {c.ld * elem};
     const cuuint32_t box[2] = {kLinearChunk, 32}, estr[2] = {1, 1};
-    const CUresult r = enc(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, estr,
+    const CUresult r = enc(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c.base, dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, elem == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {

@@ -1,0 +1,84 @@
+// The products of a gated feed-forward layer's backward pass as one launch of linear_kernel (included by clpk_linear.cuh).
+//
+//   dx = dg Wg + du Wu;   dWg = dg^T x, dWu = du^T x        (dg and du: gate_gradients_kernel)
+//
+//  * Operands that are contiguous along M or N instead of K: dx = dg Wg takes Wg as it lies ([K][N]), dW = dg^T x takes dg and x
+//    as they lie ([K][M] and [K][N]); nothing is transposed.  A stage is then boxes of 64 elements along M or N times 64 of K, in
+//    the same 128-byte swizzle; the descriptors' leading offset is the distance between two boxes, their stride that of eight rows
+//    of K.
+//  * dx is a sum over two pairs of operands, one K range of 2 f.
+//  * The tiles of dx and those of dWg and dWu are of different length.  The longer ones come first; a cluster that has one of them
+//    less gets more of the others (share_a, share_b).
+#pragma once
+
+constexpr uint32_t kMnLead = 64 * kRowBytesK;               // bytes from one box of 64 elements along M or N to the next
+constexpr uint32_t kMnStep = 16 * kRowBytesK / 16;          // 16 rows of K, in the descriptor's units of 16 bytes
+
+struct GradMaps {
+    CUtensorMap dg[2], dg_t[2];                             // dg and du: boxes of 128 tokens (dx), of 64 (dW)
+    CUtensorMap w[2], x;
+    CUtensorMap c[3];
+};
+
+// tiles of the same length: those of dx, or those of dWg and dWu
+struct GradTiles {
+    uint32_t tiles, tiles_m, blocks;                        // `blocks`: of K, of each
+    uint32_t which;                                         // the result that the first of them belong to: 0 dx, 1 dWg
+};
+
+struct GradParams : LinearParams {
+    GradTiles first, second;
+    uint32_t share_a, share_b;                              // of the second ones, for clusters below first.tiles % clusters, and for the others
+    uint32_t segment;                                       // K blocks of dx with dg
+};
+
+// the i-th tile of a cluster
+__device__ __forceinline__ bool grad_tile(const GradParams &p, uint32_t cluster, uint32_t clusters, uint32_t i, uint32_t &which, uint32_t &mb, uint32_t &nb,
+                                          uint32_t &k_blocks)
+{
+    const uint32_t have = p.first.tiles > cluster ? (p.first.tiles - cluster - 1) / clusters + 1 : 0;
+    const GradTiles &set = i < have ? p.first : p.second;
+    uint32_t tile;
+    if (i < have) {
+        tile = cluster + i * clusters;
+    } else {
+        // What clusters get that have one of the first ones less comes before what all get, so that from there on all are in step
+        // and ask for the same blocks of K together: the other way round the L2 had to fetch them again (3 % at 8192 x 2048 x 8192).
+        const uint32_t more = p.first.tiles % clusters, extra = cluster >= more ? p.share_b - p.share_a : 0, j = i - have;
+        if (j < extra)
+            tile = j * (clusters - more) + cluster - more;
+        else if (j < extra + p.share_a)
+            tile = (p.share_b - p.share_a) * (clusters - more) + (j - extra) * clusters + cluster;
+        else
+            return false;
+        if (tile >= set.tiles)
+            return false;
+    }
+    which = set.which;
+    if (which == 1 && tile >= set.tiles_m * p.tiles_n) {
+        which = 2;
+        tile -= set.tiles_m * p.tiles_n;
+    }
+    k_blocks = set.blocks;
+    dense_tile_coords(tile, set.tiles_m, p.tiles_n, p.group, mb, nb);
+    return true;
+}
+
+// a K block of a tile
+__device__ __forceinline__ void grad_load(const GradMaps &maps, const GradParams &p, uint32_t which, uint8_t *blk, uint32_t kb, uint32_t row_a, uint32_t row_b,
+                                          uint32_t bar)
+{
+    const CUtensorMap *b = &maps.x;
+    if (which == 0) {
+        const uint32_t o = kb >= p.segment ? 1 : 0;
+        kb -= o * p.segment;
+        tma_load_pair_at(blk, &maps.dg[o], (int32_t)(kb * kRowBytesK), (int32_t)row_a, bar);
+        b = &maps.w[o];
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 128; i += 64)
+            tma_load_pair_at(blk + i * kRowBytesK, &maps.dg_t[which - 1], (int32_t)((row_a + i) * 2), (int32_t)(kb * kLinearK), bar);
+    }
+    for (uint32_t i = 0; i < p.tn / 2; i += 64)
+        tma_load_pair_at(blk + kHalfTileBytes + i * kRowBytesK, b, (int32_t)((row_b + i) * 2), (int32_t)(kb * kLinearK), bar);
+}

@@ -20,82 +20,6 @@ namespace clpk {
 #include "../clpk_linear.cuh"
 #include "../clpk_linear_few.cuh"
 
-// ---- dg = dh * u * act'(g) and du = dh * act(g) -----------------------------------------------------------
-//
-// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements per step and thread.
-struct GradParams {
-    const void *dh, *g, *u;
-    void *dg, *du;
-    uint64_t ldh, ldw;                  // of the first three, and of the two in the workspace
-    uint32_t m, f;
-    uint32_t vectors;                   // of eight elements in a row
-};
-
-template <int DT>
-__device__ __forceinline__ float2 widen(uint32_t w)
-{
-    if constexpr (DT == CLPK_DT_F16)
-        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-    else
-        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-
-// eight elements of a row of `f`, zeros beyond it
-__device__ __forceinline__ uint4 load8(const void *base, uint64_t at, uint32_t left)
-{
-    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
-    if (left >= 8)
-        return *reinterpret_cast<const uint4 *>(p);
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (uint32_t i = 0; i < 8; i++)
-        if (i < left)
-            w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <int DT, int ACT>
-__global__ void __launch_bounds__(256) gate_gradients_kernel(GradParams p)
-{
-    griddep_wait();
-    griddep_launch_dependents();
-    const uint64_t all = (uint64_t)p.m * p.vectors;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t row = i / p.vectors;
-        const uint32_t col = (uint32_t)(i - row * p.vectors) * 8, left = p.f - col;
-        const uint64_t at = row * p.ldh + col;
-        const uint4 vdh = load8(p.dh, at, left), vg = load8(p.g, at, left), vu = load8(p.u, at, left);
-        const uint32_t dh[4] = {vdh.x, vdh.y, vdh.z, vdh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
-        uint32_t dg[4], du[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 h2 = widen<DT>(dh[j]), g2 = widen<DT>(g[j]), u2 = widen<DT>(u[j]);
-            float ax, dx, ay, dy;
-            activate_both<ACT>(g2.x, ax, dx);
-            activate_both<ACT>(g2.y, ay, dy);
-            dg[j] = pack16(h2.x * u2.x * dx, h2.y * u2.y * dy, DT);
-            du[j] = pack16(h2.x * ax, h2.y * ay, DT);
-        }
-        const uint64_t to = row * p.ldw + col;          // whole vectors: the workspace's pitch has room for them
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dg) + to) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.du) + to) = make_uint4(du[0], du[1], du[2], du[3]);
-    }
-}
-
-template <int DT>
-static int launch_gradients(const GradParams &p, int act, cudaStream_t s)
-{
-    const uint64_t blocks = ((uint64_t)p.m * p.vectors + 255) / 256;
-    const unsigned grid = (unsigned)std::min<uint64_t>(blocks, 1u << 30);
-    switch (act) {
-    case CLPK_ACT_SILU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SILU>, "gate_gradients", grid, 256, 0, s, p);
-    case CLPK_ACT_GELU_TANH: return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU_TANH>, "gate_gradients", grid, 256, 0, s, p);
-    case CLPK_ACT_GELU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU>, "gate_gradients", grid, 256, 0, s, p);
-    case CLPK_ACT_RELU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_RELU>, "gate_gradients", grid, 256, 0, s, p);
-    default:                 return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SIGMOID>, "gate_gradients", grid, 256, 0, s, p);
-    }
-}
-
 // ---- the products -------------------------------------------------------------------------------------------
 
 struct Matrix {
@@ -106,9 +30,8 @@ struct Matrix {
 // One product of a layer: sums over `k` of an m x n result.
 struct Product {
     uint32_t m, n, k;
-    Matrix a[2], b[2];                  // kGated: b[0] = Wg, b[1] = Wu
-    int segments, products;             // pairs of operands that are added; products of the same shape
-    void *c[3];                         // of each product; kGated: h, g, u
+    Matrix a, b[2];                     // kGated: b[0] = Wg, b[1] = Wu
+    void *c[3];                         // kGated: h, g, u
     uint64_t ldc;
     int out, activation;
     const float *a_scale, *b_scale, *u_scale;
@@ -116,30 +39,47 @@ struct Product {
     uint32_t *status;
 };
 
+static uint64_t elem_bytes(int dtype) { return dtype == CLPK_DT_F32 ? 4 : dtype == CLPK_DT_I8 ? 1 : 2; }
+
+// K blocks of 128 bytes
+static uint32_t linear_k_blocks(uint32_t k, int dtype) { return (uint32_t)(((uint64_t)k * elem_bytes(dtype) + kRowBytesK - 1) / kRowBytesK); }
+
+static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a - 1) / b + 1; }
+
 struct LinearPlan {
     uint32_t tn, splits;
 };
 
-static uint64_t elem_bytes(int dtype) { return dtype == CLPK_DT_F32 ? 4 : dtype == CLPK_DT_I8 ? 1 : 2; }
-
-// K blocks of 128 bytes (64 of 16-bit elements, whichever way they lie)
-static uint32_t linear_k_blocks(const Product &w, int dtype) { return (uint32_t)(((uint64_t)w.k * elem_bytes(dtype) + kRowBytesK - 1) / kRowBytesK); }
-
-static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks, bool b_mn)
+// Clusters of `splits` pairs that the chip holds at a time.
+static uint32_t linear_resident(uint32_t splits)
 {
-    const uint32_t pairs = (uint32_t)num_sms() / 2, cols = form == kGated ? 2 * w.n : w.n;
+    const uint32_t pairs = (uint32_t)num_sms() / 2;
+    return splits == 1 ? pairs : splits == 2 ? pairs * 33 / 74 : pairs * 15 / 74;
+}
+
+// Microseconds of linear_kernel besides its launch: `blocks` K blocks and `tiles` tiles one after another.  The terms are those of
+// gemm_tiles_kernel (plan_tiles in gemm.cu), whose main loop it is: 0.118 to issue a block, 0.265 for its instructions and its
+// loads at tn = 256, and 1.2 of epilogue; an exchange of partial sums 1 + 4.3.
+static float linear_estimate(float blocks, float tiles, uint32_t tn, uint32_t splits)
+{
+    const float wide = (float)tn / 256.0f;
+    return blocks * (0.118f + 0.265f * wide) + tiles * (1.2f * wide + (splits > 1 ? 1.0f + 4.3f * wide : 0.0f));
+}
+
+// Tile width and K ranges: the cheapest by the estimate.  It took the fastest, or one within 2 % of it, for 19 of 23 shapes that
+// were timed with every choice (256 x 4096 x 11008 int8: 18.0 us in two ranges of K with one block per stage, 19.8 as it is).
+static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks)
+{
+    const uint32_t cols = form == kGated ? 2 * w.n : w.n;
     LinearPlan plan = {256, 1};
     float best = 1e30f;
     for (uint32_t splits = 1; splits <= 4 && splits <= k_blocks; splits *= 2)
-        for (uint32_t tn = b_mn ? 128 : 64; tn <= 256; tn += b_mn ? 128 : 64) {
-            const uint32_t resident = splits == 1 ? pairs : splits == 2 ? pairs * 33 / 74 : pairs * 15 / 74;
-            const uint64_t tiles = (uint64_t)w.products * ((w.m - 1) / kLinearM + 1) * ((cols - 1) / tn + 1);
-            if (resident == 0)
+        for (uint32_t tn = 64; tn <= 256; tn += 64) {
+            const uint64_t tiles = (uint64_t)ceil_div(w.m, kLinearM) * ceil_div(cols, tn);
+            if (linear_resident(splits) == 0)
                 continue;
-            const float waves = (float)((tiles - 1) / resident + 1), wide = (float)tn / 256.0f;
-            float t = 3.9f + waves * ((float)((k_blocks - 1) / splits + 1) * (0.118f + 0.265f * wide) + 1.2f * wide);
-            if (splits > 1)
-                t += waves * (1.0f + 4.3f * wide);
+            const float waves = (float)((tiles - 1) / linear_resident(splits) + 1);
+            const float t = linear_estimate(waves * (float)ceil_div(k_blocks, splits), waves, tn, splits);
             if (t < best) {
                 best = t;
                 plan = {tn, splits};
@@ -148,66 +88,59 @@ static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_bloc
     return plan;
 }
 
-template <int DT, LinearForm FORM, bool kAMn, bool kBMn>
-static int launch_linear(const Product &w, LinearPlan plan, uint32_t k_blocks, cudaStream_t s)
+// what a launch of linear_kernel has in common
+template <int DT, LinearForm FORM, typename Maps, typename Params>
+static int launch_linear_tiles(const Maps &maps, Params &p, LinearPlan plan, uint32_t n_tiles, const char *what, cudaStream_t s)
 {
-    const uint64_t elem = elem_bytes(DT);
-    LinearMaps maps = {};
-    int rc = CLPK_OK;
-    for (int i = 0; i < 2; i++) {
-        if (w.a[i].base) {
-            rc = kAMn ? make_matrix_map(&maps.a[i], w.a[i].base, w.k, w.m * elem, w.a[i].ld * elem, 64)
-                      : make_matrix_map(&maps.a[i], w.a[i].base, w.m, w.k * elem, w.a[i].ld * elem, 128);
-            if (rc != CLPK_OK)
-                return rc;
-        }
-        if (w.b[i].base) {
-            rc = kBMn ? make_matrix_map(&maps.b[i], w.b[i].base, w.k, w.n * elem, w.b[i].ld * elem, 64)
-                      : make_matrix_map(&maps.b[i], w.b[i].base, w.n, w.k * elem, w.b[i].ld * elem, plan.tn / 2);
-            if (rc != CLPK_OK)
-                return rc;
-        }
-    }
-    for (int i = 0; i < 3; i++)
-        if (w.c[i]) {
-            rc = make_result_map(&maps.c[i], w.c[i], w.m, w.n, w.ldc, w.out);
-            if (rc != CLPK_OK)
-                return rc;
-        }
-    LinearParams p = {};
-    p.m = w.m;
-    p.n = w.n;
-    p.products = (uint32_t)w.products;
-    p.tiles_m = (w.m - 1) / kLinearM + 1;
-    const uint32_t tile_cols = FORM == kGated ? plan.tn / 2 : plan.tn;
-    p.tiles_n = (w.n - 1) / tile_cols + 1;
     p.group = 8;
-    p.k_segment = k_blocks;
-    p.k_blocks = k_blocks * (uint32_t)w.segments;
     p.tn = plan.tn;
     p.splits = plan.splits;
-    p.out = w.out;
-    p.activation = w.activation;
-    p.keep = FORM == kGated && w.c[1] ? 1 : 0;
-    p.ragged = w.n * elem_bytes(w.out) % 16 != 0;
-    std::copy(w.c, w.c + 3, p.c);
-    p.ldc = w.ldc;
-    p.a_scale = w.a_scale;
-    p.b_scale = w.b_scale;
-    p.u_scale = w.u_scale;
-    p.bias = w.bias;
-    p.status = w.status;
-    const uint32_t n_tiles = p.products * p.tiles_m * p.tiles_n, pairs = (uint32_t)num_sms() / 2;
-    const uint32_t clusters = plan.splits > 1 ? n_tiles : std::min(n_tiles, pairs);
+    const uint32_t clusters = plan.splits > 1 ? n_tiles : std::min(n_tiles, linear_resident(1));
     constexpr size_t fixed = kEpilogueWarps * kStagingBytes + sizeof(LinearSmem) + 1024;
+    // two K blocks per stage halve the hand-overs; at tn = 192 and 256 too few stages would be left
     p.kps = plan.tn <= 128 ? 2 : 1;
     const uint32_t stage_bytes = p.kps * linear_block_bytes(plan.tn);
     p.stages = std::min<uint32_t>((uint32_t)((kSmemMax - fixed) / stage_bytes), kLinearMaxStages);
     p.tmem_cols = 32;
     while (p.tmem_cols < (n_tiles > clusters ? 2 : 1) * plan.tn)
         p.tmem_cols *= 2;
-    return launch_clusters(linear_kernel<DT, FORM, kAMn, kBMn>, "linear", clusters * 2 * plan.splits, kLinearThreads,
-                           p.stages * stage_bytes + fixed, 2 * plan.splits, s, maps, p);
+    return launch_clusters(linear_kernel<DT, FORM>, what, clusters * 2 * plan.splits, kLinearThreads, p.stages * stage_bytes + fixed, 2 * plan.splits, s, maps, p);
+}
+
+static LinearResult linear_result(void *base, uint64_t ld, uint32_t m, uint32_t n, int type)
+{
+    return {base, ld, m, n, n * elem_bytes(type) % 16 != 0 ? 1u : 0u, type};
+}
+
+template <int DT, LinearForm FORM>
+static int launch_linear(const Product &w, uint32_t k_blocks, cudaStream_t s)
+{
+    const uint64_t elem = elem_bytes(DT);
+    const LinearPlan plan = plan_linear(w, FORM, k_blocks);
+    const uint32_t tile_cols = FORM == kGated ? plan.tn / 2 : plan.tn;
+    LinearMaps maps = {};
+    int rc = make_matrix_map(&maps.a, w.a.base, w.m, w.k * elem, w.a.ld * elem, 128);
+    for (int i = 0; i < (FORM == kGated ? 2 : 1) && rc == CLPK_OK; i++)
+        rc = make_matrix_map(&maps.b[i], w.b[i].base, w.n, w.k * elem, w.b[i].ld * elem, plan.tn / 2);
+    LinearParams p = {};
+    for (int i = 0; i < 3 && rc == CLPK_OK; i++)
+        if (w.c[i]) {
+            p.c[i] = linear_result(w.c[i], w.ldc, w.m, w.n, w.out);
+            rc = make_result_map(&maps.c[i], p.c[i]);
+        }
+    if (rc != CLPK_OK)
+        return rc;
+    p.tiles_m = ceil_div(w.m, kLinearM);
+    p.tiles_n = ceil_div(w.n, tile_cols);
+    p.k_blocks = k_blocks;
+    p.activation = w.activation;
+    p.keep = w.c[1] ? 1 : 0;
+    p.a_scale = w.a_scale;
+    p.b_scale = w.b_scale;
+    p.u_scale = w.u_scale;
+    p.bias = w.bias;
+    p.status = w.status;
+    return launch_linear_tiles<DT, FORM>(maps, p, plan, p.tiles_m * p.tiles_n, "linear", s);
 }
 
 template <LinearForm FORM> constexpr uint32_t few_cols = FORM == kGated ? 64 : 128;      // features of a tile
@@ -256,7 +189,7 @@ static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
     p.tmem_cols = 32;
     while (p.tmem_cols < p.tokens)
         p.tmem_cols *= 2;
-    const uint32_t tiles = (w.n - 1) / tile_cols + 1, sms = (uint32_t)num_sms();
+    const uint32_t tiles = ceil_div(w.n, tile_cols), sms = (uint32_t)num_sms();
     p.splits = few_splits(w.m, tiles, k_blocks, sms);
     // as many CTAs as an SM gets share its memory; a ring has two stages at least, and is as large as the sums
     const uint32_t stage_bytes = kHalfTileBytes + p.tokens * kRowBytesK, sums = p.splits * ((p.m + p.splits - 1) / p.splits) * kFewRows * 4;
@@ -287,7 +220,7 @@ static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
     p.bias = w.bias;
     p.status = w.status;
     FewMaps maps = {};
-    int rc = make_matrix_map(&maps.x, w.a[0].base, w.m, w.k * elem, w.a[0].ld * elem, p.tokens);
+    int rc = make_matrix_map(&maps.x, w.a.base, w.m, w.k * elem, w.a.ld * elem, p.tokens);
     for (int i = 0; i < (FORM == kGated ? 2 : 1) && rc == CLPK_OK; i++)
         rc = make_matrix_map(&maps.w[i], w.b[i].base, w.n, w.k * elem, w.b[i].ld * elem, tile_cols);
     if (rc != CLPK_OK)
@@ -295,22 +228,186 @@ static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
     return launch_clusters(linear_few_kernel<DT, FORM>, "linear_few", tiles * p.splits, kFewThreads, p.smem_bytes + sizeof(FewSmem) + 1024, p.splits, s, maps, p);
 }
 
-// a product whose operands are contiguous along K, with few tokens or many
+// a product with few tokens or many
 template <int DT, LinearForm FORM>
 static int run_tokens(const Product &w, cudaStream_t s)
 {
-    const uint32_t k_blocks = linear_k_blocks(w, DT);
-    if (few_tokens(w.m, (w.n - 1) / few_cols<FORM> + 1, k_blocks, (uint32_t)num_sms()))
+    const uint32_t k_blocks = linear_k_blocks(w.k, DT);
+    if (few_tokens(w.m, ceil_div(w.n, few_cols<FORM>), k_blocks, (uint32_t)num_sms()))
         return launch_few<DT, FORM>(w, k_blocks, s);
-    return launch_linear<DT, FORM, false, false>(w, plan_linear(w, FORM, k_blocks, false), k_blocks, s);
+    return launch_linear<DT, FORM>(w, k_blocks, s);
 }
 
-// a product of the backward pass: B contiguous along N, A along K or M
-template <int DT, bool kAMn>
-static int run_gradient(const Product &w, cudaStream_t s)
+// ---- the backward pass ----------------------------------------------------------------------------------------
+
+// ---- dg = dh * u * act'(g) and du = dh * act(g) -----------------------------------------------------------
+//
+// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements per step and thread.
+struct GateParams {
+    const void *dh, *g, *u;
+    void *dg, *du;
+    uint64_t ldh, ldw;                  // of the first three, and of the two in the workspace
+    uint32_t m, f;
+    uint32_t vectors;                   // of eight elements in a row
+};
+
+template <int DT>
+__device__ __forceinline__ float2 widen(uint32_t w)
 {
-    const uint32_t k_blocks = linear_k_blocks(w, DT);
-    return launch_linear<DT, kPlain, kAMn, true>(w, plan_linear(w, kPlain, k_blocks * (uint32_t)w.segments, true), k_blocks, s);
+    if constexpr (DT == CLPK_DT_F16)
+        return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+// eight elements of a row of `f`, zeros beyond it
+__device__ __forceinline__ uint4 load8(const void *base, uint64_t at, uint32_t left)
+{
+    const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+    if (left >= 8)
+        return *reinterpret_cast<const uint4 *>(p);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; i++)
+        if (i < left)
+            w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int DT, int ACT>
+__global__ void __launch_bounds__(256) gate_gradients_kernel(GateParams p)
+{
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint64_t all = (uint64_t)p.m * p.vectors;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = i / p.vectors;
+        const uint32_t col = (uint32_t)(i - row * p.vectors) * 8, left = p.f - col;
+        const uint64_t at = row * p.ldh + col;
+        const uint4 vdh = load8(p.dh, at, left), vg = load8(p.g, at, left), vu = load8(p.u, at, left);
+        const uint32_t dh[4] = {vdh.x, vdh.y, vdh.z, vdh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
+        uint32_t dg[4], du[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 h2 = widen<DT>(dh[j]), g2 = widen<DT>(g[j]), u2 = widen<DT>(u[j]);
+            float ax, dx, ay, dy;
+            activate_both<ACT>(g2.x, ax, dx);
+            activate_both<ACT>(g2.y, ay, dy);
+            dg[j] = pack16(h2.x * u2.x * dx, h2.y * u2.y * dy, DT);
+            du[j] = pack16(h2.x * ax, h2.y * ay, DT);
+        }
+        const uint64_t to = row * p.ldw + col;          // whole vectors: the workspace's pitch has room for them
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dg) + to) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.du) + to) = make_uint4(du[0], du[1], du[2], du[3]);
+    }
+}
+
+template <int DT>
+static int launch_gradients(const GateParams &p, int act, cudaStream_t s)
+{
+    const uint64_t blocks = ((uint64_t)p.m * p.vectors + 255) / 256;
+    const unsigned grid = (unsigned)std::min<uint64_t>(blocks, 1u << 30);
+    switch (act) {
+    case CLPK_ACT_SILU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SILU>, "gate_gradients", grid, 256, 0, s, p);
+    case CLPK_ACT_GELU_TANH: return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU_TANH>, "gate_gradients", grid, 256, 0, s, p);
+    case CLPK_ACT_GELU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU>, "gate_gradients", grid, 256, 0, s, p);
+    case CLPK_ACT_RELU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_RELU>, "gate_gradients", grid, 256, 0, s, p);
+    default:                 return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SIGMOID>, "gate_gradients", grid, 256, 0, s, p);
+    }
+}
+
+// elements from one row of dg or du to the next in the workspace
+static uint64_t gradient_pitch(uint32_t f) { return ((uint64_t)f + 7) / 8 * 8; }
+
+// The second tiles of the clusters that have one of the first more (a) and of the others (b), so that the longest cluster is as
+// short as it gets; returns its K blocks.
+static uint64_t share_tiles(const GradTiles &first, const GradTiles &second, uint32_t clusters, uint32_t &share_a, uint32_t &share_b)
+{
+    const uint32_t more = first.tiles % clusters, each = first.tiles / clusters;
+    uint64_t longest = ~0ull;
+    for (uint32_t a = second.tiles / clusters + 1;; a--) {
+        const uint32_t rest = (uint64_t)a * clusters < second.tiles ? second.tiles - a * clusters : 0;
+        const uint32_t b = a + (rest ? ceil_div(rest, clusters - more) : 0);
+        const uint64_t t = std::max(more ? (uint64_t)(each + 1) * first.blocks + (uint64_t)a * second.blocks : 0, (uint64_t)each * first.blocks + (uint64_t)b * second.blocks);
+        if (t < longest) {
+            longest = t;
+            share_a = a;
+            share_b = b;
+        }
+        if (a == 0)
+            return longest;
+    }
+}
+
+template <int DT>
+static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
+{
+    const uint64_t pitch = gradient_pitch(a.f);
+    uint16_t *const dg = static_cast<uint16_t *>(a.d_workspace), *const du = dg + a.m * pitch;
+    const GateParams gates = {a.d_dh, a.d_g, a.d_u, dg, du, a.ldh, pitch, a.m, a.f, (uint32_t)(pitch / 8)};
+    int rc = launch_gradients<DT>(gates, a.activation, s);
+    if (rc != CLPK_OK)
+        return rc;
+
+    GradParams p = {};
+    p.segment = linear_k_blocks(a.f, DT);
+    p.status = a.d_status;
+    LinearPlan plan = {256, 1};
+    float best = 1e30f;
+    for (uint32_t splits = 1; splits <= 4; splits *= 2)
+        for (uint32_t tn = 128; tn <= 256; tn += 128) {
+            const uint32_t tiles_n = ceil_div(a.d, tn), x_tiles_m = ceil_div(a.m, kLinearM), w_tiles_m = ceil_div(a.f, kLinearM), resident = linear_resident(splits);
+            const GradTiles x = {a.d_dx ? x_tiles_m * tiles_n : 0, x_tiles_m, 2 * p.segment, 0};
+            const GradTiles w = {a.d_dwg ? 2 * w_tiles_m * tiles_n : 0, w_tiles_m, linear_k_blocks(a.m, DT), 1};
+            const bool x_first = w.tiles == 0 || (x.tiles > 0 && x.blocks >= w.blocks);
+            const GradTiles &first = x_first ? x : w, &second = x_first ? w : x;
+            const uint32_t tiles = first.tiles + second.tiles;
+            if (resident == 0 || splits > first.blocks || (second.tiles && splits > second.blocks))
+                continue;
+            uint32_t share_a = 0, share_b = second.tiles ? 1 : 0;
+            float t;
+            if (splits == 1) {
+                const uint32_t clusters = std::min(tiles, resident);
+                t = linear_estimate((float)share_tiles(first, second, clusters, share_a, share_b), (float)ceil_div(tiles, clusters), tn, 1);
+            } else {
+                // one tile per cluster, in the order of their numbers
+                const float waves = (float)tiles / (float)resident, all = (float)(first.tiles * ceil_div(first.blocks, splits) + second.tiles * ceil_div(second.blocks, splits));
+                t = linear_estimate(std::max(all / (float)resident, (float)ceil_div(first.blocks, splits)), std::max(waves, 1.0f), tn, splits);
+                t += 3.9f * std::max(waves - 1.0f, 0.0f);
+            }
+            if (t < best) {
+                best = t;
+                plan = {tn, splits};
+                p.tiles_n = tiles_n;
+                p.first = first;
+                p.second = second;
+                p.share_a = share_a;
+                p.share_b = share_b;
+            }
+        }
+
+    GradMaps maps = {};
+    for (int i = 0; i < 2 && rc == CLPK_OK; i++) {
+        const void *grad = i ? du : dg, *w = i ? a.d_wu : a.d_wg;
+        if (a.d_dx) {
+            rc = make_matrix_map(&maps.dg[i], grad, a.m, (uint64_t)a.f * 2, pitch * 2, 128);
+            if (rc == CLPK_OK)
+                rc = make_matrix_map(&maps.w[i], w, a.f, (uint64_t)a.d * 2, a.ldw * 2, kLinearK);
+        }
+        if (rc == CLPK_OK && a.d_dwg)
+            rc = make_matrix_map(&maps.dg_t[i], grad, a.m, (uint64_t)a.f * 2, pitch * 2, kLinearK);
+    }
+    if (rc == CLPK_OK && a.d_dwg)
+        rc = make_matrix_map(&maps.x, a.d_x, a.m, (uint64_t)a.d * 2, a.ldx * 2, kLinearK);
+    void *const out[3] = {a.d_dx, a.d_dwg, a.d_dwu};
+    for (int i = 0; i < 3 && rc == CLPK_OK; i++)
+        if (out[i]) {
+            p.c[i] = linear_result(out[i], i ? a.ldw : a.ldx, i ? a.f : a.m, a.d, DT);
+            rc = make_result_map(&maps.c[i], p.c[i]);
+        }
+    if (rc != CLPK_OK)
+        return rc;
+    return launch_linear_tiles<DT, kGradients>(maps, p, plan, p.first.tiles + p.second.tiles, "linear (gradients)", s);
 }
 
 // ---- what the calls ask of their arguments ------------------------------------------------------------
@@ -358,9 +455,6 @@ static int check_sizes(const char *what, uint32_t m, uint32_t n, uint32_t k, uin
     return CLPK_OK;
 }
 
-// bytes of one of the two gradients that the workspace holds
-static uint64_t gradient_pitch(uint32_t f) { return ((uint64_t)f + 7) / 8 * 8; }
-
 } // namespace clpk
 
 using namespace clpk;
@@ -392,9 +486,8 @@ int clpk_gemm_i8_scaled(const clpk_gemm_i8_scaled_args_t *args, void *stream)
     w.m = a.m;
     w.n = a.n;
     w.k = a.k;
-    w.a[0] = {a.d_a, a.lda};
+    w.a = {a.d_a, a.lda};
     w.b[0] = {a.d_b, a.ldb};
-    w.segments = w.products = 1;
     w.c[0] = a.d_c;
     w.ldc = a.ldc;
     w.out = a.out_dtype;
@@ -443,10 +536,9 @@ int clpk_gated_ffn(const clpk_gated_ffn_args_t *args, void *stream)
     w.m = a.m;
     w.n = a.f;
     w.k = a.d;
-    w.a[0] = {a.d_x, a.ldx};
+    w.a = {a.d_x, a.ldx};
     w.b[0] = {a.d_wg, a.ldw};
     w.b[1] = {a.d_wu, a.ldw};
-    w.segments = w.products = 1;
     w.c[0] = a.d_h;
     w.c[1] = a.d_g;
     w.c[2] = a.d_u;
@@ -510,45 +602,7 @@ int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *st
     if (a.d_dwg)
         CLPK_TRY(check_matrix(what, "d_x", a.d_x, a.d, &a.ldx, a.dtype));
 
-    const uint64_t ld = gradient_pitch(a.f);
-    uint8_t *dg = static_cast<uint8_t *>(a.d_workspace), *du = dg + a.m * ld * 2;
-    const GradParams gp = {a.d_dh, a.d_g, a.d_u, dg, du, a.ldh, ld, a.m, a.f, (uint32_t)(ld / 8)};
-    CLPK_TRY(a.dtype == CLPK_DT_F16 ? launch_gradients<CLPK_DT_F16>(gp, a.activation, s) : launch_gradients<CLPK_DT_BF16>(gp, a.activation, s));
-    if (a.d_dx) {
-        Product w = {};
-        w.m = a.m;
-        w.n = a.d;
-        w.k = a.f;
-        w.a[0] = {dg, ld};
-        w.a[1] = {du, ld};
-        w.b[0] = {a.d_wg, a.ldw};
-        w.b[1] = {a.d_wu, a.ldw};
-        w.segments = 2;
-        w.products = 1;
-        w.c[0] = a.d_dx;
-        w.ldc = a.ldx;
-        w.out = a.dtype;
-        w.status = a.d_status;
-        CLPK_TRY((a.dtype == CLPK_DT_F16 ? run_gradient<CLPK_DT_F16, false>(w, s) : run_gradient<CLPK_DT_BF16, false>(w, s)));
-    }
-    if (a.d_dwg) {
-        Product w = {};
-        w.m = a.f;
-        w.n = a.d;
-        w.k = a.m;
-        w.a[0] = {dg, ld};
-        w.a[1] = {du, ld};
-        w.b[0] = {a.d_x, a.ldx};
-        w.segments = 1;
-        w.products = 2;
-        w.c[0] = a.d_dwg;
-        w.c[1] = a.d_dwu;
-        w.ldc = a.ldw;
-        w.out = a.dtype;
-        w.status = a.d_status;
-        CLPK_TRY((a.dtype == CLPK_DT_F16 ? run_gradient<CLPK_DT_F16, true>(w, s) : run_gradient<CLPK_DT_BF16, true>(w, s)));
-    }
-    return CLPK_OK;
+    return a.dtype == CLPK_DT_F16 ? run_backward<CLPK_DT_F16>(a, s) : run_backward<CLPK_DT_BF16>(a, s);
 }
 
 } // extern "C"
