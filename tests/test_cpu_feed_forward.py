@@ -1,0 +1,72 @@
+"""What of the feed-forward operators can be told without a GPU: their structures, workspace sizes, and that calls without one fail."""
+import ctypes as C
+import re
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from clpeak_b200 import native as N
+
+ROOT = Path(__file__).resolve().parent.parent
+STRUCTS = {"clpk_gemm_i8_scaled_args_t": N.GemmI8ScaledArgs, "clpk_gated_ffn_args_t": N.GatedFfnArgs, "clpk_gated_ffn_backward_args_t": N.GatedFfnBackwardArgs}
+CALLS = [("clpk_gemm_i8_scaled", N.GemmI8ScaledArgs), ("clpk_gated_ffn", N.GatedFfnArgs), ("clpk_gated_ffn_backward", N.GatedFfnBackwardArgs)]
+
+
+def test_structures_are_the_headers(tmp_path):
+    """Names, offsets and sizes as a C compiler has them."""
+    lines = []
+    for name, struct in STRUCTS.items():
+        lines += [f'printf("{name} . %zu\\n", sizeof({name}));'] + [f'printf("{name} {f} %zu\\n", offsetof({name}, {f}));' for f, _ in struct._fields_]
+    src = tmp_path / "offsets.c"
+    src.write_text('#include <stdio.h>\n#include "clpeak_b200_kernels.h"\nint main(void){%s return 0;}\n' % "".join(lines))
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "offsets")], check=True)
+    for line in subprocess.run([str(tmp_path / "offsets")], capture_output=True, text=True, check=True).stdout.split("\n")[:-1]:
+        name, field, at = line.split()
+        struct = STRUCTS[name]
+        assert int(at) == (C.sizeof(struct) if field == "." else getattr(struct, field).offset), line
+
+
+def test_activations_are_numbered_as_in_the_header():
+    text = (ROOT / "include" / "clpeak_b200_kernels.h").read_text()
+    header = {name: int(v) for name, v in re.findall(r"#define CLPK_(ACT_\w+)\s+(\d+)", text)}
+    assert header.pop("ACT_COUNT") == len(header) == 5
+    assert all(getattr(N, name) == v for name, v in header.items())
+
+
+@pytest.mark.parametrize("m,f,want", [(0, 8, 0), (1, 1, 2 * 8 * 2), (3, 8, 2 * 3 * 8 * 2), (1000, 1401, 2 * 1000 * 1408 * 2), (1 << 20, 16384, 2 * (1 << 20) * 16384 * 2)])
+def test_workspace_of_the_backward_pass(K, m, f, want):
+    """Two matrices of 16-bit gradients with rows of 16 bytes, more than 4 GiB of them too."""
+    for dtype in (N.DT_BF16, N.DT_F16):
+        need = C.c_size_t(99)
+        K.clpk_gated_ffn_backward_workspace_bytes(dtype, m, 64, f, C.byref(need))
+        assert need.value == want
+    with pytest.raises(N.ClpkError, match="not BF16 or F16"):
+        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_I8, m, 64, f, C.byref(C.c_size_t()))
+    with pytest.raises(N.ClpkError, match="NULL"):
+        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, 64, f, None)
+
+
+def test_no_call_without_a_gpu(K):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    for call, args in [(getattr(K, name), (C.byref(struct()), None)) for name, struct in CALLS] + [(K.clpk_quantize_rows_i8, (None, None, None, 0, 0, 0, 0, N.DT_F32, None))]:
+        with pytest.raises(N.ClpkError) as e:
+            call(*args)
+        assert e.value.code in (N.ERR_NO_DEVICE, N.ERR_CUDA, N.ERR_UNSUPPORTED)
+
+
+@pytest.mark.skipif(N._calls() is None, reason="built without the interpreter's headers")
+@pytest.mark.parametrize("name,struct", CALLS)
+def test_the_same_answer_as_through_ctypes(K, name, struct):
+    """Structures by reference, arrays of them, and structures of another call."""
+    def outcome(f, args):
+        try:
+            return f(*args)
+        except Exception as e:                                      # noqa: BLE001: whatever either raises
+            return type(e), str(e)
+    array = (struct * 2)()
+    for args in [(C.byref(struct()), 0), (C.byref(struct()), None), (C.byref(array[1]), 0), (C.byref(array), 0), (struct(), 0), (None, 0), (C.byref(N.GemmArgs()), 0),
+                 (C.byref(C.c_int()), 0), (C.byref(struct()),), (0, 0), (C.byref(array[0], C.sizeof(struct)), 0), (C.byref(struct()), -1)]:
+        assert outcome(getattr(K, name), args) == outcome(lambda *a: K.call(name, *a), args)

@@ -14,6 +14,16 @@ pytestmark = pytest.mark.gpu
 # (tokens, model width, hidden width)
 SIZES = [(1, 1, 1), (1, 4096, 1000), (2, 65, 33), (3, 1024, 4097), (16, 200, 128), (17, 2048, 136), (37, 1000, 2712), (64, 640, 520),
          (65, 96, 1016), (128, 72, 264), (129, 520, 64), (200, 64, 8), (257, 333, 257), (513, 128, 1400), (1000, 1, 40), (2500, 264, 700)]
+# one for every way to split the work: tile widths of 64 to 256 and K in one, two or four ranges on CTA pairs, and one to eight ranges
+# of the few-token kernel, whose partial sums lie behind its ring or in it (16-bit operands; in 8 bits K is twice as long for that)
+SPLIT_PAIRS = [(130, 1000, 8), (130, 2000, 520), (300, 4096, 700), (130, 4096, 520), (130, 4096, 2712), (300, 4096, 520), (130, 8200, 4096), (300, 8200, 700)]
+SPLIT_FEW = [(1, 520, 8), (2, 1000, 8), (1, 520, 2712), (1, 8200, 1400), (97, 2000, 8), (112, 2000, 1000), (5, 1000, 16000), (33, 1000, 16000),
+             (96, 1000, 16000), (1, 64, 30000)]
+SPLIT_SCALED = [(130, 2000, 8), (130, 4096, 1000), (300, 8200, 1400), (130, 8200, 1000), (130, 8200, 6000), (130, 8200, 2712), (300, 16000, 4096),
+                (300, 16000, 1400), (520, 64, 6000), (1, 1000, 8), (1, 2000, 8), (97, 4096, 8), (112, 4096, 2712), (33, 2000, 30000), (96, 2000, 30000), (1, 8200, 20000)]
+SPLIT_BACKWARD = [(64, 64, 64), (200, 64, 64), (8000, 264, 2816), (4000, 520, 1000), (1000, 2048, 520), (520, 2048, 520), (2000, 64, 64), (100, 64, 1000),
+                  (2000, 64, 100), (200, 64, 520), (520, 2048, 200), (2000, 2048, 520), (4000, 2048, 520), (520, 2048, 264), (2000, 2048, 1000),
+                  (4000, 520, 4096), (8000, 136, 2816), (4000, 136, 2816)]
 LARGE = [(1, 8192, 14336), (48, 4096, 11008), (2049, 2056, 1032), (4096, 1024, 2816)]
 
 
@@ -58,6 +68,11 @@ def test_gated_sizes(K, cuda, dtype, m, d, f):
     forward(K, dtype, "gelu_tanh", m, d, f, pad=f % 2, keep=True)
 
 
+@pytest.mark.parametrize("m,d,f", SPLIT_PAIRS + SPLIT_FEW)
+def test_gated_splits(K, cuda, m, d, f):
+    forward(K, "bf16", "silu", m, d, f, pad=m % 2, keep=True)
+
+
 @pytest.mark.parametrize("act", sorted(F.ACTS))
 @pytest.mark.parametrize("m", [5, 300])
 def test_gated_activations(K, cuda, act, m):
@@ -86,9 +101,7 @@ def test_gated_infinities_and_nans_stay_in_their_rows(K, cuda):
 
 # ---- 8 bits --------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("m,k,n", SIZES + LARGE[1:])
-def test_scaled_product(K, cuda, out, m, k, n):
+def scaled(K, out, m, k, n):
     pad = (m + n) % 3
     a, b = F.filled(integers(1, m, k), "i8", pad), F.filled(integers(2, n, k), "i8", pad)
     sa, sb = scales(3, m, 0.02), scales(4, n, 1e-3)
@@ -97,6 +110,17 @@ def test_scaled_product(K, cuda, out, m, k, n):
         K.clpk_gemm_i8_scaled(C.byref(F.linear_args(a, b, c, sa, sb, status, out, bias)), F.stream())
         F.check(c, *F.linear64(a, b, sa, sb, out, bias), "c")
         assert status.item() == 0 and F.untouched(c)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,k,n", SIZES + LARGE[1:])
+def test_scaled_product(K, cuda, out, m, k, n):
+    scaled(K, out, m, k, n)
+
+
+@pytest.mark.parametrize("m,k,n", SPLIT_SCALED)
+def test_scaled_product_splits(K, cuda, m, k, n):
+    scaled(K, "f32", m, k, n)
 
 
 @pytest.mark.parametrize("m", [1, 130])
@@ -121,9 +145,7 @@ def test_a_row_without_a_scale_is_nan_or_zero(K, cuda):
     assert bool(torch.isnan(c[1]).all()) and not c[2].any() and bool(torch.isfinite(c[[0, 3]]).all())
 
 
-@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("m,d,f", SIZES + LARGE[1:])
-def test_gated_8_bits(K, cuda, out, m, d, f):
+def gated_i8(K, out, m, d, f):
     pad = (m + f) % 2
     x, wg, wu = (F.filled(integers(s, rows, d), "i8", pad) for s, rows in ((1, m), (2, f), (3, f)))
     ss = scales(4, m, 0.02), scales(5, f, 0.02 / d ** 0.5), scales(6, f, 0.02 / d ** 0.5)
@@ -132,6 +154,17 @@ def test_gated_8_bits(K, cuda, out, m, d, f):
     K.clpk_gated_ffn(C.byref(F.ffn_args("i8", act, x, wg, wu, h, status, scales=ss, out=out)), F.stream())
     F.check(h, *F.gated64(act, x, wg, wu, "i8", out, ss)[0], "h")
     assert status.item() == 0 and F.untouched(h)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,d,f", SIZES + LARGE[1:])
+def test_gated_8_bits(K, cuda, out, m, d, f):
+    gated_i8(K, out, m, d, f)
+
+
+@pytest.mark.parametrize("m,d,f", SPLIT_PAIRS + SPLIT_FEW)
+def test_gated_8_bits_splits(K, cuda, m, d, f):
+    gated_i8(K, "f32", m, 2 * d, f)
 
 
 # ---- backward ------------------------------------------------------------------------------------------
@@ -158,6 +191,11 @@ def backward(K, dtype, act, m, d, f, pad=0, dx=True, dw=True, spread=1.0):
 @pytest.mark.parametrize("m,d,f", SIZES)
 def test_backward_sizes(K, cuda, dtype, m, d, f):
     backward(K, dtype, "silu", m, d, f, pad=m % 2)
+
+
+@pytest.mark.parametrize("m,d,f", SPLIT_BACKWARD)
+def test_backward_splits(K, cuda, m, d, f):
+    backward(K, "bf16", "silu", m, d, f, pad=f % 3 % 2)
 
 
 @pytest.mark.parametrize("act", sorted(F.ACTS))
@@ -285,6 +323,31 @@ def test_a_chain_of_calls_on_a_stream_of_its_own(K, cuda, m):
     want = F.quantize64(h)
     assert torch.equal(hq, want[0]) and torch.equal(hs, want[1])
     F.check(y, *F.linear64(hq, q[3][0], hs, q[3][1], "f32"), "y")
+
+
+@pytest.mark.parametrize("m,log_pitch", [(3, 30), (130, 25)])
+def test_rows_beyond_32_bits(K, cuda, m, log_pitch):
+    """Tokens that lie more than 2^32 bytes into x, g, u, h and the gradients, for few of them and for many."""
+    d, f, step = 72, 136, 1 << log_pitch
+
+    def far(cols, fill):
+        # columns of one allocation: a matrix of its own for each would not fit the card many times over
+        far.at += 256
+        return torch.as_strided(far.all, (m, cols), (step, 1), far.at - 256).copy_(fill) if fill is not None else torch.as_strided(far.all, (m, cols), (step, 1), far.at - 256)
+    far.at, far.all = 0, torch.empty((m - 1) * step + 4096, dtype=torch.bfloat16, device="cuda")
+    x, dh = far(d, normal(1, m, d)), far(f, normal(4, m, f))
+    h, g, u, dx = far(f, None), far(f, None), far(f, None), far(d, None)
+    wg, wu = (F.filled(normal(s, f, d, d ** -0.5), "bf16") for s in (2, 3))
+    status = F.word()
+    K.clpk_gated_ffn(C.byref(F.ffn_args("bf16", "silu", x, wg, wu, h, status, g, u)), F.stream())
+    for got, want, name in zip((h, g, u), F.gated64("silu", x, wg, wu, "bf16", "bf16"), "hgu"):
+        F.check(got, *want, name)
+    dwg, dwu = (F.matrix(f, d, "bf16") for _ in range(2))
+    ws = F.workspace(K, "bf16", m, d, f)
+    K.clpk_gated_ffn_backward(C.byref(F.backward_args("bf16", "silu", x, wg, wu, dh, g, u, dx, dwg, dwu, ws, status)), F.stream())
+    for got, want, name in zip((dx, dwg, dwu), F.backward64("silu", x, wg, wu, dh, g, u, "bf16"), ("dx", "dwg", "dwu")):
+        F.check(got, *want, name)
+    assert status.item() == 0
 
 
 # ---- refusals ------------------------------------------------------------------------------------------------

@@ -1,0 +1,98 @@
+"""The layer of clpeak_b200.feed_forward: its calls together, as a program makes them."""
+import pytest
+import torch
+
+from clpeak_b200 import native as N
+from clpeak_b200.feed_forward import FeedForward, ServedFeedForward, fit
+from tests import ff_util as F
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(seed, rows, cols, std=1.0):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return (torch.randn(rows, cols, generator=gen, device="cuda") * std).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+@pytest.mark.parametrize("act", [N.ACT_SILU, N.ACT_GELU_TANH])
+def test_layer_in_16_bits(cuda, m, act):
+    """y and the gradients, each from what the layer's call before it has left."""
+    d, f = 136, 264
+    layer = FeedForward(d, f, 300, act)
+    name = {v: k for k, v in F.ACTS.items()}[act]
+    x, dy = normal(1, m, d), normal(2, m, d, 0.1)
+    y = layer.forward(x)
+    h, g, u = (t[:m] for t in (layer.h, layer.g, layer.u))
+    for got, want, what in zip((h, g, u), F.gated64(name, x, layer.wg, layer.wu, "bf16", "bf16"), "hgu"):
+        F.check(got, *want, what)
+    want = h.double() @ layer.wd.double().T
+    F.check(y, want, F.rounded(want, "bf16") + F.sums(f) * (h.double().abs() @ layer.wd.double().abs().T), "y")
+    grads = layer.backward(dy)
+    want = dy.double() @ layer.wd.double()
+    F.check(layer.dh[:m], want, F.rounded(want, "bf16") + F.sums(d) * (dy.double().abs() @ layer.wd.double().abs()), "dh")
+    for got, want, what in zip(grads, F.backward64(name, x, layer.wg, layer.wu, layer.dh[:m], g, u, "bf16"), ("dx", "dwg", "dwu")):
+        F.check(got, *want, what)
+    layer.check()
+
+
+def test_x_may_be_a_slice(cuda):
+    layer = FeedForward(64, 128, 50)
+    wide = normal(1, 50, 200)
+    x, dy = wide[:, 8:72], normal(2, 50, 64)
+    y = layer.forward(x).clone()
+    grads = [t.clone() for t in layer.backward(dy)]
+    assert torch.equal(y, layer.forward(x.contiguous())) and all(torch.equal(a, b) for a, b in zip(grads, layer.backward(dy)))
+
+
+def test_a_few_steps_of_descent(cuda):
+    target, layer = FeedForward(64, 128, 512, seed=1), FeedForward(64, 128, 512, seed=2)
+    layer.wd.copy_(target.wd)
+    layer.wd_t.copy_(target.wd_t)
+    losses = fit(layer, target, 30, 0.5)
+    assert losses[-1] < 0.7 * losses[0]                         # 64 bits: 0.24 of it; at four times the rate it diverges there too
+
+
+@pytest.mark.parametrize("m", [0, 1, 48, 300])
+def test_served_in_8_bits(cuda, m):
+    """Every stage from what the stage before has left; and all of it near the layer in bf16: three quantised operands on the
+    way, each off by at most 1 / 254 of its rows' largest element, of the order of 1 % of a row's norm each."""
+    d, f = 520, 1400
+    layer = FeedForward(d, f, 300, N.ACT_SILU)
+    served = ServedFeedForward(layer)
+    x = normal(3, m, d)
+    y = served.forward(x)
+    assert y.shape == (m, d)
+    if m == 0:
+        return
+    xq, hq, h = served.xq[:m], served.hq[:m], served.h[:m]
+    for name in ("wg", "wu", "wd"):
+        want = F.quantize64(getattr(layer, name))
+        assert torch.equal(served.weights[name][0], want[0]) and torch.equal(served.weights[name][1], want[1])
+    want = F.quantize64(x)
+    assert torch.equal(xq, want[0]) and torch.equal(served.xs[:m], want[1])
+    (wg, sg), (wu, su), (wd, sd) = (served.weights[n] for n in ("wg", "wu", "wd"))
+    F.check(h, *F.gated64("silu", xq, wg, wu, "i8", "bf16", (served.xs[:m], sg, su))[0], "h")
+    want = F.quantize64(h)
+    assert torch.equal(hq, want[0]) and torch.equal(served.hs[:m], want[1])
+    F.check(y, *F.linear64(hq, wd, served.hs[:m], sd, "bf16"), "y")
+    assert not served.status.any()
+    full = layer.forward(x).double()
+    assert (y.double() - full).norm() < 0.05 * full.norm()
+
+
+def test_what_the_layer_refuses(cuda):
+    with pytest.raises(ValueError, match="multiples of 8"):
+        FeedForward(60, 64, 4)
+    layer = FeedForward(64, 64, 4)
+    with pytest.raises(RuntimeError, match="without forward"):
+        layer.backward(normal(1, 4, 64))
+    for x in (normal(1, 5, 64), normal(1, 4, 72), normal(1, 4, 64).float(), normal(1, 64, 4).T):
+        with pytest.raises(ValueError, match="x must be"):
+            layer.forward(x)
+        with pytest.raises(ValueError, match="x must be"):
+            ServedFeedForward(layer).forward(x)
+    layer.forward(normal(1, 3, 64))
+    with pytest.raises(ValueError, match="dy must be"):
+        layer.backward(normal(1, 4, 64))
