@@ -153,27 +153,43 @@ __device__ __forceinline__ float bias_at(const void *bias, int type, uint32_t co
     return type == CLPK_DT_F16 ? __half2float(static_cast<const __half *>(bias)[col]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(bias)[col]);
 }
 
+// What a unit of 8-bit sums is finished with: the scale of the lane's row, and of column `col` + lane those of the one or two
+// products, or scale and bias.  They are asked for a unit ahead.
+struct LinearScales {
+    float row = 1.0f, col0 = 1.0f, col1 = 0.0f;
+
+    template <int DT, LinearForm FORM>
+    __device__ __forceinline__ void rows(const LinearParams &p, uint32_t row0, int lane)
+    {
+        if constexpr (DT == CLPK_DT_I8)
+            row = row0 + lane < p.c[0].m ? p.a_scale[row0 + lane] : 0.0f;
+    }
+    template <int DT, LinearForm FORM>
+    __device__ __forceinline__ void cols(const LinearParams &p, uint32_t first, int lane)
+    {
+        if constexpr (DT == CLPK_DT_I8) {
+            const uint32_t c = first + lane;
+            const bool there = c < p.c[0].n;
+            col0 = there ? p.b_scale[c] : 0.0f;
+            if constexpr (FORM == kGated)
+                col1 = there ? p.u_scale[c] : 0.0f;
+            else
+                col1 = p.bias && there ? bias_at(p.bias, p.c[0].type, c) : 0.0f;
+        }
+    }
+};
+
 // What becomes of a unit of sums: one chunk of 32 columns, or with kGated the chunk of g and that of u.  `which`: the result
 // that plain sums (kGradients) belong to.
 template <int DT, LinearForm FORM>
-__device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const LinearParams &p, const uint32_t (&s0)[32], const uint32_t (&s1)[32], uint32_t which,
-                                              uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int lane)
+__device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const LinearParams &p, const LinearScales &scales, const uint32_t (&s0)[32],
+                                              const uint32_t (&s1)[32], uint32_t which, uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int lane)
 {
-    float row_scale = 1.0f, scale0 = 1.0f, scale1 = 1.0f, bias = 0.0f;
-    if constexpr (DT == CLPK_DT_I8) {
-        const uint32_t c = col + lane;
-        row_scale = row + lane < p.c[0].m ? p.a_scale[row + lane] : 0.0f;
-        scale0 = c < p.c[0].n ? p.b_scale[c] : 0.0f;
-        if constexpr (FORM == kGated)
-            scale1 = c < p.c[0].n ? p.u_scale[c] : 0.0f;
-        else
-            bias = p.bias && c < p.c[0].n ? bias_at(p.bias, p.c[0].type, c) : 0.0f;
-    }
     float v[32];
-    scaled32<DT>(v, s0, row_scale, scale0);
+    scaled32<DT>(v, s0, scales.row, scales.col0);
     if constexpr (FORM == kGated) {
         float u[32];
-        scaled32<DT>(u, s1, row_scale, scale1);
+        scaled32<DT>(u, s1, scales.row, scales.col1);
         if (p.keep) {
             linear_store(v, p.c[1], boxes, n_stored, maps + 1, col, row, lane);
             linear_store(u, p.c[2], boxes, n_stored, maps + 2, col, row, lane);
@@ -183,7 +199,7 @@ __device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const Lin
         if (p.bias) {
 #pragma unroll
             for (int i = 0; i < 32; i++)
-                v[i] += __shfl_sync(0xffffffffu, bias, i);
+                v[i] += __shfl_sync(0xffffffffu, scales.col1, i);
         }
     }
     linear_store(v, p.c[which], boxes, n_stored, maps + which, col, row, lane);
@@ -373,6 +389,15 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         // ---------------- epilogue, K not split: the two warps of a lane quarter take every other unit ----------------
         for (uint32_t i = 0; linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
             const uint32_t acc = i & 1, use = i >> 1;
+            const uint32_t row = t.mb * kLinearM + r * 128 + q * 32, col = t.nb * unit_cols;
+            // the two chunks that a step reads are g and u of one unit (kGated), or two units
+            constexpr uint32_t kStep = FORM == kGated ? 2 : 4;
+            LinearScales scales[2];
+            for (int o = 0; o < 2; o++) {
+                scales[o].rows<DT, FORM>(p, row, lane);
+                if (o == 0 || FORM != kGated)
+                    scales[o].cols<DT, FORM>(p, col + (half + 2 * o) * kLinearChunk, lane);
+            }
             if (!warp_wait(&sh->tmem_full[acc], use & 1)) {
                 if (lane == 0)
                     atomicCAS(p.status, 0u, 0x304u);
@@ -380,24 +405,34 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             }
             tc_fence_after_sync();
             const uint32_t taddr = tmem + acc * p.tn + ((q * 32) << 16);
-            const uint32_t row = t.mb * kLinearM + r * 128 + q * 32;
             auto release = [&]() {
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], leader);
             };
-            if (half >= units)
+            if (half >= units) {
                 release();
-            for (uint32_t c = half; c < units; c += 2) {
+                continue;
+            }
+            for (uint32_t c = half; c < units; c += kStep) {
+                const bool two = FORM != kGated && c + 2 < units;
                 uint32_t s0[32], s1[32];
                 tmem_ld_32x32b_x32(taddr + c * kLinearChunk, s0);
-                if constexpr (kSubs == 2)
-                    tmem_ld_32x32b_x32(taddr + p.tn / 2 + c * kLinearChunk, s1);
+                if (FORM == kGated || two)
+                    tmem_ld_32x32b_x32(taddr + (FORM == kGated ? p.tn / 2 + c * kLinearChunk : (c + 2) * kLinearChunk), s1);
                 tmem_ld_wait();
-                if (c + 2 >= units)
+                if (c + kStep >= units)
                     release();
-                linear_finish<DT, FORM>(maps.c, p, s0, s1, t.which, row, t.nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
+                LinearScales next[2] = {scales[0], scales[1]};
+                if (c + kStep < units)
+                    for (int o = 0; o < (FORM == kGated ? 1 : 2); o++)
+                        next[o].cols<DT, FORM>(p, col + (c + kStep + 2 * o) * kLinearChunk, lane);
+                linear_finish<DT, FORM>(maps.c, p, scales[0], s0, s1, t.which, row, col + c * kLinearChunk, boxes, n_stored, lane);
+                if (two)
+                    linear_finish<DT, FORM>(maps.c, p, scales[1], s1, s1, t.which, row, col + (c + 2) * kLinearChunk, boxes, n_stored, lane);
+                scales[0] = next[0];
+                scales[1] = next[1];
             }
         }
     } else if (!warp_wait(&sh->tmem_full[0], 0)) {
@@ -439,6 +474,9 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             const uint32_t row = t.mb * kLinearM + r * 128 + q * 32;
             for (uint32_t j = half; split + j * p.splits < units; j += 2) {
                 const uint32_t c = split + j * p.splits;
+                LinearScales scales;
+                scales.rows<DT, FORM>(p, row, lane);
+                scales.cols<DT, FORM>(p, t.nb * unit_cols + c * kLinearChunk, lane);
                 uint32_t sum[2][32];
 #pragma unroll
                 for (uint32_t sub = 0; sub < kSubs; sub++) {
@@ -466,7 +504,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                         }
                     }
                 }
-                linear_finish<DT, FORM>(maps.c, p, sum[0], sum[kSubs - 1], t.which, row, t.nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
+                linear_finish<DT, FORM>(maps.c, p, scales, sum[0], sum[kSubs - 1], t.which, row, t.nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
             }
         }
     }
