@@ -91,7 +91,9 @@ __device__ __forceinline__ void linear_store(const float (&v)[32], const LinearR
     if (c.ragged && col < c.n && c.n - col < kLinearChunk) {
         __syncwarp();
         const uint32_t left = c.n - col, j = lane * (wide ? 4 : 2), piece = j >> 4, in_piece = j & 15;
-        for (uint32_t i = 0; i < 32 && row + i < c.m; i++) {
+        const uint32_t rows = c.m > row ? (c.m - row < 32 ? c.m - row : 32) : 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < rows; i++) {
             const uint64_t at = (uint64_t)(row + i) * c.ld + col + lane;
             if (lane < left) {
                 if (wide)
@@ -205,6 +207,11 @@ __device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const Lin
     linear_store(v, p.c[which], boxes, n_stored, maps + which, col, row, lane);
 }
 
+// a tile: which result, where in it (rows of 256, and for the result; columns of tn), and which K blocks of it this pair adds
+struct LinearTile {
+    uint32_t which, mb, mb_out, nb, kb0, kb1;
+};
+
 #include "clpk_linear_grad.cuh"
 
 struct LinearMaps {
@@ -213,24 +220,21 @@ struct LinearMaps {
 template <LinearForm FORM> using LinearMapsOf = std::conditional_t<FORM == kGradients, GradMaps, LinearMaps>;
 template <LinearForm FORM> using LinearParamsOf = std::conditional_t<FORM == kGradients, GradParams, LinearParams>;
 
-// a tile: which result, where in it, and over how many K blocks
-struct LinearTile {
-    uint32_t which, mb, nb, k_blocks;
-};
-
 // the i-th tile of a cluster; false: it has no more
 template <LinearForm FORM>
-__device__ __forceinline__ bool linear_tile(const LinearParamsOf<FORM> &p, uint32_t cluster, uint32_t clusters, uint32_t i, LinearTile &t)
+__device__ __forceinline__ bool linear_tile(const LinearParamsOf<FORM> &p, uint32_t cluster, uint32_t clusters, uint32_t split, uint32_t i, LinearTile &t)
 {
     if constexpr (FORM == kGradients) {
-        return grad_tile(p, cluster, clusters, i, t.which, t.mb, t.nb, t.k_blocks);
+        return grad_tile(p, cluster, clusters, i, t);
     } else {
         const uint32_t tile = cluster + i * clusters;
-        t.which = 0;
-        t.k_blocks = p.k_blocks;
         if (tile >= p.tiles_m * p.tiles_n)
             return false;
         dense_tile_coords(tile, p.tiles_m, p.tiles_n, p.group, t.mb, t.nb);
+        t.mb_out = t.mb;
+        t.which = 0;
+        t.kb0 = split * p.k_blocks / p.splits;
+        t.kb1 = (split + 1) * p.k_blocks / p.splits;
         return true;
     }
 }
@@ -288,10 +292,10 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         const uint32_t full0 = cluster_addr(&sh->full[0], leader);
         uint32_t s = 0, parity = 1;                            // parity of the empty barrier's previous phase
         bool ok = true;
-        for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
+        for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, split, i, t); i++) {
             const uint32_t row_a = t.mb * kLinearM + r * 128;
             const uint32_t row_b = FORM == kGated ? t.nb * (p.tn / 2) : t.nb * p.tn + r * (p.tn / 2);
-            const uint32_t kb0 = split * t.k_blocks / p.splits, kb1 = (split + 1) * t.k_blocks / p.splits;
+            const uint32_t kb0 = t.kb0, kb1 = t.kb1;
             for (uint32_t kb = kb0; kb < kb1; kb += p.kps) {
                 const uint32_t nk = kb1 - kb < p.kps ? kb1 - kb : p.kps;
                 if (!warp_wait(&sh->empty[s], parity)) {       // a fresh barrier's preceding phase counts as complete
@@ -330,9 +334,9 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             const uint16_t pair_mask = (uint16_t)(3u << leader);
             uint32_t s = 0, parity = 0;
             bool ok = true;
-            for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
+            for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, split, i, t); i++) {
                 const uint32_t acc = i & 1, use = i >> 1;
-                const uint32_t kb0 = split * t.k_blocks / p.splits, kb1 = (split + 1) * t.k_blocks / p.splits;
+                const uint32_t kb0 = t.kb0, kb1 = t.kb1;
                 if (use > 0 && !warp_wait(&sh->tmem_empty[acc], (use - 1) & 1)) {
                     if (lane == 0)
                         atomicCAS(p.status, 0u, 0x302u);
@@ -387,9 +391,9 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         }
     } else if (p.splits == 1) {
         // ---------------- epilogue, K not split: the two warps of a lane quarter take every other unit ----------------
-        for (uint32_t i = 0; linear_tile<FORM>(p, cluster, clusters, i, t); i++) {
+        for (uint32_t i = 0; linear_tile<FORM>(p, cluster, clusters, split, i, t); i++) {
             const uint32_t acc = i & 1, use = i >> 1;
-            const uint32_t row = t.mb * kLinearM + r * 128 + q * 32, col = t.nb * unit_cols;
+            const uint32_t row = t.mb_out * kLinearM + r * 128 + q * 32, col = t.nb * unit_cols;
             // the two chunks that a step reads are g and u of one unit (kGated), or two units
             constexpr uint32_t kStep = FORM == kGated ? 2 : 4;
             LinearScales scales[2];
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             atomicCAS(p.status, 0u, 0x305u);
     }
 
-    if (p.splits > 1) {
+    if (FORM != kGradients && p.splits > 1) {
         // ---------------- K split over the cluster's pairs (one tile per cluster) ----------------
         // Every pair's instructions have retired, so the stages of the ring are free to take partial sums: slot (src, j) of CTA
         // (owner, r) holds pair src's sums of the owner's j-th unit, src counted without the owner.  They are added in the order
@@ -470,8 +474,8 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         }
         __syncwarp();
         cluster_sync();
-        if (epilogue && linear_tile<FORM>(p, cluster, clusters, 0, t)) {
-            const uint32_t row = t.mb * kLinearM + r * 128 + q * 32;
+        if (epilogue && linear_tile<FORM>(p, cluster, clusters, split, 0, t)) {
+            const uint32_t row = t.mb_out * kLinearM + r * 128 + q * 32;
             for (uint32_t j = half; split + j * p.splits < units; j += 2) {
                 const uint32_t c = split + j * p.splits;
                 LinearScales scales;

@@ -319,24 +319,135 @@ static int launch_gradients(const GateParams &p, int act, cudaStream_t s)
 // elements from one row of dg or du to the next in the workspace
 static uint64_t gradient_pitch(uint32_t f) { return ((uint64_t)f + 7) / 8 * 8; }
 
-// The second tiles of the clusters that have one of the first more (a) and of the others (b), so that the longest cluster is as
-// short as it gets; returns its K blocks.
+// Partial sums of K in the workspace -> the result.  Four columns per thread and step; 4 bytes an element and part, mostly from the
+// L2 that they have just been written to.
+struct JoinResult {
+    const float *parts;                 // [parts][rows_all][cols_all]
+    void *out;                          // [rows][cols], pitch ld
+    uint64_t ld;
+    uint32_t rows, rows_all, n_parts;
+};
+struct JoinParams {
+    JoinResult r[3];
+    uint32_t cols, cols_all;            // cols_all: a multiple of four
+    uint32_t results;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(256) join_parts_kernel(JoinParams p)
+{
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t vectors = p.cols_all / 4;
+    for (uint32_t o = 0; o < p.results; o++) {
+        const JoinResult &r = p.r[o];
+        const uint64_t all = (uint64_t)r.rows * vectors, part = (uint64_t)r.rows_all * vectors;
+        for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+            const float4 *from = reinterpret_cast<const float4 *>(r.parts) + i;
+            float4 sum = *from;
+#pragma unroll 4
+            for (uint32_t k = 1; k < r.n_parts; k++) {
+                const float4 v = from[k * part];
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+            }
+            const uint64_t row = i / vectors;
+            const uint32_t col = (uint32_t)(i - row * vectors) * 4;
+            const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+            few_store(r.out, DT, row * r.ld + col, p.cols - col, v);
+        }
+    }
+}
+
+// What a tile counts for, in K blocks: a short sum takes as long as the tile before it takes to be stored, 1.5 us (tn = 128) to 2.7.
+static uint32_t tile_blocks(const GradTiles &t) { return t.tiles ? std::max(ceil_div(t.blocks, t.parts), 7u) : 1; }
+
+// The second tiles of the clusters that have one of the first more (a) and of the others (b), so that the longest cluster is about
+// as short as it gets; returns its K blocks.
 static uint64_t share_tiles(const GradTiles &first, const GradTiles &second, uint32_t clusters, uint32_t &share_a, uint32_t &share_b)
 {
     const uint32_t more = first.tiles % clusters, each = first.tiles / clusters;
+    const uint32_t fb = tile_blocks(first), sb = tile_blocks(second);
+    // b - a is what one of the first is worth
+    const uint64_t without = more ? (uint64_t)(clusters - more) * (fb / sb) : 0;
+    const uint32_t about = second.tiles > without ? (uint32_t)((second.tiles - without) / clusters) : 0;
     uint64_t longest = ~0ull;
-    for (uint32_t a = second.tiles / clusters + 1;; a--) {
+    for (uint32_t a = about ? about - 1 : 0; a <= about + 2; a++) {
         const uint32_t rest = (uint64_t)a * clusters < second.tiles ? second.tiles - a * clusters : 0;
         const uint32_t b = a + (rest ? ceil_div(rest, clusters - more) : 0);
-        const uint64_t t = std::max(more ? (uint64_t)(each + 1) * first.blocks + (uint64_t)a * second.blocks : 0, (uint64_t)each * first.blocks + (uint64_t)b * second.blocks);
+        const uint64_t t = std::max(more ? (uint64_t)(each + 1) * fb + (uint64_t)a * sb : 0, (uint64_t)each * fb + (uint64_t)b * sb);
         if (t < longest) {
             longest = t;
             share_a = a;
             share_b = b;
         }
-        if (a == 0)
-            return longest;
     }
+    return longest;
+}
+
+constexpr uint32_t kGradPairs = 74;                         // of a whole B200: the workspace's size may not depend on the card at hand
+
+// How the products of the backward pass are cut: tile width and parts of K, the cheapest by the estimate.
+struct GradPlan {
+    uint32_t tn, x_parts, w_parts;
+};
+
+static GradTiles x_tiles(uint32_t m, uint32_t d, uint32_t f, uint32_t tn, uint32_t parts)
+{
+    const uint32_t tiles_m = ceil_div(m, kLinearM);
+    return {parts * tiles_m * ceil_div(d, tn), tiles_m, 2 * ceil_div(f, kLinearK), parts, 1};
+}
+static GradTiles w_tiles(uint32_t m, uint32_t d, uint32_t f, uint32_t tn, uint32_t parts)
+{
+    const uint32_t tiles_m = ceil_div(f, kLinearM);
+    return {2 * parts * tiles_m * ceil_div(d, tn), tiles_m, ceil_div(m, kLinearK), parts, 2};
+}
+
+static uint64_t part_cols(uint32_t d) { return ((uint64_t)d + 3) / 4 * 4; }
+
+// bytes of the fp32 results of all parts; none where K is whole
+static uint64_t part_bytes(const GradTiles &t, uint32_t d) { return t.parts > 1 ? (uint64_t)t.products * t.parts * t.tiles_m * kLinearM * part_cols(d) * 4 : 0; }
+
+static const GradTiles &longer(const GradTiles &x, const GradTiles &w)
+{
+    return w.tiles == 0 || (x.tiles > 0 && x.blocks / x.parts >= w.blocks / w.parts) ? x : w;
+}
+
+static GradPlan plan_backward(uint32_t m, uint32_t d, uint32_t f)
+{
+    GradPlan plan = {256, 1, 1};
+    float best = 1e30f;
+    for (uint32_t tn = 128; tn <= 256; tn += 128) {
+        const GradTiles x1 = x_tiles(m, d, f, tn, 1), w1 = w_tiles(m, d, f, tn, 1);
+        // parts that leave each tile what a cluster would do if all shared the work, and ten K blocks at least
+        const uint64_t all = (uint64_t)x1.tiles * tile_blocks(x1) + (uint64_t)w1.tiles * tile_blocks(w1);
+        const uint32_t fair = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(all / kGradPairs, 1u << 20), 10);
+        const uint32_t most = 32, xp = std::min(ceil_div(x1.blocks, fair), most), wp = std::min(ceil_div(w1.blocks, fair), most);
+        for (uint32_t cut = 0; cut < 4; cut++) {
+            if (((cut & 1) && xp == 1) || ((cut & 2) && wp == 1))
+                continue;
+            const GradTiles x = x_tiles(m, d, f, tn, cut & 1 ? xp : 1), w = w_tiles(m, d, f, tn, cut & 2 ? wp : 1);
+            const GradTiles &first = longer(x, w), &second = &first == &x ? w : x;
+            const uint32_t clusters = std::min(x.tiles + w.tiles, kGradPairs);
+            uint32_t a, b;
+            float t = linear_estimate((float)share_tiles(first, second, clusters, a, b), (float)ceil_div(x.tiles + w.tiles, clusters), tn, 1);
+            if (cut)                    // a launch, and each part's sums written and read
+                t += 3.0f + (float)(part_bytes(x, d) + part_bytes(w, d)) / 2.5e6f;
+            if (t < best) {
+                best = t;
+                plan = {tn, x.parts, w.parts};
+            }
+        }
+    }
+    return plan;
+}
+
+static uint64_t backward_bytes(uint32_t m, uint32_t d, uint32_t f)
+{
+    const uint64_t gradients = 2 * (uint64_t)m * gradient_pitch(f) * 2;
+    if (m == 0 || d == 0 || f == 0)
+        return gradients;
+    const GradPlan plan = plan_backward(m, d, f);
+    return gradients + part_bytes(x_tiles(m, d, f, plan.tn, plan.x_parts), d) + part_bytes(w_tiles(m, d, f, plan.tn, plan.w_parts), d);
 }
 
 template <int DT>
@@ -344,70 +455,69 @@ static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
 {
     const uint64_t pitch = gradient_pitch(a.f);
     uint16_t *const dg = static_cast<uint16_t *>(a.d_workspace), *const du = dg + a.m * pitch;
+    float *parts = reinterpret_cast<float *>(du + a.m * pitch);
     const GateParams gates = {a.d_dh, a.d_g, a.d_u, dg, du, a.ldh, pitch, a.m, a.f, (uint32_t)(pitch / 8)};
     int rc = launch_gradients<DT>(gates, a.activation, s);
     if (rc != CLPK_OK)
         return rc;
 
+    const GradPlan cut = plan_backward(a.m, a.d, a.f);
+    const LinearPlan plan = {cut.tn, 1};
+    GradTiles x = x_tiles(a.m, a.d, a.f, cut.tn, cut.x_parts), w = w_tiles(a.m, a.d, a.f, cut.tn, cut.w_parts);
+    if (!a.d_dx)
+        x.tiles = 0;
+    if (!a.d_dwg)
+        w.tiles = 0;
     GradParams p = {};
-    p.segment = linear_k_blocks(a.f, DT);
+    p.tiles_n = ceil_div(a.d, cut.tn);
+    p.segment = ceil_div(a.f, kLinearK);
     p.status = a.d_status;
-    LinearPlan plan = {256, 1};
-    float best = 1e30f;
-    for (uint32_t splits = 1; splits <= 4; splits *= 2)
-        for (uint32_t tn = 128; tn <= 256; tn += 128) {
-            const uint32_t tiles_n = ceil_div(a.d, tn), x_tiles_m = ceil_div(a.m, kLinearM), w_tiles_m = ceil_div(a.f, kLinearM), resident = linear_resident(splits);
-            const GradTiles x = {a.d_dx ? x_tiles_m * tiles_n : 0, x_tiles_m, 2 * p.segment, 0};
-            const GradTiles w = {a.d_dwg ? 2 * w_tiles_m * tiles_n : 0, w_tiles_m, linear_k_blocks(a.m, DT), 1};
-            const bool x_first = w.tiles == 0 || (x.tiles > 0 && x.blocks >= w.blocks);
-            const GradTiles &first = x_first ? x : w, &second = x_first ? w : x;
-            const uint32_t tiles = first.tiles + second.tiles;
-            if (resident == 0 || splits > first.blocks || (second.tiles && splits > second.blocks))
-                continue;
-            uint32_t share_a = 0, share_b = second.tiles ? 1 : 0;
-            float t;
-            if (splits == 1) {
-                const uint32_t clusters = std::min(tiles, resident);
-                t = linear_estimate((float)share_tiles(first, second, clusters, share_a, share_b), (float)ceil_div(tiles, clusters), tn, 1);
-            } else {
-                // one tile per cluster, in the order of their numbers
-                const float waves = (float)tiles / (float)resident, all = (float)(first.tiles * ceil_div(first.blocks, splits) + second.tiles * ceil_div(second.blocks, splits));
-                t = linear_estimate(std::max(all / (float)resident, (float)ceil_div(first.blocks, splits)), std::max(waves, 1.0f), tn, splits);
-                t += 3.9f * std::max(waves - 1.0f, 0.0f);
-            }
-            if (t < best) {
-                best = t;
-                plan = {tn, splits};
-                p.tiles_n = tiles_n;
-                p.first = first;
-                p.second = second;
-                p.share_a = share_a;
-                p.share_b = share_b;
-            }
-        }
+    p.first = longer(x, w);
+    p.second = &longer(x, w) == &x ? w : x;
+    const uint32_t n_tiles = x.tiles + w.tiles;
+    share_tiles(p.first, p.second, std::min(n_tiles, linear_resident(1)), p.share_a, p.share_b);
 
     GradMaps maps = {};
     for (int i = 0; i < 2 && rc == CLPK_OK; i++) {
-        const void *grad = i ? du : dg, *w = i ? a.d_wu : a.d_wg;
+        const void *grad = i ? du : dg, *weight = i ? a.d_wu : a.d_wg;
         if (a.d_dx) {
             rc = make_matrix_map(&maps.dg[i], grad, a.m, (uint64_t)a.f * 2, pitch * 2, 128);
             if (rc == CLPK_OK)
-                rc = make_matrix_map(&maps.w[i], w, a.f, (uint64_t)a.d * 2, a.ldw * 2, kLinearK);
+                rc = make_matrix_map(&maps.w[i], weight, a.f, (uint64_t)a.d * 2, a.ldw * 2, kLinearK);
         }
         if (rc == CLPK_OK && a.d_dwg)
             rc = make_matrix_map(&maps.dg_t[i], grad, a.m, (uint64_t)a.f * 2, pitch * 2, kLinearK);
     }
     if (rc == CLPK_OK && a.d_dwg)
         rc = make_matrix_map(&maps.x, a.d_x, a.m, (uint64_t)a.d * 2, a.ldx * 2, kLinearK);
+    JoinParams join = {};
+    join.cols = a.d;
+    join.cols_all = (uint32_t)part_cols(a.d);
+    uint64_t joined = 0;                                    // vectors of the largest result
     void *const out[3] = {a.d_dx, a.d_dwg, a.d_dwu};
-    for (int i = 0; i < 3 && rc == CLPK_OK; i++)
-        if (out[i]) {
-            p.c[i] = linear_result(out[i], i ? a.ldw : a.ldx, i ? a.f : a.m, a.d, DT);
-            rc = make_result_map(&maps.c[i], p.c[i]);
+    for (int i = 0; i < 3 && rc == CLPK_OK; i++) {
+        if (!out[i])
+            continue;
+        const GradTiles &set = i ? w : x;
+        const uint32_t rows = i ? a.f : a.m, rows_all = set.tiles_m * kLinearM;
+        const uint64_t ld = i ? a.ldw : a.ldx;
+        if (set.parts > 1) {
+            p.c[i] = linear_result(parts, join.cols_all, set.parts * rows_all, join.cols_all, CLPK_DT_F32);
+            join.r[join.results++] = {parts, out[i], ld, rows, rows_all, set.parts};
+            joined = std::max(joined, (uint64_t)rows * join.cols_all / 4);
+            parts += (uint64_t)set.parts * rows_all * join.cols_all;
+        } else {
+            p.c[i] = linear_result(out[i], ld, rows, a.d, DT);
         }
+        rc = make_result_map(&maps.c[i], p.c[i]);
+    }
     if (rc != CLPK_OK)
         return rc;
-    return launch_linear_tiles<DT, kGradients>(maps, p, plan, p.first.tiles + p.second.tiles, "linear (gradients)", s);
+    rc = launch_linear_tiles<DT, kGradients>(maps, p, plan, n_tiles, "linear (gradients)", s);
+    if (rc != CLPK_OK || join.results == 0)
+        return rc;
+    const unsigned grid = (unsigned)std::min<uint64_t>((joined + 255) / 256, 8u * (uint32_t)num_sms());
+    return launch_behind(join_parts_kernel<DT>, "join_parts", grid, 256, 0, s, join);
 }
 
 // ---- what the calls ask of their arguments ------------------------------------------------------------
@@ -560,8 +670,7 @@ int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, u
     CLPK_REQUIRE(bytes, "bytes is NULL");
     *bytes = 0;
     CLPK_REQUIRE(dtype == CLPK_DT_BF16 || dtype == CLPK_DT_F16, "clpk_gated_ffn_backward: dtype %d is not BF16 or F16", dtype);
-    (void)d;
-    *bytes = 2 * (size_t)m * gradient_pitch(f) * 2;
+    *bytes = (size_t)backward_bytes(m, d, f);
     return CLPK_OK;
 }
 

@@ -34,17 +34,21 @@ def test_activations_are_numbered_as_in_the_header():
     assert all(getattr(N, name) == v for name, v in header.items())
 
 
-@pytest.mark.parametrize("m,f,want", [(0, 8, 0), (1, 1, 2 * 8 * 2), (3, 8, 2 * 3 * 8 * 2), (1000, 1401, 2 * 1000 * 1408 * 2), (1 << 20, 16384, 2 * (1 << 20) * 16384 * 2)])
-def test_workspace_of_the_backward_pass(K, m, f, want):
-    """Two matrices of 16-bit gradients with rows of 16 bytes, more than 4 GiB of them too."""
+@pytest.mark.parametrize("m,d,f,parts", [(0, 64, 8, 0), (1, 64, 1, 0), (3, 8, 8, 0), (8192, 2048, 8192, 0), (1 << 20, 64, 16384, 0), (4000, 520, 1000, 0),
+                                         (147, 656, 7749, 1), (8000, 96, 200, 2)])
+def test_workspace_of_the_backward_pass(K, m, d, f, parts):
+    """Two matrices of 16-bit gradients with rows of 16 bytes, more than 4 GiB of them too; and where a sum over K is cut, an fp32
+    result for each part: at most 32 of them, of dx (1) or of dWg and dWu (2), with rows in whole 256s."""
+    gradients = 2 * m * -(-f // 8) * 8 * 2
     for dtype in (N.DT_BF16, N.DT_F16):
         need = C.c_size_t(99)
-        K.clpk_gated_ffn_backward_workspace_bytes(dtype, m, 64, f, C.byref(need))
-        assert need.value == want
+        K.clpk_gated_ffn_backward_workspace_bytes(dtype, m, d, f, C.byref(need))
+        one = (0, -(-m // 256) * 256 * d * 4, 2 * -(-f // 256) * 256 * d * 4)[parts]
+        assert need.value == gradients if parts == 0 else (need.value - gradients) % one == 0 and 2 <= (need.value - gradients) // one <= 32
     with pytest.raises(N.ClpkError, match="not BF16 or F16"):
-        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_I8, m, 64, f, C.byref(C.c_size_t()))
+        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_I8, m, d, f, C.byref(C.c_size_t()))
     with pytest.raises(N.ClpkError, match="NULL"):
-        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, 64, f, None)
+        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, d, f, None)
 
 
 def test_no_call_without_a_gpu(K):

@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 # (tokens, model width, hidden width)
 SIZES = [(1, 1, 1), (1, 4096, 1000), (2, 65, 33), (3, 1024, 4097), (16, 200, 128), (17, 2048, 136), (37, 1000, 2712), (64, 640, 520),
          (65, 96, 1016), (128, 72, 264), (129, 520, 64), (200, 64, 8), (257, 333, 257), (513, 128, 1400), (1000, 1, 40), (2500, 264, 700)]
-# one for every way to split the work: tile widths of 64 to 256 and K in one, two or four ranges on CTA pairs, and one to eight ranges
+# one for every way to split the work: tile widths of 64 to 256, K in one, two or four ranges on CTA pairs, and one to eight ranges
 # of the few-token kernel, whose partial sums lie behind its ring or in it (16-bit operands; in 8 bits K is twice as long for that)
 SPLIT_PAIRS = [(130, 1000, 8), (130, 2000, 520), (300, 4096, 700), (130, 4096, 520), (130, 4096, 2712), (300, 4096, 520), (130, 8200, 4096), (300, 8200, 700)]
 SPLIT_FEW = [(1, 520, 8), (2, 1000, 8), (1, 520, 2712), (1, 8200, 1400), (97, 2000, 8), (112, 2000, 1000), (5, 1000, 16000), (33, 1000, 16000),
@@ -23,7 +23,10 @@ SPLIT_SCALED = [(130, 2000, 8), (130, 4096, 1000), (300, 8200, 1400), (130, 8200
                 (300, 16000, 1400), (520, 64, 6000), (1, 1000, 8), (1, 2000, 8), (97, 4096, 8), (112, 4096, 2712), (33, 2000, 30000), (96, 2000, 30000), (1, 8200, 20000)]
 SPLIT_BACKWARD = [(64, 64, 64), (200, 64, 64), (8000, 264, 2816), (4000, 520, 1000), (1000, 2048, 520), (520, 2048, 520), (2000, 64, 64), (100, 64, 1000),
                   (2000, 64, 100), (200, 64, 520), (520, 2048, 200), (2000, 2048, 520), (4000, 2048, 520), (520, 2048, 264), (2000, 2048, 1000),
-                  (4000, 520, 4096), (8000, 136, 2816), (4000, 136, 2816)]
+                  (4000, 520, 4096), (8000, 136, 2816), (4000, 136, 2816),
+                  # sums in parts: of dx, of dW, of both
+                  (362, 96, 11829), (147, 654, 7749), (100, 4096, 8192), (9, 1436, 6644), (689, 1, 904), (8000, 96, 200), (16000, 40, 100), (1860, 1, 284),
+                  (4653, 1818, 8), (1702, 1, 582), (1235, 3, 781), (3585, 132, 1088)]
 LARGE = [(1, 8192, 14336), (48, 4096, 11008), (2049, 2056, 1032), (4096, 1024, 2816)]
 
 
@@ -210,8 +213,9 @@ def test_backward_large(K, cuda, m, d, f):
 
 
 @pytest.mark.parametrize("dx,dw", [(True, False), (False, True), (False, False)])
-def test_backward_of_what_is_asked_for(K, cuda, dx, dw):
-    backward(K, "bf16", "silu", 70, 136, 264, dx=dx, dw=dw)
+@pytest.mark.parametrize("m,d,f", [(70, 136, 264), (1702, 1, 582), (2049, 520, 1032)])
+def test_backward_of_what_is_asked_for(K, cuda, dx, dw, m, d, f):
+    backward(K, "bf16", "silu", m, d, f, dx=dx, dw=dw)
 
 
 @pytest.mark.parametrize("act", sorted(F.ACTS))
