@@ -10,6 +10,11 @@
 // it adds them in the order of K and finishes them.  Sending instead of fetching, because a fetch is a round trip of a microsecond
 // per CTA that is asked; and, where a CTA's share of the SM has room for it, to a place behind the owner's ring, which may still be
 // at work (in the ring it takes a barrier more).  Nothing goes through global memory.  CTAs are small: several share an SM, and one's set-up and exchange lie under another's loads.
+//
+// What bounds it: the weights' way from memory, and for few of them the chain from launch to launch (2.7 us).  bf16 1 x 4096 x
+// 11008: 180 MB in 31.3 us, 5.8 TB/s; int8 1 x 16384 x 4096 13.5 us against 10.3 at the copy rate, 1 x 4096 x 4096 5.2 against
+// 2.6; int8 48 x 4096 x 11008 20.0 against 14.0, of which 2.3 are the finishing of 48 tokens after the last product.  With 256
+// tokens' rows of A and the weights as B, as the pairs have it, the same calls take 16 to 64 us.
 #pragma once
 
 constexpr int kFewThreads = 256, kFewResident = 4;             // CTAs that an SM has registers for

@@ -242,7 +242,11 @@ static int run_tokens(const Product &w, cudaStream_t s)
 
 // ---- dg = dh * u * act'(g) and du = dh * act(g) -----------------------------------------------------------
 //
-// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements per step and thread.
+// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements per step and thread; 8192 x 8192
+// in 96 us, 7.0 TB/s.  The rounding of dg and du to 16 bits is what lets the tensor cores multiply them at full rate: it adds to
+// the gradients an error of the size of their own rounding (bf16 0.0017 -> 0.0023 of the norm).
+// Making them inside the products' launch, by warps that wait for a first tile, was built and measured: in a program that
+// keeps the card at its power limit nothing is gained by overlap (1023 against 988 us at 8192 x 2048 x 8192).
 struct GateParams {
     const void *dh, *g, *u;
     void *dg, *du;

