@@ -2,6 +2,7 @@
 
 Sizes: single tokens, tokens just below and above a tile's, odd widths, one column, sums of one element."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -352,6 +353,95 @@ def test_rows_beyond_32_bits(K, cuda, m, log_pitch):
     for got, want, name in zip((dx, dwg, dwu), F.backward64("silu", x, wg, wu, dh, g, u, "bf16"), ("dx", "dwg", "dwu")):
         F.check(got, *want, name)
     assert status.item() == 0
+
+
+@pytest.mark.parametrize("m", [3, 300])
+def test_scales_and_bias_at_any_word(K, cuda, m):
+    """They are aligned to their elements and no further."""
+    n, k = 200, 130
+    a, b = F.filled(integers(1, m, k), "i8"), F.filled(integers(2, n, k), "i8")
+    sa, sb, su = scales(3, m + 1, 0.02)[1:], scales(4, n + 3, 1e-3)[3:], scales(5, n + 2, 1e-3)[2:]
+    bias = normal(5, 1, n + 1)[0].to(torch.bfloat16)[1:]
+    c, status = F.matrix(m, n, "bf16"), F.word()
+    K.clpk_gemm_i8_scaled(C.byref(F.linear_args(a, b, c, sa, sb, status, "bf16", bias)), F.stream())
+    F.check(c, *F.linear64(a, b, sa, sb, "bf16", bias), "c")
+    K.clpk_gated_ffn(C.byref(F.ffn_args("i8", "relu", a, b, b, c, status, scales=(sa, sb, su), out="bf16")), F.stream())
+    F.check(c, *F.gated64("relu", a, b, b, "i8", "bf16", (sa, sb, su))[0], "h")
+
+
+@pytest.mark.parametrize("m,d,f", [(2, 520, 1032), (300, 520, 1032), (1702, 8, 584)])
+def test_calls_captured_in_a_graph(K, cuda, m, d, f):
+    """Forward and backward captured once and replayed on inputs that have changed since."""
+    x, wg, wu, dh = (F.matrix(r, c, "bf16") for r, c in ((m, d), (f, d), (f, d), (m, f)))
+    h, g, u = (F.matrix(m, f, "bf16") for _ in range(3))
+    grads = [F.matrix(rows, d, "bf16") for rows in (m, f, f)]
+    ws, status = F.workspace(K, "bf16", m, d, f), F.word()
+    xq, xs = F.matrix(m, d, "i8"), torch.empty(m, device="cuda")
+    forward_args = F.ffn_args("bf16", "silu", x, wg, wu, h, status, g, u)
+    backward_args = F.backward_args("bf16", "silu", x, wg, wu, dh, g, u, *grads, ws, status)
+
+    def calls(s):
+        K.clpk_quantize_rows_i8(xq.data_ptr(), xs.data_ptr(), x.data_ptr(), m, d, xq.stride(0), x.stride(0), N.DT_BF16, s)
+        K.clpk_gated_ffn(C.byref(forward_args), s)
+        K.clpk_gated_ffn_backward(C.byref(backward_args), s)
+    for t in (x, wg, wu, dh):
+        t.fill_(1)
+    calls(F.stream())                                                   # what a first call sets up is not for a capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(F.stream())
+    for seed in (1, 11):
+        x.copy_(normal(seed, m, d))
+        wg.copy_(normal(seed + 1, f, d, d ** -0.5))
+        wu.copy_(normal(seed + 2, f, d, d ** -0.5))
+        dh.copy_(normal(seed + 3, m, f, 0.1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = F.quantize64(x)
+        assert torch.equal(xq, want[0]) and torch.equal(xs, want[1])
+        for got, w, name in zip((h, g, u), F.gated64("silu", x, wg, wu, "bf16", "bf16"), "hgu"):
+            F.check(got, *w, name)
+        for got, w, name in zip(grads, F.backward64("silu", x, wg, wu, dh, g, u, "bf16"), ("dx", "dwg", "dwu")):
+            F.check(got, *w, name)
+    assert status.item() == 0
+
+
+def test_threads_with_streams_of_their_own(K, cuda):
+    """Two host threads, each with its buffers: few tokens on one stream, many on the other, results as of one alone."""
+    sizes, alone, failed = ((3, 1032, 2056), (400, 264, 1400)), [], []
+
+    def buffers(i):
+        m, d, f = sizes[i]
+        x, wg, wu, dh = (F.filled(normal(10 * i + s, r, c, 0.1), "bf16") for s, r, c in ((1, m, d), (2, f, d), (3, f, d), (4, m, f)))
+        return x, wg, wu, dh, [F.matrix(r, c, "bf16") for r, c in ((m, f), (m, f), (m, f), (m, d), (f, d), (f, d))], F.workspace(K, "bf16", m, d, f), F.word()
+
+    def calls(b, s):
+        x, wg, wu, dh, out, ws, status = b
+        K.clpk_gated_ffn(C.byref(F.ffn_args("bf16", "silu", x, wg, wu, out[0], status, out[1], out[2])), s)
+        K.clpk_gated_ffn_backward(C.byref(F.backward_args("bf16", "silu", x, wg, wu, dh, out[1], out[2], *out[3:], ws, status)), s)
+    both = [buffers(0), buffers(1)]
+    for b in both:
+        calls(b, F.stream())
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in b[4]])
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        for _ in range(40):
+            for t in both[i][4]:
+                with torch.cuda.stream(stream):
+                    t.zero_()
+            calls(both[i], stream.cuda_stream)
+            stream.synchronize()
+            if both[i][6].item() != 0 or not all(torch.equal(a, t) for a, t in zip(alone[i], both[i][4])):
+                failed.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
 
 
 # ---- refusals ------------------------------------------------------------------------------------------------
