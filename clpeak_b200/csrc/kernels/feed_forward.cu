@@ -283,34 +283,34 @@ __global__ void __launch_bounds__(256) gate_gradients_kernel(GateParams p)
 {
     griddep_wait();
     griddep_launch_dependents();
-    const uint64_t all = (uint64_t)p.m * p.vectors;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t row = i / p.vectors;
-        const uint32_t col = (uint32_t)(i - row * p.vectors) * 8, left = p.f - col;
-        const uint64_t at = row * p.ldh + col;
-        const uint4 vdh = load8(p.dh, at, left), vg = load8(p.g, at, left), vu = load8(p.u, at, left);
-        const uint32_t dh[4] = {vdh.x, vdh.y, vdh.z, vdh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
-        uint32_t dg[4], du[4];
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / p.vectors;
+    if (row >= p.m)
+        return;
+    const uint32_t col = (i - row * p.vectors) * 8, left = p.f - col;
+    const uint64_t at = row * p.ldh + col;
+    const uint4 vdh = load8(p.dh, at, left), vg = load8(p.g, at, left), vu = load8(p.u, at, left);
+    const uint32_t dh[4] = {vdh.x, vdh.y, vdh.z, vdh.w}, g[4] = {vg.x, vg.y, vg.z, vg.w}, u[4] = {vu.x, vu.y, vu.z, vu.w};
+    uint32_t dg[4], du[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 h2 = widen<DT>(dh[j]), g2 = widen<DT>(g[j]), u2 = widen<DT>(u[j]);
-            float ax, dx, ay, dy;
-            activate_both<ACT>(g2.x, ax, dx);
-            activate_both<ACT>(g2.y, ay, dy);
-            dg[j] = pack16(h2.x * u2.x * dx, h2.y * u2.y * dy, DT);
-            du[j] = pack16(h2.x * ax, h2.y * ay, DT);
-        }
-        const uint64_t to = row * p.ldw + col;          // whole vectors: the workspace's pitch has room for them
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dg) + to) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.du) + to) = make_uint4(du[0], du[1], du[2], du[3]);
+    for (int j = 0; j < 4; j++) {
+        const float2 h2 = widen<DT>(dh[j]), g2 = widen<DT>(g[j]), u2 = widen<DT>(u[j]);
+        float ax, dx, ay, dy;
+        activate_both<ACT>(g2.x, ax, dx);
+        activate_both<ACT>(g2.y, ay, dy);
+        dg[j] = pack16(h2.x * u2.x * dx, h2.y * u2.y * dy, DT);
+        du[j] = pack16(h2.x * ax, h2.y * ay, DT);
     }
+    const uint64_t to = row * p.ldw + col;          // whole vectors: the workspace's pitch has room for them
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.dg) + to) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.du) + to) = make_uint4(du[0], du[1], du[2], du[3]);
 }
 
 template <int DT>
 static int launch_gradients(const GateParams &p, int act, cudaStream_t s)
 {
-    const uint64_t blocks = ((uint64_t)p.m * p.vectors + 255) / 256;
-    const unsigned grid = (unsigned)std::min<uint64_t>(blocks, 1u << 30);
+    const uint64_t vectors = (uint64_t)p.m * p.vectors;
+    CLPK_REQUIRE(vectors <= (1ull << 32) - 256, "clpk_gated_ffn_backward: %u x %u is too large", p.m, p.f);
+    const unsigned grid = (unsigned)((vectors + 255) / 256);
     switch (act) {
     case CLPK_ACT_SILU:      return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_SILU>, "gate_gradients", grid, 256, 0, s, p);
     case CLPK_ACT_GELU_TANH: return launch_behind(gate_gradients_kernel<DT, CLPK_ACT_GELU_TANH>, "gate_gradients", grid, 256, 0, s, p);
