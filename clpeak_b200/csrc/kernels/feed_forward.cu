@@ -39,6 +39,8 @@ struct Product {
     uint32_t *status;
 };
 
+constexpr uint32_t kMostRows = 0x7FFFFF00u;         // coordinates of whole tiles are signed 32-bit numbers
+
 static uint64_t elem_bytes(int dtype) { return dtype == CLPK_DT_F32 ? 4 : dtype == CLPK_DT_I8 ? 1 : 2; }
 
 // K blocks of 128 bytes
@@ -66,8 +68,8 @@ static float linear_estimate(float blocks, float tiles, uint32_t tn, uint32_t sp
     return blocks * (0.118f + 0.265f * wide) + tiles * (1.2f * wide + (splits > 1 ? 1.0f + 4.3f * wide : 0.0f));
 }
 
-// Tile width and K ranges: the cheapest by the estimate.  It took the fastest, or one within 2 % of it, for 19 of 23 shapes that
-// were timed with every choice (256 x 4096 x 11008 int8: 18.0 us in two ranges of K with one block per stage, 19.8 as it is).
+// Tile width and K ranges: the cheapest by the estimate.  Of thirteen shapes that were timed with every choice in turn (200 to 8192
+// tokens) it took the fastest for twelve and one 2 % slower for the other.
 static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks)
 {
     const uint32_t cols = form == kGated ? 2 * w.n : w.n;
@@ -146,7 +148,7 @@ static int launch_linear(const Product &w, uint32_t k_blocks, cudaStream_t s)
 template <LinearForm FORM> constexpr uint32_t few_cols = FORM == kGated ? 64 : 128;      // features of a tile
 
 // K ranges of linear_few_kernel: as many as the chip holds CTAs for at once, as long as each has some blocks of K; with long sums
-// also where that loads the SMs more evenly.  Of 160 shapes (1 to 128 tokens) it is 1 % slower than the fastest in the geometric
+// also where that loads the SMs more evenly.  Over 70 shapes of 1 to 64 tokens it is 1 % slower than the fastest in the geometric
 // mean.  What it decides: int8 1 x 4096 x 4096 in one range 9.2 us, in four 5.2; 8 x 30080 x 4096 (235 tiles) 26.7, in two 22.8.
 static uint32_t few_splits(uint32_t tokens, uint32_t tiles, uint32_t k_blocks, uint32_t sms)
 {
@@ -238,12 +240,10 @@ static int run_tokens(const Product &w, cudaStream_t s)
     return launch_linear<DT, FORM>(w, k_blocks, s);
 }
 
-// ---- the backward pass ----------------------------------------------------------------------------------------
-
-// ---- dg = dh * u * act'(g) and du = dh * act(g) -----------------------------------------------------------
+// ---- the backward pass: dg = dh * u * act'(g) and du = dh * act(g) ----------------------------------------
 //
-// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements per step and thread; 8192 x 8192
-// in 96 us, 7.0 TB/s.  The rounding of dg and du to 16 bits is what lets the tensor cores multiply them at full rate: it adds to
+// Five arrays of 16-bit numbers pass by, ten bytes an element: bound by memory.  Eight elements a thread; 8192 x 8192 in 96 us, 7.0
+// TB/s, and 125 behind products that have just written theirs.  The rounding of dg and du to 16 bits is what lets the tensor cores multiply them at full rate: it adds to
 // the gradients an error of the size of their own rounding (bf16 0.0017 -> 0.0023 of the norm).
 // Making them inside the products' launch, by warps that wait for a first tile, was built and measured: in a program that
 // keeps the card at its power limit nothing is gained by overlap (1023 against 988 us at 8192 x 2048 x 8192).
@@ -445,6 +445,14 @@ static GradPlan plan_backward(uint32_t m, uint32_t d, uint32_t f)
     return plan;
 }
 
+// Sizes whose tiles and parts 32 bits can count: 2^25 of dx, and of dWg, are more than any card holds the results of.
+static int check_backward_sizes(uint32_t m, uint32_t d, uint32_t f)
+{
+    const uint64_t cols = ((uint64_t)d + 127) / 128, x = ((uint64_t)m + kLinearM - 1) / kLinearM * cols, w = ((uint64_t)f + kLinearM - 1) / kLinearM * cols;
+    CLPK_REQUIRE(m <= kMostRows && d <= kMostRows / 4 && f <= kMostRows / 4 && x <= 1u << 25 && w <= 1u << 25, "clpk_gated_ffn_backward: %u x %u x %u is too large", m, d, f);
+    return CLPK_OK;
+}
+
 static uint64_t backward_bytes(uint32_t m, uint32_t d, uint32_t f)
 {
     const uint64_t gradients = 2 * (uint64_t)m * gradient_pitch(f) * 2;
@@ -560,12 +568,12 @@ static int check_scales(const char *what, const char *name, const float *scales)
 }
 
 constexpr uint32_t kMostI8 = 131071;                // products of magnitude 2^14 that a 32-bit sum holds
-constexpr uint32_t kMostRows = 0x7FFFFF00u;         // coordinates of whole tiles are signed 32-bit numbers
 
 static int check_sizes(const char *what, uint32_t m, uint32_t n, uint32_t k, uint64_t elem)
 {
     CLPK_REQUIRE(n > 0 && k > 0, "%s: only the number of tokens may be 0 (got %u x %u)", what, n, k);
-    CLPK_REQUIRE(m <= kMostRows && n * elem <= kMostRows && k * elem <= kMostRows, "%s: %u x %u x %u is too large", what, m, n, k);
+    const uint64_t tiles = ((uint64_t)m + kLinearM - 1) / kLinearM * (((uint64_t)n + 31) / 32);           // at most
+    CLPK_REQUIRE(m <= kMostRows && n * elem <= kMostRows && k * elem <= kMostRows && tiles <= 1u << 31, "%s: %u x %u x %u is too large", what, m, n, k);
     return CLPK_OK;
 }
 
@@ -674,6 +682,7 @@ int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, u
     CLPK_REQUIRE(bytes, "bytes is NULL");
     *bytes = 0;
     CLPK_REQUIRE(dtype == CLPK_DT_BF16 || dtype == CLPK_DT_F16, "clpk_gated_ffn_backward: dtype %d is not BF16 or F16", dtype);
+    CLPK_TRY(check_backward_sizes(m, d, f));
     *bytes = (size_t)backward_bytes(m, d, f);
     return CLPK_OK;
 }

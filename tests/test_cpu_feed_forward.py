@@ -51,6 +51,23 @@ def test_workspace_of_the_backward_pass(K, m, d, f, parts):
         K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, d, f, None)
 
 
+@pytest.mark.parametrize("m,d,f", [(2 ** 32 - 1, 64, 64), (64, 2 ** 32 - 1, 64), (64, 64, 2 ** 32 - 1), (2 ** 31 - 256, 2 ** 29 - 64, 8), (8, 2 ** 29 - 64, 2 ** 29 - 64),
+                                   (2 ** 24, 2 ** 17, 8)])
+def test_sizes_that_cannot_be_counted(K, m, d, f):
+    need = C.c_size_t(99)
+    with pytest.raises(N.ClpkError, match="too large") as e:
+        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, d, f, C.byref(need))
+    assert e.value.code == N.ERR_BAD_ARG and need.value == 0
+
+
+@pytest.mark.parametrize("m,d,f", [(2 ** 22, 2 ** 18, 8), (8, 2 ** 18, 2 ** 22), (2 ** 30, 1, 1), (1, 1, 2 ** 28), (1, 2 ** 28, 1), (1, 1, 1)])
+def test_the_largest_sizes_have_a_workspace(K, m, d, f):
+    need = C.c_size_t(0)
+    K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, d, f, C.byref(need))
+    gradients = 2 * m * -(-f // 8) * 8 * 2
+    assert gradients <= need.value < gradients + (1 << 41)
+
+
 def test_no_call_without_a_gpu(K):
     import torch
     if torch.cuda.is_available():

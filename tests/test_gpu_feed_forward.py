@@ -469,7 +469,8 @@ def test_refusals_of_the_scaled_product(K, cuda):
                      ({"d_c": None}, "d_c is NULL"), ({"d_a": at + 1}, "d_a must start on 16"), ({"d_c": c.data_ptr() + 4}, "d_c must start on 16"),
                      ({"lda": 63}, "pitch of d_a"), ({"lda": 65}, "d_a must start"), ({"ldb": 72}, "d_b must start"), ({"ldc": 42}, "d_c must start"),
                      ({"lda": 1 << 36}, "too large"), ({"d_a_scale": None}, "d_a_scale"), ({"d_b_scale": s.data_ptr() + 2}, "d_b_scale"),
-                     ({"d_bias": s.data_ptr() + 2}, "d_bias"), ({"d_status": None}, "d_status"), ({"m": 0xFFFFFFFF}, "too large")]:
+                     ({"d_bias": s.data_ptr() + 2}, "d_bias"), ({"d_status": None}, "d_status"), ({"m": 0xFFFFFFFF}, "too large"),
+                     ({"m": 1 << 30, "n": 1 << 28, "ldc": 1 << 28}, "too large")]:
         refused(K.clpk_gemm_i8_scaled, changed(good, **kw), text)
     refused(K.clpk_gemm_i8_scaled, None, "args is NULL")
 
