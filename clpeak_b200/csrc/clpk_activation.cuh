@@ -4,7 +4,7 @@
 // where the sigmoid it stands in has long been 0 or 1; below |x| = 8 it is under 5e-7.  Quotients are products with rcp.approx (1
 // ulp).  Both flush what is below 2^-126 to 0, which 1 + exp(x) does not see and 1 / (1 + exp(x)) is not missed in; without
 // that each takes three instructions more.  tanh-GELU is a sigmoid too: (1 + tanh y) / 2 = 1 / (1 + exp(-2 y)).
-// An element then takes two special-function results, sixteen cycles of a scheduler, and six other instructions.
+// An element then takes two special-function results, sixteen cycles of a scheduler, and three other instructions (activate2).
 //
 // GELU's normal distribution function is Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x),
 // x >= 0, off by 1.5e-7 at most; in fp32 the function is within 3.0e-7 and GELU within 4.2e-7, which is what erff and its sum with 1
@@ -18,12 +18,16 @@
 
 namespace clpk {
 
-__device__ __forceinline__ float exp_approx(float x)
+constexpr float kLog2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2_approx(float x)
 {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+__device__ __forceinline__ float exp_approx(float x) { return ex2_approx(x * kLog2E); }
 
 __device__ __forceinline__ float rcp_approx(float x)
 {
@@ -34,15 +38,26 @@ __device__ __forceinline__ float rcp_approx(float x)
 
 __device__ __forceinline__ float sigmoid(float x) { return rcp_approx(1.0f + exp_approx(-x)); }
 
+// a NaN stays one
+__device__ __forceinline__ float relu(float g)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(g));
+    return y;
+}
+
 constexpr float kGeluC = 0.7978845608028654f;       // sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
+
+constexpr float kSqrtHalf = 0.7071067811865476f;
+constexpr float kErfP = 0.3275911f, kErf1 = 0.254829592f, kErf2 = -0.284496736f, kErf3 = 1.421413741f, kErf4 = -1.453152027f, kErf5 = 1.061405429f;
 
 // (1 + erf(g / sqrt(2))) / 2, and exp(-g^2 / 2)
 __device__ __forceinline__ float normal_cdf(float g, float &e)
 {
-    const float x = fabsf(g) * 0.7071067811865476f, t = rcp_approx(1.0f + 0.3275911f * x);
+    const float x = fabsf(g) * kSqrtHalf, t = rcp_approx(1.0f + kErfP * x);
     e = exp_approx(-0.5f * g * g);
-    const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float q = 0.5f * e * t * (kErf1 + t * (kErf2 + t * (kErf3 + t * (kErf4 + t * kErf5))));
     return g < 0.0f ? q : 1.0f - q;
 }
 
@@ -58,9 +73,72 @@ __device__ __forceinline__ float activate(float g)
         return g * normal_cdf(g, e);
     }
     else if constexpr (ACT == CLPK_ACT_RELU)
-        return g < 0.0f ? 0.0f : g;                                 // a NaN stays one
+        return relu(g);
     else
         return sigmoid(g);
+}
+
+// Two floats with one instruction.  act(g) of two: sums and products of two take half the issue slots, which the special-function
+// results leave too few of (gated bf16 4096 x 128 x 14336 with GELU 67 -> 63 us, with its tanh form 60 -> 55).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 c;
+    asm("{\n\t"
+        ".reg .b64 a, b;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t"
+        "}\n"
+        : "=f"(c.x), "=f"(c.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    asm("{\n\t"
+        ".reg .b64 a, b, c;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%0, %1};\n\t"
+        "fma.rn.f32x2 c, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, c;\n\t"
+        "}\n"
+        : "+f"(c.x), "+f"(c.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 1 / (1 + 2^y)
+__device__ __forceinline__ float2 sigmoid2_of(float2 y)
+{
+    const float2 d = fma2(make_float2(ex2_approx(y.x), ex2_approx(y.y)), both(1.0f), both(1.0f));
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 activate2(float2 g)
+{
+    if constexpr (ACT == CLPK_ACT_SILU) {
+        return mul2(g, sigmoid2_of(mul2(g, both(-kLog2E))));
+    } else if constexpr (ACT == CLPK_ACT_GELU_TANH) {
+        const float2 cubic = fma2(mul2(g, g), both(kGeluCubic), both(1.0f));
+        return mul2(g, sigmoid2_of(mul2(mul2(g, both(-2.0f * kGeluC * kLog2E)), cubic)));
+    } else if constexpr (ACT == CLPK_ACT_GELU) {
+        const float2 d = fma2(make_float2(fabsf(g.x), fabsf(g.y)), both(kErfP * kSqrtHalf), both(1.0f));
+        const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y)), y = mul2(mul2(g, both(-0.5f * kLog2E)), g);
+        float2 q = fma2(t, both(kErf5), both(kErf4));
+        q = fma2(t, q, both(kErf3));
+        q = fma2(t, q, both(kErf2));
+        q = fma2(t, q, both(kErf1));
+        q = mul2(mul2(q, t), mul2(make_float2(ex2_approx(y.x), ex2_approx(y.y)), both(0.5f)));
+        return mul2(g, make_float2(g.x < 0.0f ? q.x : 1.0f - q.x, g.y < 0.0f ? q.y : 1.0f - q.y));
+    } else if constexpr (ACT == CLPK_ACT_RELU) {
+        return make_float2(relu(g.x), relu(g.y));
+    } else {
+        return sigmoid2_of(mul2(g, both(-kLog2E)));
+    }
 }
 
 // act(g) and act'(g)
@@ -82,7 +160,7 @@ __device__ __forceinline__ void activate_both(float g, float &a, float &da)
         a = g * cdf;
         da = cdf + g * e * 0.3989422804014327f;                     // 1 / sqrt(2 pi)
     } else if constexpr (ACT == CLPK_ACT_RELU) {
-        a = g < 0.0f ? 0.0f : g;
+        a = relu(g);
         da = g > 0.0f ? 1.0f : 0.0f;
     } else {
         const float p = sigmoid(g);

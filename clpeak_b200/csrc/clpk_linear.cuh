@@ -14,8 +14,12 @@
 // library's plain product of that size 800 to 813 in the same minutes, and int8 8192^3 with scales and bias 389 to 393 (2.8
 // POPS) where clpk_gemm's with 32-bit results takes 400.  A K block of a 256 x 256 tile is 512 tensor cycles: 0.28 us while half of
 // the SMs work, 0.39 to 0.44 when all do.  Tiles of 512 rows, which fetch a quarter less, were 5 to 11 % slower in every form:
-// tensor memory then holds one accumulator, and an epilogue with activations is too long to stand exposed.  Short sums: the
-// epilogue, 1 us a unit of 32 x 32 results and warp (gated: two special-function results an element).
+// tensor memory then holds one accumulator, and an epilogue with activations is too long to stand exposed.
+//
+// Short sums: the epilogue and the results' way to memory.  16-bit results of 4096 x 14336 x 256 leave in 35 us, and a memset of them
+// takes 33; gated bf16 4096 x 128 x 14336 43 us with ReLU and 53 with SiLU, of whose two special-function results an element the
+// schedulers' share is 28.  Sixteen warps do it, four on each scheduler, so that one's waits -- for tensor memory, for its box, for
+// shared memory -- lie under the others' work: eight, with two boxes each, issued in a third of the cycles (66 us, ReLU 50).
 #pragma once
 
 enum LinearForm { kGated = 0, kScaled = 1, kGradients = 2 };
@@ -23,10 +27,13 @@ enum LinearForm { kGated = 0, kScaled = 1, kGradients = 2 };
 constexpr int kLinearMaxStages = 12;
 constexpr uint32_t kLinearM = 256;
 constexpr uint32_t kLinearK = 64;                                   // of 16-bit elements: 128 bytes; 128 of the 8-bit ones
-constexpr uint32_t kLinearChunk = 32;                               // columns per tcgen05.ld and per box of C
-constexpr int kLinearThreads = 64 + 32 * kEpilogueWarps;
+constexpr uint32_t kLinearChunk = 32, kLinearPart = 16;             // columns that a warp takes in turn, and at once
+constexpr int kLinearSets = 4, kLinearEpilogueWarps = 4 * kLinearSets;     // a set: a warp for each lane quarter
+constexpr uint32_t kLinearBoxBytes = 2048;                          // 32 rows of 64 bytes
+constexpr int kLinearThreads = 64 + 32 * kLinearEpilogueWarps;
 
 struct LinearSmem {
+    alignas(16) float cols[kLinearEpilogueWarps][32];               // a warp's scales and bias
     uint64_t full[kLinearMaxStages];
     uint64_t empty[kLinearMaxStages];
     uint64_t tmem_full[2];
@@ -39,12 +46,47 @@ struct LinearResult {
     void *base;
     uint64_t ld;
     uint32_t m, n;
-    uint32_t ragged;                                // its rows end inside 16 bytes
+    uint32_t whole;                                 // columns up to the last 16 bytes that a row fills
     int type;                                       // CLPK_DT_*
 };
 
+// n / d for n < 2^31 by the multiplication of Granlund and Montgomery (1994); a division takes some 25 instructions
+struct Divider {
+    uint32_t mul, shift;
+};
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divider &d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
+static Divider divider(uint32_t d)
+{
+    uint32_t shift = 0;
+    while ((1ull << shift) < d)
+        shift++;
+    return {(uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+
+// Tiles are walked in groups of eight columns, M fastest inside a row of a group's.
+constexpr uint32_t kLinearGroup = 8;
+struct TileOrder {
+    uint32_t tiles_m, tiles_n;
+    Divider group, last;                            // by the tiles of a group, and by the columns of the last one where they are fewer
+};
+static TileOrder tile_order(uint32_t tiles_m, uint32_t tiles_n)
+{
+    return {tiles_m, tiles_n, divider(kLinearGroup * tiles_m), divider(std::max(tiles_n % kLinearGroup, 1u))};
+}
+__device__ __forceinline__ void tile_coords(const TileOrder &o, uint32_t tile, uint32_t &mb, uint32_t &nb)
+{
+    const uint32_t g = divide(tile, o.group), within = tile - g * kLinearGroup * o.tiles_m, first_n = g * kLinearGroup, width = o.tiles_n - first_n;
+    if (width >= kLinearGroup) {
+        mb = within / kLinearGroup;
+        nb = first_n + within % kLinearGroup;
+    } else {
+        mb = divide(within, o.last);
+        nb = first_n + within - mb * width;
+    }
+}
+
 struct LinearParams {
-    uint32_t tiles_m, tiles_n, group;
+    TileOrder order;
     uint32_t k_blocks;                              // of 128 bytes
     uint32_t tn, splits, stages, kps, tmem_cols;    // kps: K blocks per stage
     int activation;                                 // CLPK_ACT_*
@@ -68,105 +110,119 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type)
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// 32 columns of one row per lane -> the warp's staging box (rows of 64 or 128 bytes in the swizzle of that width) -> one TMA
-// store, which clips what lies beyond C -- in units of 16 bytes: where a row of C ends inside one, the box that holds its end is
-// written element by element, so that what lies behind the row stays as it is.
-__device__ __forceinline__ void linear_store(const float (&v)[32], const LinearResult &c, uint8_t *boxes, uint32_t &n_stored, const CUtensorMap *map, uint32_t col,
-                                             uint32_t row, int lane)
+// What a warp finishes at a time: `kLinearPart` columns of 32 rows, a row in each lane.
+//
+// A warp's staging is a box of 32 rows of 64 bytes, in the swizzle of that width: two parts of 16-bit results or one of fp32.  (A
+// second box for fp32 gained nothing: 8192 x 8192 x 512 64.0 and 64.6 us.)  TMA stores it and clips what lies beyond C -- in units of 16 bytes: where a row of C ends inside one,
+// the map's rows end before it and each lane writes the rest of its row, so that what lies behind the row stays as it is.
+template <int TYPE>
+__device__ __forceinline__ void fill_box(const float (&v)[kLinearPart], uint8_t *box, uint32_t first, int lane)
 {
-    const bool wide = c.type == CLPK_DT_F32;
-    // 16 bits: two 2 KiB boxes in turn: the one filled now was handed to TMA two stores ago
-    uint8_t *box = wide ? boxes : boxes + (n_stored & 1) * 2048;
-    if (lane == 0) {
-        if (wide)
-            bulk_wait_read<0>();
-        else
-            bulk_wait_read<1>();
-    }
-    __syncwarp();
-    if (wide) {
+    constexpr uint32_t kPieces = TYPE == CLPK_DT_F32 ? 4 : 2;
 #pragma unroll
-        for (uint32_t j = 0; j < 8; j++)
-            *reinterpret_cast<float4 *>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
+    for (uint32_t j = 0; j < kPieces; j++) {
+        uint4 w;
+        if constexpr (TYPE == CLPK_DT_F32) {
+            const float *x = v + 4 * j;
+            w = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+        } else {
             const float *x = v + 8 * j;
-            *reinterpret_cast<uint4 *>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(pack16(x[0], x[1], c.type), pack16(x[2], x[3], c.type), pack16(x[4], x[5], c.type), pack16(x[6], x[7], c.type));
+            w = make_uint4(pack16(x[0], x[1], TYPE), pack16(x[2], x[3], TYPE), pack16(x[4], x[5], TYPE), pack16(x[6], x[7], TYPE));
         }
+        *reinterpret_cast<uint4 *>(box + lane * 64 + (((first + j) ^ ((lane >> 1) & 3)) << 4)) = w;
     }
-    if (c.ragged && col < c.n && c.n - col < kLinearChunk) {
-        __syncwarp();
-        const uint32_t left = c.n - col, j = lane * (wide ? 4 : 2), piece = j >> 4, in_piece = j & 15;
-        const uint32_t rows = c.m > row ? (c.m - row < 32 ? c.m - row : 32) : 0;
-#pragma unroll 8
-        for (uint32_t i = 0; i < rows; i++) {
-            const uint64_t at = (uint64_t)(row + i) * c.ld + col + lane;
-            if (lane < left) {
-                if (wide)
-                    static_cast<float *>(c.base)[at] = *reinterpret_cast<const float *>(box + i * 128 + ((piece ^ (i & 7)) << 4) + in_piece);
-                else
-                    static_cast<uint16_t *>(c.base)[at] = *reinterpret_cast<const uint16_t *>(box + i * 64 + ((piece ^ ((i >> 1) & 3)) << 4) + in_piece);
-            }
-        }
-        __syncwarp();
-        if (lane == 0)
-            bulk_commit();                              // an empty group: the boxes' turns are counted in groups
-    } else {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store_box(const LinearResult &c, const uint8_t *box, const CUtensorMap *map, uint32_t col, uint32_t row, int lane)
+{
+    constexpr uint32_t kElem = TYPE == CLPK_DT_F32 ? 4 : 2, kCols = 64 / kElem;
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        if (col < c.whole)
             tma_store_2d(map, box, (int32_t)col, (int32_t)row);
-            bulk_commit();
-        }
+        bulk_commit();
     }
-    n_stored++;
+    if (c.n != c.whole && c.whole - col < kCols && row + lane < c.m) {
+        uint4 v = *reinterpret_cast<const uint4 *>(box + lane * 64 + (((c.whole - col) * kElem / 16 ^ ((lane >> 1) & 3)) << 4));
+        uint8_t *to = static_cast<uint8_t *>(c.base) + ((uint64_t)(row + lane) * c.ld + c.whole) * kElem;
+        const uint32_t bytes = (c.n - c.whole) * kElem;
+        if (bytes & 8) {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(v.x, v.y);
+            to += 8;
+            v.x = v.z;
+            v.y = v.w;
+        }
+        if (bytes & 4) {
+            *reinterpret_cast<uint32_t *>(to) = v.x;
+            to += 4;
+            v.x = v.y;
+        }
+        if (bytes & 2)
+            *reinterpret_cast<uint16_t *>(to) = (uint16_t)v.x;
+    }
 }
 
 template <int ACT>
-__device__ __forceinline__ void gate32(float (&h)[32], const float (&u)[32])
+__device__ __forceinline__ void gate(float (&h)[kLinearPart], const float (&u)[kLinearPart])
 {
 #pragma unroll
-    for (int i = 0; i < 32; i++)
-        h[i] = activate<ACT>(h[i]) * u[i];
+    for (int i = 0; i < kLinearPart; i += 2) {
+        const float2 v = mul2(activate2<ACT>(make_float2(h[i], h[i + 1])), make_float2(u[i], u[i + 1]));
+        h[i] = v.x;
+        h[i + 1] = v.y;
+    }
 }
 
-__device__ __forceinline__ void gate32_by(int act, float (&h)[32], const float (&u)[32])
+__device__ __forceinline__ void gate_by(int act, float (&h)[kLinearPart], const float (&u)[kLinearPart])
 {
     switch (act) {
-    case CLPK_ACT_SILU:      gate32<CLPK_ACT_SILU>(h, u); break;
-    case CLPK_ACT_GELU_TANH: gate32<CLPK_ACT_GELU_TANH>(h, u); break;
-    case CLPK_ACT_GELU:      gate32<CLPK_ACT_GELU>(h, u); break;
-    case CLPK_ACT_RELU:      gate32<CLPK_ACT_RELU>(h, u); break;
-    default:                 gate32<CLPK_ACT_SIGMOID>(h, u); break;
+    case CLPK_ACT_SILU:      gate<CLPK_ACT_SILU>(h, u); break;
+    case CLPK_ACT_GELU_TANH: gate<CLPK_ACT_GELU_TANH>(h, u); break;
+    case CLPK_ACT_GELU:      gate<CLPK_ACT_GELU>(h, u); break;
+    case CLPK_ACT_RELU:      gate<CLPK_ACT_RELU>(h, u); break;
+    default:                 gate<CLPK_ACT_SIGMOID>(h, u); break;
     }
 }
 
-// the sums of a chunk in fp32; those of 8-bit integers with their scales, of which lane i has that of column i
+// the sums of a part in fp32; those of 8-bit integers with the scale of the lane's row and those of the columns
 template <int DT>
-__device__ __forceinline__ void scaled32(float (&v)[32], const uint32_t (&sum)[32], float row_scale, float col_scale)
+__device__ __forceinline__ void scaled(float (&v)[kLinearPart], const uint32_t (&sum)[kLinearPart], float row_scale, const float *cols)
 {
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-        if constexpr (DT == CLPK_DT_I8)
-            v[i] = (float)(int32_t)sum[i] * row_scale * __shfl_sync(0xffffffffu, col_scale, i);
-        else
-            v[i] = __uint_as_float(sum[i]);
+    for (int i = 0; i < kLinearPart; i += 4) {
+        if constexpr (DT == CLPK_DT_I8) {
+            const float4 c = *reinterpret_cast<const float4 *>(cols + i);
+            const float2 rows = make_float2(row_scale, row_scale);
+            const float2 a = mul2(mul2(make_float2((float)(int32_t)sum[i], (float)(int32_t)sum[i + 1]), rows), make_float2(c.x, c.y));
+            const float2 b = mul2(mul2(make_float2((float)(int32_t)sum[i + 2], (float)(int32_t)sum[i + 3]), rows), make_float2(c.z, c.w));
+            v[i] = a.x; v[i + 1] = a.y; v[i + 2] = b.x; v[i + 3] = b.y;
+        } else {
+            for (int j = i; j < i + 4; j++)
+                v[j] = __uint_as_float(sum[j]);
+        }
     }
 }
 
-__device__ __forceinline__ float bias_at(const void *bias, int type, uint32_t col)
+__device__ __forceinline__ uint32_t bias_bits(const void *bias, int type, uint32_t col)
 {
-    if (type == CLPK_DT_F32)
-        return static_cast<const float *>(bias)[col];
-    return type == CLPK_DT_F16 ? __half2float(static_cast<const __half *>(bias)[col]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(bias)[col]);
+    return type == CLPK_DT_F32 ? static_cast<const uint32_t *>(bias)[col] : static_cast<const uint16_t *>(bias)[col];
 }
 
-// What a unit of 8-bit sums is finished with: the scale of the lane's row, and of column `col` + lane those of the one or two
-// products, or scale and bias.  They are asked for a unit ahead.
+__device__ __forceinline__ float bias_value(uint32_t bits, int type)
+{
+    if (type == CLPK_DT_F32)
+        return __uint_as_float(bits);
+    return type == CLPK_DT_F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+
+// What a chunk's 8-bit sums are finished with: the scale of the lane's row, and of each part a column's of Wg's or B's for the lower
+// half of the lanes and of Wu's, or bias, for the upper.  They are asked for a chunk ahead, and go to the lanes through shared
+// memory: with a shuffle for each column the pipe that shuffles was the bound (bf16 results, 4096 x 14336 x 256 with bias 63 us, so 53).
 struct LinearScales {
-    float row = 1.0f, col0 = 1.0f, col1 = 0.0f;
+    float row = 0.0f;
+    uint32_t col[2] = {};
 
     template <int DT, LinearForm FORM>
     __device__ __forceinline__ void rows(const LinearParams &p, uint32_t row0, int lane)
@@ -178,41 +234,114 @@ struct LinearScales {
     __device__ __forceinline__ void cols(const LinearParams &p, uint32_t first, int lane)
     {
         if constexpr (DT == CLPK_DT_I8) {
-            const uint32_t c = first + lane;
-            const bool there = c < p.c[0].n;
-            col0 = there ? p.b_scale[c] : 0.0f;
-            if constexpr (FORM == kGated)
-                col1 = there ? p.u_scale[c] : 0.0f;
-            else
-                col1 = p.bias && there ? bias_at(p.bias, p.c[0].type, c) : 0.0f;
+#pragma unroll
+            for (uint32_t h = 0; h < 2; h++) {
+                const uint32_t c = first + h * kLinearPart + lane % kLinearPart;
+                col[h] = 0;
+                if (c < p.c[0].n) {
+                    if (lane < kLinearPart)
+                        col[h] = __float_as_uint(p.b_scale[c]);
+                    else if (FORM == kGated)
+                        col[h] = __float_as_uint(p.u_scale[c]);
+                    else if (p.bias)
+                        col[h] = bias_bits(p.bias, p.c[0].type, c);
+                }
+            }
         }
+    }
+    template <LinearForm FORM>
+    __device__ __forceinline__ float value(const LinearParams &p, uint32_t h, int lane) const
+    {
+        const uint32_t bits = h ? col[1] : col[0];
+        return FORM == kGated || lane < kLinearPart ? __uint_as_float(bits) : bias_value(bits, p.c[0].type);
     }
 };
 
-// What becomes of a unit of sums: one chunk of 32 columns, or with kGated the chunk of g and that of u.  `which`: the result
-// that plain sums (kGradients) belong to.
-template <int DT, LinearForm FORM>
-__device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const LinearParams &p, const LinearScales &scales, const uint32_t (&s0)[32],
-                                              const uint32_t (&s1)[32], uint32_t which, uint32_t row, uint32_t col, uint8_t *boxes, uint32_t &n_stored, int lane)
+// a row's part of an exchanged unit, four columns every 2 KiB
+__device__ __forceinline__ void load_part(uint32_t (&v)[kLinearPart], const uint8_t *at)
 {
-    float v[32];
-    scaled32<DT>(v, s0, scales.row, scales.col0);
-    if constexpr (FORM == kGated) {
-        float u[32];
-        scaled32<DT>(u, s1, scales.row, scales.col1);
-        if (p.keep) {
-            linear_store(v, p.c[1], boxes, n_stored, maps + 1, col, row, lane);
-            linear_store(u, p.c[2], boxes, n_stored, maps + 2, col, row, lane);
-        }
-        gate32_by(p.activation, v, u);
-    } else if constexpr (FORM == kScaled) {
-        if (p.bias) {
 #pragma unroll
-            for (int i = 0; i < 32; i++)
-                v[i] += __shfl_sync(0xffffffffu, scales.col1, i);
-        }
+    for (uint32_t g = 0; g < kLinearPart / 4; g++) {
+        const uint4 e = *reinterpret_cast<const uint4 *>(at + g * 2048);
+        v[4 * g] = e.x; v[4 * g + 1] = e.y; v[4 * g + 2] = e.z; v[4 * g + 3] = e.w;
     }
-    linear_store(v, p.c[which], boxes, n_stored, maps + which, col, row, lane);
+}
+
+// what a warp of the epilogue works with
+struct LinearWarp {
+    uint8_t *box;
+    float *cols;                                        // of a part: 32 scales, or scales and bias
+    int lane;
+};
+
+// What becomes of a chunk of sums, or with kGated of that of g and that of u.  fetch(h, s0, s1, last): the sums of a part; `last`:
+// they are not asked for again.  `which`: the result that plain sums (kGradients) belong to.
+template <int DT, LinearForm FORM, int TYPE, typename Fetch>
+__device__ __forceinline__ void linear_finish_as(const CUtensorMap *maps, const LinearParams &p, const LinearScales &scales, uint32_t which, uint32_t row,
+                                                 uint32_t col, const LinearWarp &w, Fetch fetch)
+{
+    // kGated: g and u go out first where they are kept
+    for (uint32_t out = FORM == kGated && DT != CLPK_DT_I8 && p.keep ? 2 : 0;; out--) {
+        const uint32_t to = FORM == kGated ? out : which;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; h++) {
+            uint32_t s0[kLinearPart], s1[kLinearPart];
+            fetch(h, s0, s1, out == 0 && h == 1);
+            if constexpr (DT == CLPK_DT_I8) {
+                w.cols[w.lane] = scales.value<FORM>(p, h, w.lane);       // all lanes have read the last ones: a box's turn lies between
+                __syncwarp();
+            }
+            float v[kLinearPart];
+            scaled<DT>(v, s0, scales.row, w.cols);
+            if constexpr (FORM == kGated) {
+                float u[kLinearPart];
+                scaled<DT>(u, s1, scales.row, w.cols + kLinearPart);
+                if (DT == CLPK_DT_I8 || out == 0) {
+                    gate_by(p.activation, v, u);
+                } else if (out == 2) {
+#pragma unroll
+                    for (int i = 0; i < kLinearPart; i++)
+                        v[i] = u[i];
+                }
+            } else if constexpr (FORM == kScaled) {
+                if (p.bias) {
+#pragma unroll
+                    for (int i = 0; i < kLinearPart; i += 4) {
+                        const float4 c = *reinterpret_cast<const float4 *>(w.cols + kLinearPart + i);
+                        v[i] += c.x; v[i + 1] += c.y; v[i + 2] += c.z; v[i + 3] += c.w;
+                    }
+                }
+            }
+            constexpr bool kWide = TYPE == CLPK_DT_F32;
+            if ((kWide || h == 0) && w.lane == 0)
+                bulk_wait_read<0>();
+            __syncwarp();
+            fill_box<TYPE>(v, w.box, kWide ? 0 : 2 * h, w.lane);
+            if (kWide || h == 1)
+                store_box<TYPE>(p.c[to], w.box, maps + to, kWide ? col + h * kLinearPart : col, row, w.lane);
+        }
+        if (out == 0)
+            break;
+    }
+}
+
+template <int DT, LinearForm FORM, typename Fetch>
+__device__ __forceinline__ void linear_finish(const CUtensorMap *maps, const LinearParams &p, const LinearScales &scales, uint32_t which, uint32_t row, uint32_t col,
+                                              const LinearWarp &w, Fetch fetch)
+{
+    const int type = p.c[which].type;
+    if constexpr (DT != CLPK_DT_I8) {                   // its own type, or fp32 for a part of a gradient's sum
+        if (FORM == kGradients && type == CLPK_DT_F32)
+            linear_finish_as<DT, FORM, CLPK_DT_F32>(maps, p, scales, which, row, col, w, fetch);
+        else
+            linear_finish_as<DT, FORM, DT>(maps, p, scales, which, row, col, w, fetch);
+    } else if (type == CLPK_DT_F32) {
+        linear_finish_as<DT, FORM, CLPK_DT_F32>(maps, p, scales, which, row, col, w, fetch);
+    } else if (type == CLPK_DT_F16) {
+        linear_finish_as<DT, FORM, CLPK_DT_F16>(maps, p, scales, which, row, col, w, fetch);
+    } else {
+        linear_finish_as<DT, FORM, CLPK_DT_BF16>(maps, p, scales, which, row, col, w, fetch);
+    }
 }
 
 // a tile: which result, where in it (rows of 256, and for the result; columns of tn), and which K blocks of it this pair adds
@@ -236,9 +365,9 @@ __device__ __forceinline__ bool linear_tile(const LinearParamsOf<FORM> &p, uint3
         return grad_tile(p, cluster, clusters, i, t);
     } else {
         const uint32_t tile = cluster + i * clusters;
-        if (tile >= p.tiles_m * p.tiles_n)
+        if (tile >= p.order.tiles_m * p.order.tiles_n)
             return false;
-        dense_tile_coords(tile, p.tiles_m, p.tiles_n, p.group, t.mb, t.nb);
+        tile_coords(p.order, tile, t.mb, t.nb);
         t.mb_out = t.mb;
         t.which = 0;
         t.kb0 = split * p.k_blocks / p.splits;
@@ -251,10 +380,18 @@ template <int DT, LinearForm FORM>
 __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_constant__ LinearMapsOf<FORM> maps, const __grid_constant__ LinearParamsOf<FORM> p)
 {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *const smem = smem_raw;
+    // The ring and the scales leave no room to move the base up to 1024 bytes, the swizzle's period; a launch whose memory does not
+    // start there, as it is declared, says so instead of computing.
+    if (smem_u32(smem) % 1024 != 0) {
+        griddep_wait();
+        if (threadIdx.x == 0)
+            *p.status = 0x306u;
+        return;
+    }
     const uint32_t block_bytes = linear_block_bytes(p.tn), stage_bytes = p.kps * block_bytes;
     uint8_t *staging = smem + (size_t)p.stages * stage_bytes;
-    LinearSmem *sh = reinterpret_cast<LinearSmem *>(staging + kEpilogueWarps * kStagingBytes);
+    LinearSmem *sh = reinterpret_cast<LinearSmem *>(staging + kLinearEpilogueWarps * kLinearBoxBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank(), r = rank & 1, leader = rank & ~1u, split = rank >> 1;
@@ -267,7 +404,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         }
         for (int acc = 0; acc < 2; acc++) {
             mbar_init(&sh->tmem_full[acc], 1);
-            mbar_init(&sh->tmem_empty[acc], 2 * kEpilogueWarps);
+            mbar_init(&sh->tmem_empty[acc], 2 * kLinearEpilogueWarps);
         }
         mbar_fence_init();
         if constexpr (FORM != kGradients) {
@@ -288,11 +425,11 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         *p.status = 0u;
     griddep_launch_dependents();
 
-    const uint32_t q = (uint32_t)(warp & 3), half = (uint32_t)(warp - 2) >> 2;     // epilogue warps
+    const uint32_t q = (uint32_t)(warp & 3), set = (uint32_t)(warp - 2) >> 2;      // epilogue warps
     const uint32_t unit_cols = FORM == kGated ? p.tn / 2 : p.tn, units = unit_cols / kLinearChunk;
     constexpr uint32_t kSubs = FORM == kGated ? 2 : 1;                             // chunks per unit, tn / 2 columns apart
-    uint8_t *boxes = staging + (size_t)(warp - 2) * kStagingBytes;
-    uint32_t n_stored = 0;
+    const uint32_t me = warp < 2 ? 0 : warp - 2;
+    const LinearWarp w = {staging + me * kLinearBoxBytes, sh->cols[me], lane};
     LinearTile t;
 
     if (warp == 0) {
@@ -398,18 +535,18 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
             }
         }
     } else if (p.splits == 1) {
-        // ---------------- epilogue, K not split: the two warps of a lane quarter take every other unit ----------------
-        for (uint32_t i = 0; linear_tile<FORM>(p, cluster, clusters, split, i, t); i++) {
-            const uint32_t acc = i & 1, use = i >> 1;
+        // ---------------- epilogue, K not split: the warps of a lane quarter take chunks in turn ----------------
+        auto ask = [&](LinearScales &scales) {                 // for a tile's first chunk
+            scales.template rows<DT, FORM>(p, t.mb_out * kLinearM + r * 128 + q * 32, lane);
+            scales.template cols<DT, FORM>(p, t.nb * unit_cols + set * kLinearChunk, lane);
+        };
+        LinearScales scales;
+        bool more = linear_tile<FORM>(p, cluster, clusters, split, 0, t);
+        if (more)
+            ask(scales);
+        for (uint32_t i = 0; more; i++) {
+            const uint32_t acc = i & 1, use = i >> 1, which = t.which;
             const uint32_t row = t.mb_out * kLinearM + r * 128 + q * 32, col = t.nb * unit_cols;
-            // the two chunks that a step reads are g and u of one unit (kGated), or two units
-            constexpr uint32_t kStep = FORM == kGated ? 2 : 4;
-            LinearScales scales[2];
-            for (int o = 0; o < 2; o++) {
-                scales[o].rows<DT, FORM>(p, row, lane);
-                if (o == 0 || FORM != kGated)
-                    scales[o].cols<DT, FORM>(p, col + (half + 2 * o) * kLinearChunk, lane);
-            }
             if (!warp_wait(&sh->tmem_full[acc], use & 1)) {
                 if (lane == 0)
                     atomicCAS(p.status, 0u, 0x304u);
@@ -423,28 +560,29 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                 if (lane == 0)
                     mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], leader);
             };
-            if (half >= units) {
+            if (set >= units) {
                 release();
+                more = linear_tile<FORM>(p, cluster, clusters, split, i + 1, t);
                 continue;
             }
-            for (uint32_t c = half; c < units; c += kStep) {
-                const bool two = FORM != kGated && c + 2 < units;
-                uint32_t s0[32], s1[32];
-                tmem_ld_32x32b_x32(taddr + c * kLinearChunk, s0);
-                if (FORM == kGated || two)
-                    tmem_ld_32x32b_x32(taddr + (FORM == kGated ? p.tn / 2 + c * kLinearChunk : (c + 2) * kLinearChunk), s1);
-                tmem_ld_wait();
-                if (c + kStep >= units)
-                    release();
-                LinearScales next[2] = {scales[0], scales[1]};
-                if (c + kStep < units)
-                    for (int o = 0; o < (FORM == kGated ? 1 : 2); o++)
-                        next[o].cols<DT, FORM>(p, col + (c + kStep + 2 * o) * kLinearChunk, lane);
-                linear_finish<DT, FORM>(maps.c, p, scales[0], s0, s1, t.which, row, col + c * kLinearChunk, boxes, n_stored, lane);
-                if (two)
-                    linear_finish<DT, FORM>(maps.c, p, scales[1], s1, s1, t.which, row, col + (c + 2) * kLinearChunk, boxes, n_stored, lane);
-                scales[0] = next[0];
-                scales[1] = next[1];
+            for (uint32_t c = set; c < units; c += kLinearSets) {
+                const bool last_chunk = c + kLinearSets >= units;
+                LinearScales next = scales;
+                if (!last_chunk)
+                    next.template cols<DT, FORM>(p, col + (c + kLinearSets) * kLinearChunk, lane);
+                else if ((more = linear_tile<FORM>(p, cluster, clusters, split, i + 1, t)))
+                    ask(next);
+                linear_finish<DT, FORM>(maps.c, p, scales, which, row, col + c * kLinearChunk, w,
+                                        [&](uint32_t h, uint32_t (&s0)[kLinearPart], uint32_t (&s1)[kLinearPart], bool last) {
+                                            const uint32_t at = taddr + c * kLinearChunk + h * kLinearPart;
+                                            tmem_ld_32x32b_x16(at, s0);
+                                            if (FORM == kGated)
+                                                tmem_ld_32x32b_x16(at + p.tn / 2, s1);
+                                            tmem_ld_wait();
+                                            if (last && last_chunk)
+                                                release();
+                                        });
+                scales = next;
             }
         }
     } else if (!warp_wait(&sh->tmem_full[0], 0)) {
@@ -466,7 +604,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         const uint32_t taddr = tmem + ((q * 32) << 16), my_row = q * 32 + lane;
         const bool epilogue = warp >= 2;
         if (epilogue) {
-            for (uint32_t i = half; i < kSubs * units; i += 2) {
+            for (uint32_t i = set; i < kSubs * units; i += kLinearSets) {
                 const uint32_t c = i / kSubs, sub = i % kSubs, owner = c % p.splits;
                 if (owner == split)
                     continue;
@@ -484,39 +622,47 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
         cluster_sync();
         if (epilogue && linear_tile<FORM>(p, cluster, clusters, split, 0, t)) {
             const uint32_t row = t.mb_out * kLinearM + r * 128 + q * 32;
-            for (uint32_t j = half; split + j * p.splits < units; j += 2) {
-                const uint32_t c = split + j * p.splits;
-                LinearScales scales;
-                scales.rows<DT, FORM>(p, row, lane);
-                scales.cols<DT, FORM>(p, t.nb * unit_cols + c * kLinearChunk, lane);
-                uint32_t sum[2][32];
+            // the four warps of a lane quarter share the sums, each of which takes the place of the first of its terms
+            constexpr uint32_t kParts = kLinearChunk / kLinearPart * kSubs;
+#pragma unroll 1
+            for (uint32_t i = set; split + i / kParts * p.splits < units; i += kLinearSets) {
+                const uint32_t j = i / kParts, c = split + j * p.splits, sub = i % kParts / 2, h = i % 2;
+                uint8_t *const slot = smem + (size_t)j * kUnitBytes + sub * (kUnitBytes / kSubs) + h * 8192 + my_row * 16;
+                uint32_t own[kLinearPart], sum[kLinearPart] = {};
+                tmem_ld_32x32b_x16(taddr + sub * (p.tn / 2) + c * kLinearChunk + h * kLinearPart, own);
+                tmem_ld_wait();
+#pragma unroll 1
+                for (uint32_t src = 0; src < p.splits; src++) {
+                    uint32_t theirs[kLinearPart];
+                    if (src != split)
+                        load_part(theirs, slot + (size_t)(src < split ? src : src - 1) * slots * kUnitBytes);
 #pragma unroll
-                for (uint32_t sub = 0; sub < kSubs; sub++) {
-                    uint32_t own[32];
-                    tmem_ld_32x32b_x32(taddr + sub * (p.tn / 2) + c * kLinearChunk, own);
-                    tmem_ld_wait();
-                    for (uint32_t src = 0; src < p.splits; src++) {
-                        const uint8_t *slot = smem + (size_t)((src < split ? src : src - 1) * slots + j) * kUnitBytes + sub * (kUnitBytes / kSubs) + my_row * 16;
-#pragma unroll
-                        for (uint32_t g = 0; g < 8; g++) {
-                            uint4 v = make_uint4(own[4 * g], own[4 * g + 1], own[4 * g + 2], own[4 * g + 3]);
-                            if (src != split)
-                                v = *reinterpret_cast<const uint4 *>(slot + g * 2048);
-                            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (uint32_t l = 0; l < 4; l++) {
-                                uint32_t &x = sum[sub][4 * g + l];
-                                if (src == 0)
-                                    x = e[l];
-                                else if constexpr (DT == CLPK_DT_I8)
-                                    x += e[l];
-                                else
-                                    x = __float_as_uint(__uint_as_float(x) + __uint_as_float(e[l]));
-                            }
-                        }
+                    for (uint32_t l = 0; l < kLinearPart; l++) {
+                        const uint32_t e = src == split ? own[l] : theirs[l];
+                        if (src == 0)
+                            sum[l] = e;
+                        else if constexpr (DT == CLPK_DT_I8)
+                            sum[l] += e;
+                        else
+                            sum[l] = __float_as_uint(__uint_as_float(sum[l]) + __uint_as_float(e));
                     }
                 }
-                linear_finish<DT, FORM>(maps.c, p, scales, sum[0], sum[kSubs - 1], t.which, row, t.nb * unit_cols + c * kLinearChunk, boxes, n_stored, lane);
+#pragma unroll
+                for (uint32_t g = 0; g < kLinearPart / 4; g++)
+                    *reinterpret_cast<uint4 *>(slot + g * 2048) = make_uint4(sum[4 * g], sum[4 * g + 1], sum[4 * g + 2], sum[4 * g + 3]);
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "n"(32 * kLinearSets) : "memory");
+            for (uint32_t j = set; split + j * p.splits < units; j += kLinearSets) {
+                const uint32_t c = split + j * p.splits, col = t.nb * unit_cols + c * kLinearChunk;
+                const uint8_t *const at = smem + (size_t)j * kUnitBytes + my_row * 16;
+                LinearScales scales;
+                scales.rows<DT, FORM>(p, row, lane);
+                scales.cols<DT, FORM>(p, col, lane);
+                linear_finish<DT, FORM>(maps.c, p, scales, t.which, row, col, w, [&](uint32_t h, uint32_t (&s0)[kLinearPart], uint32_t (&s1)[kLinearPart], bool) {
+                    load_part(s0, at + h * 8192);
+                    if (FORM == kGated)
+                        load_part(s1, at + kUnitBytes / 2 + h * 8192);
+                });
             }
         }
     }
@@ -551,7 +697,7 @@ static int make_matrix_map(CUtensorMap *map, const void *base, uint64_t rows, ui
     return CLPK_OK;
 }
 
-// a result, in boxes of 32 x 32
+// a result, in boxes of 32 rows of 64 bytes
 static int make_result_map(CUtensorMap *map, const LinearResult &c)
 {
     EncodeTiledFn enc = nullptr;
@@ -559,10 +705,10 @@ static int make_result_map(CUtensorMap *map, const LinearResult &c)
     if (rc != CLPK_OK)
         return rc;
     const uint32_t elem = c.type == CLPK_DT_F32 ? 4 : 2;
-    const cuuint64_t dims[2] = {c.n, c.m}, strides[1] = {c.ld * elem};
-    const cuuint32_t box[2] = {kLinearChunk, 32}, estr[2] = {1, 1};
+    const cuuint64_t dims[2] = {std::max(c.whole, 16 / elem), c.m}, strides[1] = {c.ld * elem};
+    const cuuint32_t box[2] = {64 / elem, 32}, estr[2] = {1, 1};
     const CUresult r = enc(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c.base, dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, elem == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled (result) failed with CUresult %d", (int)r);

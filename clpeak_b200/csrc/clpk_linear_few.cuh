@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) linear_few_kernel(c
             if constexpr (FORM == kGated)
                 u_scale[i] = i < left ? p.u_scale[col + i] : 0.0f;
             else
-                u_scale[i] = p.bias && i < left ? bias_at(p.bias, p.out, col + i) : 0.0f;
+                u_scale[i] = p.bias && i < left ? bias_value(bias_bits(p.bias, p.out, col + i), p.out) : 0.0f;
         }
         if (threadIdx.x < p.m)
             sh->a_scale[threadIdx.x] = p.a_scale[threadIdx.x];

@@ -28,11 +28,15 @@ struct GradTiles {
     uint32_t tiles, tiles_m, blocks;                        // `blocks`: of K, of all parts together
     uint32_t parts;                                         // that K is cut into; `tiles` counts each
     uint32_t products;                                      // dx, or dWg and dWu
+    // of the launch
+    TileOrder order;
+    Divider by_product, by_parts;                           // by the tiles of a product's part, by the parts
 };
 
 struct GradParams : LinearParams {
     GradTiles first, second;
-    uint32_t share_a, share_b;                              // of the second ones, for clusters below first.tiles % clusters, and for the others
+    uint32_t first_each, first_more;                        // of the first ones: what each cluster has, and how many have one more
+    uint32_t share_a, share_b;                              // of the second ones, for clusters below first_more, and for the others
     uint32_t segment;                                       // K blocks of dx with dg
 };
 
@@ -40,7 +44,7 @@ struct GradParams : LinearParams {
 // part's results lie behind in the workspace.
 __device__ __forceinline__ bool grad_tile(const GradParams &p, uint32_t cluster, uint32_t clusters, uint32_t i, LinearTile &t)
 {
-    const uint32_t have = p.first.tiles > cluster ? (p.first.tiles - cluster - 1) / clusters + 1 : 0;
+    const uint32_t more = p.first_more, have = p.first_each + (cluster < more ? 1 : 0);
     const GradTiles &set = i < have ? p.first : p.second;
     uint32_t tile;
     if (i < have) {
@@ -48,7 +52,7 @@ __device__ __forceinline__ bool grad_tile(const GradParams &p, uint32_t cluster,
     } else {
         // What clusters get that have one of the first ones less comes before what all get, so that from there on all are in step
         // and ask for the same blocks of K together: the other way round the L2 had to fetch them again (3 % at 8192 x 2048 x 8192).
-        const uint32_t more = p.first.tiles % clusters, extra = cluster >= more ? p.share_b - p.share_a : 0, j = i - have;
+        const uint32_t extra = cluster >= more ? p.share_b - p.share_a : 0, j = i - have;
         if (j < extra)
             tile = j * (clusters - more) + cluster - more;
         else if (j < extra + p.share_a)
@@ -58,11 +62,11 @@ __device__ __forceinline__ bool grad_tile(const GradParams &p, uint32_t cluster,
         if (tile >= set.tiles)
             return false;
     }
-    const uint32_t each = set.tiles_m * p.tiles_n, unit = tile / each, part = unit / set.products;
+    const uint32_t each = set.tiles_m * set.order.tiles_n, unit = divide(tile, set.by_product), part = unit >> (set.products - 1);
     t.which = set.products == 1 ? 0 : 1 + unit % 2;
-    t.kb0 = part * set.blocks / set.parts;
-    t.kb1 = (part + 1) * set.blocks / set.parts;
-    dense_tile_coords(tile - unit * each, set.tiles_m, p.tiles_n, p.group, t.mb, t.nb);
+    t.kb0 = divide(part * set.blocks, set.by_parts);
+    t.kb1 = divide((part + 1) * set.blocks, set.by_parts);
+    tile_coords(set.order, tile - unit * each, t.mb, t.nb);
     t.mb_out = part * set.tiles_m + t.mb;
     return true;
 }

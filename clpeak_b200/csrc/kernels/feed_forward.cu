@@ -94,11 +94,10 @@ static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_bloc
 template <int DT, LinearForm FORM, typename Maps, typename Params>
 static int launch_linear_tiles(const Maps &maps, Params &p, LinearPlan plan, uint32_t n_tiles, const char *what, cudaStream_t s)
 {
-    p.group = 8;
     p.tn = plan.tn;
     p.splits = plan.splits;
     const uint32_t clusters = plan.splits > 1 ? n_tiles : std::min(n_tiles, linear_resident(1));
-    constexpr size_t fixed = kEpilogueWarps * kStagingBytes + sizeof(LinearSmem) + 1024;
+    constexpr size_t fixed = kLinearEpilogueWarps * kLinearBoxBytes + sizeof(LinearSmem);
     // two K blocks per stage halve the hand-overs; at tn = 192 and 256 too few stages would be left
     p.kps = plan.tn <= 128 ? 2 : 1;
     const uint32_t stage_bytes = p.kps * linear_block_bytes(plan.tn);
@@ -111,7 +110,7 @@ static int launch_linear_tiles(const Maps &maps, Params &p, LinearPlan plan, uin
 
 static LinearResult linear_result(void *base, uint64_t ld, uint32_t m, uint32_t n, int type)
 {
-    return {base, ld, m, n, n * elem_bytes(type) % 16 != 0 ? 1u : 0u, type};
+    return {base, ld, m, n, n - n % (uint32_t)(16 / elem_bytes(type)), type};
 }
 
 template <int DT, LinearForm FORM>
@@ -132,8 +131,8 @@ static int launch_linear(const Product &w, uint32_t k_blocks, cudaStream_t s)
         }
     if (rc != CLPK_OK)
         return rc;
-    p.tiles_m = ceil_div(w.m, kLinearM);
-    p.tiles_n = ceil_div(w.n, tile_cols);
+    const uint32_t tiles_m = ceil_div(w.m, kLinearM), tiles_n = ceil_div(w.n, tile_cols);
+    p.order = tile_order(tiles_m, tiles_n);
     p.k_blocks = k_blocks;
     p.activation = w.activation;
     p.keep = w.c[1] ? 1 : 0;
@@ -142,7 +141,7 @@ static int launch_linear(const Product &w, uint32_t k_blocks, cudaStream_t s)
     p.u_scale = w.u_scale;
     p.bias = w.bias;
     p.status = w.status;
-    return launch_linear_tiles<DT, FORM>(maps, p, plan, p.tiles_m * p.tiles_n, "linear", s);
+    return launch_linear_tiles<DT, FORM>(maps, p, plan, tiles_m * tiles_n, "linear", s);
 }
 
 template <LinearForm FORM> constexpr uint32_t few_cols = FORM == kGated ? 64 : 128;      // features of a tile
@@ -481,13 +480,20 @@ static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
     if (!a.d_dwg)
         w.tiles = 0;
     GradParams p = {};
-    p.tiles_n = ceil_div(a.d, cut.tn);
     p.segment = ceil_div(a.f, kLinearK);
     p.status = a.d_status;
     p.first = longer(x, w);
     p.second = &longer(x, w) == &x ? w : x;
     const uint32_t n_tiles = x.tiles + w.tiles;
-    share_tiles(p.first, p.second, std::min(n_tiles, linear_resident(1)), p.share_a, p.share_b);
+    const uint32_t clusters = std::min(n_tiles, linear_resident(1)), tiles_n = ceil_div(a.d, cut.tn);
+    share_tiles(p.first, p.second, clusters, p.share_a, p.share_b);
+    p.first_each = p.first.tiles / clusters;
+    p.first_more = p.first.tiles % clusters;
+    for (GradTiles *set : {&p.first, &p.second}) {
+        set->order = tile_order(set->tiles_m, tiles_n);
+        set->by_product = divider(set->tiles_m * tiles_n);
+        set->by_parts = divider(set->parts);
+    }
 
     GradMaps maps = {};
     for (int i = 0; i < 2 && rc == CLPK_OK; i++) {
