@@ -48,10 +48,10 @@ namespace clpk {
 // Launches a kernel with the programmatic-serialisation attribute: its first CTAs take their places under the tail of
 // the kernel before it in the stream.  The kernel must therefore wait (griddep_wait) before it touches memory.
 template <typename... Params, typename... Args>
-int launch_behind(void (*kernel)(Params...), const char *what, unsigned grid, int threads, size_t smem, cudaStream_t s, Args... args)
+int launch_behind(void (*kernel)(Params...), const char *what, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

@@ -59,17 +59,17 @@ static uint32_t linear_resident(uint32_t splits)
     return splits == 1 ? pairs : splits == 2 ? pairs * 33 / 74 : pairs * 15 / 74;
 }
 
-// Microseconds of linear_kernel besides its launch: `blocks` K blocks and `tiles` tiles one after another.  The terms are those of
-// gemm_tiles_kernel (plan_tiles in gemm.cu), whose main loop it is: 0.118 to issue a block, 0.265 for its instructions and its
-// loads at tn = 256, and 1.2 of epilogue; an exchange of partial sums 1 + 4.3.
+// Microseconds of linear_kernel besides its launch: `blocks` K blocks and `tiles` tiles one after another, with an exchange of
+// partial sums where K is split.  Fitted to what 60 shapes of 131 to 8192 tokens took with every width and split, and 73 backward
+// passes with every width and number of parts.
 static float linear_estimate(float blocks, float tiles, uint32_t tn, uint32_t splits)
 {
     const float wide = (float)tn / 256.0f;
-    return blocks * (0.118f + 0.265f * wide) + tiles * (1.2f * wide + (splits > 1 ? 1.0f + 4.3f * wide : 0.0f));
+    return blocks * (0.12f + 0.15f * wide) + tiles * (0.8f + 1.3f * wide + (splits > 1 ? 3.5f + 2.0f * wide : 0.0f));
 }
 
-// Tile width and K ranges: the cheapest by the estimate.  Of thirteen shapes that were timed with every choice in turn (200 to 8192
-// tokens) it took the fastest for twelve and one 2 % slower for the other.
+// Tile width and K ranges: the cheapest by the estimate.  Of those 60 shapes it takes the fastest choice for 53; one is 14 % slower,
+// and the geometric mean 0.6 %.
 static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks)
 {
     const uint32_t cols = form == kGated ? 2 * w.n : w.n;
@@ -333,31 +333,28 @@ struct JoinResult {
 struct JoinParams {
     JoinResult r[3];
     uint32_t cols, cols_all;            // cols_all: a multiple of four
-    uint32_t results;
 };
 
 template <int DT>
-__global__ void __launch_bounds__(256) join_parts_kernel(JoinParams p)
+__global__ void __launch_bounds__(128) join_parts_kernel(JoinParams p)
 {
     griddep_wait();
     griddep_launch_dependents();
+    const JoinResult &r = p.r[blockIdx.y];
     const uint32_t vectors = p.cols_all / 4;
-    for (uint32_t o = 0; o < p.results; o++) {
-        const JoinResult &r = p.r[o];
-        const uint64_t all = (uint64_t)r.rows * vectors, part = (uint64_t)r.rows_all * vectors;
-        for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
-            const float4 *from = reinterpret_cast<const float4 *>(r.parts) + i;
-            float4 sum = *from;
-#pragma unroll 4
-            for (uint32_t k = 1; k < r.n_parts; k++) {
-                const float4 v = from[k * part];
-                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-            }
-            const uint64_t row = i / vectors;
-            const uint32_t col = (uint32_t)(i - row * vectors) * 4;
-            const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-            few_store(r.out, DT, row * r.ld + col, p.cols - col, v);
+    const uint64_t all = (uint64_t)r.rows * vectors, part = (uint64_t)r.rows_all * vectors;
+    for (uint64_t i = (uint64_t)blockIdx.x * 128 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 128) {
+        const float4 *from = reinterpret_cast<const float4 *>(r.parts) + i;
+        float4 sum = *from;
+#pragma unroll 8
+        for (uint32_t k = 1; k < r.n_parts; k++) {
+            const float4 v = from[k * part];
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
+        const uint64_t row = i / vectors;
+        const uint32_t col = (uint32_t)(i - row * vectors) * 4;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        few_store(r.out, DT, row * r.ld + col, p.cols - col, v);
     }
 }
 
@@ -389,7 +386,10 @@ static uint64_t share_tiles(const GradTiles &first, const GradTiles &second, uin
 
 constexpr uint32_t kGradPairs = 74;                         // of a whole B200: the workspace's size may not depend on the card at hand
 
-// How the products of the backward pass are cut: tile width and parts of K, the cheapest by the estimate.
+// How the products of the backward pass are cut: tile width and parts of K, the cheapest by the estimate.  A set of tiles that fills
+// the chip is whole, and so is one of the two (no shape gained more than 1 % by cutting both).  Over 73 shapes that were timed with
+// every choice this is 0.9 % slower than the fastest in the geometric mean, 9 % at most; 4103 x 170 x 3591 takes 71 us in tiles of
+// 128 columns, 58 in tiles of 256 and dx in two parts.
 struct GradPlan {
     uint32_t tn, x_parts, w_parts;
 };
@@ -420,26 +420,25 @@ static GradPlan plan_backward(uint32_t m, uint32_t d, uint32_t f)
     GradPlan plan = {256, 1, 1};
     float best = 1e30f;
     for (uint32_t tn = 128; tn <= 256; tn += 128) {
-        const GradTiles x1 = x_tiles(m, d, f, tn, 1), w1 = w_tiles(m, d, f, tn, 1);
-        // parts that leave each tile what a cluster would do if all shared the work, and ten K blocks at least
-        const uint64_t all = (uint64_t)x1.tiles * tile_blocks(x1) + (uint64_t)w1.tiles * tile_blocks(w1);
-        const uint32_t fair = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(all / kGradPairs, 1u << 20), 10);
-        const uint32_t most = 32, xp = std::min(ceil_div(x1.blocks, fair), most), wp = std::min(ceil_div(w1.blocks, fair), most);
-        for (uint32_t cut = 0; cut < 4; cut++) {
-            if (((cut & 1) && xp == 1) || ((cut & 2) && wp == 1))
-                continue;
-            const GradTiles x = x_tiles(m, d, f, tn, cut & 1 ? xp : 1), w = w_tiles(m, d, f, tn, cut & 2 ? wp : 1);
+        const GradTiles whole[2] = {x_tiles(m, d, f, tn, 1), w_tiles(m, d, f, tn, 1)};
+        const auto look = [&](uint32_t x_parts, uint32_t w_parts) {
+            const GradTiles x = x_tiles(m, d, f, tn, x_parts), w = w_tiles(m, d, f, tn, w_parts);
             const GradTiles &first = longer(x, w), &second = &first == &x ? w : x;
             const uint32_t clusters = std::min(x.tiles + w.tiles, kGradPairs);
             uint32_t a, b;
             float t = linear_estimate((float)share_tiles(first, second, clusters, a, b), (float)ceil_div(x.tiles + w.tiles, clusters), tn, 1);
-            if (cut)                    // a launch, and each part's sums written and read
-                t += 3.0f + (float)(part_bytes(x, d) + part_bytes(w, d)) / 2.5e6f;
+            if (x_parts + w_parts > 2)      // a launch, and each part's sums written and read
+                t += 2.0f + (float)(part_bytes(x, d) + part_bytes(w, d)) / 1.5e6f;
             if (t < best) {
                 best = t;
-                plan = {tn, x.parts, w.parts};
+                plan = {tn, x_parts, w_parts};
             }
-        }
+        };
+        look(1, 1);
+        for (int which = 0; which < 2; which++)
+            for (const uint32_t parts : {2, 3, 4, 6, 8, 12, 16, 24, 32})
+                if (whole[which].tiles < kGradPairs && whole[which].blocks >= 8 * parts)
+                    look(which ? 1 : parts, which ? parts : 1);
     }
     return plan;
 }
@@ -452,17 +451,17 @@ static int check_backward_sizes(uint32_t m, uint32_t d, uint32_t f)
     return CLPK_OK;
 }
 
-static uint64_t backward_bytes(uint32_t m, uint32_t d, uint32_t f)
+static uint64_t backward_bytes(uint32_t m, uint32_t d, uint32_t f, GradPlan &plan)
 {
     const uint64_t gradients = 2 * (uint64_t)m * gradient_pitch(f) * 2;
     if (m == 0 || d == 0 || f == 0)
         return gradients;
-    const GradPlan plan = plan_backward(m, d, f);
+    plan = plan_backward(m, d, f);
     return gradients + part_bytes(x_tiles(m, d, f, plan.tn, plan.x_parts), d) + part_bytes(w_tiles(m, d, f, plan.tn, plan.w_parts), d);
 }
 
 template <int DT>
-static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
+static int run_backward(const clpk_gated_ffn_backward_args_t &a, const GradPlan &cut, cudaStream_t s)
 {
     const uint64_t pitch = gradient_pitch(a.f);
     uint16_t *const dg = static_cast<uint16_t *>(a.d_workspace), *const du = dg + a.m * pitch;
@@ -472,7 +471,6 @@ static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
     if (rc != CLPK_OK)
         return rc;
 
-    const GradPlan cut = plan_backward(a.m, a.d, a.f);
     const LinearPlan plan = {cut.tn, 1};
     GradTiles x = x_tiles(a.m, a.d, a.f, cut.tn, cut.x_parts), w = w_tiles(a.m, a.d, a.f, cut.tn, cut.w_parts);
     if (!a.d_dx)
@@ -509,6 +507,7 @@ static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
     if (rc == CLPK_OK && a.d_dwg)
         rc = make_matrix_map(&maps.x, a.d_x, a.m, (uint64_t)a.d * 2, a.ldx * 2, kLinearK);
     JoinParams join = {};
+    uint32_t results = 0;
     join.cols = a.d;
     join.cols_all = (uint32_t)part_cols(a.d);
     uint64_t joined = 0;                                    // vectors of the largest result
@@ -521,7 +520,7 @@ static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
         const uint64_t ld = i ? a.ldw : a.ldx;
         if (set.parts > 1) {
             p.c[i] = linear_result(parts, join.cols_all, set.parts * rows_all, join.cols_all, CLPK_DT_F32);
-            join.r[join.results++] = {parts, out[i], ld, rows, rows_all, set.parts};
+            join.r[results++] = {parts, out[i], ld, rows, rows_all, set.parts};
             joined = std::max(joined, (uint64_t)rows * join.cols_all / 4);
             parts += (uint64_t)set.parts * rows_all * join.cols_all;
         } else {
@@ -532,10 +531,10 @@ static int run_backward(const clpk_gated_ffn_backward_args_t &a, cudaStream_t s)
     if (rc != CLPK_OK)
         return rc;
     rc = launch_linear_tiles<DT, kGradients>(maps, p, plan, n_tiles, "linear (gradients)", s);
-    if (rc != CLPK_OK || join.results == 0)
+    if (rc != CLPK_OK || results == 0)
         return rc;
-    const unsigned grid = (unsigned)std::min<uint64_t>((joined + 255) / 256, 8u * (uint32_t)num_sms());
-    return launch_behind(join_parts_kernel<DT>, "join_parts", grid, 256, 0, s, join);
+    const unsigned grid = (unsigned)std::min<uint64_t>((joined + 127) / 128, 16u * (uint32_t)num_sms());
+    return launch_behind(join_parts_kernel<DT>, "join_parts", dim3(grid, results), 128, 0, s, join);
 }
 
 // ---- what the calls ask of their arguments ------------------------------------------------------------
@@ -689,7 +688,8 @@ int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, u
     *bytes = 0;
     CLPK_REQUIRE(dtype == CLPK_DT_BF16 || dtype == CLPK_DT_F16, "clpk_gated_ffn_backward: dtype %d is not BF16 or F16", dtype);
     CLPK_TRY(check_backward_sizes(m, d, f));
-    *bytes = (size_t)backward_bytes(m, d, f);
+    GradPlan plan;
+    *bytes = (size_t)backward_bytes(m, d, f, plan);
     return CLPK_OK;
 }
 
@@ -699,8 +699,10 @@ int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *st
     const char *what = "clpk_gated_ffn_backward";
     CLPK_REQUIRE(args, "%s: args is NULL", what);
     clpk_gated_ffn_backward_args_t a = *args;
-    size_t need = 0;
-    CLPK_TRY(clpk_gated_ffn_backward_workspace_bytes(a.dtype, a.m, a.d, a.f, &need));
+    CLPK_REQUIRE(a.dtype == CLPK_DT_BF16 || a.dtype == CLPK_DT_F16, "%s: dtype %d is not BF16 or F16", what, a.dtype);
+    CLPK_TRY(check_backward_sizes(a.m, a.d, a.f));
+    GradPlan cut = {};
+    const size_t need = (size_t)backward_bytes(a.m, a.d, a.f, cut);
     CLPK_REQUIRE(a.activation >= 0 && a.activation < CLPK_ACT_COUNT, "%s: unknown activation %d", what, a.activation);
     CLPK_TRY(check_sizes(what, a.m, a.f, a.d, 4));
     CLPK_TRY(check_status(what, a.d_status));
@@ -730,7 +732,7 @@ int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *st
     if (a.d_dwg)
         CLPK_TRY(check_matrix(what, "d_x", a.d_x, a.d, &a.ldx, a.dtype));
 
-    return a.dtype == CLPK_DT_F16 ? run_backward<CLPK_DT_F16>(a, s) : run_backward<CLPK_DT_BF16>(a, s);
+    return a.dtype == CLPK_DT_F16 ? run_backward<CLPK_DT_F16>(a, cut, s) : run_backward<CLPK_DT_BF16>(a, cut, s);
 }
 
 } // extern "C"
