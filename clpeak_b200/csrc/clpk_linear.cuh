@@ -9,9 +9,9 @@
 //    features, a thread of the epilogue holds both, and h = act(g) * u leaves without g or u having been anywhere.
 //  * kGradients: the products of the backward pass (clpk_linear_grad.cuh).
 //
-// What bounds it.  Long sums: the tensor cores and the card's power limit.  Gated bf16 4096^3 keeps the tensor pipe busy for 94.5 % of
-// the SMs' active cycles, at 1.51 GHz; 8192 x 4096 x 8192 takes 782 to 817 us in a running program (1.34 to 1.41 PFLOPS), the
-// library's plain product of that size 800 to 813 in the same minutes, and int8 8192^3 with scales and bias 389 to 393 (2.8
+// What bounds it.  Long sums: the tensor cores and the card's power limit.  Gated bf16 4096^3 keeps the tensor pipe busy for 94.9 % of
+// the SMs' active cycles, at 1.53 GHz; 8192 x 4096 x 8192 takes 784 to 795 us in a running program (1.38 to 1.40 PFLOPS), the
+// library's plain product of that size 800 to 813 in the same minutes, and int8 8192^3 with scales and bias 383 to 393 (2.8
 // POPS) where clpk_gemm's with 32-bit results takes 400.  A K block of a 256 x 256 tile is 512 tensor cycles: 0.28 us while half of
 // the SMs work, 0.39 to 0.44 when all do.  Tiles of 512 rows, which fetch a quarter less, were 5 to 11 % slower in every form:
 // tensor memory then holds one accumulator, and an epilogue with activations is too long to stand exposed.

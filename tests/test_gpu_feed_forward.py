@@ -25,7 +25,7 @@ SPLIT_SCALED = [(130, 2000, 8), (130, 4096, 1000), (300, 8200, 1400), (130, 8200
 SPLIT_BACKWARD = [(64, 64, 64), (200, 64, 64), (8000, 264, 2816), (4000, 520, 1000), (1000, 2048, 520), (520, 2048, 520), (2000, 64, 64), (100, 64, 1000),
                   (2000, 64, 100), (200, 64, 520), (520, 2048, 200), (2000, 2048, 520), (4000, 2048, 520), (520, 2048, 264), (2000, 2048, 1000),
                   (4000, 520, 4096), (8000, 136, 2816), (4000, 136, 2816),
-                  # sums in parts: of dx, of dW, of both
+                  # sums in parts: of dx, of dW
                   (362, 96, 11829), (147, 654, 7749), (100, 4096, 8192), (9, 1436, 6644), (689, 1, 904), (8000, 96, 200), (16000, 40, 100), (1860, 1, 284),
                   (4653, 1818, 8), (1702, 1, 582), (1235, 3, 781), (3585, 132, 1088)]
 LARGE = [(1, 8192, 14336), (48, 4096, 11008), (2049, 2056, 1032), (4096, 1024, 2816)]
@@ -508,3 +508,27 @@ def test_refusals_of_the_gradients(K, cuda):
     refused(K.clpk_gated_ffn_backward, None, "args is NULL")
     with pytest.raises(N.ClpkError, match="dtype"):
         K.clpk_gated_ffn_backward_workspace_bytes(N.DT_F32, 1, 1, 1, C.byref(C.c_size_t(0)))
+
+
+# ---- choices and row ends that the sizes above do not reach -------------------------------------------------
+
+# a width of 64 columns with K in two and four ranges, 128 and 192 in two, and several tiles a cluster at 192
+@pytest.mark.parametrize("m,d,f", [(4100, 4090, 7), (129, 2559, 7), (4100, 6397, 39), (257, 6397, 1399), (257, 63, 5999)])
+def test_gated_in_every_width(K, cuda, m, d, f):
+    forward(K, "bf16", "silu", m, d, f, pad=m % 2, keep=f < 1000)
+    gated_i8(K, "bf16", m, 2 * d, f)
+
+
+@pytest.mark.parametrize("m,k,n", [(4100, 8190, 7), (129, 5119, 7), (2049, 12799, 263), (257, 12799, 2711), (257, 127, 13999)])
+def test_scaled_product_in_every_width(K, cuda, m, k, n):
+    scaled(K, "f16", m, k, n)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [*range(1, 18), 23, 31, 33, 34, 47, 63, 65, 100, 129, 250])
+def test_rows_that_end_anywhere(K, cuda, out, n):
+    """The last 16 bytes of a row, whole or in part, in each place of a box, with rows that end a tile early."""
+    scaled(K, out, 150, 200, n)
+    if out == "bf16":
+        forward(K, out, "sigmoid", 150, 72, n, pad=n % 2, keep=True)
+        backward(K, out, "relu", 150, n, 40)
