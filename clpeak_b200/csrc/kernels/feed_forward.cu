@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(128) join_parts_kernel(JoinParams p)
     }
 }
 
-// What a tile counts for, in K blocks: a short sum takes as long as the tile before it takes to be stored, 1.5 us (tn = 128) to 2.7.
+// What a tile counts for, in K blocks: a short sum takes as long as the tile before it takes to be stored, 1.5 us (tn = 128) to 2.1.
 static uint32_t tile_blocks(const GradTiles &t) { return t.tiles ? std::max(ceil_div(t.blocks, t.parts), 7u) : 1; }
 
 // The second tiles of the clusters that have one of the first more (a) and of the others (b), so that the longest cluster is about
