@@ -32,6 +32,15 @@ def _wide(rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty(rows, -(-cols // unit) * unit, dtype=dtype, device="cuda")[:, :cols]
 
 
+def _rows(x: torch.Tensor):
+    """x and its pitch as the calls take it.  A stride of 0 is one row for all tokens to torch, and rows one behind another to the
+    calls: rows that share elements are copied.  The stride of a single row says nothing."""
+    m, d = x.shape
+    if m > 1 and x.stride(0) < d:
+        x = x.contiguous()
+    return x, x.stride(0) if m > 1 else d
+
+
 class FeedForward:
     """The layer in bf16 for up to `tokens` tokens.  The down projection is frozen: its transpose is kept beside it, for the
     gradient of h is a product with it.  `d` and `f` are multiples of 8 (rows of 16 bytes, which clpk_gemm asks for)."""
@@ -71,9 +80,10 @@ class FeedForward:
         if m == 0:
             self.x = x
             return self.y[:0]
+        x, ldx = _rows(x)
         self.x = x
         args = N.GatedFfnArgs(dtype=N.DT_BF16, activation=self.activation, m=m, d=self.d, f=self.f, d_x=x.data_ptr(), d_wg=self.wg.data_ptr(),
-                              d_wu=self.wu.data_ptr(), d_h=self.h.data_ptr(), d_g=self.g.data_ptr(), d_u=self.u.data_ptr(), ldx=x.stride(0),
+                              d_wu=self.wu.data_ptr(), d_h=self.h.data_ptr(), d_g=self.g.data_ptr(), d_u=self.u.data_ptr(), ldx=ldx,
                               d_status=self._status(0))
         self.K.clpk_gated_ffn(C.byref(args), _stream())
         self._gemm(self.h[:m], self.wd, self.y, 1)
@@ -89,7 +99,7 @@ class FeedForward:
         if m:
             self._gemm(dy, self.wd_t, self.dh, 2)
         # x's pitch is that of dx as well: a pitch of dx's own where x is a slice
-        if m and x.stride(0) != self.d:
+        if m > 1 and x.stride(0) != self.d:
             x = x.contiguous()
         args = N.GatedFfnBackwardArgs(dtype=N.DT_BF16, activation=self.activation, m=m, d=self.d, f=self.f, d_x=x.data_ptr(), d_wg=self.wg.data_ptr(),
                                       d_wu=self.wu.data_ptr(), d_dh=self.dh.data_ptr(), d_g=self.g.data_ptr(), d_u=self.u.data_ptr(),
@@ -132,9 +142,10 @@ class ServedFeedForward:
         m = x.shape[0]
         if x.dtype != torch.bfloat16 or x.shape[1] != self.d or x.stride(1) != 1 or m > self.tokens:
             raise ValueError(f"x must be bf16 [up to {self.tokens}][{self.d}] with rows of neighbours")
+        x, ldx = _rows(x)
         s, K = _stream(), self.K
         self.gated.m = self.down.m = m
-        K.clpk_quantize_rows_i8(self.xq.data_ptr(), self.xs.data_ptr(), x.data_ptr(), m, self.d, self.xq.stride(0), x.stride(0), N.DT_BF16, s)
+        K.clpk_quantize_rows_i8(self.xq.data_ptr(), self.xs.data_ptr(), x.data_ptr(), m, self.d, self.xq.stride(0), ldx, N.DT_BF16, s)
         K.clpk_gated_ffn(C.byref(self.gated), s)
         K.clpk_quantize_rows_i8(self.hq.data_ptr(), self.hs.data_ptr(), self.h.data_ptr(), m, self.f, self.hq.stride(0), self.h.stride(0), N.DT_BF16, s)
         K.clpk_gemm_i8_scaled(C.byref(self.down), s)

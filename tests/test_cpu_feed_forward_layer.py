@@ -1,0 +1,110 @@
+"""What the feed-forward layer hands to the kernels, and what it refuses, with its tensors in host memory and the calls written down
+instead of made."""
+import ctypes as C
+
+import pytest
+import torch
+
+from clpeak_b200 import feed_forward as ff
+from clpeak_b200 import native as N
+
+
+class HostTorch:
+    """torch, whose "cuda" is host memory."""
+
+    def __getattr__(self, name):
+        made = getattr(torch, name)
+        if name not in ("Generator", "empty", "randn", "zeros"):
+            return made
+        return lambda *args, **kw: made(*args, **{**kw, "device": "cpu" if kw.get("device") == "cuda" else kw.get("device")})
+
+
+class Calls(list):
+    """Calls in place of the kernels: (name, arguments), structures by their fields; "x" is what the call finds as x in 16 bits, as a
+    copy that it reads may be gone after it.  Sizes come from the library itself."""
+
+    def __init__(self, K):
+        self.K = K
+
+    def __getattr__(self, name):
+        if name.endswith("_workspace_bytes"):
+            return getattr(self.K, name)
+
+        def call(*args):
+            args = [{f: getattr(a._obj, f) for f, _ in a._obj._fields_} if isinstance(a, type(C.byref(C.c_int()))) else a for a in args]
+            if isinstance(args[0], dict) and args[0].get("d_x") and args[0]["dtype"] == N.DT_BF16 and args[0]["m"]:
+                args[0]["x"] = rows_at(args[0]["d_x"], args[0]["m"], args[0]["d"], args[0]["ldx"])
+            self.append((name, *args))
+        return call
+
+    def of(self, name):
+        return [args for called, *args in self if called == name]
+
+
+@pytest.fixture
+def calls(K, monkeypatch):
+    made = Calls(K)
+    monkeypatch.setattr(ff, "torch", HostTorch())
+    monkeypatch.setattr(ff, "_stream", lambda *_: 0)
+    monkeypatch.setattr(ff.N, "kernels", lambda: made)
+    return made
+
+
+def values(rows, cols, seed=0):
+    gen = torch.Generator()
+    gen.manual_seed(seed)
+    return torch.randn(rows, cols, generator=gen).to(torch.bfloat16)
+
+
+def rows_at(address, m, d, pitch):
+    """The m rows that a call finds behind an address with a pitch; 0: one behind another."""
+    pitch = pitch or d
+    flat = (C.c_uint16 * ((m - 1) * pitch + d)).from_address(address)
+    return torch.tensor([[flat[r * pitch + c] for c in range(d)] for r in range(m)], dtype=torch.int32)
+
+
+def bits(x):
+    return x.contiguous().view(torch.int16).to(torch.int32) & 0xFFFF
+
+
+# ---- rows that share elements ---------------------------------------------------------------------------------
+
+def shared_rows():
+    """A row for all tokens, a window that moves by eight elements, one row whatever its stride, and rows as they should lie."""
+    row = values(1, 64)
+    return [row.expand(4, 64), torch.as_strided(values(1, 96), (5, 64), (8, 1)), torch.as_strided(values(1, 64), (1, 64), (0, 1)),
+            torch.as_strided(values(1, 64), (1, 64), (3, 1)), values(3, 64), values(3, 200)[:, 8:72]]
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_rows_that_share_elements_reach_the_calls_as_rows(calls, i):
+    """A stride of 0 says the same row again to torch and rows one behind another to the calls: what they read has to be x."""
+    x = shared_rows()[i]
+    m = x.shape[0]
+    layer = ff.FeedForward(64, 128, 8)
+    layer.forward(x)
+    args, = [a[0] for a in calls.of("clpk_gated_ffn")]
+    assert args["ldx"] >= 64 and torch.equal(args["x"], bits(x))
+    layer.backward(values(m, 64))
+    args, = [a[0] for a in calls.of("clpk_gated_ffn_backward")]
+    assert torch.equal(args["x"], bits(x))
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_rows_that_share_elements_reach_the_quantiser_as_rows(calls, i):
+    x, read = shared_rows()[i], []
+    m = x.shape[0]
+
+    class Quantiser:                                            # the copy lives as long as the call
+        def clpk_quantize_rows_i8(self, q, scales, src, rows, cols, ld_q, ld, dtype, stream):
+            assert ld >= cols
+            read.append(bits(x) if cols != 64 else rows_at(src, rows, cols, ld))
+
+        def clpk_gated_ffn(self, args, stream):
+            assert args._obj.m == m
+
+        clpk_gemm_i8_scaled = clpk_gated_ffn
+    served = ff.ServedFeedForward(ff.FeedForward(64, 128, 8))
+    served.K = Quantiser()
+    served.forward(x)
+    assert len(read) == 2 and torch.equal(read[0], bits(x))

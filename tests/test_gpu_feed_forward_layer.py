@@ -96,3 +96,13 @@ def test_what_the_layer_refuses(cuda):
     layer.forward(normal(1, 3, 64))
     with pytest.raises(ValueError, match="dy must be"):
         layer.backward(normal(1, 4, 64))
+
+
+def test_x_may_be_one_row_for_all_tokens(cuda):
+    layer = FeedForward(64, 128, 50)
+    served = ServedFeedForward(layer)
+    for x in (normal(1, 1, 64).expand(37, 64), torch.as_strided(normal(2, 1, 400), (37, 64), (8, 1)), torch.as_strided(normal(3, 1, 64), (1, 64), (0, 1))):
+        rows, dy = torch.empty(x.shape, dtype=x.dtype, device="cuda").copy_(x), normal(4, x.shape[0], 64)
+        got = [layer.forward(x).clone(), served.forward(x).clone(), *(t.clone() for t in layer.backward(dy))]
+        want = [layer.forward(rows), served.forward(rows), *layer.backward(dy)]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
