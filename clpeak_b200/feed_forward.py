@@ -18,8 +18,16 @@ import torch
 from . import native as N
 
 
-def _stream() -> int:
+def _stream(device: torch.device) -> int:
+    """The current stream, which has to be one of the GPU that the layer's tensors lie on."""
+    if torch.cuda.current_device() != device.index:
+        raise ValueError(f"the layer is on {device}, the current device is cuda:{torch.cuda.current_device()}")
     return torch.cuda.current_stream().cuda_stream
+
+
+def _check_device(name: str, t: torch.Tensor, device: torch.device) -> None:
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, as the layer (got {t.device})")
 
 
 def _bytes(n: int) -> torch.Tensor:
@@ -54,6 +62,7 @@ class FeedForward:
         weight = lambda rows, cols: (torch.randn(rows, cols, generator=gen, device="cuda") * cols ** -0.5).to(torch.bfloat16)  # noqa: E731
         self.wg, self.wu, self.wd = weight(f, d), weight(f, d), weight(d, f)
         self.wd_t = self.wd.T.contiguous()
+        self.device = self.wg.device
         # a matrix of h's shape for each: what the forward pass keeps, and the gradient of h
         self.h, self.g, self.u, self.dh = (torch.empty(tokens, f, dtype=torch.bfloat16, device="cuda") for _ in range(4))
         self.y, self.dx = (torch.empty(tokens, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
@@ -71,12 +80,13 @@ class FeedForward:
     def _gemm(self, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, i: int) -> None:
         args = N.GemmArgs(dtype=N.DT_BF16, m=a.shape[0], n=b.shape[0], k=a.shape[1], d_a=a.data_ptr(), d_b=b.data_ptr(), d_c=c.data_ptr(),
                           alpha=1.0, d_status=self._status(i))
-        self.K.clpk_gemm(C.byref(args), _stream())
+        self.K.clpk_gemm(C.byref(args), _stream(self.device))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         m = x.shape[0]
         if x.dtype != torch.bfloat16 or x.shape[1] != self.d or x.stride(1) != 1 or m > self.tokens:
             raise ValueError(f"x must be bf16 [up to {self.tokens}][{self.d}] with rows of neighbours")
+        _check_device("x", x, self.device)
         if m == 0:
             self.x = x
             return self.y[:0]
@@ -85,7 +95,7 @@ class FeedForward:
         args = N.GatedFfnArgs(dtype=N.DT_BF16, activation=self.activation, m=m, d=self.d, f=self.f, d_x=x.data_ptr(), d_wg=self.wg.data_ptr(),
                               d_wu=self.wu.data_ptr(), d_h=self.h.data_ptr(), d_g=self.g.data_ptr(), d_u=self.u.data_ptr(), ldx=ldx,
                               d_status=self._status(0))
-        self.K.clpk_gated_ffn(C.byref(args), _stream())
+        self.K.clpk_gated_ffn(C.byref(args), _stream(self.device))
         self._gemm(self.h[:m], self.wd, self.y, 1)
         return self.y[:m]
 
@@ -96,6 +106,7 @@ class FeedForward:
         x, m = self.x, self.x.shape[0]
         if dy.dtype != torch.bfloat16 or tuple(dy.shape) != (m, self.d) or not dy.is_contiguous():
             raise ValueError(f"dy must be contiguous bf16 [{m}][{self.d}]")
+        _check_device("dy", dy, self.device)
         if m:
             self._gemm(dy, self.wd_t, self.dh, 2)
         # x's pitch is that of dx as well: a pitch of dx's own where x is a slice
@@ -105,7 +116,7 @@ class FeedForward:
                                       d_wu=self.wu.data_ptr(), d_dh=self.dh.data_ptr(), d_g=self.g.data_ptr(), d_u=self.u.data_ptr(),
                                       d_dx=self.dx.data_ptr(), d_dwg=self.dwg.data_ptr(), d_dwu=self.dwu.data_ptr(),
                                       d_workspace=self.workspace.data_ptr(), workspace_bytes=self.workspace.numel(), d_status=self._status(3))
-        self.K.clpk_gated_ffn_backward(C.byref(args), _stream())
+        self.K.clpk_gated_ffn_backward(C.byref(args), _stream(self.device))
         return self.dx[:m], self.dwg, self.dwu
 
     def check(self) -> None:
@@ -119,6 +130,7 @@ class ServedFeedForward:
 
     def __init__(self, layer: FeedForward, tokens: int | None = None):
         self.d, self.f, self.tokens, self.activation, self.K = layer.d, layer.f, tokens or layer.tokens, layer.activation, layer.K
+        self.device = layer.device
         self.weights = {name: self._quantize(getattr(layer, name)) for name in ("wg", "wu", "wd")}
         self.xq, self.hq = _wide(self.tokens, self.d, torch.int8), _wide(self.tokens, self.f, torch.int8)
         self.xs, self.hs = (torch.empty(self.tokens, device="cuda") for _ in range(2))
@@ -135,15 +147,16 @@ class ServedFeedForward:
 
     def _quantize(self, w: torch.Tensor):
         q, scale = _wide(*w.shape, torch.int8), torch.empty(w.shape[0], device="cuda")
-        self.K.clpk_quantize_rows_i8(q.data_ptr(), scale.data_ptr(), w.data_ptr(), *w.shape, q.stride(0), w.stride(0), N.DT_BF16, _stream())
+        self.K.clpk_quantize_rows_i8(q.data_ptr(), scale.data_ptr(), w.data_ptr(), *w.shape, q.stride(0), w.stride(0), N.DT_BF16, _stream(self.device))
         return q, scale
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         m = x.shape[0]
         if x.dtype != torch.bfloat16 or x.shape[1] != self.d or x.stride(1) != 1 or m > self.tokens:
             raise ValueError(f"x must be bf16 [up to {self.tokens}][{self.d}] with rows of neighbours")
+        _check_device("x", x, self.device)
         x, ldx = _rows(x)
-        s, K = _stream(), self.K
+        s, K = _stream(self.device), self.K
         self.gated.m = self.down.m = m
         K.clpk_quantize_rows_i8(self.xq.data_ptr(), self.xs.data_ptr(), x.data_ptr(), m, self.d, self.xq.stride(0), ldx, N.DT_BF16, s)
         K.clpk_gated_ffn(C.byref(self.gated), s)

@@ -108,3 +108,30 @@ def test_rows_that_share_elements_reach_the_quantiser_as_rows(calls, i):
     served.K = Quantiser()
     served.forward(x)
     assert len(read) == 2 and torch.equal(read[0], bits(x))
+
+
+# ---- where x and dy lie ------------------------------------------------------------------------------------------
+
+def test_tensors_elsewhere_are_refused_before_any_call(calls):
+    """"meta" stands for another GPU, or for host memory under a layer on a GPU: a device that is not the layer's."""
+    layer = ff.FeedForward(64, 128, 8)
+    served = ff.ServedFeedForward(layer)
+    calls.clear()
+    for run in (layer.forward, served.forward):
+        for m in (0, 1, 4):
+            with pytest.raises(ValueError, match="x must be on cpu"):
+                run(values(m, 64).to("meta"))
+    layer.forward(values(4, 64))
+    calls.clear()
+    with pytest.raises(ValueError, match="dy must be on cpu"):
+        layer.backward(values(4, 64).to("meta"))
+    assert not calls
+
+
+def test_a_stream_of_another_gpu_is_refused(monkeypatch):
+    """Launches go to the current GPU, which cannot read the layer's tensors if that is another one."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: type("Stream", (), {"cuda_stream": 77}))
+    assert ff._stream(torch.device("cuda", 1)) == 77
+    with pytest.raises(ValueError, match="cuda:0.*cuda:1"):
+        ff._stream(torch.device("cuda", 0))

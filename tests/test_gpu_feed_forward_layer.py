@@ -106,3 +106,13 @@ def test_x_may_be_one_row_for_all_tokens(cuda):
         got = [layer.forward(x).clone(), served.forward(x).clone(), *(t.clone() for t in layer.backward(dy))]
         want = [layer.forward(rows), served.forward(rows), *layer.backward(dy)]
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_host_memory_is_refused(cuda):
+    layer = FeedForward(64, 128, 8)
+    for run in (layer.forward, ServedFeedForward(layer).forward):
+        with pytest.raises(ValueError, match="x must be on cuda:0"):
+            run(normal(1, 4, 64).cpu())
+    layer.forward(normal(1, 4, 64))
+    with pytest.raises(ValueError, match="dy must be on cuda:0"):
+        layer.backward(normal(2, 4, 64).cpu())
