@@ -40,6 +40,12 @@ def _wide(rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty(rows, -(-cols // unit) * unit, dtype=dtype, device="cuda")[:, :cols]
 
 
+def _check_x(x: torch.Tensor, layer) -> None:
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != layer.d or x.stride(1) != 1 or x.shape[0] > layer.tokens:
+        raise ValueError(f"x must be bf16 [up to {layer.tokens}][{layer.d}] with rows of neighbours")
+    _check_device("x", x, layer.device)
+
+
 def _rows(x: torch.Tensor):
     """x and its pitch as the calls take it.  A stride of 0 is one row for all tokens to torch, and rows one behind another to the
     calls: rows that share elements are copied.  The stride of a single row says nothing."""
@@ -83,10 +89,8 @@ class FeedForward:
         self.K.clpk_gemm(C.byref(args), _stream(self.device))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _check_x(x, self)
         m = x.shape[0]
-        if x.dtype != torch.bfloat16 or x.shape[1] != self.d or x.stride(1) != 1 or m > self.tokens:
-            raise ValueError(f"x must be bf16 [up to {self.tokens}][{self.d}] with rows of neighbours")
-        _check_device("x", x, self.device)
         if m == 0:
             self.x = x
             return self.y[:0]
@@ -151,10 +155,8 @@ class ServedFeedForward:
         return q, scale
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _check_x(x, self)
         m = x.shape[0]
-        if x.dtype != torch.bfloat16 or x.shape[1] != self.d or x.stride(1) != 1 or m > self.tokens:
-            raise ValueError(f"x must be bf16 [up to {self.tokens}][{self.d}] with rows of neighbours")
-        _check_device("x", x, self.device)
         x, ldx = _rows(x)
         s, K = _stream(self.device), self.K
         self.gated.m = self.down.m = m

@@ -135,3 +135,16 @@ def test_a_stream_of_another_gpu_is_refused(monkeypatch):
     assert ff._stream(torch.device("cuda", 1)) == 77
     with pytest.raises(ValueError, match="cuda:0.*cuda:1"):
         ff._stream(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 64, 1), (64, 1, 1)), ((4, 64, 3), (64, 1, 256)), ((64,), (1,)), ((), ())])
+def test_x_that_is_no_matrix_is_refused(calls, shape, strides):
+    """One of three dimensions whose second one has the layer's width is not its first slice."""
+    layer = ff.FeedForward(64, 128, 8)
+    served = ff.ServedFeedForward(layer)
+    calls.clear()
+    x = torch.as_strided(values(1, 1024), shape, strides)
+    for run in (layer.forward, served.forward):
+        with pytest.raises(ValueError, match="x must be bf16"):
+            run(x)
+    assert not calls
