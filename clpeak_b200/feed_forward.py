@@ -95,12 +95,13 @@ class FeedForward:
             self.x = x
             return self.y[:0]
         x, ldx = _rows(x)
-        self.x = x
+        self.x = None                                   # until h, g, u and y are of this x
         args = N.GatedFfnArgs(dtype=N.DT_BF16, activation=self.activation, m=m, d=self.d, f=self.f, d_x=x.data_ptr(), d_wg=self.wg.data_ptr(),
                               d_wu=self.wu.data_ptr(), d_h=self.h.data_ptr(), d_g=self.g.data_ptr(), d_u=self.u.data_ptr(), ldx=ldx,
                               d_status=self._status(0))
         self.K.clpk_gated_ffn(C.byref(args), _stream(self.device))
         self._gemm(self.h[:m], self.wd, self.y, 1)
+        self.x = x
         return self.y[:m]
 
     def backward(self, dy: torch.Tensor):

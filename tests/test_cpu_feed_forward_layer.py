@@ -148,3 +148,23 @@ def test_x_that_is_no_matrix_is_refused(calls, shape, strides):
         with pytest.raises(ValueError, match="x must be bf16"):
             run(x)
     assert not calls
+
+
+# ---- a call that fails -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("failing", ["clpk_gated_ffn", "clpk_gemm"])
+def test_no_backward_pass_of_a_forward_pass_that_failed(calls, failing):
+    """The kept g and u are those of an earlier x then, or of this one without a y: gradients would mix the two."""
+    layer = ff.FeedForward(64, 128, 8)
+    layer.forward(values(8, 64))
+
+    def fails(args, stream):
+        raise N.ClpkError(N.ERR_BAD_ARG, "refused", failing)
+    setattr(calls, failing, fails)
+    with pytest.raises(N.ClpkError):
+        layer.forward(values(4, 64))
+    delattr(calls, failing)
+    with pytest.raises(RuntimeError, match="without forward"):
+        layer.backward(values(4, 64))
+    layer.forward(values(4, 64))
+    layer.backward(values(4, 64))
