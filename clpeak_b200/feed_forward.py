@@ -75,13 +75,17 @@ class FeedForward:
         self.dwg, self.dwu = torch.empty_like(self.wg), torch.empty_like(self.wu)
         self.status = torch.zeros(4, dtype=torch.int32, device="cuda")
         self.K = N.kernels()
-        need = C.c_size_t(0)
-        self.K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, tokens, d, f, C.byref(need))
-        self.workspace = _bytes(need.value)
+        # fewer tokens can need more (their sums are cut into more parts); the most is that of a multiple of 64 or of all
+        self.workspace = _bytes(max(self._need(m) for m in (*range(64, tokens, 64), tokens)))
         self.x = None
 
     def _status(self, i: int) -> int:
         return self.status.data_ptr() + 4 * i
+
+    def _need(self, m: int) -> int:
+        need = C.c_size_t(0)
+        self.K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, self.d, self.f, C.byref(need))
+        return need.value
 
     def _gemm(self, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, i: int) -> None:
         args = N.GemmArgs(dtype=N.DT_BF16, m=a.shape[0], n=b.shape[0], k=a.shape[1], d_a=a.data_ptr(), d_b=b.data_ptr(), d_c=c.data_ptr(),

@@ -564,6 +564,9 @@ typedef struct clpk_gated_ffn_backward_args {
     uint32_t     *d_status;
 } clpk_gated_ffn_backward_args_t;
 
+/* For these sizes and no others: fewer tokens can need more, since their sums are cut into more parts.  From one token more than a
+ * multiple of 64 up to the next multiple the need grows with m, so the most for any m up to M is that of M or of a multiple of 64
+ * below it. */
 CLPK_API int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, uint32_t f, size_t *bytes);
 CLPK_API int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *stream);
 

@@ -168,3 +168,30 @@ def test_no_backward_pass_of_a_forward_pass_that_failed(calls, failing):
         layer.backward(values(4, 64))
     layer.forward(values(4, 64))
     layer.backward(values(4, 64))
+
+
+# ---- workspace ---------------------------------------------------------------------------------------------------
+
+def needed(K, m, d, f):
+    need = C.c_size_t(0)
+    K.clpk_gated_ffn_backward_workspace_bytes(N.DT_BF16, m, d, f, C.byref(need))
+    return need.value
+
+
+@pytest.mark.parametrize("d,f,tokens", [(1024, 2816, 1024), (512, 1408, 1024), (2048, 2816, 640), (4096, 4096, 264), (4096, 11008, 512), (136, 264, 300),
+                                        (8, 8, 1), (64, 128, 65), (1024, 2816, 704), (8, 1408, 2000), (2048, 8, 700)])
+def test_the_workspace_does_for_every_number_of_tokens(calls, K, d, f, tokens):
+    """Fewer tokens can need more than all of them: their sums are cut into more parts."""
+    layer = ff.FeedForward(d, f, tokens)
+    layer.x = values(0, d)
+    layer.backward(values(0, d))
+    args, = [a[0] for a in calls.of("clpk_gated_ffn_backward")]
+    most = max(needed(K, m, d, f) for m in range(tokens + 1))
+    assert args["workspace_bytes"] == max(most, 16) and layer.workspace.data_ptr() == args["d_workspace"]
+
+
+@pytest.mark.parametrize("d,f", [(1024, 2816), (4096, 4096), (1, 1), (333, 77), (64, 11008), (2048, 40)])
+def test_the_need_grows_within_64_tokens(K, d, f):
+    """As the header says: up to a number of tokens, the most is that of a multiple of 64 or of the number itself."""
+    need = [needed(K, m, d, f) for m in range(1500)]
+    assert all(need[m] >= need[m - 1] for m in range(1, 1500) if (m - 1) % 64)

@@ -116,3 +116,14 @@ def test_host_memory_is_refused(cuda):
     layer.forward(normal(1, 4, 64))
     with pytest.raises(ValueError, match="dy must be on cuda:0"):
         layer.backward(normal(2, 4, 64).cpu())
+
+
+@pytest.mark.parametrize("m", [513, 600])
+def test_fewer_tokens_that_need_a_larger_workspace(cuda, m):
+    layer = FeedForward(1024, 2816, 1024)
+    x, dy = normal(1, m, 1024), normal(2, m, 1024, 0.1)
+    layer.forward(x)
+    grads = layer.backward(dy)
+    for got, want, what in zip(grads, F.backward64("silu", x, layer.wg, layer.wu, layer.dh[:m], layer.g[:m], layer.u[:m], "bf16"), ("dx", "dwg", "dwu")):
+        F.check(got, *want, what)
+    layer.check()
