@@ -46,6 +46,11 @@ def _check_x(x: torch.Tensor, layer) -> None:
     _check_device("x", x, layer.device)
 
 
+def _check_status(status: torch.Tensor, what: str) -> None:
+    if status.any():
+        raise N.ClpkError(N.ERR_TIMEOUT, f"status words {status.tolist()}", what)
+
+
 def _rows(x: torch.Tensor):
     """x and its pitch as the calls take it.  A stride of 0 is one row for all tokens to torch, and rows one behind another to the
     calls: rows that share elements are copied.  The stride of a single row says nothing."""
@@ -129,9 +134,9 @@ class FeedForward:
         return self.dx[:m], self.dwg, self.dwu
 
     def check(self) -> None:
-        """Raises if a device-side wait of an earlier call expired.  Waits for the stream."""
-        if self.status.any():
-            raise N.ClpkError(N.ERR_TIMEOUT, f"status words {self.status.tolist()}", "feed-forward layer")
+        """Raises if a device-side wait expired in the last forward or backward pass, whose results are wrong then.  Waits for the
+        stream."""
+        _check_status(self.status, "feed-forward layer")
 
 
 class ServedFeedForward:
@@ -170,6 +175,10 @@ class ServedFeedForward:
         K.clpk_quantize_rows_i8(self.hq.data_ptr(), self.hs.data_ptr(), self.h.data_ptr(), m, self.f, self.hq.stride(0), self.h.stride(0), N.DT_BF16, s)
         K.clpk_gemm_i8_scaled(C.byref(self.down), s)
         return self.y[:m]
+
+    def check(self) -> None:
+        """Raises if a device-side wait expired in the last pass, whose results are wrong then.  Waits for the stream."""
+        _check_status(self.status, "feed-forward layer in 8 bits")
 
 
 def fit(layer: FeedForward, target: FeedForward, steps: int, rate: float, seed: int = 1) -> list[float]:
@@ -210,6 +219,7 @@ def main() -> None:
             served.forward(x[:m])
         end.record()
         end.synchronize()
+        served.check()
         print(f"served in 8 bits, {m} tokens: {float(off):.4f} off the layer in bf16, {begin.elapsed_time(end) / 50 * 1e3:.1f} us a call")
 
 

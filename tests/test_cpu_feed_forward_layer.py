@@ -195,3 +195,17 @@ def test_the_need_grows_within_64_tokens(K, d, f):
     """As the header says: up to a number of tokens, the most is that of a multiple of 64 or of the number itself."""
     need = [needed(K, m, d, f) for m in range(1500)]
     assert all(need[m] >= need[m - 1] for m in range(1, 1500) if (m - 1) % 64)
+
+
+# ---- waits that ran out --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("word", range(4))
+def test_a_wait_that_ran_out_is_told(calls, word):
+    layer = ff.FeedForward(64, 128, 8)
+    for checked in (layer, ff.ServedFeedForward(layer)):
+        checked.check()
+        if word < checked.status.numel():
+            checked.status[word] = 0x303
+            with pytest.raises(N.ClpkError) as e:
+                checked.check()
+            assert e.value.code == N.ERR_TIMEOUT and str(0x303) in str(e.value)
