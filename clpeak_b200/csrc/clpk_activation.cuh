@@ -46,6 +46,15 @@ __device__ __forceinline__ float relu(float g)
     return y;
 }
 
+// g in [-most, most]; a NaN stays one
+__device__ __forceinline__ float clamped(float g, float most)
+{
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(g), "f"(most));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(y), "f"(-most));
+    return y;
+}
+
 constexpr float kGeluC = 0.7978845608028654f;       // sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
 
@@ -141,7 +150,7 @@ __device__ __forceinline__ float2 activate2(float2 g)
     }
 }
 
-// act(g) and act'(g)
+// act(g) and act'(g).  Both are NaN where g is one: dWg says so too then, and not only dx and dWu.
 template <int ACT>
 __device__ __forceinline__ void activate_both(float g, float &a, float &da)
 {
@@ -150,7 +159,7 @@ __device__ __forceinline__ void activate_both(float g, float &a, float &da)
         a = g * p;
         da = p * (1.0f + g * (1.0f - p));
     } else if constexpr (ACT == CLPK_ACT_GELU_TANH) {
-        const float c = fminf(fmaxf(g, -30.0f), 30.0f);             // beyond, p is 0 or 1 and the second term 0, whatever its factors
+        const float c = clamped(g, 30.0f);                          // beyond, p is 0 or 1 and the second term 0, whatever its factors
         const float p = sigmoid(2.0f * kGeluC * c * (1.0f + kGeluCubic * c * c));
         a = g * p;
         da = p + c * p * (1.0f - p) * (2.0f * kGeluC) * (1.0f + 3.0f * kGeluCubic * c * c);
@@ -161,7 +170,7 @@ __device__ __forceinline__ void activate_both(float g, float &a, float &da)
         da = cdf + g * e * 0.3989422804014327f;                     // 1 / sqrt(2 pi)
     } else if constexpr (ACT == CLPK_ACT_RELU) {
         a = relu(g);
-        da = g > 0.0f ? 1.0f : 0.0f;
+        da = g > 0.0f ? 1.0f : a;                                   // a: 0 or NaN
     } else {
         const float p = sigmoid(g);
         a = p;

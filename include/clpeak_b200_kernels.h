@@ -547,7 +547,7 @@ CLPK_API int clpk_gated_ffn(const clpk_gated_ffn_args_t *args, void *stream);
  *   dg = dh * u * act'(g),  du = dh * act(g)      in fp32, rounded to `dtype` (the workspace holds them)
  *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x      sums in fp32, rounded once
  * d_dx may be NULL, and so may d_dwg and d_dwu (both or neither): what is not asked for is not computed.  Sums are formed
- * in the same order in every call. */
+ * in the same order in every call.  A NaN in g makes act(g) and act'(g) NaN, whatever the activation. */
 typedef struct clpk_gated_ffn_backward_args {
     int           dtype;
     int           activation;

@@ -532,3 +532,45 @@ def test_rows_that_end_anywhere(K, cuda, out, n):
     if out == "bf16":
         forward(K, out, "sigmoid", 150, 72, n, pad=n % 2, keep=True)
         backward(K, out, "relu", 150, n, 40)
+
+
+# ---- gradients that are not finite --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("act", sorted(F.ACTS))
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,d,f", [(9, 33, 40), (300, 520, 1032), (100, 64, 1000)])
+def test_a_nan_stays_one_through_the_backward_pass(K, cuda, act, dtype, m, d, f):
+    """A NaN in g, u or dh of one token and feature: dg and du of it are NaN as far as they depend on it, and with them the token's row
+    of dx and the feature's row of dWg or dWu; everything else is finite."""
+    for bad, to_dg, to_du in (("g", True, True), ("u", True, False), ("dh", True, True)):
+        x = F.filled(normal(1, m, d), dtype)
+        wg, wu = (F.filled(normal(s, f, d, d ** -0.5), dtype) for s in (2, 3))
+        kept = {"dh": normal(4, m, f, 0.1), "g": normal(5, m, f), "u": normal(6, m, f)}
+        kept[bad][3, 7] = float("nan")
+        kept = {n: F.filled(t, dtype) for n, t in kept.items()}
+        dx, dwg, dwu = (F.matrix(rows, d, dtype) for rows in (m, f, f))
+        ws, status = F.workspace(K, dtype, m, d, f), F.word()
+        K.clpk_gated_ffn_backward(C.byref(F.backward_args(dtype, act, x, wg, wu, kept["dh"], kept["g"], kept["u"], dx, dwg, dwu, ws, status)), F.stream())
+        for got, row, nan in ((dx, 3, True), (dwg, 7, to_dg), (dwu, 7, to_du)):
+            want = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+            want[row] = nan
+            assert torch.equal(torch.isnan(got), want) and torch.equal(~torch.isfinite(got), want), (bad, row)
+        assert status.item() == 0
+
+
+@pytest.mark.parametrize("act", sorted(F.ACTS))
+def test_gates_far_from_zero(K, cuda, act):
+    """Where an activation is its argument, or nothing, so is its derivative 1 or 0, up to the largest numbers of the type."""
+    m, d, f = 8, 16, 24
+    x, w = F.filled(normal(1, m, d), "bf16"), F.filled(normal(2, f, d, 0.25), "bf16")
+    size = torch.tensor([40.0, 100.0, 1e4, 1e10, 1e19, 1e25, 1e30, 3e38], device="cuda")[:, None]
+    sign = torch.where(torch.arange(f, device="cuda") % 2 == 0, 1.0, -1.0)
+    g, u, dh = F.filled(size * sign, "bf16"), F.filled(torch.full((m, f), 0.5, device="cuda"), "bf16"), F.filled(torch.full((m, f), 2.0 ** -130, device="cuda"), "bf16")
+    dx, dwg, dwu = F.matrix(m, d, "bf16"), F.matrix(f, d, "bf16"), F.matrix(f, d, "bf16")
+    ws, status = F.workspace(K, "bf16", m, d, f), F.word()
+    K.clpk_gated_ffn_backward(C.byref(F.backward_args("bf16", act, x, w, w, dh, g, u, dx, dwg, dwu, ws, status)), F.stream())
+    for t in (dx, dwg, dwu):
+        assert bool(torch.isfinite(t).all())
+    if act != "sigmoid":                                        # there a is 1 or 0 and its derivative 0
+        assert not dwg[1::2].any() and not dwu[1::2].any()
+    assert status.item() == 0
