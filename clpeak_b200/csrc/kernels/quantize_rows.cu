@@ -202,13 +202,17 @@ static int launch_rows(const RowParams &p, uint64_t vectors, cudaStream_t s)
         return launch_behind(quantize_rows_kernel<DT, THREADS, 1>, "quantize_rows", grid, threads, 0, s, p);
     if (each <= 2)
         return launch_behind(quantize_rows_kernel<DT, THREADS, 2>, "quantize_rows", grid, threads, 0, s, p);
-    if (each <= 4)
+    if constexpr (THREADS == 32) {                      // four at most, see quantize_rows
         return launch_behind(quantize_rows_kernel<DT, THREADS, 4>, "quantize_rows", grid, threads, 0, s, p);
-    if (each <= 8)
-        return launch_behind(quantize_rows_kernel<DT, THREADS, 8>, "quantize_rows", grid, threads, 0, s, p);
-    if (each <= 12)
-        return launch_behind(quantize_rows_kernel<DT, THREADS, 12>, "quantize_rows", grid, threads, 0, s, p);
-    return launch_behind(quantize_rows_kernel<DT, THREADS, 16>, "quantize_rows", grid, threads, 0, s, p);
+    } else {
+        if (each <= 4)
+            return launch_behind(quantize_rows_kernel<DT, THREADS, 4>, "quantize_rows", grid, threads, 0, s, p);
+        if (each <= 8)
+            return launch_behind(quantize_rows_kernel<DT, THREADS, 8>, "quantize_rows", grid, threads, 0, s, p);
+        if (each <= 12)
+            return launch_behind(quantize_rows_kernel<DT, THREADS, 12>, "quantize_rows", grid, threads, 0, s, p);
+        return launch_behind(quantize_rows_kernel<DT, THREADS, 16>, "quantize_rows", grid, threads, 0, s, p);
+    }
 }
 
 template <int DT>
