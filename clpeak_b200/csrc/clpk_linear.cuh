@@ -24,7 +24,7 @@
 
 enum LinearForm { kGated = 0, kScaled = 1, kGradients = 2 };
 
-constexpr int kLinearMaxStages = 12;
+constexpr uint32_t kLinearMaxStages = 6;                            // of the widths there are, see linear_stages
 constexpr uint32_t kLinearM = 256;
 constexpr uint32_t kLinearK = 64;                                   // of 16-bit elements: 128 bytes; 128 of the 8-bit ones
 constexpr uint32_t kLinearChunk = 32, kLinearPart = 16;             // columns that a warp takes in turn, and at once
@@ -99,6 +99,15 @@ struct LinearParams {
 
 // bytes of one K block in a CTA: its 128 rows of A and its half of the tile's columns of B
 __host__ __device__ constexpr uint32_t linear_block_bytes(uint32_t tn) { return kHalfTileBytes + tn / 2 * kRowBytesK; }
+
+// two K blocks per stage halve the hand-overs; at tn = 192 and 256 too few stages would be left
+constexpr uint32_t linear_kps(uint32_t tn) { return tn <= 128 ? 2 : 1; }
+
+// what a CTA has besides its ring, and the stages that fit beside it
+constexpr uint32_t kLinearFixedBytes = kLinearEpilogueWarps * kLinearBoxBytes + (uint32_t)sizeof(LinearSmem);
+constexpr uint32_t linear_stages(uint32_t tn) { return (kSmemMax - kLinearFixedBytes) / (linear_kps(tn) * linear_block_bytes(tn)); }
+static_assert(linear_stages(64) == 4 && linear_stages(128) == 4 && linear_stages(192) == kLinearMaxStages && linear_stages(256) == 6,
+              "the barriers are as many as the stages of the width that has most");
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, int type)
 {

@@ -97,15 +97,12 @@ static int launch_linear_tiles(const Maps &maps, Params &p, LinearPlan plan, uin
     p.tn = plan.tn;
     p.splits = plan.splits;
     const uint32_t clusters = plan.splits > 1 ? n_tiles : std::min(n_tiles, linear_resident(1));
-    constexpr size_t fixed = kLinearEpilogueWarps * kLinearBoxBytes + sizeof(LinearSmem);
-    // two K blocks per stage halve the hand-overs; at tn = 192 and 256 too few stages would be left
-    p.kps = plan.tn <= 128 ? 2 : 1;
-    const uint32_t stage_bytes = p.kps * linear_block_bytes(plan.tn);
-    p.stages = std::min<uint32_t>((uint32_t)((kSmemMax - fixed) / stage_bytes), kLinearMaxStages);
+    p.kps = linear_kps(plan.tn);
+    p.stages = linear_stages(plan.tn);
     p.tmem_cols = 32;
     while (p.tmem_cols < (n_tiles > clusters ? 2 : 1) * plan.tn)
         p.tmem_cols *= 2;
-    return launch_clusters(linear_kernel<DT, FORM>, what, clusters * 2 * plan.splits, kLinearThreads, p.stages * stage_bytes + fixed, 2 * plan.splits, s, maps, p);
+    return launch_clusters(linear_kernel<DT, FORM>, what, clusters * 2 * plan.splits, kLinearThreads, p.stages * p.kps * linear_block_bytes(plan.tn) + kLinearFixedBytes, 2 * plan.splits, s, maps, p);
 }
 
 static LinearResult linear_result(void *base, uint64_t ld, uint32_t m, uint32_t n, int type)
