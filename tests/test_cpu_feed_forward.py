@@ -1,5 +1,6 @@
 """What of the feed-forward operators can be told without a GPU: their structures, workspace sizes, and that calls without one fail."""
 import ctypes as C
+import random
 import re
 import subprocess
 from pathlib import Path
@@ -91,3 +92,30 @@ def test_the_same_answer_as_through_ctypes(K, name, struct):
     for args in [(C.byref(struct()), 0), (C.byref(struct()), None), (C.byref(array[1]), 0), (C.byref(array), 0), (struct(), 0), (None, 0), (C.byref(N.GemmArgs()), 0),
                  (C.byref(C.c_int()), 0), (C.byref(struct()),), (0, 0), (C.byref(array[0], C.sizeof(struct)), 0), (C.byref(struct()), -1)]:
         assert outcome(getattr(K, name), args) == outcome(lambda *a: K.call(name, *a), args)
+
+
+def parts_that_may_be(m, d, f):
+    """Bytes of fp32 results that the products of the backward pass may be cut into: one of dx and dW, in tiles of 128 or 256 columns,
+    where the tiles are fewer than the 74 pairs of the chip and a part has eight blocks of 64 at least."""
+    up = lambda a, b: -(-a // b)                                    # noqa: E731
+    legal = {0}
+    for columns in (128, 256):
+        for rows, blocks, products in ((m, 2 * up(f, 64), 1), (f, up(m, 64), 2)):
+            if products * up(rows, 256) * up(d, columns) < 74:
+                legal |= {products * parts * up(rows, 256) * 256 * up(d, 4) * 4 * 4 for parts in (2, 3, 4, 6, 8, 12, 16, 24, 32) if blocks >= 8 * parts}
+    return legal
+
+
+def test_every_workspace_is_what_its_parts_take(K):
+    rng = random.Random(3)
+    size = lambda most: round(most ** rng.random())                 # noqa: E731: even over its logarithm
+    cases = [(size(1 << 22), size(1 << 14), size(1 << 16)) for _ in range(4000)]
+    cases += [(2 ** 22, 2 ** 18, 8), (8, 2 ** 18, 2 ** 22), (2 ** 30, 1, 1), (1, 1, 2 ** 28), (1, 2 ** 28, 1), (1, 1, 1)]
+    cut = 0
+    for m, d, f in cases:
+        need = C.c_size_t(0)
+        K.clpk_gated_ffn_backward_workspace_bytes(N.DT_F16, m, d, f, C.byref(need))
+        parts = need.value - 2 * m * -(-f // 8) * 8 * 2
+        assert parts in parts_that_may_be(m, d, f), (m, d, f, parts)
+        cut += parts > 0
+    assert cut > 200
