@@ -174,25 +174,18 @@ static bool few_tokens(uint32_t tokens, uint32_t tiles, uint32_t k_blocks, uint3
     return tokens <= 128 && k_blocks >= 20 && few_splits(tokens, tiles, k_blocks, sms) >= 4;
 }
 
-template <int DT, LinearForm FORM>
-static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
+// How linear_few_kernel is launched: K ranges, the ring, and where the partial sums lie.
+static void plan_few(FewParams &p, uint32_t tiles, uint32_t sms)
 {
-    constexpr uint32_t tile_cols = few_cols<FORM>;
-    const uint64_t elem = elem_bytes(DT);
-    FewParams p = {};
-    p.m = w.m;
-    p.n = w.n;
-    p.k_blocks = k_blocks;
-    p.tokens = (w.m + 15) / 16 * 16;
+    p.tokens = (p.m + 15) / 16 * 16;
     p.tmem_cols = 32;
     while (p.tmem_cols < p.tokens)
         p.tmem_cols *= 2;
-    const uint32_t tiles = ceil_div(w.n, tile_cols), sms = (uint32_t)num_sms();
-    p.splits = few_splits(w.m, tiles, k_blocks, sms);
+    p.splits = few_splits(p.m, tiles, p.k_blocks, sms);
     // as many CTAs as an SM gets share its memory; a ring has two stages at least, and is as large as the sums
     const uint32_t stage_bytes = kHalfTileBytes + p.tokens * kRowBytesK, sums = p.splits * ((p.m + p.splits - 1) / p.splits) * kFewRows * 4;
     uint32_t each = std::min((tiles * p.splits - 1) / sms + 1, (uint32_t)kFewResident), budget = 0;
-    if ((each == 2 || (each == 1 && k_blocks < 32 * p.splits)) && 227 * 1024 / (each + 1) >= 3 * stage_bytes + 4096)
+    if ((each == 2 || (each == 1 && p.k_blocks < 32 * p.splits)) && 227 * 1024 / (each + 1) >= 3 * stage_bytes + 4096)
         each++;
     for (;; each--) {
         budget = 227 * 1024 / each - 1024 - 1024 - (uint32_t)sizeof(FewSmem);
@@ -206,6 +199,19 @@ static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
         p.sums_at = p.stages * stage_bytes;
     }
     p.smem_bytes = p.sums_at ? p.sums_at + sums : std::max(p.stages * stage_bytes, std::max(sums, p.tokens * kFewRows * 4));
+}
+
+template <int DT, LinearForm FORM>
+static int launch_few(const Product &w, uint32_t k_blocks, cudaStream_t s)
+{
+    constexpr uint32_t tile_cols = few_cols<FORM>;
+    const uint64_t elem = elem_bytes(DT);
+    FewParams p = {};
+    p.m = w.m;
+    p.n = w.n;
+    p.k_blocks = k_blocks;
+    const uint32_t tiles = ceil_div(w.n, tile_cols);
+    plan_few(p, tiles, (uint32_t)num_sms());
     p.out = w.out;
     p.activation = w.activation;
     p.c = w.c[0];

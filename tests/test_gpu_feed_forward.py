@@ -574,3 +574,28 @@ def test_gates_far_from_zero(K, cuda, act):
     if act != "sigmoid":                                        # there a is 1 or 0 and its derivative 0
         assert not dwg[1::2].any() and not dwu[1::2].any()
     assert status.item() == 0
+
+
+# ---- the choices that the lists above leave out (tests/test_cpu_feed_forward_plans.py says which there are) ---------------
+
+PAIRS_GATED, PAIRS_GATED_8 = [(9804, 2, 138), (99, 3, 4743)], [(9616, 3, 130), (100, 3, 4761)]
+PAIRS_SCALED = [(9675, 2, 266)]
+# every number of parts of dx and of dW in tiles of 128 and of 256 columns, with the longer sum in either
+PARTS_BACKWARD = [(6083, 2, 196), (8137, 2, 196), (1345, 2, 1), (12939, 2, 258), (1475, 2, 1), (16341, 2, 1), (1998, 3, 193), (3017, 2, 1), (3091, 2, 197),
+                  (4045, 2, 1), (4167, 2, 193), (519, 2, 3059), (2, 2, 3015), (1076, 2, 5637), (792, 2, 722), (2, 2, 642), (590, 3, 6430), (2, 2, 6249),
+                  (2, 2, 12806), (516, 2, 982), (517, 2, 1491), (2, 2, 1489), (516, 3, 1988), (2, 2, 1986), (6663, 129, 1), (6608, 134, 207), (8660, 133, 1),
+                  (8965, 142, 193), (4657, 1289, 1), (5477, 132, 1360), (2635, 777, 1), (3900, 279, 604), (2765, 522, 1), (4952, 145, 593), (3437, 398, 1),
+                  (3356, 385, 220), (4807, 270, 1), (5453, 145, 261), (523, 139, 3369), (2, 129, 3746), (2, 130, 4117), (2, 132, 6140), (1230, 302, 1819),
+                  (2, 1211, 1124), (1325, 133, 2577), (592, 257, 1824), (769, 146, 3223)]
+
+
+@pytest.mark.parametrize("m,d,f", PARTS_BACKWARD)
+def test_backward_in_every_number_of_parts(K, cuda, m, d, f):
+    backward(K, "bf16", "silu", m, d, f, pad=m % 2)
+
+
+@pytest.mark.parametrize("i", range(2))
+def test_gated_pairs_of_every_width(K, cuda, i):
+    forward(K, "bf16", "silu", *PAIRS_GATED[i], 0, True)
+    gated_i8(K, "f32", *PAIRS_GATED_8[i])
+    scaled(K, "bf16", *PAIRS_SCALED[0])
