@@ -544,7 +544,8 @@ typedef struct clpk_gated_ffn_args {
 CLPK_API int clpk_gated_ffn(const clpk_gated_ffn_args_t *args, void *stream);
 
 /* Gradients of clpk_gated_ffn in CLPK_DT_BF16 or F16, from that of h and the g and u that it kept:
- *   dg = dh * u * act'(g),  du = dh * act(g)      in fp32, rounded to `dtype` (the workspace holds them)
+ *   dg = dh * u * act'(g),  du = dh * act(g)      in fp32, rounded to `dtype` (the workspace holds them):
+ *                                                 in F16 above 65504 infinite and below 2^-25 nothing; scale dh where that matters
  *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x      sums in fp32, rounded once
  * d_dx may be NULL, and so may d_dwg and d_dwu (both or neither): what is not asked for is not computed.  Sums are formed
  * in the same order in every call.  A NaN in g makes act(g) and act'(g) NaN, whatever the activation. */

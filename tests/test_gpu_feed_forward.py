@@ -599,3 +599,22 @@ def test_gated_pairs_of_every_width(K, cuda, i):
     forward(K, "bf16", "silu", *PAIRS_GATED[i], 0, True)
     gated_i8(K, "f32", *PAIRS_GATED_8[i])
     scaled(K, "bf16", *PAIRS_SCALED[0])
+
+
+def test_gradients_beyond_the_range_of_fp16(K, cuda):
+    """dg = dh * u is rounded to fp16 on the way: beyond 65504 it is an infinity and below 2^-25 nothing, though dWg = dg^T x has room
+    for what it would be; dh times a power of two (and the gradients divided by it) is the caller's way out."""
+    m, d, f = 4, 16, 8
+
+    def dwg(dh, u, x):
+        g = F.filled(torch.full((m, f), 2.0, device="cuda"), "f16")
+        x, dh, u = (F.filled(torch.full(s, v, device="cuda"), "f16") for s, v in (((m, d), x), ((m, f), dh), ((m, f), u)))
+        w = F.filled(torch.ones(f, d, device="cuda"), "f16")
+        out, ws, status = [F.matrix(r, d, "f16") for r in (m, f, f)], F.workspace(K, "f16", m, d, f), F.word()
+        K.clpk_gated_ffn_backward(C.byref(F.backward_args("f16", "relu", x, w, w, dh, g, u, *out, ws, status)), F.stream())
+        assert status.item() == 0 and bool((out[2] == 4 * 2 * dh[0, 0] * x[0, 0]).all())
+        return out[1]
+    assert bool((dwg(300.0, 256.0, 2.0 ** -10) == float("inf")).all())                       # 4 * 76800 / 1024 = 300
+    assert bool((dwg(75.0, 256.0, 2.0 ** -10) == 75).all())
+    assert not dwg(2.0 ** -14, 2.0 ** -12, 1024.0).any()                                     # 2^-14
+    assert bool((dwg(2.0 ** -8, 2.0 ** -12, 1024.0) == 2.0 ** -8).all())
