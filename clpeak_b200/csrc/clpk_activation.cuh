@@ -9,7 +9,8 @@
 // GELU's normal distribution function is Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x),
 // x >= 0, off by 1.5e-7 at most; in fp32 the function is within 3.0e-7 and GELU within 4.2e-7, which is what erff and its sum with 1
 // lose too (4.5e-7).  Below 0, where that sum cancels, the error here falls with exp(-x^2) (g = -5: -1.4355e-6 for -1.4332e-6,
-// with erff -1.4901e-6).  Gated bf16 4096 x 512 x 4096 38.2 -> 35.0 us, int8 1378 x 144 x 13968 45.4 -> 39.0, both with eight epilogue warps (now 34 and 29).
+// with erff -1.4901e-6).  In place of erff it took gated bf16 4096 x 512 x 4096 from 38.2 to 35.0 us and int8 1378 x 144 x 13968 from 45.4
+// to 39.0, with eight epilogue warps; with sixteen they take 29 and 29, and 28.5 and 22 with ReLU.
 #pragma once
 
 #include <stdint.h>

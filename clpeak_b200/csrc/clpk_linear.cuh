@@ -10,14 +10,14 @@
 //  * kGradients: the products of the backward pass (clpk_linear_grad.cuh).
 //
 // What bounds it.  Long sums: the tensor cores and the card's power limit.  Gated bf16 4096^3 keeps the tensor pipe busy for 94.9 % of
-// the SMs' active cycles, at 1.53 GHz; 8192 x 4096 x 8192 takes 784 to 795 us in a running program (1.38 to 1.40 PFLOPS), the
-// library's plain product of that size 800 to 813 in the same minutes, and int8 8192^3 with scales and bias 383 to 393 (2.8
-// POPS) where clpk_gemm's with 32-bit results takes 400.  A K block of a 256 x 256 tile is 512 tensor cycles: 0.28 us while half of
+// the SMs' active cycles, at 1.53 GHz; 8192 x 4096 x 8192 takes 784 to 820 us in a running program, by the card (1.34 to 1.40
+// PFLOPS; where it took 784 to 795, the library's plain product of that size took 800 to 813), and int8 8192^3 with scales and bias 375 to
+// 393 (2.8 to 2.9 POPS), clpk_gemm's with 32-bit results 400.  A K block of a 256 x 256 tile is 512 tensor cycles: 0.28 us while half of
 // the SMs work, 0.39 to 0.44 when all do.  Tiles of 512 rows, which fetch a quarter less, were 5 to 11 % slower in every form:
 // tensor memory then holds one accumulator, and an epilogue with activations is too long to stand exposed.
 //
 // Short sums: the epilogue and the results' way to memory.  16-bit results of 4096 x 14336 x 256 leave in 35 us, and a memset of them
-// takes 33; gated bf16 4096 x 128 x 14336 43 us with ReLU and 53 with SiLU, of whose two special-function results an element the
+// takes 33; gated bf16 4096 x 128 x 14336 37 to 43 us with ReLU and 53 to 55 with SiLU, of whose two special-function results an element the
 // schedulers' share is 28.  Sixteen warps do it, four on each scheduler, so that one's waits -- for tensor memory, for its box, for
 // shared memory -- lie under the others' work: eight, with two boxes each, issued in a third of the cycles (66 us, ReLU 50).
 #pragma once
@@ -228,7 +228,8 @@ __device__ __forceinline__ float bias_value(uint32_t bits, int type)
 
 // What a chunk's 8-bit sums are finished with: the scale of the lane's row, and of each part a column's of Wg's or B's for the lower
 // half of the lanes and of Wu's, or bias, for the upper.  They are asked for a chunk ahead, and go to the lanes through shared
-// memory: with a shuffle for each column the pipe that shuffles was the bound (bf16 results, 4096 x 14336 x 256 with bias 63 us, so 53).
+// memory: with a shuffle for each column the pipe that shuffles was the bound (bf16 results, 4096 x 14336 x 256 with
+// bias 63 us and so 53, both with eight epilogue warps; 35 to 38 with sixteen).
 struct LinearScales {
     float row = 0.0f;
     uint32_t col[2] = {};

@@ -52,7 +52,8 @@ struct LinearPlan {
     uint32_t tn, splits;
 };
 
-// Clusters of `splits` pairs that the chip holds at a time.
+// Clusters of `splits` pairs that the chip holds at a time: of a whole B200's 148 SMs, 33 of four CTAs that take an SM each and 15 of
+// eight, as cudaOccupancyMaxActiveClusters counts them for every tile width.
 static uint32_t linear_resident(uint32_t splits)
 {
     const uint32_t pairs = (uint32_t)num_sms() / 2;
@@ -68,8 +69,8 @@ static float linear_estimate(float blocks, float tiles, uint32_t tn, uint32_t sp
     return blocks * (0.12f + 0.15f * wide) + tiles * (0.8f + 1.3f * wide + (splits > 1 ? 3.5f + 2.0f * wide : 0.0f));
 }
 
-// Tile width and K ranges: the cheapest by the estimate.  Of those 60 shapes it takes the fastest choice for 53; one is 14 % slower,
-// and the geometric mean 0.6 %.
+// Tile width and K ranges: the cheapest by the estimate.  Of the 60 shapes it was fitted to it takes the fastest choice for
+// 53, and the geometric mean is 0.6 % slower; of 60 others 59 are within 1 % of the fastest, and one is 3 % slower.
 static LinearPlan plan_linear(const Product &w, LinearForm form, uint32_t k_blocks)
 {
     const uint32_t cols = form == kGated ? 2 * w.n : w.n;
@@ -144,8 +145,10 @@ static int launch_linear(const Product &w, uint32_t k_blocks, cudaStream_t s)
 template <LinearForm FORM> constexpr uint32_t few_cols = FORM == kGated ? 64 : 128;      // features of a tile
 
 // K ranges of linear_few_kernel: as many as the chip holds CTAs for at once, as long as each has some blocks of K; with long sums
-// also where that loads the SMs more evenly.  Over 70 shapes of 1 to 64 tokens it is 1 % slower than the fastest in the geometric
-// mean.  What it decides: int8 1 x 4096 x 4096 in one range 9.2 us, in four 5.2; 8 x 30080 x 4096 (235 tiles) 26.7, in two 22.8.
+// also where that loads the SMs more evenly.  Fitted to 70 shapes of 1 to 64 tokens (1 % slower than the fastest in the
+// geometric mean); over 70 others of up to 128 tokens, with few_tokens, it is 2.4 % slower, 53 are within 2 %, and the worst takes
+// 49 us in one range where four would take 39 (64 x 10039 x 15855).  What it decides: int8 1 x 4096 x 4096 in one range 9.2 us, in
+// four 5.2; 8 x 30080 x 4096 (235 tiles) 26.7, in two 23.0.
 static uint32_t few_splits(uint32_t tokens, uint32_t tiles, uint32_t k_blocks, uint32_t sms)
 {
     uint32_t splits = 1;
@@ -390,9 +393,10 @@ static uint64_t share_tiles(const GradTiles &first, const GradTiles &second, uin
 constexpr uint32_t kGradPairs = 74;                         // of a whole B200: the workspace's size may not depend on the card at hand
 
 // How the products of the backward pass are cut: tile width and parts of K, the cheapest by the estimate.  A set of tiles that fills
-// the chip is whole, and so is one of the two (no shape gained more than 1 % by cutting both).  Over 73 shapes that were timed with
-// every choice this is 0.9 % slower than the fastest in the geometric mean, 9 % at most; 4103 x 170 x 3591 takes 71 us in tiles of
-// 128 columns, 58 in tiles of 256 and dx in two parts.
+// the chip is whole, and so is one of the two (no shape gained more than 1 % by cutting both).  Over the 73 shapes that the
+// estimate was fitted to this is 0.9 % slower than the fastest in the geometric mean, 9 % at most; over 73 others 1.7 %, where 59 are within
+// 2 % and the worst takes 18.2 us uncut and 14.9 with dW in three parts (2467 x 919 x 138).  4103 x 170 x 3591 takes 71 us in tiles of 128
+// columns, 58 in tiles of 256 and dx in two parts.
 struct GradPlan {
     uint32_t tn, x_parts, w_parts;
 };
