@@ -187,7 +187,7 @@ def fit(layer: FeedForward, target: FeedForward, steps: int, rate: float, seed: 
     gen = torch.Generator(device="cuda")
     gen.manual_seed(seed)
     wg, wu = layer.wg.float(), layer.wu.float()
-    losses = []
+    losses, waits = [], torch.zeros_like(layer.status)
     for _ in range(steps):
         x = torch.randn(layer.tokens, layer.d, generator=gen, device="cuda").to(torch.bfloat16)
         off = layer.forward(x).float() - target.forward(x).float()
@@ -197,7 +197,8 @@ def fit(layer: FeedForward, target: FeedForward, steps: int, rate: float, seed: 
         wu -= rate * dwu.float()
         layer.wg.copy_(wg)
         layer.wu.copy_(wu)
-    layer.check()
+        waits |= layer.status | target.status
+    _check_status(waits, "fit")
     return [float(v) for v in losses]
 
 

@@ -209,3 +209,20 @@ def test_a_wait_that_ran_out_is_told(calls, word):
             with pytest.raises(N.ClpkError) as e:
                 checked.check()
             assert e.value.code == N.ERR_TIMEOUT and str(0x303) in str(e.value)
+
+
+@pytest.mark.parametrize("step,which", [(1, 0), (3, 0), (2, 1)])
+def test_a_wait_that_ran_out_in_any_step_of_a_fit(calls, step, which):
+    """Every call clears its status word, so that of a step is gone with the next one."""
+    layers = ff.FeedForward(64, 128, 8), ff.FeedForward(64, 128, 8)
+    for t in layers:
+        t.y.zero_()
+    steps = [0, 0]
+
+    def gated(args, stream):
+        i = [t.wg.data_ptr() for t in layers].index(args._obj.d_wg)
+        steps[i] += 1
+        layers[i].status[0] = 0x301 if (steps[i], i) == (step, which) else 0
+    calls.clpk_gated_ffn = gated
+    with pytest.raises(N.ClpkError, match=str(0x301)):
+        ff.fit(*layers, steps=3, rate=0.1)
