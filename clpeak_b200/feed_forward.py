@@ -6,7 +6,10 @@
     served = ServedFeedForward(layer)         # weights quantised once, one scale for each output channel
     y = served.forward(x)                     # tokens quantised on the way, one scale for each
 
-Buffers, workspaces and argument structures are set up once and used again by every call; calls run on torch's current stream.
+Buffers, workspaces and argument structures are set up once and used again by every call; calls run on torch's current stream.  What a
+call returns is a view of them: it is good until the layer's next call of that kind, and a program that needs it longer copies it.  x
+is read again by backward() and has to be as it was until then.  A layer is for one stream and one host thread at a time: every
+call of another stream or thread needs a layer of its own, or has to come after the calls before it.
 ``python -m clpeak_b200.feed_forward`` fits the projections of a small layer to those of another one and then serves it.
 """
 from __future__ import annotations
