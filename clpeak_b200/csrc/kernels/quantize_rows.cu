@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) quantize_rows_k
     }
 }
 
-// Rows that are not aligned, or longer than the registers hold: element by element, read twice.
+// Rows that are not aligned, or longer than the registers hold: element by element, read twice.  fp32 4096 x 11008 65 us (aligned
+// 36), 4096 x 28672 265 us where its bytes take 90.
 template <int DT>
 __global__ void __launch_bounds__(256) quantize_rows_plain_kernel(RowParams p)
 {
