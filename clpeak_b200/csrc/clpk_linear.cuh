@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         const uint32_t full0 = cluster_addr(&sh->full[0], leader);
-        uint32_t s = 0, parity = 1;                            // parity of the empty barrier's previous phase
+        uint32_t s = 0, parity = 1, issued = 0;                // parity of the empty barrier's previous phase
         bool ok = true;
         for (uint32_t i = 0; ok && linear_tile<FORM>(p, cluster, clusters, split, i, t); i++) {
             const uint32_t row_a = t.mb * kLinearM + r * 128;
@@ -476,12 +476,15 @@ __global__ void __launch_bounds__(kLinearThreads) linear_kernel(const __grid_con
                         }
                 }
                 __syncwarp();
+                issued++;
                 if (++s == p.stages) {
                     s = 0;
                     parity ^= 1;
                 }
             }
         }
+        if (r == 0)                                            // its barriers count the loads of both; nothing else waits for this warp
+            ring_settled(sh->full, p.stages, issued);
     } else if (warp == 1) {
         // ---------------- MMA issuer (the pair's leader) ----------------
         if (r == 0) {

@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) linear_few_kernel(c
         *p.status = 0u;
     griddep_launch_dependents();
 
+    uint32_t issued = 0;
     if (warp == 0) {
         // ---------------- TMA producer ----------------
         uint32_t s = 0, parity = 1;
@@ -232,6 +233,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) linear_few_kernel(c
                 tma_load_own(st + kHalfTileBytes, &maps.x, x, 0, &sh->full[s]);
             }
             __syncwarp();
+            issued++;
             if (++s == p.stages) {
                 s = 0;
                 parity ^= 1;
@@ -294,8 +296,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) linear_few_kernel(c
     // ---------------- partial sums -> shared memory of the token's owner, [K range][token of its][128 rows] ----------------
     // All instructions have retired, hence all loads have landed: where K is not split the ring is free.  A wait that ran out
     // leaves sums that are wrong, and a status that says so; every CTA still comes to the barriers.
-    if (!warp_wait(&sh->done, 0) && lane == 0)
-        atomicCAS(p.status, 0u, 0x313u);
+    if (!warp_wait(&sh->done, 0)) {
+        if (lane == 0)
+            atomicCAS(p.status, 0u, 0x313u);
+        if (warp == 0)
+            ring_settled(sh->full, p.stages, issued);
+    }
     tc_fence_after_sync();
     if (p.splits > 1) {
         if (!p.sums_at)

@@ -51,6 +51,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity)
     return __all_sync(0xffffffffu, mbar_wait(bar, parity) ? 1 : 0) != 0;
 }
 
+// Where a wait has run out, whoever consumed the stages of a ring may have given up while loads into them are on their way: they have
+// to land before the CTA's shared memory goes away.  Only a stage's last use can be on its way; each wait has its limit.
+__device__ __forceinline__ void ring_settled(uint64_t *full, uint32_t stages, uint32_t issued)
+{
+    for (uint32_t use = issued > stages ? issued - stages : 0; use < issued; use++)
+        warp_wait(&full[use % stages], use / stages & 1);
+}
+
 constexpr int kEpilogueWarps = 8;
 constexpr uint32_t kStagingBytes = 32 * 128;                       // 32 rows x 128 bytes of C
 
