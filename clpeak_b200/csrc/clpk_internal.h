@@ -81,6 +81,13 @@ int launch_behind(void (*kernel)(Params...), const char *what, dim3 grid, int th
         }                                                        \
     } while (0)
 
+#define CLPK_TRY(call)                                           \
+    do {                                                         \
+        const int rc__ = (call);                                 \
+        if (rc__ != CLPK_OK)                                     \
+            return rc__;                                         \
+    } while (0)
+
 #define CLPK_LAUNCH_CHECK(name)                                  \
     do {                                                         \
         cudaError_t e__ = cudaGetLastError();                    \

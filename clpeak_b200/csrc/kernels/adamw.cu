@@ -1,0 +1,404 @@
+// One step of Adam with decoupled weight decay over many tensors.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound by memory: every array passes by once.  bf16 parameters with master copies and 32-bit moments move 28 bytes an element, with
+// 8-bit moments and no master copy 10 or 12.  The table of tensors travels with the launch, so that a call is one launch for up to 440
+// tensors, whatever their sizes: a CTA has a chunk of 2048 elements, and finds the tensor that its chunk belongs to by halving the
+// list of the tensors' first chunks.
+//
+// Moments in 8 bits.  A warp has a block of 256 elements, eight in each lane: the moments are computed in fp32, the largest of the block is
+// found by one reduction over the lanes, and codes are rounded from registers.  The codes stand for m = s q |q| and
+// sqrt(v) = s c^2: the square spreads 127 steps over a range of 2^14, and 255 over 2^16 of sqrt(v), 2^32 of v, where equal steps would
+// round to zero whatever is below 2^-8 and 2^-9 of the block's largest.  A v that is not zero keeps a code that is not: an
+// element with a small v beside a large one is taken for larger than it is, and its step gets shorter, never divided by eps alone.
+// Every operation is rounded by itself (no fused multiply-add), so that moments and codes have one value that can be told in
+// any arithmetic.
+#include "../clpk_elements.cuh"
+#include "../clpk_internal.h"
+#include "../clpk_ptx.cuh"
+
+#include <cmath>
+
+namespace clpk {
+
+constexpr int kStepThreads = 256, kStepElems = 8;
+constexpr uint32_t kStepChunk = kStepThreads * kStepElems;
+static_assert(32 * kStepElems == CLPK_ADAMW_BLOCK, "a warp has one block of 8-bit moments");
+
+struct StepTensor {
+    uint64_t n;
+    void *param;
+    const void *grad;
+    float *master;
+    void *m, *v;
+    float *m_scale, *v_scale;
+};
+
+// the step's numbers
+struct StepRates {
+    float b1, b1_rest, b2, b2_rest, eps;
+    float keep, root_scale, rate;                       // 1 - lr wd, 1 / sqrt(1 - b2^t), lr / (1 - b1^t)
+};
+
+struct StepCommon {
+    StepRates rates;
+    double lr, beta1, beta2, decay;                     // with d_lr or d_step
+    uint64_t step;
+    const float *d_lr;
+    const uint32_t *d_step;
+    const float *grad_scale;
+    uint32_t count;
+};
+
+template <int CAP> struct StepTable {
+    StepCommon c;
+    StepTensor tensors[CAP];
+    uint32_t first[CAP];                                // chunk of the launch; `aligned` in the top bit
+};
+constexpr uint32_t kStepAligned = 0x80000000u;
+constexpr int kStepFew = 48, kStepMany = 440;
+static_assert(sizeof(StepTable<kStepFew>) <= 4096 && sizeof(StepTable<kStepMany>) <= 32764, "parameters of a kernel");
+
+__host__ __device__ __forceinline__ void set_rates(StepRates &r, double lr, double beta1, double beta2, double decay, double step)
+{
+    // 1 - beta^t without the digits that a beta near 1 loses
+    const double c1 = beta1 > 0 ? -expm1(step * log(beta1)) : 1.0, c2 = beta2 > 0 ? -expm1(step * log(beta2)) : 1.0;
+    r.keep = (float)(1.0 - lr * decay);
+    r.root_scale = (float)(1.0 / sqrt(c2));
+    r.rate = (float)(lr / c1);
+}
+
+// The code of size >= 0 with 1 / scale; the scale of a block from its largest one, whose bits order like the values
+__device__ __forceinline__ float step_code(float size, float inverse) { return rintf(__fsqrt_rn(__fmul_rn(size, inverse))); }
+__device__ __forceinline__ float step_scale(uint32_t top, float squared_steps, float &scale)
+{
+    if (top >= 0x7F800000u) {
+        scale = __uint_as_float(0x7FC00000u);
+        return 0.0f;
+    }
+    scale = __fdiv_rn(__uint_as_float(top), squared_steps);
+    if (scale < 1.17549435e-38f) {
+        scale = 0.0f;
+        return 0.0f;
+    }
+    return __frcp_rn(scale);
+}
+
+// Eight elements of a thread.  FAST: neighbours, in whole vectors; otherwise 32 apart, one at a time, those below `left` only.
+template <int DT, int GDT, int SDT, bool MASTER, bool FAST>
+__device__ __forceinline__ void step_elements(const StepTensor &t, const StepRates &r, float grad_scale, bool scaled, uint64_t at, uint32_t left)
+{
+    using P = Element<DT>;
+    using G = Element<GDT>;
+    constexpr int N = kStepElems;
+    constexpr bool kSmall = SDT == CLPK_DT_I8;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t block = at;                          // the warp's first element
+    typename P::T *const param = static_cast<typename P::T *>(t.param) + block;
+    const typename G::T *const grad = static_cast<const typename G::T *>(t.grad) + block;
+    float *const master = MASTER ? t.master + block : nullptr;
+    float p[N], g[N], m[N], v[N];
+    auto mine = [&](int j) { return lane + 32 * j; };
+
+    if constexpr (FAST) {
+        Raw<GDT, N> raw_g;
+        raw_g.load(grad + lane * N);
+        if constexpr (MASTER) {
+            Raw<CLPK_DT_F32, N> raw;
+            raw.load(master + lane * N);
+            raw.widen(p);
+        } else {
+            Raw<DT, N> raw;
+            raw.load(param + lane * N);
+            raw.widen(p);
+        }
+        if constexpr (kSmall) {
+            const uint2 qm = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(t.m) + block + lane * N);
+            const uint2 qv = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(t.v) + block + lane * N);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                m[j] = (float)(int8_t)((j < 4 ? qm.x : qm.y) >> (8 * (j & 3)));
+                v[j] = (float)(uint8_t)((j < 4 ? qv.x : qv.y) >> (8 * (j & 3)));
+            }
+        } else {
+            Raw<CLPK_DT_F32, N> raw_m, raw_v;
+            raw_m.load(static_cast<const float *>(t.m) + block + lane * N);
+            raw_v.load(static_cast<const float *>(t.v) + block + lane * N);
+            raw_m.widen(m);
+            raw_v.widen(v);
+        }
+        raw_g.widen(g);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            p[j] = g[j] = m[j] = v[j] = 0.0f;
+            if (mine(j) < left) {
+                g[j] = G::widen(grad[mine(j)]);
+                p[j] = MASTER ? master[mine(j)] : P::widen(param[mine(j)]);
+                if constexpr (kSmall) {
+                    m[j] = static_cast<const int8_t *>(t.m)[block + mine(j)];
+                    v[j] = static_cast<const uint8_t *>(t.v)[block + mine(j)];
+                } else {
+                    m[j] = static_cast<const float *>(t.m)[block + mine(j)];
+                    v[j] = static_cast<const float *>(t.v)[block + mine(j)];
+                }
+            }
+        }
+    }
+    float root[N];
+    if constexpr (kSmall) {
+        const float sm = t.m_scale[block / CLPK_ADAMW_BLOCK], sv = t.v_scale[block / CLPK_ADAMW_BLOCK];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            m[j] = __fmul_rn(m[j] * fabsf(m[j]), sm);   // whole numbers below 2^16: their products are exact
+            const float old = __fmul_rn(v[j] * v[j], sv);
+            v[j] = __fmul_rn(old, old);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        if (scaled)
+            g[j] = __fmul_rn(g[j], grad_scale);
+        m[j] = __fadd_rn(__fmul_rn(m[j], r.b1), __fmul_rn(g[j], r.b1_rest));
+        v[j] = __fadd_rn(__fmul_rn(v[j], r.b2), __fmul_rn(__fmul_rn(g[j], g[j]), r.b2_rest));
+        root[j] = __fsqrt_rn(v[j]);
+        const float step = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(root[j], r.root_scale), r.eps));
+        p[j] = __fsub_rn(__fmul_rn(p[j], r.keep), __fmul_rn(step, r.rate));
+    }
+
+    uint32_t qm[2] = {}, qv[2] = {};
+    if constexpr (kSmall) {
+        uint32_t top_m = 0, top_v = 0;                  // zeros behind the last element are the largest of nothing
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            if (FAST || mine(j) < left) {
+                top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+                top_v = max(top_v, __float_as_uint(root[j]) & 0x7FFFFFFFu);
+            }
+        }
+        top_m = __reduce_max_sync(0xffffffffu, top_m);
+        top_v = __reduce_max_sync(0xffffffffu, top_v);
+        float sm, sv;
+        const float im = step_scale(top_m, 127.0f * 127.0f, sm), iv = step_scale(top_v, 255.0f * 255.0f, sv);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const float cm = step_code(fabsf(m[j]), im), cv = step_code(root[j], iv);
+            const int q = im > 0.0f ? (int)copysignf(cm, m[j]) : 0;
+            const uint32_t c = iv > 0.0f ? (root[j] > 0.0f ? max((uint32_t)cv, 1u) : 0u) : 0u;
+            qm[j / 4] |= ((uint32_t)q & 0xFFu) << (8 * (j & 3));
+            qv[j / 4] |= c << (8 * (j & 3));
+        }
+        if (lane == 0 && (FAST || left > 0)) {
+            t.m_scale[block / CLPK_ADAMW_BLOCK] = sm;
+            t.v_scale[block / CLPK_ADAMW_BLOCK] = sv;
+        }
+    }
+
+    if constexpr (FAST) {
+        Raw<DT, N> out;
+        out.round(p);
+        out.store(param + lane * N);
+        Raw<CLPK_DT_F32, N> raw;
+        if constexpr (MASTER) {
+            raw.round(p);
+            raw.store(master + lane * N);
+        }
+        if constexpr (kSmall) {
+            *reinterpret_cast<uint2 *>(static_cast<int8_t *>(t.m) + block + lane * N) = make_uint2(qm[0], qm[1]);
+            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(t.v) + block + lane * N) = make_uint2(qv[0], qv[1]);
+        } else {
+            raw.round(m);
+            raw.store(static_cast<float *>(t.m) + block + lane * N);
+            raw.round(v);
+            raw.store(static_cast<float *>(t.v) + block + lane * N);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (mine(j) < left) {
+                param[mine(j)] = P::round(p[j]);
+                if constexpr (MASTER)
+                    master[mine(j)] = p[j];
+                if constexpr (kSmall) {
+                    static_cast<int8_t *>(t.m)[block + mine(j)] = (int8_t)(qm[j / 4] >> (8 * (j & 3)));
+                    static_cast<uint8_t *>(t.v)[block + mine(j)] = (uint8_t)(qv[j / 4] >> (8 * (j & 3)));
+                } else {
+                    static_cast<float *>(t.m)[block + mine(j)] = m[j];
+                    static_cast<float *>(t.v)[block + mine(j)] = v[j];
+                }
+            }
+    }
+}
+
+template <int DT, int GDT, int SDT, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kStepThreads) adamw_kernel(const __grid_constant__ StepTable<CAP> table)
+{
+    __shared__ StepRates told;
+    griddep_wait();
+    griddep_launch_dependents();
+    // the last tensor whose first chunk is not behind this one
+    uint32_t lo = 0, hi = table.c.count;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if ((table.first[mid] & ~kStepAligned) <= blockIdx.x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const StepTensor &t = table.tensors[lo];
+    const uint64_t at = (uint64_t)(blockIdx.x - (table.first[lo] & ~kStepAligned)) * kStepChunk + (threadIdx.x & ~31u) * kStepElems;
+    StepRates r = table.c.rates;
+    if (table.c.d_lr || table.c.d_step) {
+        if (threadIdx.x == 0) {
+            const double lr = table.c.d_lr ? (double)*table.c.d_lr : table.c.lr;
+            set_rates(told, lr, table.c.beta1, table.c.beta2, table.c.decay, table.c.d_step ? (double)*table.c.d_step : (double)table.c.step);
+        }
+        __syncthreads();
+        r.keep = told.keep;
+        r.root_scale = told.root_scale;
+        r.rate = told.rate;
+    }
+    const bool scaled = table.c.grad_scale != nullptr;
+    const float grad_scale = scaled ? *table.c.grad_scale : 1.0f;
+    if (at >= t.n)                                      // whole warps, behind the last barrier
+        return;
+    const uint64_t left = t.n - at;
+    if ((table.first[lo] & kStepAligned) && left >= CLPK_ADAMW_BLOCK)
+        step_elements<DT, GDT, SDT, MASTER, true>(t, r, grad_scale, scaled, at, CLPK_ADAMW_BLOCK);
+    else
+        step_elements<DT, GDT, SDT, MASTER, false>(t, r, grad_scale, scaled, at, left < CLPK_ADAMW_BLOCK ? (uint32_t)left : CLPK_ADAMW_BLOCK);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------
+
+constexpr uint64_t kStepMostChunks = 0x7FFFFFFFu;       // of a launch
+
+template <int DT, int GDT, int SDT, bool MASTER, int CAP>
+static int launch_step(StepTable<CAP> &table, const clpk_adamw_tensor_t *tensors, uint32_t count, cudaStream_t s)
+{
+    uint64_t chunks = 0;
+    const auto flush = [&]() {
+        const int rc = table.c.count ? launch_behind(adamw_kernel<DT, GDT, SDT, MASTER, CAP>, "adamw", (unsigned)chunks, kStepThreads, 0, s, table) : CLPK_OK;
+        table.c.count = 0;
+        chunks = 0;
+        return rc;
+    };
+    for (uint32_t i = 0; i < count; i++) {
+        const clpk_adamw_tensor_t &t = tensors[i];
+        const uint64_t own = (t.n + kStepChunk - 1) / kStepChunk;
+        if (own == 0)
+            continue;
+        if (table.c.count == CAP || chunks + own > kStepMostChunks)
+            CLPK_TRY(flush());
+        uintptr_t at = (uintptr_t)t.d_param | (uintptr_t)t.d_grad | (uintptr_t)t.d_master;
+        if (SDT == CLPK_DT_F32)
+            at |= (uintptr_t)t.d_m | (uintptr_t)t.d_v;
+        const bool aligned = at % 16 == 0 && (SDT == CLPK_DT_F32 || ((uintptr_t)t.d_m | (uintptr_t)t.d_v) % 8 == 0);
+        table.tensors[table.c.count] = {t.n, t.d_param, t.d_grad, t.d_master, t.d_m, t.d_v, t.d_m_scale, t.d_v_scale};
+        table.first[table.c.count++] = (uint32_t)chunks | (aligned ? kStepAligned : 0);
+        chunks += own;
+    }
+    return flush();
+}
+
+template <int DT, int GDT, int SDT, bool MASTER>
+static int run_step(const StepCommon &c, const clpk_adamw_tensor_t *tensors, uint32_t count, cudaStream_t s)
+{
+    if (count <= kStepFew) {                            // less to send along with the launch
+        StepTable<kStepFew> table;
+        table.c = c;
+        return launch_step<DT, GDT, SDT, MASTER>(table, tensors, count, s);
+    }
+    StepTable<kStepMany> table;
+    table.c = c;
+    return launch_step<DT, GDT, SDT, MASTER>(table, tensors, count, s);
+}
+
+template <int DT, int GDT>
+static int run_step_by(const StepCommon &c, int state, bool master, const clpk_adamw_tensor_t *tensors, uint32_t count, cudaStream_t s)
+{
+    if constexpr (DT != CLPK_DT_F32)
+        if (master)
+            return state == CLPK_DT_I8 ? run_step<DT, GDT, CLPK_DT_I8, true>(c, tensors, count, s) : run_step<DT, GDT, CLPK_DT_F32, true>(c, tensors, count, s);
+    return state == CLPK_DT_I8 ? run_step<DT, GDT, CLPK_DT_I8, false>(c, tensors, count, s) : run_step<DT, GDT, CLPK_DT_F32, false>(c, tensors, count, s);
+}
+
+static int check_part(uint32_t i, const char *name, const void *base, uint64_t elem)
+{
+    CLPK_REQUIRE(base && (uintptr_t)base % elem == 0, "clpk_adamw: %s of tensor %u is NULL or not aligned to its elements", name, i);
+    return CLPK_OK;
+}
+
+static int check_step_tensor(const clpk_adamw_args_t &a, uint32_t i, bool master)
+{
+    const clpk_adamw_tensor_t &t = a.h_tensors[i];
+    if (t.n == 0)
+        return CLPK_OK;
+    CLPK_REQUIRE(t.n <= 1ull << 40, "clpk_adamw: tensor %u has %llu elements", i, (unsigned long long)t.n);
+    CLPK_TRY(check_part(i, "d_param", t.d_param, element_bytes(a.dtype)));
+    CLPK_TRY(check_part(i, "d_grad", t.d_grad, element_bytes(a.grad_dtype)));
+    CLPK_REQUIRE((t.d_master != nullptr) == master, "clpk_adamw: d_master: give it for every tensor, or for none (tensor %u)", i);
+    if (master)
+        CLPK_TRY(check_part(i, "d_master", t.d_master, 4));
+    const uint64_t state = element_bytes(a.state_dtype);
+    CLPK_TRY(check_part(i, "d_m", t.d_m, state));
+    CLPK_TRY(check_part(i, "d_v", t.d_v, state));
+    if (a.state_dtype == CLPK_DT_I8) {
+        CLPK_TRY(check_part(i, "d_m_scale", t.d_m_scale, 4));
+        CLPK_TRY(check_part(i, "d_v_scale", t.d_v_scale, 4));
+    }
+    return CLPK_OK;
+}
+
+} // namespace clpk
+
+using namespace clpk;
+
+extern "C" int clpk_adamw(const clpk_adamw_args_t *args, void *stream)
+{
+    CLPK_TRY(require_sm100());
+    const char *what = "clpk_adamw";
+    CLPK_REQUIRE(args, "%s: args is NULL", what);
+    const clpk_adamw_args_t &a = *args;
+    CLPK_REQUIRE(a.dtype == CLPK_DT_F32 || a.dtype == CLPK_DT_F16 || a.dtype == CLPK_DT_BF16, "%s: dtype %d is not F32, F16 or BF16", what, a.dtype);
+    CLPK_REQUIRE(a.grad_dtype == a.dtype || a.grad_dtype == CLPK_DT_F32, "%s: grad_dtype %d is neither dtype nor F32", what, a.grad_dtype);
+    CLPK_REQUIRE(a.state_dtype == CLPK_DT_F32 || a.state_dtype == CLPK_DT_I8, "%s: state_dtype %d is not F32 or I8", what, a.state_dtype);
+    CLPK_REQUIRE(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0, "%s: beta1 %g, beta2 %g: both in [0, 1)", what, a.beta1, a.beta2);
+    CLPK_REQUIRE((float)a.eps > 0.0f && a.eps < 1e30, "%s: eps %g is not above 0 in fp32", what, a.eps);
+    CLPK_REQUIRE(std::isfinite(a.weight_decay) && a.weight_decay >= 0.0 && (a.d_lr || (std::isfinite(a.lr) && a.lr >= 0.0)), "%s: lr %g, weight_decay %g", what, a.lr, a.weight_decay);
+    CLPK_REQUIRE(a.d_step || a.step > 0, "%s: steps are counted from 1", what);
+    CLPK_REQUIRE((uintptr_t)a.d_lr % 4 == 0 && (uintptr_t)a.d_step % 4 == 0 && (uintptr_t)a.d_grad_scale % 4 == 0, "%s: d_lr, d_step or d_grad_scale is not aligned to its elements", what);
+    CLPK_REQUIRE(a.count == 0 || a.h_tensors, "%s: h_tensors is NULL", what);
+    bool master = false;
+    for (uint32_t i = 0; i < a.count && !master; i++)
+        master = a.h_tensors[i].n > 0 && a.h_tensors[i].d_master;
+    CLPK_REQUIRE(!master || a.dtype != CLPK_DT_F32, "%s: parameters in fp32 have no master copies", what);
+    for (uint32_t i = 0; i < a.count; i++)
+        CLPK_TRY(check_step_tensor(a, i, master));
+
+    StepCommon c = {};
+    c.rates.b1 = (float)a.beta1;
+    c.rates.b1_rest = (float)(1.0 - a.beta1);
+    c.rates.b2 = (float)a.beta2;
+    c.rates.b2_rest = (float)(1.0 - a.beta2);
+    c.rates.eps = (float)a.eps;
+    if (!a.d_lr && !a.d_step)
+        set_rates(c.rates, a.lr, a.beta1, a.beta2, a.weight_decay, (double)a.step);
+    c.lr = a.lr;
+    c.beta1 = a.beta1;
+    c.beta2 = a.beta2;
+    c.decay = a.weight_decay;
+    c.step = a.step;
+    c.d_lr = a.d_lr;
+    c.d_step = a.d_step;
+    c.grad_scale = a.d_grad_scale;
+    cudaStream_t s = as_stream(stream);
+    if (a.dtype == CLPK_DT_F32)
+        return run_step_by<CLPK_DT_F32, CLPK_DT_F32>(c, a.state_dtype, master, a.h_tensors, a.count, s);
+    if (a.dtype == CLPK_DT_BF16)
+        return a.grad_dtype == CLPK_DT_F32 ? run_step_by<CLPK_DT_BF16, CLPK_DT_F32>(c, a.state_dtype, master, a.h_tensors, a.count, s)
+                                           : run_step_by<CLPK_DT_BF16, CLPK_DT_BF16>(c, a.state_dtype, master, a.h_tensors, a.count, s);
+    return a.grad_dtype == CLPK_DT_F32 ? run_step_by<CLPK_DT_F16, CLPK_DT_F32>(c, a.state_dtype, master, a.h_tensors, a.count, s)
+                                       : run_step_by<CLPK_DT_F16, CLPK_DT_F16>(c, a.state_dtype, master, a.h_tensors, a.count, s);
+}

@@ -560,13 +560,6 @@ static int check_matrix(const char *what, const char *name, const void *base, ui
     return CLPK_OK;
 }
 
-#define CLPK_TRY(call)            \
-    do {                          \
-        const int rc__ = (call);  \
-        if (rc__ != CLPK_OK)      \
-            return rc__;          \
-    } while (0)
-
 static int check_status(const char *what, const uint32_t *status)
 {
     CLPK_REQUIRE(status && (uintptr_t)status % 4 == 0, "%s: d_status must be a device word", what);

@@ -121,6 +121,51 @@ class GatedFfnBackwardArgs(C.Structure):
     ]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("weight_dtype", C.c_int),
+        ("m", C.c_uint32), ("d", C.c_uint32),
+        ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_bias", C.c_void_p),
+        ("d_y", C.c_void_p), ("d_mean", C.c_void_p), ("d_rstd", C.c_void_p),
+        ("ldx", C.c_uint64), ("ldy", C.c_uint64),
+        ("eps", C.c_float),
+    ]
+
+
+class LayerNormBackwardArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("weight_dtype", C.c_int),
+        ("m", C.c_uint32), ("d", C.c_uint32),
+        ("d_x", C.c_void_p), ("d_weight", C.c_void_p), ("d_dy", C.c_void_p),
+        ("d_mean", C.c_void_p), ("d_rstd", C.c_void_p),
+        ("d_dx", C.c_void_p), ("d_dweight", C.c_void_p), ("d_dbias", C.c_void_p),
+        ("ldx", C.c_uint64), ("lddy", C.c_uint64), ("lddx", C.c_uint64),
+        ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [
+        ("n", C.c_uint64),
+        ("d_param", C.c_void_p), ("d_grad", C.c_void_p), ("d_master", C.c_void_p),
+        ("d_m", C.c_void_p), ("d_v", C.c_void_p),
+        ("d_m_scale", C.c_void_p), ("d_v_scale", C.c_void_p),
+    ]
+
+
+class AdamwArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("grad_dtype", C.c_int), ("state_dtype", C.c_int),
+        ("count", C.c_uint32),
+        ("h_tensors", C.c_void_p),
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+        ("step", C.c_uint64),
+        ("d_lr", C.c_void_p), ("d_step", C.c_void_p), ("d_grad_scale", C.c_void_p),
+    ]
+
+
+ADAMW_BLOCK = 256                   # elements that share a scale, moments in 8 bits
+
 _vp, _u64, _u32, _i, _f = C.c_void_p, C.c_uint64, C.c_uint32, C.c_int, C.c_float
 
 # name -> argtypes; every function returns int unless listed in _RESTYPES.
@@ -189,11 +234,16 @@ KERNEL_API = {
     "clpk_gated_ffn": [C.POINTER(GatedFfnArgs), _vp],
     "clpk_gated_ffn_backward_workspace_bytes": [_i, _u32, _u32, _u32, C.POINTER(C.c_size_t)],
     "clpk_gated_ffn_backward": [C.POINTER(GatedFfnBackwardArgs), _vp],
+    "clpk_layer_norm": [C.POINTER(LayerNormArgs), _vp],
+    "clpk_layer_norm_backward_workspace_bytes": [_u32, _u32, C.POINTER(C.c_size_t)],
+    "clpk_layer_norm_backward": [C.POINTER(LayerNormBackwardArgs), _vp],
+    "clpk_adamw": [C.POINTER(AdamwArgs), _vp],
     "clpk_set_tuning": [_i, _i],
     "clpk_get_tuning": [_i, C.POINTER(_i)],
 }
 # the structure that a call of the extension takes by reference, where it is not GemmArgs
-_ARGUMENTS = {"clpk_gemm_i8_scaled": GemmI8ScaledArgs, "clpk_gated_ffn": GatedFfnArgs, "clpk_gated_ffn_backward": GatedFfnBackwardArgs}
+_ARGUMENTS = {"clpk_gemm_i8_scaled": GemmI8ScaledArgs, "clpk_gated_ffn": GatedFfnArgs, "clpk_gated_ffn_backward": GatedFfnBackwardArgs,
+              "clpk_layer_norm": LayerNormArgs, "clpk_layer_norm_backward": LayerNormBackwardArgs, "clpk_adamw": AdamwArgs}
 _RESTYPES = {
     "clpk_last_error": C.c_char_p,
     "clpk_version": C.c_char_p,

@@ -571,6 +571,100 @@ typedef struct clpk_gated_ffn_backward_args {
 CLPK_API int clpk_gated_ffn_backward_workspace_bytes(int dtype, uint32_t m, uint32_t d, uint32_t f, size_t *bytes);
 CLPK_API int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args, void *stream);
 
+/* ---- training a block ---------------------------------------------------------------------------
+ * What stands around a layer's products while it is trained: the norm in front of it and the optimiser's step.  No
+ * counterpart in the reference. */
+
+/* y = (x - mean) * rstd * weight + bias for each of m rows of d elements, with
+ *   mean = sum x / d,   rstd = 1 / sqrt(sum (x - mean)^2 / d + eps)
+ * in fp32 and rounded once.  dtype: CLPK_DT_F32, F16 or BF16, of x and y; weight_dtype: `dtype` or CLPK_DT_F32.  Rows lie ld*
+ * elements apart, 0: one behind another; any alignment, pitch and length will do (rows that start on 16 bytes and have up to
+ * 32768 elements are faster).  What lies between rows is neither read into a result nor written; y does not overlap x.  A row
+ * with an infinity or a NaN is NaN, and so is an fp32 row whose sum or sum of squares goes beyond fp32. */
+typedef struct clpk_layer_norm_args {
+    int           dtype;
+    int           weight_dtype;
+    uint32_t      m, d;           /* m may be 0                                      */
+    const void   *d_x;            /* [m][d], pitch ldx                               */
+    const void   *d_weight;       /* [d], or NULL: ones                              */
+    const void   *d_bias;         /* [d], or NULL: zeros                             */
+    void         *d_y;            /* [m][d], pitch ldy                               */
+    float        *d_mean;         /* [m], or NULL: for the backward pass             */
+    float        *d_rstd;         /* [m], or NULL                                    */
+    uint64_t      ldx, ldy;
+    float         eps;            /* >= 0; with 0 a row of equal elements is NaN     */
+} clpk_layer_norm_args_t;
+
+CLPK_API int clpk_layer_norm(const clpk_layer_norm_args_t *args, void *stream);
+
+/* Gradients of clpk_layer_norm, from that of y and the mean and rstd that it kept: with xhat = (x - mean) * rstd, g = dy * weight
+ *   dx = rstd * (g - sum g / d - xhat * sum (g * xhat) / d),   dweight = sum over rows of dy * xhat,   dbias = sum over rows of dy
+ * in fp32 and rounded once.  Any of d_dx, d_dweight and d_dbias may be NULL: what is not asked for is not computed.  Sums are formed
+ * in the same order in every call.  m = 0: dweight and dbias are zeros. */
+typedef struct clpk_layer_norm_backward_args {
+    int           dtype;          /* of x, dy and dx                                 */
+    int           weight_dtype;   /* of weight, dweight and dbias                    */
+    uint32_t      m, d;
+    const void   *d_x;            /* [m][d], pitch ldx                               */
+    const void   *d_weight;       /* [d], or NULL: ones                              */
+    const void   *d_dy;           /* [m][d], pitch lddy                              */
+    const float  *d_mean;         /* [m]                                             */
+    const float  *d_rstd;         /* [m]                                             */
+    void         *d_dx;           /* [m][d], pitch lddx                              */
+    void         *d_dweight;      /* [d]                                             */
+    void         *d_dbias;        /* [d]                                             */
+    uint64_t      ldx, lddy, lddx;
+    void         *d_workspace;    /* 16-byte aligned; for d_dweight and d_dbias      */
+    size_t        workspace_bytes;
+} clpk_layer_norm_backward_args_t;
+
+/* What does for m rows does for fewer. */
+CLPK_API int clpk_layer_norm_backward_workspace_bytes(uint32_t m, uint32_t d, size_t *bytes);
+CLPK_API int clpk_layer_norm_backward(const clpk_layer_norm_backward_args_t *args, void *stream);
+
+/* One step of Adam with decoupled weight decay over all tensors of a list, in fp32 whatever their types, each operation rounded:
+ *   g' = g * grad_scale
+ *   m  = beta1 * m + (1 - beta1) * g'
+ *   v  = beta2 * v + (1 - beta2) * g' * g'
+ *   p  = p * (1 - lr * weight_decay) - m / (sqrt(v) * (1 / sqrt(1 - beta2^step)) + eps) * (lr / (1 - beta1^step))
+ * Moments in 32 bits (state_dtype CLPK_DT_F32), or in 8 (CLPK_DT_I8): each 256 elements of a tensor, the last ones fewer, share two
+ * scales, and m and the root of v are their scales times squares of whole numbers:
+ *   m = m_scale * q * |q|,        q = sign(m) * rint(sqrt(|m| * (1 / m_scale))) in [-127, 127],  m_scale = max |m| / 127^2
+ *   sqrt(v) = v_scale * c^2,      c = max(1, rint(sqrt(sqrt(v) * (1 / v_scale)))) in [1, 255],   v_scale = max sqrt(v) / 255^2
+ * with c = 0 only where v is 0; zeros and zero scales are moments of zero.  The step itself takes the moments before they are
+ * rounded.  A block whose scale would be below 2^-126 has the scale 0 and codes of 0; one with an infinity or a NaN has the scale NaN
+ * and codes of 0.
+ * With a master copy the step is taken on it and the parameter is its rounded value.  Tensors and arrays do not overlap; any
+ * alignment and length will do, 0 included (those that start on 16 bytes are faster).  Element types and their alignment:
+ * those of the arrays. */
+#define CLPK_ADAMW_BLOCK 256
+
+typedef struct clpk_adamw_tensor {
+    uint64_t      n;              /* elements                                        */
+    void         *d_param;        /* [n] of `dtype`                                  */
+    const void   *d_grad;         /* [n] of `grad_dtype`                             */
+    float        *d_master;       /* [n]: of all tensors, or NULL of all             */
+    void         *d_m;            /* [n] float, or int8_t                            */
+    void         *d_v;            /* [n] float, or uint8_t                           */
+    float        *d_m_scale;      /* [ceil(n / 256)]; 8 bits only                    */
+    float        *d_v_scale;      /* [ceil(n / 256)]; 8 bits only                    */
+} clpk_adamw_tensor_t;
+
+typedef struct clpk_adamw_args {
+    int           dtype;          /* CLPK_DT_F32, F16 or BF16: of the parameters     */
+    int           grad_dtype;     /* `dtype` or CLPK_DT_F32                          */
+    int           state_dtype;    /* CLPK_DT_F32 or CLPK_DT_I8                       */
+    uint32_t      count;
+    const clpk_adamw_tensor_t *h_tensors;   /* [count], read before the call returns */
+    double        lr, beta1, beta2, eps, weight_decay;
+    uint64_t      step;           /* from 1; unused with d_step                      */
+    const float  *d_lr;           /* NULL, or read by the step in place of lr        */
+    const uint32_t *d_step;       /* NULL, or read by the step in place of step      */
+    const float  *d_grad_scale;   /* NULL: 1                                         */
+} clpk_adamw_args_t;
+
+CLPK_API int clpk_adamw(const clpk_adamw_args_t *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
