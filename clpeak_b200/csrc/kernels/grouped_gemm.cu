@@ -1,0 +1,900 @@
+// Products of rows that lie sorted by group (tokens by expert), each group with weights of its own, and their gradients.
+//
+//   forward    C[r] = A[r] W[e]^T              rows r of group e
+//   backward   dA[r] = dC[r] W[e],  dW[e] = sum over the group's rows of dC[r]^T A[r]
+//
+// On CTA pairs: TMA ring, M = 256 instructions of a pair, two accumulators in tensor memory.  The side of 256 is always the side that
+// is contiguous in the result: features of C, of dA or of dW's rows.  The side of N is what is ragged: a group's rows (or the
+// rows of dW[e]), any multiple of 32 up to 256.  A group of one row then costs an instruction of N = 32 and loads of 16 rows, one of
+// 300 two of 160, and no tile reaches into the next group's results.  In tensor memory a lane has a feature and a column a row, so
+// that a warp's 32 lanes store 32 neighbours of each row, and rows that are no group's are never touched.
+//
+//   forward    M side: W[e], K contiguous             N side: rows of A, K contiguous
+//   dA         M side: W[e]^T as it lies, M contiguous  N side: rows of dC, K contiguous
+//   dW         M side: A^T as it lies, M contiguous     N side: dC^T as it lies, N contiguous; K: the group's rows
+//
+// dW's sums are ragged in K: the last block of 64 rows reaches into the next group.  Its loads land on a barrier of each CTA's own, a
+// warp overwrites the rows behind the group with zeros -- in these layouts a row is 128 bytes of a box, whatever the swizzle -- and then
+// tells the pair's barrier.
+//
+// Sizes of groups are known on the device alone.  grouped_plan_kernel turns them into tiles, in front of the main kernel: most are
+// dealt to the pairs in turn, so that neighbours share operands in the L2, and the last half to one and a half rounds are cut by cost, also inside
+// their sums, so that all pairs finish together (pairs_start).  A tile that several pairs have summed is finished by the
+// one that comes last, in the order of K: the sums are the same in every call.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "../clpk_elements.cuh"
+#include "../clpk_internal.h"
+#include "../clpk_pair.cuh"
+#include "../clpk_ptx.cuh"
+
+namespace clpk {
+
+enum GroupedKind : uint32_t { kForward = 0, kRowGrad = 1, kWeightGrad = 2 };
+
+constexpr uint32_t kGroupedMost = 1024;                         // groups
+constexpr uint32_t kGroupedPairs = 74;                          // of a whole B200: the workspace's size may not depend on the card at hand
+constexpr uint32_t kGroupedM = 256, kGroupedN = 256, kGroupedK = 64;
+constexpr uint32_t kGroupedStages = 6, kGroupedStageBytes = 2 * kHalfTileBytes;
+constexpr int kGroupedSets = 4, kGroupedEpilogueWarps = 4 * kGroupedSets;
+constexpr int kGroupedZeroWarp = 2 + kGroupedEpilogueWarps;
+constexpr int kGroupedThreads = 32 * (kGroupedZeroWarp + 1);
+constexpr uint32_t kGroupedChunk = 32;                          // columns of an accumulator that a warp takes at a time
+constexpr uint32_t kGroupedUnits = 2 * 4 * (kGroupedN / kGroupedChunk);     // of a tile: CTA, lane quarter, chunk
+constexpr uint32_t kGroupedCutTiles = 2 * kGroupedPairs;        // tiles that may be cut, at most
+constexpr uint32_t kGroupedSlotFloats = kGroupedM * kGroupedN;
+constexpr uint32_t kGroupedLeast = 6;                           // K blocks of a part; fewer stay with the pair before or behind
+constexpr uint32_t kGroupedTileCost = 6;                        // what a tile takes besides its K blocks, in K blocks
+
+constexpr uint32_t kMnLead = 64 * kRowBytesK;                   // as in clpk_linear_grad.cuh: from one box of 64 elements along M or N to the next
+constexpr uint32_t kMnStep = 16 * kRowBytesK / 16;              // 16 rows of K, in the descriptor's units of 16 bytes
+
+constexpr uint32_t kBadOffsets = 0x401u;
+
+// Sums over rows are written group after group: `lists` of `groups` entries each, with a kind.
+struct GroupedShape {
+    uint32_t m, groups, lists;
+    uint32_t kind[2];
+    uint32_t feature_tiles[3], k_blocks[3];                     // by kind; k_blocks of dW: by group
+    uint32_t dw_cols, dw_width;                                 // tiles along dW's rows, and their width
+    uint32_t pairs;
+};
+
+struct GroupTiles {
+    uint32_t cols, width, features, k_blocks;                   // tiles along N and their width, tiles along M
+};
+
+__host__ __device__ __forceinline__ GroupTiles group_tiles(const GroupedShape &p, uint32_t kind, uint32_t rows)
+{
+    if (kind == kWeightGrad)
+        return {p.dw_cols, p.dw_width, p.feature_tiles[kind], rows ? (rows + kGroupedK - 1) / kGroupedK : 1};   // of none: zeros
+    const uint32_t cols = (rows + kGroupedN - 1) / kGroupedN;
+    return {cols, cols ? ((rows + cols - 1) / cols + 31) / 32 * 32 : 32, p.feature_tiles[kind], p.k_blocks[kind]};
+}
+
+// What a K block takes, in units of a column: loading and multiplying 256 features and `width` rows
+__device__ __forceinline__ uint32_t block_cost(uint32_t width) { return 200 + width; }
+
+// A place in the list of tiles
+struct GroupedPlace {
+    uint32_t tile, kb;
+};
+
+// In the workspace, in front of the partial sums.
+struct GroupedPlan {
+    uint32_t n_tiles, whole;                                    // `whole`: tiles that are dealt out, a multiple of the pairs
+    GroupedPlace start[kGroupedPairs + 1];                      // of each pair in the rest
+    uint32_t offsets[kGroupedMost + 1];
+    uint32_t first[2 * kGroupedMost + 1];                       // tile of each entry
+    alignas(16) uint32_t done[kGroupedCutTiles * kGroupedUnits];        // K blocks that have been added
+};
+constexpr uint64_t kGroupedPartsAt = (sizeof(GroupedPlan) + 1023) / 1024 * 1024;
+constexpr uint64_t kGroupedWorkspace = kGroupedPartsAt + 2ull * kGroupedPairs * kGroupedSlotFloats * 4;
+
+// ---- the plan -------------------------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 512;
+
+template <typename T>
+__device__ __forceinline__ T plan_scan(T own, T *warps, T &total)       // exclusive, over the CTA
+{
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const T v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= (uint32_t)o)
+            sum += v;
+    }
+    __syncthreads();                                            // the last scan's words have been read
+    if (lane == 31)
+        warps[warp] = sum;
+    __syncthreads();
+    T before = 0;
+    total = 0;
+    for (uint32_t w = 0; w < kPlanThreads / 32; w++) {
+        if (w < warp)
+            before += warps[w];
+        total += warps[w];
+    }
+    return before + sum - own;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) grouped_plan_kernel(const int32_t *offsets, GroupedPlan *plan, uint32_t *status, GroupedShape p)
+{
+    __shared__ uint32_t off[kGroupedMost + 1], first[2 * kGroupedMost + 1];
+    __shared__ unsigned long long rest[2 * kGroupedMost + 1], load[kGroupedPairs], begins[kGroupedPairs + 1], warps64[kPlanThreads / 32];
+    __shared__ uint32_t warps32[kPlanThreads / 32];
+    const uint32_t t = threadIdx.x, entries = p.lists * p.groups;
+    griddep_wait();
+    griddep_launch_dependents();
+    bool bad = false;
+    for (uint32_t i = t; i <= p.groups; i += kPlanThreads) {
+        const int32_t v = offsets[i];
+        off[i] = (uint32_t)v;
+        bad |= v < 0 || (uint32_t)v > p.m || (i > 0 && offsets[i - 1] > v);
+    }
+    for (uint32_t i = t; i < kGroupedPairs; i += kPlanThreads)
+        load[i] = 0;
+    bad = __syncthreads_or(bad);
+    if (t == 0)
+        *status = bad ? kBadOffsets : 0u;
+
+    auto shape = [&](uint32_t i, unsigned long long &cost) {
+        const uint32_t list = i / p.groups, e = i - list * p.groups;
+        const GroupTiles g = group_tiles(p, p.kind[list], off[e + 1] - off[e]);
+        cost = (unsigned long long)(g.k_blocks + kGroupedTileCost) * block_cost(g.width);
+        return g;
+    };
+    // tiles of the entries, one behind another
+    const uint32_t each = (entries + kPlanThreads - 1) / kPlanThreads, i0 = min(t * each, entries), i1 = min(i0 + each, entries);
+    unsigned long long cost;
+    uint32_t own = 0, n_tiles;
+    for (uint32_t i = i0; i < i1 && !bad; i++) {
+        const GroupTiles g = shape(i, cost);
+        own += g.cols * g.features;
+    }
+    uint32_t at = plan_scan(own, warps32, n_tiles);
+    for (uint32_t i = i0; i < i1; i++) {
+        first[i] = at;
+        if (!bad) {
+            const GroupTiles g = shape(i, cost);
+            at += g.cols * g.features;
+        }
+    }
+    if (t == 0)
+        first[entries] = n_tiles;
+    // half a round to one and a half are left for cutting
+    const uint32_t whole = n_tiles >= p.pairs + p.pairs / 2 ? (n_tiles - p.pairs / 2) / p.pairs * p.pairs : 0;
+    __syncthreads();
+    // what each pair has of the others
+    if (whole) {
+        const uint32_t c = t % 128;
+        unsigned long long sum = 0;
+        if (c < p.pairs) {
+            const auto below = [&](uint32_t x) { return (x + p.pairs - 1 - c) / p.pairs; };     // tiles of this pair in front of x
+            for (uint32_t i = t / 128; i < entries && first[i] < whole; i += kPlanThreads / 128) {
+                const uint32_t n = below(min(first[i + 1], whole)) - below(first[i]);
+                if (n) {
+                    shape(i, cost);
+                    sum += n * cost;
+                }
+            }
+            atomicAdd(&load[c], sum);
+        }
+    }
+    // cost of the rest, entry after entry
+    unsigned long long mine = 0, total;
+    for (uint32_t i = i0; i < i1; i++)
+        if (first[i + 1] > whole) {
+            shape(i, cost);
+            mine += (first[i + 1] - max(first[i], whole)) * cost;
+        }
+    unsigned long long from = plan_scan(mine, warps64, total);
+    for (uint32_t i = i0; i < i1; i++) {
+        rest[i] = from;
+        if (first[i + 1] > whole) {
+            shape(i, cost);
+            from += (first[i + 1] - max(first[i], whole)) * cost;
+        }
+    }
+    if (t == 0)
+        rest[entries] = total;
+    __syncthreads();
+    // Where the pairs begin in the rest: each fills up to one level what it has.
+    if (t < 32) {
+        constexpr uint32_t kEach = (kGroupedPairs + 31) / 32;
+        double have[kEach], level = 0;
+        for (int round = 0; round < 6; round++) {
+            double sum = 0;
+            uint32_t count = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kEach; j++) {
+                const uint32_t c = t * kEach + j;
+                have[j] = c < p.pairs ? (double)load[c] : 1e300;
+                if (c < p.pairs && (round == 0 || have[j] < level)) {
+                    sum += have[j];
+                    count++;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                count += __shfl_xor_sync(0xffffffffu, count, o);
+            }
+            level = ((double)total + sum) / (double)max(count, 1u);
+        }
+        double room[kEach], sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++) {
+            room[j] = fmax(level - have[j], 0.0);
+            sum += room[j];
+        }
+        double before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double v = __shfl_up_sync(0xffffffffu, before, o);
+            if (t >= (uint32_t)o)
+                before += v;
+        }
+        const double all = __shfl_sync(0xffffffffu, before, 31);
+        before -= sum;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++) {
+            const uint32_t c = t * kEach + j;
+            if (c < p.pairs)
+                begins[c] = all > 0 ? min((unsigned long long)((double)total * (before / all)), total) : 0;
+            before += room[j];
+        }
+    }
+    __syncthreads();
+    for (uint32_t c = t; c <= p.pairs; c += kPlanThreads) {
+        GroupedPlace at = {c == 0 ? whole : n_tiles, 0};
+        if (c > 0 && c < p.pairs && begins[c] < total) {
+            const unsigned long long pos = begins[c];
+            uint32_t lo = 0, hi = entries;                      // the last entry that does not begin behind it
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (rest[mid] <= pos)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            const GroupTiles g = shape(lo, cost);
+            const unsigned long long in = pos - rest[lo];
+            const uint32_t tile = (uint32_t)(in / cost), blocks = (uint32_t)((in - tile * cost) / block_cost(g.width));
+            at.tile = max(first[lo], whole) + tile;
+            // the tile's own cost lies in front of its blocks
+            at.kb = blocks <= kGroupedTileCost ? 0 : blocks - kGroupedTileCost;
+            if (at.kb < kGroupedLeast)
+                at.kb = 0;
+            else if (at.kb + kGroupedLeast > g.k_blocks)
+                at = {at.tile + 1, 0};
+        }
+        plan->start[c] = at;
+    }
+    if (t == 0) {
+        plan->n_tiles = n_tiles;
+        plan->whole = whole;
+    }
+    for (uint32_t i = t; i <= p.groups; i += kPlanThreads)
+        plan->offsets[i] = off[i];
+    for (uint32_t i = t; i <= entries; i += kPlanThreads)
+        plan->first[i] = first[i];
+    uint4 *done = reinterpret_cast<uint4 *>(plan->done);
+    for (uint32_t i = t; i < (n_tiles - whole) * kGroupedUnits / 4; i += kPlanThreads)
+        done[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---- the products ---------------------------------------------------------------------------------------------
+
+struct GroupedMaps {
+    CUtensorMap w;                                              // forward: boxes of 128 features x 64 of K; dA: of 64 rows of K x 64 features
+    CUtensorMap rows[4];                                        // of A or dC, boxes of 16, 32, 64 and 128 rows x 64 of K
+    CUtensorMap a_t, dc_t;                                      // dW: boxes of 64 rows x 64 features
+};
+
+struct GroupedResult {
+    void *base;
+    uint64_t ld, stride;                                        // elements; `stride`: from one group's to the next (dW)
+    uint32_t features;
+    int type;
+};
+
+struct GroupedParams {
+    GroupedShape shape;
+    GroupedResult out[3];                                       // by kind
+    uint32_t dw_rows;                                           // rows of dW[e]
+    GroupedPlan *plan;
+    float *parts;
+    uint32_t *status;
+};
+
+struct GroupedSmem {
+    alignas(16) uint64_t full[kGroupedStages];                  // of the leader: both CTAs' loads
+    uint64_t empty[kGroupedStages];
+    uint64_t tail[kGroupedStages];                              // of each CTA: a last block of dW's rows
+    uint64_t tmem_full[2];
+    uint64_t tmem_empty[2];
+    uint32_t tmem_base;
+    uint32_t n_tiles, whole;
+    GroupedPlace start[kGroupedPairs + 1];
+    uint32_t offsets[kGroupedMost + 1];
+    uint32_t first[2 * kGroupedMost + 1];
+};
+constexpr uint32_t kGroupedSmemBytes = kGroupedStages * kGroupedStageBytes + (uint32_t)sizeof(GroupedSmem);
+static_assert(kGroupedSmemBytes <= kSmemMax, "ring, barriers and the list of groups");
+
+// A tile, or the part of its sum that falls to this pair
+struct GroupedTile {
+    uint32_t kind, group, tile;
+    uint32_t feature, row, width, rows;                         // M side; N side: first row, columns, and those of them that are the group's (or dW's)
+    uint32_t k_blocks, kb0, kb1;
+    uint32_t k_row, k_rows;                                     // dW: the group's rows
+};
+
+// The tiles of a pair, one after another; every role walks the same list.
+struct GroupedWalk {
+    const GroupedParams &p;
+    const GroupedSmem *sh;
+    uint32_t pair, i = 0, entry = 0;
+
+    __device__ __forceinline__ GroupedWalk(const GroupedParams &p, const GroupedSmem *sh, uint32_t pair) : p(p), sh(sh), pair(pair) {}
+
+    __device__ __forceinline__ bool next(GroupedTile &t)
+    {
+        const GroupedShape &s = p.shape;
+        const uint32_t rounds = sh->whole / s.pairs;
+        uint32_t tile, kb0 = 0, kb1 = 0xFFFFFFFFu;
+        if (i < rounds) {
+            tile = pair + i * s.pairs;
+        } else {
+            const GroupedPlace from = sh->start[pair], to = sh->start[pair + 1];
+            tile = from.tile + (i - rounds);
+            kb0 = i == rounds ? from.kb : 0;
+            if (tile > to.tile || (tile == to.tile && kb0 >= to.kb))
+                return false;
+            if (tile == to.tile)
+                kb1 = to.kb;
+        }
+        i++;
+        while (sh->first[entry + 1] <= tile)
+            entry++;
+        const uint32_t list = entry / s.groups, e = entry - list * s.groups, begin = sh->offsets[e], rows = sh->offsets[e + 1] - begin;
+        t.kind = s.kind[list];
+        t.group = e;
+        t.tile = tile;
+        const GroupTiles g = group_tiles(s, t.kind, rows);
+        // strips of eight tiles along N, those fastest: neighbours share what they read
+        const uint32_t at = tile - sh->first[entry], strip = at / (8 * g.features), in = at - strip * 8 * g.features, wide = min(8u, g.cols - strip * 8);
+        const uint32_t col = strip * 8 + in % wide;
+        t.feature = in / wide * kGroupedM;
+        t.width = g.width;
+        t.k_blocks = g.k_blocks;
+        t.kb0 = kb0;
+        t.kb1 = min(kb1, g.k_blocks);
+        t.k_row = begin;
+        t.k_rows = rows;
+        const uint32_t first = col * g.width, all = t.kind == kWeightGrad ? p.dw_rows : rows;
+        t.rows = all > first ? min(all - first, g.width) : 0;
+        t.row = t.kind == kWeightGrad ? first : begin + first;
+        return true;
+    }
+};
+
+// The last block of a group's rows has others behind them.
+__device__ __forceinline__ bool has_tail(const GroupedTile &t) { return t.kind == kWeightGrad && t.k_blocks * kGroupedK != t.k_rows; }
+
+__device__ __forceinline__ void tma_load_pair_3d(void *smem_dst, const CUtensorMap *tmap, int32_t x, int32_t y, int32_t z, uint32_t leader_bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(tmap), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// what another pair has written in this launch
+__device__ __forceinline__ float load_told(const float *p)
+{
+    float v;
+    asm volatile("ld.relaxed.gpu.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+
+// 32 columns of 32 lanes -> rows of the result.  In 16 bits lanes 2i and 2i + 1 exchange halves, so that each has two neighbours of
+// every other row: 4-byte stores, 64 bytes of a row by a warp.
+template <int TYPE>
+__device__ __forceinline__ void store_rows(const float (&v)[kGroupedChunk], const GroupedResult &out, uint64_t row0, uint32_t rows, uint32_t feature, int lane)
+{
+    if constexpr (TYPE == CLPK_DT_F32) {
+        float *to = static_cast<float *>(out.base) + row0 * out.ld + feature + lane;
+        if (feature + lane < out.features) {
+#pragma unroll
+            for (uint32_t j = 0; j < kGroupedChunk; j++)
+                if (j < rows)
+                    to[j * out.ld] = v[j];
+        }
+    } else {
+        const uint32_t odd = lane & 1, f = feature + (lane & ~1);
+        uint16_t *to = static_cast<uint16_t *>(out.base) + (row0 + odd) * out.ld + f;
+#pragma unroll
+        for (uint32_t j = 0; j < kGroupedChunk; j += 2) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+            const uint32_t w = odd ? Element<TYPE>::round2(got, v[j + 1]) : Element<TYPE>::round2(v[j], got);
+            if (j + odd < rows) {
+                if (f + 1 < out.features)
+                    *reinterpret_cast<uint32_t *>(to + j * out.ld) = w;
+                else if (f < out.features)
+                    to[j * out.ld] = (uint16_t)w;
+            }
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_tile_rows(const float (&v)[kGroupedChunk], const GroupedParams &p, const GroupedTile &t, uint32_t col, uint32_t lane_feature, int lane)
+{
+    const GroupedResult &out = p.out[t.kind];
+    if (col >= t.rows)
+        return;
+    const uint32_t rows = t.rows - col;
+    const uint64_t row = t.row + col;
+    GroupedResult to = out;
+    if (t.kind == kWeightGrad)
+        to.base = static_cast<uint8_t *>(out.base) + t.group * out.stride * (out.type == CLPK_DT_F32 ? 4 : 2);
+    if (out.type == CLPK_DT_F32)
+        store_rows<CLPK_DT_F32>(v, to, row, rows, t.feature + lane_feature, lane);
+    else
+        store_rows<DT>(v, to, row, rows, t.feature + lane_feature, lane);
+}
+
+template <int DT, bool BACKWARD>
+__global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedParams p)
+{
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *const smem = smem_raw;
+    if (smem_u32(smem) % 1024 != 0) {                           // the swizzle's period; it is declared so
+        griddep_wait();
+        if (threadIdx.x == 0)
+            *p.status = 0x406u;
+        return;
+    }
+    GroupedSmem *sh = reinterpret_cast<GroupedSmem *>(smem + kGroupedStages * kGroupedStageBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t r = cluster_ctarank(), pair = blockIdx.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kGroupedStages; s++) {
+            mbar_init(&sh->full[s], 2);                         // the leader's producer twice, or both CTAs' warps that write zeros
+            mbar_init(&sh->empty[s], 1);
+            mbar_init(&sh->tail[s], 1);
+        }
+        for (int acc = 0; acc < 2; acc++) {
+            mbar_init(&sh->tmem_full[acc], 1);
+            mbar_init(&sh->tmem_empty[acc], 2 * kGroupedEpilogueWarps);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1)
+        tmem_alloc<2>(&sh->tmem_base, 512);
+    griddep_wait();
+    griddep_launch_dependents();
+    if (threadIdx.x == 0) {
+        sh->n_tiles = p.plan->n_tiles;
+        sh->whole = p.plan->whole;
+    }
+    for (uint32_t i = threadIdx.x; i <= p.shape.pairs; i += kGroupedThreads)
+        sh->start[i] = p.plan->start[i];
+    for (uint32_t i = threadIdx.x; i <= p.shape.groups; i += kGroupedThreads)
+        sh->offsets[i] = p.plan->offsets[i];
+    for (uint32_t i = threadIdx.x; i <= p.shape.lists * p.shape.groups; i += kGroupedThreads)
+        sh->first[i] = p.plan->first[i];
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh->tmem_base;
+    GroupedWalk walk(p, sh, pair);
+    GroupedTile t;
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        const uint32_t full0 = cluster_addr(&sh->full[0], 0);
+        uint32_t s = 0, parity = 1, issued = 0;                 // a fresh barrier's preceding phase counts as complete
+        bool ok = true;
+        while (ok && walk.next(t)) {
+            const bool tail = has_tail(t);
+            const uint32_t half = t.width / 2, feature = t.feature + r * 128;
+            for (uint32_t kb = t.kb0; kb < t.kb1; kb++) {
+                if (!warp_wait(&sh->empty[s], parity)) {
+                    if (lane == 0)
+                        atomicCAS(p.status, 0u, 0x402u);
+                    ok = false;
+                    break;
+                }
+                uint8_t *const a = smem + (size_t)s * kGroupedStageBytes, *const b = a + kHalfTileBytes;
+                const bool last = tail && kb + 1 == t.k_blocks;
+                const uint32_t bytes = kHalfTileBytes + half * kRowBytesK;
+                if (elect_one()) {
+                    if (last) {
+                        mbar_expect_tx(&sh->tail[s], bytes);
+                    } else if (r == 0) {
+                        mbar_expect_tx(&sh->full[s], 2 * bytes);
+                        mbar_arrive(&sh->full[s]);
+                    }
+                    const uint32_t bar = full0 + 8 * s;
+                    if constexpr (!BACKWARD) {
+                        tma_load_pair_3d(a, &maps.w, (int32_t)(kb * kRowBytesK), (int32_t)feature, (int32_t)t.group, bar);
+                    } else if (t.kind == kRowGrad) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 128; i += 64)
+                            tma_load_pair_3d(a + i * kRowBytesK, &maps.w, (int32_t)((feature + i) * 2), (int32_t)(kb * kGroupedK), (int32_t)t.group, bar);
+                    } else {
+                        const int32_t row = (int32_t)(t.k_row + kb * kGroupedK);
+                        auto load = [&](uint8_t *to, const CUtensorMap *map, uint32_t x) {
+                            if (last)
+                                tma_load_own(to, map, (int32_t)(x * 2), row, &sh->tail[s]);
+                            else
+                                tma_load_pair_at(to, map, (int32_t)(x * 2), row, bar);
+                        };
+                        for (uint32_t i = 0; i < 128; i += 64)
+                            load(a + i * kRowBytesK, &maps.a_t, feature + i);
+                        for (uint32_t i = 0; i < half; i += 64)
+                            load(b + i * kRowBytesK, &maps.dc_t, t.row + r * half + i);
+                    }
+                    if (!BACKWARD || t.kind == kRowGrad) {
+                        uint32_t at = 0;
+#pragma unroll
+                        for (int i = 3; i >= 0; i--)
+                            if (half & (16u << i)) {
+                                tma_load_pair_at(b + at * kRowBytesK, &maps.rows[i], (int32_t)(kb * kRowBytesK), (int32_t)(t.row + r * half + at), bar);
+                                at += 16u << i;
+                            }
+                    }
+                }
+                __syncwarp();
+                issued++;
+                if (++s == kGroupedStages) {
+                    s = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+        if (r == 0)
+            ring_settled(sh->full, kGroupedStages, issued);
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (the pair's leader) ----------------
+        if (r == 0) {
+            constexpr uint32_t kFmt = DT == CLPK_DT_BF16 ? kFmtBF16 : kFmtF16;
+            uint32_t s = 0, parity = 0;
+            bool ok = true;
+            for (uint32_t i = 0; ok && walk.next(t); i++) {
+                const uint32_t acc = i & 1, use = i >> 1;
+                if (use > 0 && !warp_wait(&sh->tmem_empty[acc], (use - 1) & 1)) {
+                    if (lane == 0)
+                        atomicCAS(p.status, 0u, 0x403u);
+                    break;
+                }
+                tc_fence_after_sync();
+                const uint32_t d = tmem + acc * kGroupedN;
+                const bool a_mn = BACKWARD, b_mn = BACKWARD && t.kind == kWeightGrad;
+                const uint32_t idesc = make_idesc(kGroupedM, t.width, kFmt, kFmt, kAccF32) | (a_mn ? kMajorA : 0u) | (b_mn ? kMajorB : 0u);
+                const uint32_t a_lbo = a_mn ? kMnLead : 16, a_step = a_mn ? kMnStep : 2, b_lbo = b_mn ? kMnLead : 16, b_step = b_mn ? kMnStep : 2;
+                for (uint32_t kb = t.kb0; kb < t.kb1; kb++) {
+                    if (!warp_wait(&sh->full[s], parity)) {
+                        if (lane == 0)
+                            atomicCAS(p.status, 0u, 0x404u);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t base = smem_u32(smem + (size_t)s * kGroupedStageBytes), s_now = s;
+                    if (++s == kGroupedStages) {
+                        s = 0;
+                        parity ^= 1;
+                    }
+                    if (elect_one()) {
+                        const uint64_t ad = make_smem_desc(base, a_lbo, 1024, kSwizzle128B), bd = make_smem_desc(base + kHalfTileBytes, b_lbo, 1024, kSwizzle128B);
+#pragma unroll
+                        for (uint32_t kk = 0; kk < 4; kk++)
+                            mma2_f16_ss(d, ad + kk * a_step, bd + kk * b_step, idesc, (kb != t.kb0 || kk != 0) ? 1u : 0u);
+                        tc_commit_pair(&sh->empty[s_now], 3);
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one())
+                    tc_commit_pair(&sh->tmem_full[acc], 3);
+                __syncwarp();
+            }
+        }
+    } else if (warp < kGroupedZeroWarp) {
+        // ---------------- epilogue: the warps of a lane quarter take chunks in turn ----------------
+        const uint32_t q = (uint32_t)(warp & 3), set = (uint32_t)(warp - 2) >> 2;
+        const uint32_t lanes = r * 128 + q * 32;                // the warp's features in the tile
+        for (uint32_t i = 0; walk.next(t); i++) {
+            const uint32_t acc = i & 1, use = i >> 1;
+            if (!warp_wait(&sh->tmem_full[acc], use & 1)) {
+                if (lane == 0)
+                    atomicCAS(p.status, 0u, 0x405u);
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t taddr = tmem + acc * kGroupedN + ((q * 32) << 16), chunks = t.width / kGroupedChunk;
+            const bool whole = t.kb0 == 0 && t.kb1 == t.k_blocks;
+            for (uint32_t c = set; c < chunks; c += kGroupedSets) {
+                float v[kGroupedChunk];
+                tmem_ld_32x32b_x32(taddr + c * kGroupedChunk, reinterpret_cast<uint32_t(&)[kGroupedChunk]>(v));
+                tmem_ld_wait();
+                if (c + kGroupedSets >= chunks) {               // the accumulator is free as soon as it has been read
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
+                }
+                if (!whole) {
+                    // this pair's sums go to its slot; whoever brings the last blocks adds all parts, in the order of K
+                    const uint64_t unit = (uint64_t)(r * 4 + q) * kGroupedN + c * kGroupedChunk;
+                    auto slot = [&](uint32_t of, bool inside) { return p.parts + (uint64_t)(2 * of + (inside ? 0 : 1)) * kGroupedSlotFloats + unit * 32 + lane; };
+                    float *to = slot(pair, t.kb0 > 0);
+#pragma unroll
+                    for (uint32_t j = 0; j < kGroupedChunk; j++)
+                        to[j * 32] = v[j];
+                    __threadfence();
+                    __syncwarp();
+                    uint32_t before = 0;
+                    if (lane == 0)
+                        before = atomicAdd(&p.plan->done[(t.tile - sh->whole) * kGroupedUnits + (r * 4 + q) * (kGroupedN / kGroupedChunk) + c], t.kb1 - t.kb0);
+                    if (__shfl_sync(0xffffffffu, before, 0) + (t.kb1 - t.kb0) != t.k_blocks)
+                        continue;
+                    __threadfence();
+                    uint32_t of = pair;
+                    while (sh->start[of].tile == t.tile && sh->start[of].kb > 0)
+                        of--;
+                    bool begun = false;
+                    for (; of < p.shape.pairs; of++) {
+                        const GroupedPlace from = sh->start[of], end = sh->start[of + 1];
+                        if (from.tile > t.tile || (begun && from.tile == t.tile && from.kb == 0))
+                            break;
+                        if (from.tile == end.tile && from.kb == end.kb)
+                            continue;
+                        if (end.tile < t.tile || (end.tile == t.tile && end.kb == 0))
+                            continue;
+                        const float *at = slot(of, from.tile == t.tile && from.kb > 0);
+#pragma unroll
+                        for (uint32_t j = 0; j < kGroupedChunk; j++)
+                            v[j] = begun ? v[j] + load_told(at + j * 32) : load_told(at + j * 32);
+                        begun = true;
+                    }
+                }
+                store_tile_rows<DT>(v, p, t, c * kGroupedChunk, lanes, lane);
+            }
+            if (set >= chunks) {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
+            }
+        }
+    } else if (BACKWARD) {
+        // ---------------- zeros behind a group's last rows ----------------
+        uint32_t blocks = 0, uses = 0;                          // K blocks so far; a bit for each stage: the parity of its next tail
+        const uint32_t full0 = cluster_addr(&sh->full[0], 0);
+        while (walk.next(t)) {
+            if (has_tail(t) && t.kb1 == t.k_blocks) {
+                const uint32_t s = (blocks + (t.kb1 - t.kb0) - 1) % kGroupedStages;
+                if (!warp_wait(&sh->tail[s], uses >> s & 1)) {
+                    if (lane == 0)
+                        atomicCAS(p.status, 0u, 0x407u);
+                    break;
+                }
+                uses ^= 1u << s;
+                const uint32_t rows = t.k_rows - (t.k_blocks - 1) * kGroupedK;      // of none: zeros all
+                uint8_t *const st = smem + (size_t)s * kGroupedStageBytes;
+                const uint32_t boxes = 2 + t.width / 128, each = (kGroupedK - rows) * (kRowBytesK / 16);
+                for (uint32_t i = lane; i < boxes * each; i += 32) {
+                    const uint32_t box = i / each, at = i - box * each;
+                    *reinterpret_cast<uint4 *>(st + box * kMnLead + rows * kRowBytesK + at * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive_remote(full0 + 8 * s);
+            }
+            blocks += t.kb1 - t.kb0;
+        }
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1)
+        tmem_dealloc<2>(tmem, 512);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------
+
+// boxes of 128 bytes of a row times box_rows rows; of three dimensions where `groups` > 0
+static int make_grouped_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t row_elems, uint64_t pitch, uint32_t box_rows, uint64_t groups = 0, uint64_t stride = 0)
+{
+    EncodeTiledFn enc = nullptr;
+    CLPK_TRY(get_encode_fn(&enc));
+    const cuuint64_t dims[3] = {row_elems * 2, rows, groups}, strides[2] = {pitch * 2, stride * 2};
+    const cuuint32_t box[3] = {kRowBytesK, box_rows, 1}, estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, groups ? 3 : 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled (grouped) failed with CUresult %d", (int)r);
+        return CLPK_ERR_CUDA;
+    }
+    return CLPK_OK;
+}
+
+static uint32_t up_div(uint64_t a, uint32_t b) { return (uint32_t)((a + b - 1) / b); }
+
+static int run_grouped(const GroupedMaps &maps, GroupedParams &p, int dtype, bool backward, const int32_t *offsets, void *workspace, cudaStream_t s)
+{
+    p.plan = static_cast<GroupedPlan *>(workspace);
+    p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kGroupedPartsAt);
+    p.shape.pairs = std::min(kGroupedPairs, (uint32_t)num_sms() / 2);
+    CLPK_TRY(launch_behind(grouped_plan_kernel, "grouped_plan", 1, kPlanThreads, 0, s, offsets, p.plan, p.status, p.shape));
+    const uint32_t ctas = 2 * p.shape.pairs;
+    if (backward)
+        return dtype == CLPK_DT_F16 ? launch_clusters(grouped_kernel<CLPK_DT_F16, true>, "grouped (gradients)", ctas, kGroupedThreads, kGroupedSmemBytes, 2, s, maps, p)
+                                    : launch_clusters(grouped_kernel<CLPK_DT_BF16, true>, "grouped (gradients)", ctas, kGroupedThreads, kGroupedSmemBytes, 2, s, maps, p);
+    return dtype == CLPK_DT_F16 ? launch_clusters(grouped_kernel<CLPK_DT_F16, false>, "grouped", ctas, kGroupedThreads, kGroupedSmemBytes, 2, s, maps, p)
+                                : launch_clusters(grouped_kernel<CLPK_DT_BF16, false>, "grouped", ctas, kGroupedThreads, kGroupedSmemBytes, 2, s, maps, p);
+}
+
+// ---- what the calls ask of their arguments --------------------------------------------------------------------
+
+static int check_grouped(const char *what, int dtype, int out_dtype, uint32_t m, uint32_t n, uint32_t k, uint32_t groups)
+{
+    CLPK_REQUIRE(dtype == CLPK_DT_BF16 || dtype == CLPK_DT_F16, "%s: dtype %d is not BF16 or F16", what, dtype);
+    CLPK_REQUIRE(out_dtype == dtype || out_dtype == CLPK_DT_F32, "%s: results of type %d are neither dtype nor F32", what, out_dtype);
+    CLPK_REQUIRE(n > 0 && k > 0, "%s: only the number of rows may be 0 (got %u x %u)", what, n, k);
+    CLPK_REQUIRE(groups > 0 && groups <= kGroupedMost, "%s: %u groups, of 1 to %u", what, groups, kGroupedMost);
+    // whole tiles and K blocks have to have 32-bit coordinates, and the tiles of both gradients a 32-bit number
+    const uint64_t rows = m / kGroupedN + groups, tiles = (up_div(n, kGroupedM) + (uint64_t)up_div(k, kGroupedM)) * rows + (uint64_t)groups * up_div(k, kGroupedM) * up_div(n, 128);
+    CLPK_REQUIRE(m <= 0x7FFFFE00u && n <= 0x1FFFFF00u && k <= 0x1FFFFF00u && tiles <= 1u << 30, "%s: %u x %u x %u in %u groups is too large", what, m, n, k, groups);
+    return CLPK_OK;
+}
+
+// the pitch of a matrix; 0 in *ld: rows one behind another
+static int check_grouped_matrix(const char *what, const char *name, const void *base, uint64_t cols, uint64_t *ld, uint64_t elem)
+{
+    if (*ld == 0)
+        *ld = cols;
+    CLPK_REQUIRE(base, "%s: %s is NULL", what, name);
+    CLPK_REQUIRE(*ld >= cols && *ld < 1ull << 35, "%s: the pitch of %s, %llu, is shorter than its rows of %llu, or too large", what, name, (unsigned long long)*ld,
+                 (unsigned long long)cols);
+    CLPK_REQUIRE(*ld * elem % 16 == 0 && (uintptr_t)base % 16 == 0, "%s: %s must start on 16 bytes and its pitch (%llu elements of %llu bytes) be a multiple of 16 bytes",
+                 what, name, (unsigned long long)*ld, (unsigned long long)elem);
+    return CLPK_OK;
+}
+
+// the elements from one group's matrix to the next; 0 in *stride: one behind another
+static int check_grouped_stride(const char *what, const char *name, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t *stride, uint64_t elem, uint32_t groups)
+{
+    if (*stride == 0 || groups == 1)
+        *stride = rows * ld;
+    CLPK_REQUIRE(*stride >= (rows - 1) * ld + cols && *stride < 1ull << 38, "%s: %s, %llu, is shorter than %llu rows, or too large", what, name, (unsigned long long)*stride,
+                 (unsigned long long)rows);
+    CLPK_REQUIRE(*stride * elem % 16 == 0, "%s: %s (%llu elements of %llu bytes) must be a multiple of 16 bytes", what, name, (unsigned long long)*stride, (unsigned long long)elem);
+    return CLPK_OK;
+}
+
+static int check_grouped_rest(const char *what, const int32_t *offsets, const void *workspace, size_t bytes, const uint32_t *status)
+{
+    CLPK_REQUIRE(offsets && (uintptr_t)offsets % 4 == 0, "%s: d_offsets must be an array of 32-bit integers", what);
+    CLPK_REQUIRE(workspace && bytes >= kGroupedWorkspace && (uintptr_t)workspace % 16 == 0, "%s: needs a 16-byte aligned workspace of %llu bytes", what,
+                 (unsigned long long)kGroupedWorkspace);
+    CLPK_REQUIRE(status && (uintptr_t)status % 4 == 0, "%s: d_status must be a device word", what);
+    return CLPK_OK;
+}
+
+} // namespace clpk
+
+using namespace clpk;
+
+extern "C" {
+
+int clpk_grouped_gemm_workspace_bytes(uint32_t groups, size_t *bytes)
+{
+    CLPK_REQUIRE(bytes, "bytes is NULL");
+    *bytes = 0;
+    CLPK_REQUIRE(groups > 0 && groups <= kGroupedMost, "clpk_grouped_gemm: %u groups, of 1 to %u", groups, kGroupedMost);
+    *bytes = (size_t)kGroupedWorkspace;
+    return CLPK_OK;
+}
+
+int clpk_grouped_gemm(const clpk_grouped_gemm_args_t *args, void *stream)
+{
+    CLPK_TRY(require_sm100());
+    const char *what = "clpk_grouped_gemm";
+    CLPK_REQUIRE(args, "%s: args is NULL", what);
+    clpk_grouped_gemm_args_t a = *args;
+    CLPK_TRY(check_grouped(what, a.dtype, a.out_dtype, a.m, a.n, a.k, a.groups));
+    CLPK_TRY(check_grouped_rest(what, a.d_offsets, a.d_workspace, a.workspace_bytes, a.d_status));
+    cudaStream_t s = as_stream(stream);
+    if (a.m == 0) {
+        CLPK_CUDA(cudaMemsetAsync(a.d_status, 0, sizeof(uint32_t), s));
+        return CLPK_OK;
+    }
+    const uint64_t out_elem = element_bytes(a.out_dtype);
+    CLPK_TRY(check_grouped_matrix(what, "d_a", a.d_a, a.k, &a.lda, 2));
+    CLPK_TRY(check_grouped_matrix(what, "d_w", a.d_w, a.k, &a.ldw, 2));
+    CLPK_TRY(check_grouped_stride(what, "stride_w", a.n, a.k, a.ldw, &a.stride_w, 2, a.groups));
+    CLPK_TRY(check_grouped_matrix(what, "d_c", a.d_c, a.n, &a.ldc, out_elem));
+    GroupedMaps maps = {};
+    CLPK_TRY(make_grouped_map(&maps.w, a.d_w, a.n, a.k, a.ldw, 128, a.groups, a.stride_w));
+    for (uint32_t i = 0; i < 4; i++)
+        CLPK_TRY(make_grouped_map(&maps.rows[i], a.d_a, a.m, a.k, a.lda, 16u << i));
+    GroupedParams p = {};
+    p.shape.m = a.m;
+    p.shape.groups = a.groups;
+    p.shape.lists = 1;
+    p.shape.kind[0] = kForward;
+    p.shape.feature_tiles[kForward] = up_div(a.n, kGroupedM);
+    p.shape.k_blocks[kForward] = up_div(a.k, kGroupedK);
+    p.out[kForward] = {a.d_c, a.ldc, 0, a.n, a.out_dtype};
+    p.status = a.d_status;
+    return run_grouped(maps, p, a.dtype, false, a.d_offsets, a.d_workspace, s);
+}
+
+int clpk_grouped_gemm_backward(const clpk_grouped_gemm_backward_args_t *args, void *stream)
+{
+    CLPK_TRY(require_sm100());
+    const char *what = "clpk_grouped_gemm_backward";
+    CLPK_REQUIRE(args, "%s: args is NULL", what);
+    clpk_grouped_gemm_backward_args_t a = *args;
+    CLPK_TRY(check_grouped(what, a.dtype, a.dw_dtype, a.m, a.n, a.k, a.groups));
+    CLPK_TRY(check_grouped_rest(what, a.d_offsets, a.d_workspace, a.workspace_bytes, a.d_status));
+    const uint64_t dw_elem = element_bytes(a.dw_dtype);
+    if (a.d_dw) {
+        CLPK_TRY(check_grouped_matrix(what, "d_dw", a.d_dw, a.k, &a.lddw, dw_elem));
+        CLPK_TRY(check_grouped_stride(what, "stride_dw", a.n, a.k, a.lddw, &a.stride_dw, dw_elem, a.groups));
+    }
+    cudaStream_t s = as_stream(stream);
+    if (a.m == 0 || (!a.d_da && !a.d_dw)) {
+        CLPK_CUDA(cudaMemsetAsync(a.d_status, 0, sizeof(uint32_t), s));
+        for (uint32_t e = 0; e < a.groups && a.d_dw; e++)
+            CLPK_CUDA(cudaMemset2DAsync(static_cast<uint8_t *>(a.d_dw) + e * a.stride_dw * dw_elem, a.lddw * dw_elem, 0, (size_t)a.k * dw_elem, a.n, s));
+        return CLPK_OK;
+    }
+    CLPK_TRY(check_grouped_matrix(what, "d_dc", a.d_dc, a.n, &a.lddc, 2));
+    GroupedMaps maps = {};
+    GroupedParams p = {};
+    p.shape.m = a.m;
+    p.shape.groups = a.groups;
+    p.dw_rows = a.n;
+    p.status = a.d_status;
+    if (a.d_da) {
+        CLPK_TRY(check_grouped_matrix(what, "d_da", a.d_da, a.k, &a.ldda, 2));
+        CLPK_TRY(check_grouped_matrix(what, "d_w", a.d_w, a.k, &a.ldw, 2));
+        CLPK_TRY(check_grouped_stride(what, "stride_w", a.n, a.k, a.ldw, &a.stride_w, 2, a.groups));
+        CLPK_TRY(make_grouped_map(&maps.w, a.d_w, a.n, a.k, a.ldw, kGroupedK, a.groups, a.stride_w));
+        for (uint32_t i = 0; i < 4; i++)
+            CLPK_TRY(make_grouped_map(&maps.rows[i], a.d_dc, a.m, a.n, a.lddc, 16u << i));
+        p.shape.kind[p.shape.lists++] = kRowGrad;
+        p.shape.feature_tiles[kRowGrad] = up_div(a.k, kGroupedM);
+        p.shape.k_blocks[kRowGrad] = up_div(a.n, kGroupedK);
+        p.out[kRowGrad] = {a.d_da, a.ldda, 0, a.k, a.dtype};
+    }
+    if (a.d_dw) {
+        CLPK_TRY(check_grouped_matrix(what, "d_a", a.d_a, a.k, &a.lda, 2));
+        CLPK_TRY(make_grouped_map(&maps.a_t, a.d_a, a.m, a.k, a.lda, kGroupedK));
+        CLPK_TRY(make_grouped_map(&maps.dc_t, a.d_dc, a.m, a.n, a.lddc, kGroupedK));
+        p.shape.kind[p.shape.lists++] = kWeightGrad;
+        p.shape.feature_tiles[kWeightGrad] = up_div(a.k, kGroupedM);
+        p.shape.dw_width = a.n <= 128 ? 128 : 256;              // whole boxes of 64 for each CTA
+        p.shape.dw_cols = up_div(a.n, p.shape.dw_width);
+        p.out[kWeightGrad] = {a.d_dw, a.lddw, a.stride_dw, a.k, a.dw_dtype};
+    }
+    return run_grouped(maps, p, a.dtype, true, a.d_offsets, a.d_workspace, s);
+}
+
+} // extern "C"

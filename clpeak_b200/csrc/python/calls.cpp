@@ -99,7 +99,8 @@ template <> struct Arg<float> {
 // structures that a call takes by reference
 template <typename P, typename... S> constexpr bool is_one_of = (std::is_same<P, const S>::value || ...);
 template <typename P> constexpr bool is_args = is_one_of<P, clpk_gemm_args_t, clpk_gemm_i8_scaled_args_t, clpk_gated_ffn_args_t, clpk_gated_ffn_backward_args_t,
-                                                         clpk_layer_norm_args_t, clpk_layer_norm_backward_args_t, clpk_adamw_args_t>;
+                                                         clpk_layer_norm_args_t, clpk_layer_norm_backward_args_t, clpk_adamw_args_t, clpk_grouped_gemm_args_t,
+                                                         clpk_grouped_gemm_backward_args_t>;
 
 template <typename P> struct Arg<P *, std::enable_if_t<!is_args<P>>> {
     P *v;
@@ -192,7 +193,8 @@ const struct {
     vectorcallfunc invoke;
 } kCalls[] = {CALL(clpk_fill_f32), CALL(clpk_fill_i8), CALL(clpk_convert_f32), CALL(clpk_absmax_f32), CALL(clpk_quantize_fp4), CALL(clpk_stream_read),
               CALL(clpk_stream_copy), CALL(clpk_stream_triad), CALL(clpk_gemm), CALL(clpk_gemm_pack_scales), CALL(clpk_quantize_rows_i8), CALL(clpk_gemm_i8_scaled),
-              CALL(clpk_gated_ffn), CALL(clpk_gated_ffn_backward), CALL(clpk_layer_norm), CALL(clpk_layer_norm_backward), CALL(clpk_adamw)};
+              CALL(clpk_gated_ffn), CALL(clpk_gated_ffn_backward), CALL(clpk_layer_norm), CALL(clpk_layer_norm_backward), CALL(clpk_adamw),
+              CALL(clpk_grouped_gemm), CALL(clpk_grouped_gemm_backward)};
 
 int call_traverse(PyObject *self, visitproc visit, void *arg)
 {

@@ -164,6 +164,30 @@ class AdamwArgs(C.Structure):
     ]
 
 
+class GroupedGemmArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("out_dtype", C.c_int),
+        ("m", C.c_uint32), ("n", C.c_uint32), ("k", C.c_uint32), ("groups", C.c_uint32),
+        ("d_a", C.c_void_p), ("d_w", C.c_void_p), ("d_offsets", C.c_void_p), ("d_c", C.c_void_p),
+        ("lda", C.c_uint64), ("ldw", C.c_uint64), ("stride_w", C.c_uint64), ("ldc", C.c_uint64),
+        ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("d_status", C.c_void_p),
+    ]
+
+
+class GroupedGemmBackwardArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("dw_dtype", C.c_int),
+        ("m", C.c_uint32), ("n", C.c_uint32), ("k", C.c_uint32), ("groups", C.c_uint32),
+        ("d_a", C.c_void_p), ("d_w", C.c_void_p), ("d_offsets", C.c_void_p),
+        ("d_dc", C.c_void_p), ("d_da", C.c_void_p), ("d_dw", C.c_void_p),
+        ("lda", C.c_uint64), ("ldw", C.c_uint64), ("stride_w", C.c_uint64), ("lddc", C.c_uint64), ("ldda", C.c_uint64), ("lddw", C.c_uint64),
+        ("stride_dw", C.c_uint64),
+        ("d_workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("d_status", C.c_void_p),
+    ]
+
+
 ADAMW_BLOCK = 256                   # elements that share a scale, moments in 8 bits
 
 _vp, _u64, _u32, _i, _f = C.c_void_p, C.c_uint64, C.c_uint32, C.c_int, C.c_float
@@ -238,12 +262,16 @@ KERNEL_API = {
     "clpk_layer_norm_backward_workspace_bytes": [_u32, _u32, C.POINTER(C.c_size_t)],
     "clpk_layer_norm_backward": [C.POINTER(LayerNormBackwardArgs), _vp],
     "clpk_adamw": [C.POINTER(AdamwArgs), _vp],
+    "clpk_grouped_gemm_workspace_bytes": [_u32, C.POINTER(C.c_size_t)],
+    "clpk_grouped_gemm": [C.POINTER(GroupedGemmArgs), _vp],
+    "clpk_grouped_gemm_backward": [C.POINTER(GroupedGemmBackwardArgs), _vp],
     "clpk_set_tuning": [_i, _i],
     "clpk_get_tuning": [_i, C.POINTER(_i)],
 }
 # the structure that a call of the extension takes by reference, where it is not GemmArgs
 _ARGUMENTS = {"clpk_gemm_i8_scaled": GemmI8ScaledArgs, "clpk_gated_ffn": GatedFfnArgs, "clpk_gated_ffn_backward": GatedFfnBackwardArgs,
-              "clpk_layer_norm": LayerNormArgs, "clpk_layer_norm_backward": LayerNormBackwardArgs, "clpk_adamw": AdamwArgs}
+              "clpk_layer_norm": LayerNormArgs, "clpk_layer_norm_backward": LayerNormBackwardArgs, "clpk_adamw": AdamwArgs,
+              "clpk_grouped_gemm": GroupedGemmArgs, "clpk_grouped_gemm_backward": GroupedGemmBackwardArgs}
 _RESTYPES = {
     "clpk_last_error": C.c_char_p,
     "clpk_version": C.c_char_p,

@@ -665,6 +665,58 @@ typedef struct clpk_adamw_args {
 
 CLPK_API int clpk_adamw(const clpk_adamw_args_t *args, void *stream);
 
+/* ---- products of experts ------------------------------------------------------------------------
+ * Rows of A lie sorted by group (tokens by expert); group e has the rows from d_offsets[e] up to d_offsets[e + 1] and weights W[e] of
+ * its own:
+ *   C[r] = A[r] W[e]^T          sums in fp32, rounded once
+ * d_offsets: 32-bit integers on the device, read by the kernels; they do not decrease and lie in [0, m].  Where they do, *d_status
+ * becomes 0x401 and no result is written.  Groups may be empty; rows in front of the first group and behind the last stay as they are
+ * in C.  Up to 1024 groups.
+ * Matrices are row-major with pitches as those of the feed-forward layers: multiples of 16 bytes, 0: rows one behind another, and what
+ * lies between rows is neither read into a result nor written.  stride_* elements lie between one group's weights and the next, a
+ * multiple of 16 bytes; 0: one behind another.  Outputs do not overlap inputs.  *d_status is cleared by the call and set where a
+ * device-side wait expired.  The workspace belongs to one call at a time. */
+typedef struct clpk_grouped_gemm_args {
+    int            dtype;         /* CLPK_DT_BF16 or F16: of A and W                 */
+    int            out_dtype;     /* of C: `dtype` or CLPK_DT_F32                    */
+    uint32_t       m, n, k, groups;         /* m may be 0                            */
+    const void    *d_a;           /* [m][k], pitch lda                               */
+    const void    *d_w;           /* [groups][n][k], pitch ldw, stride_w             */
+    const int32_t *d_offsets;     /* [groups + 1]                                    */
+    void          *d_c;           /* [m][n], pitch ldc                               */
+    uint64_t       lda, ldw, stride_w, ldc;
+    void          *d_workspace;   /* 16-byte aligned                                 */
+    size_t         workspace_bytes;
+    uint32_t      *d_status;
+} clpk_grouped_gemm_args_t;
+
+/* For both calls, whatever their other sizes. */
+CLPK_API int clpk_grouped_gemm_workspace_bytes(uint32_t groups, size_t *bytes);
+CLPK_API int clpk_grouped_gemm(const clpk_grouped_gemm_args_t *args, void *stream);
+
+/* Gradients of clpk_grouped_gemm from that of C:
+ *   dA[r] = dC[r] W[e],   dW[e] = sum over the group's rows of dC[r]^T A[r]      sums in fp32, rounded once
+ * dA and its rows of no group as C; dW[e] of an empty group is zeros.  Rows of A and dC that are no group's are not read into a
+ * result.  d_da or d_dw may be NULL: what is not asked for is not computed.  Sums are formed in the same order in every call with the
+ * same offsets. */
+typedef struct clpk_grouped_gemm_backward_args {
+    int            dtype;         /* CLPK_DT_BF16 or F16: of A, W, dC and dA         */
+    int            dw_dtype;      /* of dW: `dtype` or CLPK_DT_F32                   */
+    uint32_t       m, n, k, groups;
+    const void    *d_a;           /* [m][k], pitch lda                               */
+    const void    *d_w;           /* [groups][n][k], pitch ldw, stride_w             */
+    const int32_t *d_offsets;     /* [groups + 1]                                    */
+    const void    *d_dc;          /* [m][n], pitch lddc                              */
+    void          *d_da;          /* [m][k], pitch ldda                              */
+    void          *d_dw;          /* [groups][n][k], pitch lddw, stride_dw           */
+    uint64_t       lda, ldw, stride_w, lddc, ldda, lddw, stride_dw;
+    void          *d_workspace;
+    size_t         workspace_bytes;
+    uint32_t      *d_status;
+} clpk_grouped_gemm_backward_args_t;
+
+CLPK_API int clpk_grouped_gemm_backward(const clpk_grouped_gemm_backward_args_t *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -205,3 +205,81 @@ def same(got, want):
         if differ.any():
             at = int(differ.nonzero()[0])
             raise AssertionError(f"{name}: {int(differ.sum())} of {a.numel()} differ, first at {at}: {a[at].item()!r}, want {b[at].item()!r}")
+
+
+# ---- products of groups ----------------------------------------------------------------------------------------
+
+def grouped_workspace(K, groups=1):
+    need = C.c_size_t(0)
+    K.clpk_grouped_gemm_workspace_bytes(groups, C.byref(need))
+    return torch.full((need.value,), 255, dtype=torch.uint8, device="cuda")
+
+
+def offsets_of(rows, first=0):
+    return torch.tensor([first] + list(rows), device="cuda").cumsum(0).to(torch.int32)
+
+
+def grouped_args(a, w, c, offsets, workspace, status, dtype, out, n):
+    groups = offsets.numel() - 1
+    return N.GroupedGemmArgs(dtype=F.DT[dtype], out_dtype=F.DT[out], m=a.shape[0], n=n, k=a.shape[1], groups=groups, d_a=a.data_ptr(), d_w=w.data_ptr(),
+                             d_offsets=offsets.data_ptr(), d_c=c.data_ptr(), lda=a.stride(0), ldw=w.stride(1), stride_w=w.stride(0), ldc=c.stride(0),
+                             d_workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(), d_status=status.data_ptr())
+
+
+def grouped_backward_args(a, w, dc, da, dw, offsets, workspace, status, dtype, out, n):
+    ptr = lambda t: None if t is None else t.data_ptr()                  # noqa: E731
+    args = N.GroupedGemmBackwardArgs(dtype=F.DT[dtype], dw_dtype=F.DT[out], m=a.shape[0], n=n, k=a.shape[1], groups=offsets.numel() - 1, d_a=ptr(a), d_w=ptr(w),
+                                     d_offsets=ptr(offsets), d_dc=ptr(dc), d_da=ptr(da), d_dw=ptr(dw), lda=a.stride(0), ldw=w.stride(1), stride_w=w.stride(0),
+                                     lddc=dc.stride(0), d_workspace=ptr(workspace), workspace_bytes=workspace.numel(), d_status=ptr(status))
+    if da is not None:
+        args.ldda = da.stride(0)
+    if dw is not None:
+        args.lddw, args.stride_dw = dw.stride(1), dw.stride(0)
+    return args
+
+
+def weights3(groups, n, k, dtype, pad=0, between=0, values=None, fill=F.SENTINEL):
+    """[groups][n][k] whose rows lie at multiples of 16 bytes and whose matrices lie `between` multiples of 16 bytes apart."""
+    t = F.TORCH[dtype]
+    unit = 16 // t.itemsize
+    step = -(-k // unit) * unit + pad * unit
+    stride = n * step + between * unit
+    whole = torch.full((groups * stride,), fill, dtype=t, device="cuda")
+    out = torch.as_strided(whole, (groups, n, k), (stride, step, 1))
+    if values is not None:
+        out.copy_(values)
+    return out
+
+
+def around(t):
+    """What lies around the elements of a matrix of weights3."""
+    whole = torch.as_strided(t, (t.shape[0] * t.stride(0),), (1,))
+    left = torch.ones_like(whole, dtype=torch.bool)
+    torch.as_strided(left, tuple(t.shape), t.stride()).fill_(False)
+    return whole[left]
+
+
+def grouped64(a, w, rows, first, out):
+    """C's rows of all groups in 64 bits, and what each element may be off: the tensor cores' sums, parts of which are added in fp32."""
+    want, off, at = [], [], first
+    for e, r in enumerate(rows):
+        x, y = a[at:at + r].double(), w[e].double()
+        want.append(x @ y.T)
+        off.append((F.sums(a.shape[1]) + 75 * U) * (x.abs() @ y.abs().T))
+        at += r
+    want, off = torch.cat(want), torch.cat(off)
+    return want, off + F.rounded(want.abs() + off, out)
+
+
+def grouped_backward64(a, w, dc, rows, first, dtype, out):
+    """(dA of all groups' rows, dW) in 64 bits, each with what it may be off."""
+    da, e_da, dw, e_dw, at = [], [], [], [], first
+    for e, r in enumerate(rows):
+        x, y, g = a[at:at + r].double(), w[e].double(), dc[at:at + r].double()
+        da.append(g @ y)
+        e_da.append((F.sums(w.shape[1]) + 75 * U) * (g.abs() @ y.abs()))
+        dw.append(g.T @ x)
+        e_dw.append((F.sums(r) + 75 * U) * (g.abs().T @ x.abs()))
+        at += r
+    da, e_da, dw, e_dw = torch.cat(da), torch.cat(e_da), torch.stack(dw), torch.stack(e_dw)
+    return (da, e_da + F.rounded(da.abs() + e_da, dtype)), (dw, e_dw + F.rounded(dw.abs() + e_dw, out))

@@ -10,8 +10,9 @@ from clpeak_b200 import native as N
 
 ROOT = Path(__file__).resolve().parent.parent
 STRUCTS = {"clpk_layer_norm_args_t": N.LayerNormArgs, "clpk_layer_norm_backward_args_t": N.LayerNormBackwardArgs, "clpk_adamw_tensor_t": N.AdamwTensor,
-           "clpk_adamw_args_t": N.AdamwArgs}
-CALLS = [("clpk_layer_norm", N.LayerNormArgs), ("clpk_layer_norm_backward", N.LayerNormBackwardArgs), ("clpk_adamw", N.AdamwArgs)]
+           "clpk_adamw_args_t": N.AdamwArgs, "clpk_grouped_gemm_args_t": N.GroupedGemmArgs, "clpk_grouped_gemm_backward_args_t": N.GroupedGemmBackwardArgs}
+CALLS = [("clpk_layer_norm", N.LayerNormArgs), ("clpk_layer_norm_backward", N.LayerNormBackwardArgs), ("clpk_adamw", N.AdamwArgs),
+         ("clpk_grouped_gemm", N.GroupedGemmArgs), ("clpk_grouped_gemm_backward", N.GroupedGemmBackwardArgs)]
 
 
 def test_structures_are_the_headers(tmp_path):
