@@ -17,14 +17,17 @@
 // warp overwrites the rows behind the group with zeros -- in these layouts a row is 128 bytes of a box, whatever the swizzle -- and then
 // tells the pair's barrier.
 //
-// Sizes of groups are known on the device alone.  grouped_plan_kernel turns them into tiles, in front of the main kernel: most are
-// dealt to the pairs in turn, so that neighbours share operands in the L2, and the last half to one and a half rounds are cut by cost, also inside
-// their sums, so that all pairs finish together (pairs_start).  A tile that several pairs have summed is finished by the
-// one that comes last, in the order of K: the sums are the same in every call.
+// Sizes of groups are known on the device alone, so every CTA makes the list of tiles for itself, before its first load: a prefix sum
+// over the groups.  Tiles are dealt to the pairs in turn, so that neighbours share operands in the L2.  Where that leaves pairs idle at
+// the end for longer than it costs to put sums together, the last half to one and a half rounds are cut by cost instead, also inside their
+// sums, so that all pairs finish together.  A tile that several pairs have summed is finished by the one that comes last, in
+// the order of K: the sums are the same in every call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 
 #include "../clpk_elements.cuh"
 #include "../clpk_internal.h"
@@ -43,11 +46,12 @@ constexpr int kGroupedSets = 4, kGroupedEpilogueWarps = 4 * kGroupedSets;
 constexpr int kGroupedZeroWarp = 2 + kGroupedEpilogueWarps;
 constexpr int kGroupedThreads = 32 * (kGroupedZeroWarp + 1);
 constexpr uint32_t kGroupedChunk = 32;                          // columns of an accumulator that a warp takes at a time
-constexpr uint32_t kGroupedUnits = 2 * 4 * (kGroupedN / kGroupedChunk);     // of a tile: CTA, lane quarter, chunk
+constexpr uint32_t kGroupedUnits = 2 * kGroupedEpilogueWarps;   // of a tile: what a warp has of it
 constexpr uint32_t kGroupedCutTiles = 2 * kGroupedPairs;        // tiles that may be cut, at most
 constexpr uint32_t kGroupedSlotFloats = kGroupedM * kGroupedN;
 constexpr uint32_t kGroupedLeast = 6;                           // K blocks of a part; fewer stay with the pair before or behind
 constexpr uint32_t kGroupedTileCost = 6;                        // what a tile takes besides its K blocks, in K blocks
+constexpr uint32_t kGroupedJoinCost = 48;                       // and to put one together, in its K blocks
 
 constexpr uint32_t kMnLead = 64 * kRowBytesK;                   // as in clpk_linear_grad.cuh: from one box of 64 elements along M or N to the next
 constexpr uint32_t kMnStep = 16 * kRowBytesK / 16;              // 16 rows of K, in the descriptor's units of 16 bytes
@@ -83,211 +87,13 @@ struct GroupedPlace {
     uint32_t tile, kb;
 };
 
-// In the workspace, in front of the partial sums.
-struct GroupedPlan {
-    uint32_t n_tiles, whole;                                    // `whole`: tiles that are dealt out, a multiple of the pairs
-    GroupedPlace start[kGroupedPairs + 1];                      // of each pair in the rest
-    uint32_t offsets[kGroupedMost + 1];
-    uint32_t first[2 * kGroupedMost + 1];                       // tile of each entry
-    alignas(16) uint32_t done[kGroupedCutTiles * kGroupedUnits];        // K blocks that have been added
-};
-constexpr uint64_t kGroupedPartsAt = (sizeof(GroupedPlan) + 1023) / 1024 * 1024;
+// The workspace: for each unit of a tile that may be cut, how many K blocks have been added, and by which launch; and the partial sums,
+// two slots for each pair.  Whoever adds the last blocks sets the word to zero, and a word of another launch counts as zero, so that
+// nothing has to be cleared in front of a launch and a captured one can be replayed.
+constexpr uint64_t kGroupedPartsAt = kGroupedCutTiles * kGroupedUnits * sizeof(unsigned long long);
 constexpr uint64_t kGroupedWorkspace = kGroupedPartsAt + 2ull * kGroupedPairs * kGroupedSlotFloats * 4;
-
-// ---- the plan -------------------------------------------------------------------------------------------------
-
-constexpr int kPlanThreads = 512;
-
-template <typename T>
-__device__ __forceinline__ T plan_scan(T own, T *warps, T &total)       // exclusive, over the CTA
-{
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    T sum = own;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const T v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= (uint32_t)o)
-            sum += v;
-    }
-    __syncthreads();                                            // the last scan's words have been read
-    if (lane == 31)
-        warps[warp] = sum;
-    __syncthreads();
-    T before = 0;
-    total = 0;
-    for (uint32_t w = 0; w < kPlanThreads / 32; w++) {
-        if (w < warp)
-            before += warps[w];
-        total += warps[w];
-    }
-    return before + sum - own;
-}
-
-__global__ void __launch_bounds__(kPlanThreads) grouped_plan_kernel(const int32_t *offsets, GroupedPlan *plan, uint32_t *status, GroupedShape p)
-{
-    __shared__ uint32_t off[kGroupedMost + 1], first[2 * kGroupedMost + 1];
-    __shared__ unsigned long long rest[2 * kGroupedMost + 1], load[kGroupedPairs], begins[kGroupedPairs + 1], warps64[kPlanThreads / 32];
-    __shared__ uint32_t warps32[kPlanThreads / 32];
-    const uint32_t t = threadIdx.x, entries = p.lists * p.groups;
-    griddep_wait();
-    griddep_launch_dependents();
-    bool bad = false;
-    for (uint32_t i = t; i <= p.groups; i += kPlanThreads) {
-        const int32_t v = offsets[i];
-        off[i] = (uint32_t)v;
-        bad |= v < 0 || (uint32_t)v > p.m || (i > 0 && offsets[i - 1] > v);
-    }
-    for (uint32_t i = t; i < kGroupedPairs; i += kPlanThreads)
-        load[i] = 0;
-    bad = __syncthreads_or(bad);
-    if (t == 0)
-        *status = bad ? kBadOffsets : 0u;
-
-    auto shape = [&](uint32_t i, unsigned long long &cost) {
-        const uint32_t list = i / p.groups, e = i - list * p.groups;
-        const GroupTiles g = group_tiles(p, p.kind[list], off[e + 1] - off[e]);
-        cost = (unsigned long long)(g.k_blocks + kGroupedTileCost) * block_cost(g.width);
-        return g;
-    };
-    // tiles of the entries, one behind another
-    const uint32_t each = (entries + kPlanThreads - 1) / kPlanThreads, i0 = min(t * each, entries), i1 = min(i0 + each, entries);
-    unsigned long long cost;
-    uint32_t own = 0, n_tiles;
-    for (uint32_t i = i0; i < i1 && !bad; i++) {
-        const GroupTiles g = shape(i, cost);
-        own += g.cols * g.features;
-    }
-    uint32_t at = plan_scan(own, warps32, n_tiles);
-    for (uint32_t i = i0; i < i1; i++) {
-        first[i] = at;
-        if (!bad) {
-            const GroupTiles g = shape(i, cost);
-            at += g.cols * g.features;
-        }
-    }
-    if (t == 0)
-        first[entries] = n_tiles;
-    // half a round to one and a half are left for cutting
-    const uint32_t whole = n_tiles >= p.pairs + p.pairs / 2 ? (n_tiles - p.pairs / 2) / p.pairs * p.pairs : 0;
-    __syncthreads();
-    // what each pair has of the others
-    if (whole) {
-        const uint32_t c = t % 128;
-        unsigned long long sum = 0;
-        if (c < p.pairs) {
-            const auto below = [&](uint32_t x) { return (x + p.pairs - 1 - c) / p.pairs; };     // tiles of this pair in front of x
-            for (uint32_t i = t / 128; i < entries && first[i] < whole; i += kPlanThreads / 128) {
-                const uint32_t n = below(min(first[i + 1], whole)) - below(first[i]);
-                if (n) {
-                    shape(i, cost);
-                    sum += n * cost;
-                }
-            }
-            atomicAdd(&load[c], sum);
-        }
-    }
-    // cost of the rest, entry after entry
-    unsigned long long mine = 0, total;
-    for (uint32_t i = i0; i < i1; i++)
-        if (first[i + 1] > whole) {
-            shape(i, cost);
-            mine += (first[i + 1] - max(first[i], whole)) * cost;
-        }
-    unsigned long long from = plan_scan(mine, warps64, total);
-    for (uint32_t i = i0; i < i1; i++) {
-        rest[i] = from;
-        if (first[i + 1] > whole) {
-            shape(i, cost);
-            from += (first[i + 1] - max(first[i], whole)) * cost;
-        }
-    }
-    if (t == 0)
-        rest[entries] = total;
-    __syncthreads();
-    // Where the pairs begin in the rest: each fills up to one level what it has.
-    if (t < 32) {
-        constexpr uint32_t kEach = (kGroupedPairs + 31) / 32;
-        double have[kEach], level = 0;
-        for (int round = 0; round < 6; round++) {
-            double sum = 0;
-            uint32_t count = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < kEach; j++) {
-                const uint32_t c = t * kEach + j;
-                have[j] = c < p.pairs ? (double)load[c] : 1e300;
-                if (c < p.pairs && (round == 0 || have[j] < level)) {
-                    sum += have[j];
-                    count++;
-                }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o /= 2) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                count += __shfl_xor_sync(0xffffffffu, count, o);
-            }
-            level = ((double)total + sum) / (double)max(count, 1u);
-        }
-        double room[kEach], sum = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kEach; j++) {
-            room[j] = fmax(level - have[j], 0.0);
-            sum += room[j];
-        }
-        double before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const double v = __shfl_up_sync(0xffffffffu, before, o);
-            if (t >= (uint32_t)o)
-                before += v;
-        }
-        const double all = __shfl_sync(0xffffffffu, before, 31);
-        before -= sum;
-#pragma unroll
-        for (uint32_t j = 0; j < kEach; j++) {
-            const uint32_t c = t * kEach + j;
-            if (c < p.pairs)
-                begins[c] = all > 0 ? min((unsigned long long)((double)total * (before / all)), total) : 0;
-            before += room[j];
-        }
-    }
-    __syncthreads();
-    for (uint32_t c = t; c <= p.pairs; c += kPlanThreads) {
-        GroupedPlace at = {c == 0 ? whole : n_tiles, 0};
-        if (c > 0 && c < p.pairs && begins[c] < total) {
-            const unsigned long long pos = begins[c];
-            uint32_t lo = 0, hi = entries;                      // the last entry that does not begin behind it
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (rest[mid] <= pos)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            const GroupTiles g = shape(lo, cost);
-            const unsigned long long in = pos - rest[lo];
-            const uint32_t tile = (uint32_t)(in / cost), blocks = (uint32_t)((in - tile * cost) / block_cost(g.width));
-            at.tile = max(first[lo], whole) + tile;
-            // the tile's own cost lies in front of its blocks
-            at.kb = blocks <= kGroupedTileCost ? 0 : blocks - kGroupedTileCost;
-            if (at.kb < kGroupedLeast)
-                at.kb = 0;
-            else if (at.kb + kGroupedLeast > g.k_blocks)
-                at = {at.tile + 1, 0};
-        }
-        plan->start[c] = at;
-    }
-    if (t == 0) {
-        plan->n_tiles = n_tiles;
-        plan->whole = whole;
-    }
-    for (uint32_t i = t; i <= p.groups; i += kPlanThreads)
-        plan->offsets[i] = off[i];
-    for (uint32_t i = t; i <= entries; i += kPlanThreads)
-        plan->first[i] = first[i];
-    uint4 *done = reinterpret_cast<uint4 *>(plan->done);
-    for (uint32_t i = t; i < (n_tiles - whole) * kGroupedUnits / 4; i += kPlanThreads)
-        done[i] = make_uint4(0, 0, 0, 0);
-}
+constexpr uint32_t kDoneBits = 28;                              // of a word: K blocks; above them the launch
+static_assert(kGroupedPartsAt % 16 == 0, "partial sums start on 16 bytes");
 
 // ---- the products ---------------------------------------------------------------------------------------------
 
@@ -308,7 +114,9 @@ struct GroupedParams {
     GroupedShape shape;
     GroupedResult out[3];                                       // by kind
     uint32_t dw_rows;                                           // rows of dW[e]
-    GroupedPlan *plan;
+    const int32_t *offsets;
+    unsigned long long *done;
+    unsigned long long launch;                                  // its number, not 0
     float *parts;
     uint32_t *status;
 };
@@ -320,13 +128,242 @@ struct GroupedSmem {
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint32_t tmem_base;
-    uint32_t n_tiles, whole;
-    GroupedPlace start[kGroupedPairs + 1];
+    uint32_t n_tiles, dealt;                                    // tiles in front of `dealt` are dealt in turn, the others cut
+    GroupedPlace start[kGroupedPairs + 1];                      // of each pair among the others
     uint32_t offsets[kGroupedMost + 1];
-    uint32_t first[2 * kGroupedMost + 1];
+    uint32_t first[2 * kGroupedMost + 1];                       // tile of each entry
+    // while the list is made
+    uint32_t warps[kGroupedThreads / 32];
+    unsigned long long load[kGroupedPairs];                     // cost of what has been dealt to a pair
+    unsigned long long rest[kGroupedCutTiles + 1];              // of the tiles that may be cut, one behind another
+    unsigned long long begins[kGroupedPairs];
+    unsigned long long warp_cost[(kGroupedCutTiles + 31) / 32], most;
+    uint32_t join;
 };
 constexpr uint32_t kGroupedSmemBytes = kGroupedStages * kGroupedStageBytes + (uint32_t)sizeof(GroupedSmem);
 static_assert(kGroupedSmemBytes <= kSmemMax, "ring, barriers and the list of groups");
+
+// ---- the list of tiles ----------------------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ T warp_before(T own)                 // exclusive sum over the lanes
+{
+    const uint32_t lane = threadIdx.x & 31;
+    T sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const T v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= (uint32_t)o)
+            sum += v;
+    }
+    return sum - own;
+}
+
+__device__ __forceinline__ uint32_t entry_of(const GroupedSmem *sh, uint32_t entries, uint32_t tile)     // the last one that does not begin behind it
+{
+    uint32_t lo = 0, hi = entries;
+#pragma unroll 1
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (sh->first[mid] <= tile)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ GroupTiles entry_tiles(const GroupedSmem *sh, const GroupedShape &p, uint32_t entry, uint32_t &kind, uint32_t &group)
+{
+    const uint32_t list = entry >= p.groups ? 1 : 0;
+    group = entry - list * p.groups;
+    kind = list ? p.kind[1] : p.kind[0];
+    return group_tiles(p, kind, sh->offsets[group + 1] - sh->offsets[group]);
+}
+
+__device__ __forceinline__ unsigned long long tile_cost(const GroupTiles &g) { return (unsigned long long)(g.k_blocks + kGroupedTileCost) * block_cost(g.width); }
+
+// All threads of a CTA; false: the offsets are none.  The code is short rather than fast: a launch meets it cold.
+__device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams &params)
+{
+    const GroupedShape &p = params.shape;
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5, entries = p.lists * p.groups, P = p.pairs;
+    uint32_t kind, group;
+    bool bad = false;
+#pragma unroll 1
+    for (uint32_t i = t; i <= p.groups; i += kGroupedThreads) {
+        const int32_t v = params.offsets[i], before = i ? params.offsets[i - 1] : 0;
+        sh->offsets[i] = (uint32_t)v;
+        bad |= v < before || v < 0 || (uint32_t)v > p.m;
+    }
+    if (t < kGroupedPairs)
+        sh->load[t] = 0;
+    if (t == 0) {
+        sh->most = 0;
+        sh->join = 0;
+    }
+    if (__syncthreads_or(bad)) {                                // nothing to walk
+        if (t == 0)
+            sh->n_tiles = sh->dealt = 0;
+        if (t <= P)
+            sh->start[t] = {0, 0};
+        __syncthreads();
+        return false;
+    }
+    const uint32_t each = (entries + kGroupedThreads - 1) / kGroupedThreads, i0 = min(t * each, entries), i1 = min(i0 + each, entries);
+    uint32_t own = 0;
+#pragma unroll 1
+    for (uint32_t i = i0; i < i1; i++) {
+        const GroupTiles g = entry_tiles(sh, p, i, kind, group);
+        own += g.cols * g.features;
+    }
+    uint32_t at = warp_before(own);
+    if (lane == 31)
+        sh->warps[warp] = at + own;
+    __syncthreads();
+    uint32_t n_tiles = 0;
+#pragma unroll 1
+    for (uint32_t w = 0; w < kGroupedThreads / 32; w++) {
+        at += w < warp ? sh->warps[w] : 0;
+        n_tiles += sh->warps[w];
+    }
+#pragma unroll 1
+    for (uint32_t i = i0; i < i1; i++) {
+        sh->first[i] = at;
+        const GroupTiles g = entry_tiles(sh, p, i, kind, group);
+        at += g.cols * g.features;
+    }
+    if (t == 0)
+        sh->first[entries] = n_tiles;
+    __syncthreads();
+
+    // What may be cut: half a round to one and a half, a thread for each of its tiles.
+    const uint32_t whole = n_tiles >= P + P / 2 ? (n_tiles - P / 2) / P * P : 0, rest = n_tiles - whole;
+    unsigned long long cost = 0;
+    if (warp < (kGroupedCutTiles + 31) / 32) {
+        uint32_t join = 0;
+        if (t < rest) {
+            const GroupTiles g = entry_tiles(sh, p, entry_of(sh, entries, whole + t), kind, group);
+            cost = tile_cost(g);
+            join = kGroupedJoinCost * block_cost(g.width);
+        }
+        unsigned long long sum = cost, most = cost;
+#pragma unroll 1
+        for (int o = 16; o > 0; o /= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        join = __reduce_max_sync(0xffffffffu, join);
+        if (lane == 0) {
+            sh->warp_cost[warp] = sum;
+            atomicMax(&sh->most, most);
+            atomicMax(&sh->join, join);
+        }
+    }
+    __syncthreads();
+    unsigned long long total = 0, from = 0;
+#pragma unroll 1
+    for (uint32_t w = 0; w < (kGroupedCutTiles + 31) / 32; w++) {
+        from += w < warp ? sh->warp_cost[w] : 0;
+        total += sh->warp_cost[w];
+    }
+    // dealt out: as many as a pair gets of the longest; cut: an equal share and the joining
+    const bool cut = ((rest + P - 1) / P) * sh->most > total / P + sh->join;
+    if (t == 0) {
+        sh->n_tiles = n_tiles;
+        sh->dealt = cut ? whole : n_tiles;
+    }
+    if (!cut) {
+        if (t <= P)
+            sh->start[t] = {n_tiles, 0};
+        __syncthreads();
+        return true;
+    }
+    if (warp < (kGroupedCutTiles + 31) / 32) {
+        from += warp_before(cost);
+        if (t <= rest)
+            sh->rest[t] = from;                                 // and the total behind the last
+    }
+    if (whole) {                                                // what each pair has of the others
+        const uint32_t c = t % 128;
+        if (c < P) {
+            unsigned long long sum = 0;
+#pragma unroll 1
+            for (uint32_t i = t / 128; i < entries && sh->first[i] < whole; i += kGroupedThreads / 128) {
+                // tiles c, c + P, ... in front of the entry's end and of its begin
+                const uint32_t n = (min(sh->first[i + 1], whole) + P - 1 - c) / P - (sh->first[i] + P - 1 - c) / P;
+                if (n)
+                    sum += n * tile_cost(entry_tiles(sh, p, i, kind, group));
+            }
+            if (t < kGroupedThreads / 128 * 128)
+                atomicAdd(&sh->load[c], sum);
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {                                            // where the pairs begin: each fills up to one level what it has
+        constexpr uint32_t kPairsEach = (kGroupedPairs + 31) / 32;
+        const float all_cost = (float)total;
+        float level = 3e38f;
+#pragma unroll 1
+        for (int round = 0; round < 5; round++) {
+            float sum = 0, count = 0;
+#pragma unroll 1
+            for (uint32_t c = lane * kPairsEach; c < min(P, (lane + 1) * kPairsEach); c++)
+                if ((float)sh->load[c] < level) {
+                    sum += (float)sh->load[c];
+                    count += 1;
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                count += __shfl_xor_sync(0xffffffffu, count, o);
+            }
+            level = (all_cost + sum) / fmaxf(count, 1.0f);
+        }
+        // in whole numbers, so that no pair begins in front of the one before it
+        const unsigned long long full = (unsigned long long)level;
+        const auto room = [&](uint32_t c) { return full > sh->load[c] ? full - sh->load[c] : 0ull; };
+        unsigned long long own_room = 0;
+#pragma unroll 1
+        for (uint32_t c = lane * kPairsEach; c < min(P, (lane + 1) * kPairsEach); c++)
+            own_room += room(c);
+        unsigned long long before = warp_before(own_room);
+        const float all = fmaxf((float)__shfl_sync(0xffffffffu, before + own_room, 31), 1.0f);
+#pragma unroll 1
+        for (uint32_t c = lane * kPairsEach; c < min(P, (lane + 1) * kPairsEach); c++) {
+            sh->begins[c] = (unsigned long long)(all_cost * ((float)before / all));
+            before += room(c);
+        }
+    }
+    __syncthreads();
+    if (t <= P) {
+        GroupedPlace to = {t == 0 ? whole : n_tiles, 0};
+        if (t > 0 && t < P && sh->begins[t] < total) {
+            const unsigned long long pos = sh->begins[t];
+            uint32_t lo = 0, hi = rest;
+#pragma unroll 1
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (sh->rest[mid] <= pos)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            const GroupTiles g = entry_tiles(sh, p, entry_of(sh, entries, whole + lo), kind, group);
+            const uint32_t blocks = (uint32_t)((pos - sh->rest[lo]) / block_cost(g.width));
+            // the tile's own cost lies in front of its blocks
+            to.tile = whole + lo;
+            to.kb = blocks <= kGroupedTileCost ? 0 : blocks - kGroupedTileCost;
+            if (to.kb < kGroupedLeast)
+                to.kb = 0;
+            else if (to.kb + kGroupedLeast > g.k_blocks)
+                to = {to.tile + 1, 0};
+        }
+        sh->start[t] = to;
+    }
+    __syncthreads();
+    return true;
+}
 
 // A tile, or the part of its sum that falls to this pair
 struct GroupedTile {
@@ -340,34 +377,31 @@ struct GroupedTile {
 struct GroupedWalk {
     const GroupedParams &p;
     const GroupedSmem *sh;
-    uint32_t pair, i = 0, entry = 0;
+    uint32_t pair, i = 0, cut = 0, entry = 0;
 
     __device__ __forceinline__ GroupedWalk(const GroupedParams &p, const GroupedSmem *sh, uint32_t pair) : p(p), sh(sh), pair(pair) {}
 
     __device__ __forceinline__ bool next(GroupedTile &t)
     {
         const GroupedShape &s = p.shape;
-        const uint32_t rounds = sh->whole / s.pairs;
-        uint32_t tile, kb0 = 0, kb1 = 0xFFFFFFFFu;
-        if (i < rounds) {
-            tile = pair + i * s.pairs;
-        } else {
+        uint32_t tile = pair + i * s.pairs, kb0 = 0, kb1 = 0xFFFFFFFFu;
+        if (tile >= sh->dealt) {
             const GroupedPlace from = sh->start[pair], to = sh->start[pair + 1];
-            tile = from.tile + (i - rounds);
-            kb0 = i == rounds ? from.kb : 0;
+            tile = from.tile + cut;
+            kb0 = cut == 0 ? from.kb : 0;
             if (tile > to.tile || (tile == to.tile && kb0 >= to.kb))
                 return false;
             if (tile == to.tile)
                 kb1 = to.kb;
+            cut++;
+        } else {
+            i++;
         }
-        i++;
         while (sh->first[entry + 1] <= tile)
             entry++;
-        const uint32_t list = entry / s.groups, e = entry - list * s.groups, begin = sh->offsets[e], rows = sh->offsets[e + 1] - begin;
-        t.kind = s.kind[list];
-        t.group = e;
+        const GroupTiles g = entry_tiles(sh, s, entry, t.kind, t.group);
+        const uint32_t begin = sh->offsets[t.group], rows = sh->offsets[t.group + 1] - begin;
         t.tile = tile;
-        const GroupTiles g = group_tiles(s, t.kind, rows);
         // strips of eight tiles along N, those fastest: neighbours share what they read
         const uint32_t at = tile - sh->first[entry], strip = at / (8 * g.features), in = at - strip * 8 * g.features, wide = min(8u, g.cols - strip * 8);
         const uint32_t col = strip * 8 + in % wide;
@@ -398,11 +432,25 @@ __device__ __forceinline__ void tma_load_pair_3d(void *smem_dst, const CUtensorM
 }
 
 // what another pair has written in this launch
-__device__ __forceinline__ float load_told(const float *p)
+__device__ __forceinline__ float4 load_told(const float4 *p)
 {
-    float v;
-    asm volatile("ld.relaxed.gpu.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    float4 v;
+    asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
     return v;
+}
+
+// K blocks to those that this launch has added so far; whether they are all
+__device__ __forceinline__ bool add_blocks(unsigned long long *done, unsigned long long launch, uint32_t blocks, uint32_t all)
+{
+    unsigned long long old = *reinterpret_cast<volatile unsigned long long *>(done);
+    while (true) {
+        const unsigned long long sum = (old >> kDoneBits == launch ? old : launch << kDoneBits) + blocks;
+        const bool last = (uint32_t)sum % (1u << kDoneBits) == all;
+        const unsigned long long seen = atomicCAS(done, old, last ? 0ull : sum);
+        if (seen == old)
+            return last;
+        old = seen;
+    }
 }
 
 // 32 columns of 32 lanes -> rows of the result.  In 16 bits lanes 2i and 2i + 1 exchange halves, so that each has two neighbours of
@@ -481,23 +529,22 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
     }
     if (warp == 1)
         tmem_alloc<2>(&sh->tmem_base, 512);
-    griddep_wait();
-    griddep_launch_dependents();
-    if (threadIdx.x == 0) {
-        sh->n_tiles = p.plan->n_tiles;
-        sh->whole = p.plan->whole;
-    }
-    for (uint32_t i = threadIdx.x; i <= p.shape.pairs; i += kGroupedThreads)
-        sh->start[i] = p.plan->start[i];
-    for (uint32_t i = threadIdx.x; i <= p.shape.groups; i += kGroupedThreads)
-        sh->offsets[i] = p.plan->offsets[i];
-    for (uint32_t i = threadIdx.x; i <= p.shape.lists * p.shape.groups; i += kGroupedThreads)
-        sh->first[i] = p.plan->first[i];
+    if (threadIdx.x == 0)
+        for (uint32_t l = 0; l < p.shape.lists; l++) {
+            const bool dw = p.shape.kind[l] == kWeightGrad;
+            tma_prefetch_desc(dw ? &maps.a_t : &maps.w);
+            tma_prefetch_desc(dw ? &maps.dc_t : &maps.rows[3]);
+        }
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync();
     tc_fence_after_sync();
     const uint32_t tmem = sh->tmem_base;
+    griddep_wait();
+    griddep_launch_dependents();
+    const bool good = list_tiles(sh, p);
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *p.status = good ? 0u : kBadOffsets;
     GroupedWalk walk(p, sh, pair);
     GroupedTile t;
 
@@ -625,6 +672,10 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
             tc_fence_after_sync();
             const uint32_t taddr = tmem + acc * kGroupedN + ((q * 32) << 16), chunks = t.width / kGroupedChunk;
             const bool whole = t.kb0 == 0 && t.kb1 == t.k_blocks;
+            // where the warp's sums of a chunk lie in a pair's slot: of the pair's part at its begin, or that at its end
+            auto slot = [&](uint32_t of, bool at_begin, uint32_t c) {
+                return reinterpret_cast<float4 *>(p.parts + (uint64_t)(2 * of + (at_begin ? 0 : 1)) * kGroupedSlotFloats + ((r * 4 + q) * kGroupedN + c * kGroupedChunk) * 32) + lane;
+            };
             for (uint32_t c = set; c < chunks; c += kGroupedSets) {
                 float v[kGroupedChunk];
                 tmem_ld_32x32b_x32(taddr + c * kGroupedChunk, reinterpret_cast<uint32_t(&)[kGroupedChunk]>(v));
@@ -635,48 +686,58 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
                     if (lane == 0)
                         mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
                 }
-                if (!whole) {
-                    // this pair's sums go to its slot; whoever brings the last blocks adds all parts, in the order of K
-                    const uint64_t unit = (uint64_t)(r * 4 + q) * kGroupedN + c * kGroupedChunk;
-                    auto slot = [&](uint32_t of, bool inside) { return p.parts + (uint64_t)(2 * of + (inside ? 0 : 1)) * kGroupedSlotFloats + unit * 32 + lane; };
-                    float *to = slot(pair, t.kb0 > 0);
+                if (whole) {
+                    store_tile_rows<DT>(v, p, t, c * kGroupedChunk, lanes, lane);
+                } else {
+                    float4 *to = slot(pair, t.kb0 > 0, c);
 #pragma unroll
-                    for (uint32_t j = 0; j < kGroupedChunk; j++)
-                        to[j * 32] = v[j];
-                    __threadfence();
-                    __syncwarp();
-                    uint32_t before = 0;
-                    if (lane == 0)
-                        before = atomicAdd(&p.plan->done[(t.tile - sh->whole) * kGroupedUnits + (r * 4 + q) * (kGroupedN / kGroupedChunk) + c], t.kb1 - t.kb0);
-                    if (__shfl_sync(0xffffffffu, before, 0) + (t.kb1 - t.kb0) != t.k_blocks)
-                        continue;
-                    __threadfence();
-                    uint32_t of = pair;
-                    while (sh->start[of].tile == t.tile && sh->start[of].kb > 0)
-                        of--;
-                    bool begun = false;
-                    for (; of < p.shape.pairs; of++) {
-                        const GroupedPlace from = sh->start[of], end = sh->start[of + 1];
-                        if (from.tile > t.tile || (begun && from.tile == t.tile && from.kb == 0))
-                            break;
-                        if (from.tile == end.tile && from.kb == end.kb)
-                            continue;
-                        if (end.tile < t.tile || (end.tile == t.tile && end.kb == 0))
-                            continue;
-                        const float *at = slot(of, from.tile == t.tile && from.kb > 0);
-#pragma unroll
-                        for (uint32_t j = 0; j < kGroupedChunk; j++)
-                            v[j] = begun ? v[j] + load_told(at + j * 32) : load_told(at + j * 32);
-                        begun = true;
-                    }
+                    for (uint32_t j = 0; j < kGroupedChunk / 4; j++)
+                        to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 }
-                store_tile_rows<DT>(v, p, t, c * kGroupedChunk, lanes, lane);
             }
             if (set >= chunks) {
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
+                continue;
+            }
+            if (whole)
+                continue;
+            // whoever brings the last blocks adds all parts, in the order of K
+            __threadfence();
+            __syncwarp();
+            bool last = false;
+            if (lane == 0)
+                last = add_blocks(p.done + (t.tile - sh->dealt) * kGroupedUnits + (r * 4 + q) * kGroupedSets + set, p.launch, t.kb1 - t.kb0, t.k_blocks);
+            if (!__shfl_sync(0xffffffffu, last, 0))
+                continue;
+            __threadfence();
+            uint32_t begin = pair;
+            while (sh->start[begin].tile == t.tile && sh->start[begin].kb > 0)
+                begin--;
+            for (uint32_t c = set; c < chunks; c += kGroupedSets) {
+                float v[kGroupedChunk] = {};
+                for (uint32_t of = begin; of < p.shape.pairs && sh->start[of].tile <= t.tile; of++) {
+                    const GroupedPlace from = sh->start[of], end = sh->start[of + 1];
+                    if ((from.tile == end.tile && from.kb == end.kb) || end.tile < t.tile || (end.tile == t.tile && end.kb == 0))
+                        continue;                               // none, or none of this tile
+                    if (from.tile == t.tile && from.kb == 0 && of != begin)
+                        break;
+                    const float4 *at = slot(of, from.tile == t.tile && from.kb > 0, c);
+                    float4 part[kGroupedChunk / 4];             // all asked for before any is waited for
+#pragma unroll
+                    for (uint32_t j = 0; j < kGroupedChunk / 4; j++)
+                        part[j] = load_told(at + j * 32);
+#pragma unroll
+                    for (uint32_t j = 0; j < kGroupedChunk / 4; j++) {
+                        v[4 * j] += part[j].x;
+                        v[4 * j + 1] += part[j].y;
+                        v[4 * j + 2] += part[j].z;
+                        v[4 * j + 3] += part[j].w;
+                    }
+                }
+                store_tile_rows<DT>(v, p, t, c * kGroupedChunk, lanes, lane);
             }
         }
     } else if (BACKWARD) {
@@ -737,10 +798,14 @@ static uint32_t up_div(uint64_t a, uint32_t b) { return (uint32_t)((a + b - 1) /
 
 static int run_grouped(const GroupedMaps &maps, GroupedParams &p, int dtype, bool backward, const int32_t *offsets, void *workspace, cudaStream_t s)
 {
-    p.plan = static_cast<GroupedPlan *>(workspace);
+    // numbers that no other launch of this process has, and hardly one of a process before it in the same memory
+    static std::atomic<unsigned long long> launches((unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() << 8);
+    constexpr unsigned long long kMost = (1ull << (64 - kDoneBits)) - 1;
+    p.launch = launches.fetch_add(1) % kMost + 1;
+    p.offsets = offsets;
+    p.done = static_cast<unsigned long long *>(workspace);
     p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kGroupedPartsAt);
     p.shape.pairs = std::min(kGroupedPairs, (uint32_t)num_sms() / 2);
-    CLPK_TRY(launch_behind(grouped_plan_kernel, "grouped_plan", 1, kPlanThreads, 0, s, offsets, p.plan, p.status, p.shape));
     const uint32_t ctas = 2 * p.shape.pairs;
     if (backward)
         return dtype == CLPK_DT_F16 ? launch_clusters(grouped_kernel<CLPK_DT_F16, true>, "grouped (gradients)", ctas, kGroupedThreads, kGroupedSmemBytes, 2, s, maps, p)
