@@ -453,32 +453,39 @@ __device__ __forceinline__ bool add_blocks(unsigned long long *done, unsigned lo
     }
 }
 
-// 32 columns of 32 lanes -> rows of the result.  In 16 bits lanes 2i and 2i + 1 exchange halves, so that each has two neighbours of
-// every other row: 4-byte stores, 64 bytes of a row by a warp.
-template <int TYPE>
+// 32 columns of 32 lanes -> rows of the result.  In 16 bits lanes 2i and 2i + 1 exchange halves of what they have of four columns, so that
+// each has two neighbours of every other row: 4-byte stores, 64 bytes of a row by a warp.
+template <int TYPE, bool WHOLE>
 __device__ __forceinline__ void store_rows(const float (&v)[kGroupedChunk], const GroupedResult &out, uint64_t row0, uint32_t rows, uint32_t feature, int lane)
 {
     if constexpr (TYPE == CLPK_DT_F32) {
         float *to = static_cast<float *>(out.base) + row0 * out.ld + feature + lane;
-        if (feature + lane < out.features) {
+        if (WHOLE || feature + lane < out.features) {
 #pragma unroll
-            for (uint32_t j = 0; j < kGroupedChunk; j++)
-                if (j < rows)
-                    to[j * out.ld] = v[j];
+            for (uint32_t j = 0; j < kGroupedChunk; j++, to += out.ld)
+                if (WHOLE || j < rows)
+                    *to = v[j];
         }
     } else {
-        const uint32_t odd = lane & 1, f = feature + (lane & ~1);
+        using E = Element<TYPE>;
+        const uint32_t odd = lane & 1, f = feature + (lane & ~1), give = odd ? 0x5410 : 0x7632, one = odd ? 0x3254 : 0x5410, two = odd ? 0x3276 : 0x7610;
         uint16_t *to = static_cast<uint16_t *>(out.base) + (row0 + odd) * out.ld + f;
-#pragma unroll
-        for (uint32_t j = 0; j < kGroupedChunk; j += 2) {
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
-            const uint32_t w = odd ? Element<TYPE>::round2(got, v[j + 1]) : Element<TYPE>::round2(v[j], got);
-            if (j + odd < rows) {
-                if (f + 1 < out.features)
-                    *reinterpret_cast<uint32_t *>(to + j * out.ld) = w;
+        const uint64_t step = 2 * out.ld;
+        auto put = [&](uint32_t j, uint32_t w) {
+            if (WHOLE || j + odd < rows) {
+                if (WHOLE || f + 1 < out.features)
+                    *reinterpret_cast<uint32_t *>(to) = w;
                 else if (f < out.features)
-                    to[j * out.ld] = (uint16_t)w;
+                    *to = (uint16_t)w;
             }
+            to += step;
+        };
+#pragma unroll
+        for (uint32_t j = 0; j < kGroupedChunk; j += 4) {
+            const uint32_t a = E::round2(v[j], v[j + 1]), b = E::round2(v[j + 2], v[j + 3]);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(a, b, give), 1);
+            put(j, __byte_perm(a, got, one));
+            put(j + 2, __byte_perm(b, got, two));
         }
     }
 }
@@ -494,10 +501,12 @@ __device__ __forceinline__ void store_tile_rows(const float (&v)[kGroupedChunk],
     GroupedResult to = out;
     if (t.kind == kWeightGrad)
         to.base = static_cast<uint8_t *>(out.base) + t.group * out.stride * (out.type == CLPK_DT_F32 ? 4 : 2);
+    const uint32_t feature = t.feature + lane_feature;
+    const bool whole = rows >= kGroupedChunk && feature + 32 <= out.features;
     if (out.type == CLPK_DT_F32)
-        store_rows<CLPK_DT_F32>(v, to, row, rows, t.feature + lane_feature, lane);
+        whole ? store_rows<CLPK_DT_F32, true>(v, to, row, rows, feature, lane) : store_rows<CLPK_DT_F32, false>(v, to, row, rows, feature, lane);
     else
-        store_rows<DT>(v, to, row, rows, t.feature + lane_feature, lane);
+        whole ? store_rows<DT, true>(v, to, row, rows, feature, lane) : store_rows<DT, false>(v, to, row, rows, feature, lane);
 }
 
 template <int DT, bool BACKWARD>
@@ -581,17 +590,20 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
                         for (uint32_t i = 0; i < 128; i += 64)
                             tma_load_pair_3d(a + i * kRowBytesK, &maps.w, (int32_t)((feature + i) * 2), (int32_t)(kb * kGroupedK), (int32_t)t.group, bar);
                     } else {
-                        const int32_t row = (int32_t)(t.k_row + kb * kGroupedK);
-                        auto load = [&](uint8_t *to, const CUtensorMap *map, uint32_t x) {
-                            if (last)
-                                tma_load_own(to, map, (int32_t)(x * 2), row, &sh->tail[s]);
-                            else
-                                tma_load_pair_at(to, map, (int32_t)(x * 2), row, bar);
-                        };
-                        for (uint32_t i = 0; i < 128; i += 64)
-                            load(a + i * kRowBytesK, &maps.a_t, feature + i);
-                        for (uint32_t i = 0; i < half; i += 64)
-                            load(b + i * kRowBytesK, &maps.dc_t, t.row + r * half + i);
+                        const int32_t row = (int32_t)(t.k_row + kb * kGroupedK), xa = (int32_t)(feature * 2), xb = (int32_t)((t.row + r * half) * 2);
+                        if (!last) {
+                            tma_load_pair_at(a, &maps.a_t, xa, row, bar);
+                            tma_load_pair_at(a + kMnLead, &maps.a_t, xa + 128, row, bar);
+                            tma_load_pair_at(b, &maps.dc_t, xb, row, bar);
+                            if (half > 64)
+                                tma_load_pair_at(b + kMnLead, &maps.dc_t, xb + 128, row, bar);
+                        } else {
+                            tma_load_own(a, &maps.a_t, xa, row, &sh->tail[s]);
+                            tma_load_own(a + kMnLead, &maps.a_t, xa + 128, row, &sh->tail[s]);
+                            tma_load_own(b, &maps.dc_t, xb, row, &sh->tail[s]);
+                            if (half > 64)
+                                tma_load_own(b + kMnLead, &maps.dc_t, xb + 128, row, &sh->tail[s]);
+                        }
                     }
                     if (!BACKWARD || t.kind == kRowGrad) {
                         uint32_t at = 0;
@@ -676,42 +688,55 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
             auto slot = [&](uint32_t of, bool at_begin, uint32_t c) {
                 return reinterpret_cast<float4 *>(p.parts + (uint64_t)(2 * of + (at_begin ? 0 : 1)) * kGroupedSlotFloats + ((r * 4 + q) * kGroupedN + c * kGroupedChunk) * 32) + lane;
             };
-            for (uint32_t c = set; c < chunks; c += kGroupedSets) {
-                float v[kGroupedChunk];
-                tmem_ld_32x32b_x32(taddr + c * kGroupedChunk, reinterpret_cast<uint32_t(&)[kGroupedChunk]>(v));
-                tmem_ld_wait();
-                if (c + kGroupedSets >= chunks) {               // the accumulator is free as soon as it has been read
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0)
-                        mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
-                }
-                if (whole) {
+            auto release = [&]() {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
+            };
+            if (set >= chunks) {
+                release();
+                continue;
+            }
+            if (whole) {
+                for (uint32_t c = set; c < chunks; c += kGroupedSets) {
+                    float v[kGroupedChunk];
+                    tmem_ld_32x32b_x32(taddr + c * kGroupedChunk, reinterpret_cast<uint32_t(&)[kGroupedChunk]>(v));
+                    tmem_ld_wait();
+                    if (c + kGroupedSets >= chunks)
+                        release();                              // the accumulator is free as soon as it has been read
                     store_tile_rows<DT>(v, p, t, c * kGroupedChunk, lanes, lane);
-                } else {
+                }
+                continue;
+            }
+            // Whoever brings the last blocks adds all parts, in the order of K.  A pair that finds all others there keeps its own where they
+            // are; another one writes them to its slot first.
+            unsigned long long *const done = p.done + (t.tile - sh->dealt) * kGroupedUnits + (r * 4 + q) * kGroupedSets + set;
+            const uint32_t blocks = t.kb1 - t.kb0;
+            bool last = false, kept = false;
+            if (lane == 0)
+                kept = *reinterpret_cast<volatile unsigned long long *>(done) == (p.launch << kDoneBits) + (t.k_blocks - blocks);
+            kept = __shfl_sync(0xffffffffu, kept, 0);
+            if (!kept) {
+                for (uint32_t c = set; c < chunks; c += kGroupedSets) {
+                    float v[kGroupedChunk];
+                    tmem_ld_32x32b_x32(taddr + c * kGroupedChunk, reinterpret_cast<uint32_t(&)[kGroupedChunk]>(v));
+                    tmem_ld_wait();
                     float4 *to = slot(pair, t.kb0 > 0, c);
 #pragma unroll
                     for (uint32_t j = 0; j < kGroupedChunk / 4; j++)
                         to[j * 32] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 }
-            }
-            if (set >= chunks) {
-                tc_fence_before_sync();
+                release();
+                __threadfence();
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive_cluster_relaxed(&sh->tmem_empty[acc], 0);
-                continue;
+                    last = add_blocks(done, p.launch, blocks, t.k_blocks);
+                if (!__shfl_sync(0xffffffffu, last, 0))
+                    continue;
+            } else if (lane == 0) {
+                *reinterpret_cast<volatile unsigned long long *>(done) = 0;
             }
-            if (whole)
-                continue;
-            // whoever brings the last blocks adds all parts, in the order of K
-            __threadfence();
-            __syncwarp();
-            bool last = false;
-            if (lane == 0)
-                last = add_blocks(p.done + (t.tile - sh->dealt) * kGroupedUnits + (r * 4 + q) * kGroupedSets + set, p.launch, t.kb1 - t.kb0, t.k_blocks);
-            if (!__shfl_sync(0xffffffffu, last, 0))
-                continue;
             __threadfence();
             uint32_t begin = pair;
             while (sh->start[begin].tile == t.tile && sh->start[begin].kb > 0)
@@ -722,21 +747,24 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
                     const GroupedPlace from = sh->start[of], end = sh->start[of + 1];
                     if ((from.tile == end.tile && from.kb == end.kb) || end.tile < t.tile || (end.tile == t.tile && end.kb == 0))
                         continue;                               // none, or none of this tile
-                    if (from.tile == t.tile && from.kb == 0 && of != begin)
-                        break;
-                    const float4 *at = slot(of, from.tile == t.tile && from.kb > 0, c);
-                    float4 part[kGroupedChunk / 4];             // all asked for before any is waited for
+                    float part[kGroupedChunk];                  // all asked for before any is waited for
+                    if (kept && of == pair) {
+                        tmem_ld_32x32b_x32(taddr + c * kGroupedChunk, reinterpret_cast<uint32_t(&)[kGroupedChunk]>(part));
+                        tmem_ld_wait();
+                    } else {
+                        const float4 *at = slot(of, from.tile == t.tile && from.kb > 0, c);
 #pragma unroll
-                    for (uint32_t j = 0; j < kGroupedChunk / 4; j++)
-                        part[j] = load_told(at + j * 32);
-#pragma unroll
-                    for (uint32_t j = 0; j < kGroupedChunk / 4; j++) {
-                        v[4 * j] += part[j].x;
-                        v[4 * j + 1] += part[j].y;
-                        v[4 * j + 2] += part[j].z;
-                        v[4 * j + 3] += part[j].w;
+                        for (uint32_t j = 0; j < kGroupedChunk / 4; j++) {
+                            const float4 f = load_told(at + j * 32);
+                            part[4 * j] = f.x; part[4 * j + 1] = f.y; part[4 * j + 2] = f.z; part[4 * j + 3] = f.w;
+                        }
                     }
+#pragma unroll
+                    for (uint32_t j = 0; j < kGroupedChunk; j++)
+                        v[j] += part[j];
                 }
+                if (kept && c + kGroupedSets >= chunks)
+                    release();
                 store_tile_rows<DT>(v, p, t, c * kGroupedChunk, lanes, lane);
             }
         }
