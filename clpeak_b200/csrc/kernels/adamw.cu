@@ -12,8 +12,8 @@
 // sqrt(v) = s c^2: the square spreads 127 steps over a range of 2^14, and 255 over 2^16 of sqrt(v), 2^32 of v, where equal steps would
 // round to zero whatever is below 2^-8 and 2^-9 of the block's largest.  A v that is not zero keeps a code that is not: an
 // element with a small v beside a large one is taken for larger than it is, and its step gets shorter, never divided by eps alone.
-// Every operation is rounded by itself (no fused multiply-add), so that moments and codes have one value that can be told in
-// any arithmetic.
+// No multiplication and addition are fused, so that moments and codes have one value that can be told in any arithmetic; with moments in
+// fp32 that holds for the parameters too.
 #include "../clpk_elements.cuh"
 #include "../clpk_internal.h"
 #include "../clpk_ptx.cuh"
@@ -39,6 +39,7 @@ struct StepTensor {
 struct StepRates {
     float b1, b1_rest, b2, b2_rest, eps;
     float keep, root_scale, rate;                       // 1 - lr wd, 1 / sqrt(1 - b2^t), lr / (1 - b1^t)
+    float none;                                         // -0
 };
 
 struct StepCommon {
@@ -69,8 +70,91 @@ __host__ __device__ __forceinline__ void set_rates(StepRates &r, double lr, doub
     r.rate = (float)(lr / c1);
 }
 
-// The code of size >= 0 with 1 / scale; the scale of a block from its largest one, whose bits order like the values
-__device__ __forceinline__ float step_code(float size, float inverse) { return rintf(__fsqrt_rn(__fmul_rn(size, inverse))); }
+// Two numbers at a time, each operation rounded by itself.  The assembler makes a fused multiply-add of mul.rn.f32x2 and a sum that
+// follows; so a product is a fused one with -0, which it does not know (`none`: StepRates::none).
+__device__ __forceinline__ float2 step_mul(float2 a, float2 b, float none)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %6};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(none));
+    return d;
+}
+__device__ __forceinline__ float2 step_add(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 step_both(float x) { return make_float2(x, x); }
+
+constexpr uint32_t kByteFloat = 0x4B000000u;            // 2^23: a byte in its lowest place is added to it
+constexpr float kRoundCode = 12582912.0f;               // 1.5 * 2^23: the sum's last place is 1
+
+// bytes j and j + 1 of `w` as numbers, less `bias`
+__device__ __forceinline__ float2 step_bytes(uint32_t w, uint32_t j, float bias)
+{
+    return step_add(make_float2(__uint_as_float(__byte_perm(w, kByteFloat, 0x7540 + j)), __uint_as_float(__byte_perm(w, kByteFloat, 0x7541 + j))),
+                    step_both(-8388608.0f - bias));
+}
+
+__device__ __forceinline__ float sqrt_near(float x)     // 2^-23 of the value off; 0 below 2^-126
+{
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_near(float x)      // 2^-23 of the value off
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Codes of four elements, as numbers that have them in their lowest byte: rint(sqrt(size * inverse)) with the sign of m for m, whose
+// size is |m|, and of 1 at least for v above 0, whose size is sqrt(v).
+//
+// Roots are taken with 2^-23 of their value first.  The one or two of them and the rounding of the product leave the last one, which is 255 at
+// most, less than 2^-13 off, and that tells the code unless it lies so near to the middle between two; then the roots are
+// rounded.  `exact`: that they are in any case.
+template <bool V>
+__device__ __forceinline__ void step_codes(float2 (&t)[2], const float2 (&of)[2], float inverse, float none, bool exact)
+{
+    const auto root_of = [&](float x, bool near) { return near ? sqrt_near(x) : __fsqrt_rn(x); };
+    const auto codes = [&](float2 x, bool near, float2 &root) {
+        const float2 size = V ? make_float2(root_of(x.x, near), root_of(x.y, near)) : make_float2(fabsf(x.x), fabsf(x.y));
+        const float2 y = step_mul(size, step_both(inverse), none);
+        root = make_float2(root_of(y.x, near), root_of(y.y, near));
+        if (V) {
+            if (x.x > 0.0f)
+                root.x = fmaxf(root.x, 1.0f);
+            if (x.y > 0.0f)
+                root.y = fmaxf(root.y, 1.0f);
+        } else {
+            root = make_float2(copysignf(root.x, x.x), copysignf(root.y, x.y));
+        }
+        return step_add(root, step_both(kRoundCode));
+    };
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        float2 root;
+        t[i] = codes(of[i], true, root);
+        const float2 c = step_add(t[i], step_both(-kRoundCode)), off = step_add(root, make_float2(-c.x, -c.y));
+        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+    }
+    if (far > 0.5f - 1.0f / 8192 || exact) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float2 root;
+            t[i] = codes(of[i], false, root);
+        }
+    }
+}
+
+// the scale of a block from its largest size, whose bits order like the values; 1 / scale, or 0 where there is none
 __device__ __forceinline__ float step_scale(uint32_t top, float squared_steps, float &scale)
 {
     if (top >= 0x7F800000u) {
@@ -85,9 +169,9 @@ __device__ __forceinline__ float step_scale(uint32_t top, float squared_steps, f
     return __frcp_rn(scale);
 }
 
-// Eight elements of a thread.  FAST: neighbours, in whole vectors; otherwise 32 apart, one at a time, those below `left` only.
+// Eight elements of a thread, in pairs.  FAST: neighbours, in whole vectors; otherwise 32 apart, one at a time, those below `left` only.
 template <int DT, int GDT, int SDT, bool MASTER, bool FAST>
-__device__ __forceinline__ void step_elements(const StepTensor &t, const StepRates &r, float grad_scale, bool scaled, uint64_t at, uint32_t left)
+__device__ __forceinline__ void step_elements(const StepTensor &t, const StepRates &r, float grad_scale, uint64_t at, uint32_t left)
 {
     using P = Element<DT>;
     using G = Element<GDT>;
@@ -99,11 +183,23 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
     const typename G::T *const grad = static_cast<const typename G::T *>(t.grad) + block;
     float *const master = MASTER ? t.master + block : nullptr;
     float p[N], g[N], m[N], v[N];
+    uint32_t qm[2] = {}, qv[2] = {};                    // codes, four a word
     auto mine = [&](int j) { return lane + 32 * j; };
 
     if constexpr (FAST) {
         Raw<GDT, N> raw_g;
         raw_g.load(grad + lane * N);
+        if constexpr (kSmall) {
+            const uint2 m8 = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(t.m) + block + lane * N);
+            const uint2 v8 = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(t.v) + block + lane * N);
+            qm[0] = m8.x; qm[1] = m8.y; qv[0] = v8.x; qv[1] = v8.y;
+        } else {
+            Raw<CLPK_DT_F32, N> raw_m, raw_v;
+            raw_m.load(static_cast<const float *>(t.m) + block + lane * N);
+            raw_v.load(static_cast<const float *>(t.v) + block + lane * N);
+            raw_m.widen(m);
+            raw_v.widen(v);
+        }
         if constexpr (MASTER) {
             Raw<CLPK_DT_F32, N> raw;
             raw.load(master + lane * N);
@@ -112,21 +208,6 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
             Raw<DT, N> raw;
             raw.load(param + lane * N);
             raw.widen(p);
-        }
-        if constexpr (kSmall) {
-            const uint2 qm = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(t.m) + block + lane * N);
-            const uint2 qv = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(t.v) + block + lane * N);
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                m[j] = (float)(int8_t)((j < 4 ? qm.x : qm.y) >> (8 * (j & 3)));
-                v[j] = (float)(uint8_t)((j < 4 ? qv.x : qv.y) >> (8 * (j & 3)));
-            }
-        } else {
-            Raw<CLPK_DT_F32, N> raw_m, raw_v;
-            raw_m.load(static_cast<const float *>(t.m) + block + lane * N);
-            raw_v.load(static_cast<const float *>(t.v) + block + lane * N);
-            raw_m.widen(m);
-            raw_v.widen(v);
         }
         raw_g.widen(g);
     } else {
@@ -137,8 +218,8 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
                 g[j] = G::widen(grad[mine(j)]);
                 p[j] = MASTER ? master[mine(j)] : P::widen(param[mine(j)]);
                 if constexpr (kSmall) {
-                    m[j] = static_cast<const int8_t *>(t.m)[block + mine(j)];
-                    v[j] = static_cast<const uint8_t *>(t.v)[block + mine(j)];
+                    qm[j / 4] |= (uint32_t)static_cast<const uint8_t *>(t.m)[block + mine(j)] << (8 * (j & 3));
+                    qv[j / 4] |= (uint32_t)static_cast<const uint8_t *>(t.v)[block + mine(j)] << (8 * (j & 3));
                 } else {
                     m[j] = static_cast<const float *>(t.m)[block + mine(j)];
                     v[j] = static_cast<const float *>(t.v)[block + mine(j)];
@@ -146,53 +227,39 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
             }
         }
     }
-    float root[N];
+    float sm = 0.0f, sv = 0.0f;
     if constexpr (kSmall) {
-        const float sm = t.m_scale[block / CLPK_ADAMW_BLOCK], sv = t.v_scale[block / CLPK_ADAMW_BLOCK];
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            m[j] = __fmul_rn(m[j] * fabsf(m[j]), sm);   // whole numbers below 2^16: their products are exact
-            const float old = __fmul_rn(v[j] * v[j], sv);
-            v[j] = __fmul_rn(old, old);
-        }
+        sm = t.m_scale[block / CLPK_ADAMW_BLOCK];
+        sv = t.v_scale[block / CLPK_ADAMW_BLOCK];
+        qm[0] ^= 0x80808080u;                           // from [-128, 127] to [0, 255]
+        qm[1] ^= 0x80808080u;
     }
+    const auto mul = [&](float2 a, float2 b) { return step_mul(a, b, r.none); };
+    // With moments in 8 bits the instructions are the bound: root and quotient come with 2^-23 of their value.  A near root is 0 where v is
+    // below 2^-126, so eps has to hide what is lost there, 2^-63: by 2^-22.
+    const bool near = kSmall && r.eps >= r.root_scale * 4.547473508864641e-13f;
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-        if (scaled)
-            g[j] = __fmul_rn(g[j], grad_scale);
-        m[j] = __fadd_rn(__fmul_rn(m[j], r.b1), __fmul_rn(g[j], r.b1_rest));
-        v[j] = __fadd_rn(__fmul_rn(v[j], r.b2), __fmul_rn(__fmul_rn(g[j], g[j]), r.b2_rest));
-        root[j] = __fsqrt_rn(v[j]);
-        const float step = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(root[j], r.root_scale), r.eps));
-        p[j] = __fsub_rn(__fmul_rn(p[j], r.keep), __fmul_rn(step, r.rate));
-    }
-
-    uint32_t qm[2] = {}, qv[2] = {};
-    if constexpr (kSmall) {
-        uint32_t top_m = 0, top_v = 0;                  // zeros behind the last element are the largest of nothing
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            if (FAST || mine(j) < left) {
-                top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-                top_v = max(top_v, __float_as_uint(root[j]) & 0x7FFFFFFFu);
-            }
+    for (int j = 0; j < N; j += 2) {
+        float2 m2 = make_float2(m[j], m[j + 1]), v2 = make_float2(v[j], v[j + 1]), p2 = make_float2(p[j], p[j + 1]), step;
+        const float2 g2 = mul(make_float2(g[j], g[j + 1]), step_both(grad_scale));
+        if constexpr (kSmall) {
+            const float2 q = step_bytes(qm[j / 4], j & 3, 128.0f), c = step_bytes(qv[j / 4], j & 3, 0.0f);
+            m2 = mul(mul(q, make_float2(fabsf(q.x), fabsf(q.y))), step_both(sm));       // whole numbers below 2^16: their products are exact
+            const float2 old = mul(mul(c, c), step_both(sv));
+            v2 = mul(old, old);
         }
-        top_m = __reduce_max_sync(0xffffffffu, top_m);
-        top_v = __reduce_max_sync(0xffffffffu, top_v);
-        float sm, sv;
-        const float im = step_scale(top_m, 127.0f * 127.0f, sm), iv = step_scale(top_v, 255.0f * 255.0f, sv);
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            const float cm = step_code(fabsf(m[j]), im), cv = step_code(root[j], iv);
-            const int q = im > 0.0f ? (int)copysignf(cm, m[j]) : 0;
-            const uint32_t c = iv > 0.0f ? (root[j] > 0.0f ? max((uint32_t)cv, 1u) : 0u) : 0u;
-            qm[j / 4] |= ((uint32_t)q & 0xFFu) << (8 * (j & 3));
-            qv[j / 4] |= c << (8 * (j & 3));
-        }
-        if (lane == 0 && (FAST || left > 0)) {
-            t.m_scale[block / CLPK_ADAMW_BLOCK] = sm;
-            t.v_scale[block / CLPK_ADAMW_BLOCK] = sv;
-        }
+        m2 = step_add(mul(m2, step_both(r.b1)), mul(g2, step_both(r.b1_rest)));
+        v2 = step_add(mul(v2, step_both(r.b2)), mul(mul(g2, g2), step_both(r.b2_rest)));
+        const float2 root = near ? make_float2(sqrt_near(v2.x), sqrt_near(v2.y)) : make_float2(__fsqrt_rn(v2.x), __fsqrt_rn(v2.y));
+        const float2 under = step_add(mul(root, step_both(r.root_scale)), step_both(r.eps));
+        step = kSmall ? mul(m2, make_float2(rcp_near(under.x), rcp_near(under.y))) : make_float2(__fdiv_rn(m2.x, under.x), __fdiv_rn(m2.y, under.y));
+        p2 = step_add(mul(p2, step_both(r.keep)), mul(step, step_both(-r.rate)));
+        p[j] = p2.x;
+        p[j + 1] = p2.y;
+        m[j] = m2.x;
+        m[j + 1] = m2.y;
+        v[j] = v2.x;
+        v[j + 1] = v2.y;
     }
 
     if constexpr (FAST) {
@@ -204,10 +271,7 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
             raw.round(p);
             raw.store(master + lane * N);
         }
-        if constexpr (kSmall) {
-            *reinterpret_cast<uint2 *>(static_cast<int8_t *>(t.m) + block + lane * N) = make_uint2(qm[0], qm[1]);
-            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(t.v) + block + lane * N) = make_uint2(qv[0], qv[1]);
-        } else {
+        if constexpr (!kSmall) {
             raw.round(m);
             raw.store(static_cast<float *>(t.m) + block + lane * N);
             raw.round(v);
@@ -220,19 +284,61 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
                 param[mine(j)] = P::round(p[j]);
                 if constexpr (MASTER)
                     master[mine(j)] = p[j];
-                if constexpr (kSmall) {
-                    static_cast<int8_t *>(t.m)[block + mine(j)] = (int8_t)(qm[j / 4] >> (8 * (j & 3)));
-                    static_cast<uint8_t *>(t.v)[block + mine(j)] = (uint8_t)(qv[j / 4] >> (8 * (j & 3)));
-                } else {
+                if constexpr (!kSmall) {
                     static_cast<float *>(t.m)[block + mine(j)] = m[j];
                     static_cast<float *>(t.v)[block + mine(j)] = v[j];
                 }
             }
     }
+
+    if constexpr (kSmall) {
+        uint32_t top_m = 0, top_v = 0;                  // zeros behind the last element are the largest of nothing
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (FAST || mine(j) < left) {
+                top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+                top_v = max(top_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+            }
+        top_m = __reduce_max_sync(0xffffffffu, top_m);
+        top_v = __reduce_max_sync(0xffffffffu, top_v);
+        // the largest root is that of the largest v; where that is below 2^-90, roots that are near lose what lies below 2^-126
+        const bool low = top_v < 0x12800000u;
+        const float im = step_scale(top_m, 127.0f * 127.0f, sm), iv = step_scale(__float_as_uint(__fsqrt_rn(__uint_as_float(top_v))), 255.0f * 255.0f, sv);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float2 c[2] = {};
+            const auto word = [&](float inverse) {
+                const uint32_t w = __byte_perm(__byte_perm(__float_as_uint(c[0].x), __float_as_uint(c[0].y), 0x0040),
+                                               __byte_perm(__float_as_uint(c[1].x), __float_as_uint(c[1].y), 0x0040), 0x5410);
+                return inverse > 0.0f ? w : 0u;
+            };
+            const float2 m4[2] = {make_float2(m[4 * h], m[4 * h + 1]), make_float2(m[4 * h + 2], m[4 * h + 3])};
+            const float2 v4[2] = {make_float2(v[4 * h], v[4 * h + 1]), make_float2(v[4 * h + 2], v[4 * h + 3])};
+            step_codes<false>(c, m4, im, r.none, false);
+            qm[h] = word(im);
+            step_codes<true>(c, v4, iv, r.none, low);
+            qv[h] = word(iv);
+        }
+        if (lane == 0 && (FAST || left > 0)) {
+            t.m_scale[block / CLPK_ADAMW_BLOCK] = sm;
+            t.v_scale[block / CLPK_ADAMW_BLOCK] = sv;
+        }
+        if constexpr (FAST) {
+            *reinterpret_cast<uint2 *>(static_cast<int8_t *>(t.m) + block + lane * N) = make_uint2(qm[0], qm[1]);
+            *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(t.v) + block + lane * N) = make_uint2(qv[0], qv[1]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (mine(j) < left) {
+                    static_cast<int8_t *>(t.m)[block + mine(j)] = (int8_t)(qm[j / 4] >> (8 * (j & 3)));
+                    static_cast<uint8_t *>(t.v)[block + mine(j)] = (uint8_t)(qv[j / 4] >> (8 * (j & 3)));
+                }
+        }
+    }
 }
 
 template <int DT, int GDT, int SDT, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kStepThreads) adamw_kernel(const __grid_constant__ StepTable<CAP> table)
+__global__ void __launch_bounds__(kStepThreads, 4) adamw_kernel(const __grid_constant__ StepTable<CAP> table)
 {
     __shared__ StepRates told;
     griddep_wait();
@@ -259,15 +365,14 @@ __global__ void __launch_bounds__(kStepThreads) adamw_kernel(const __grid_consta
         r.root_scale = told.root_scale;
         r.rate = told.rate;
     }
-    const bool scaled = table.c.grad_scale != nullptr;
-    const float grad_scale = scaled ? *table.c.grad_scale : 1.0f;
+    const float grad_scale = table.c.grad_scale ? *table.c.grad_scale : 1.0f;
     if (at >= t.n)                                      // whole warps, behind the last barrier
         return;
     const uint64_t left = t.n - at;
     if ((table.first[lo] & kStepAligned) && left >= CLPK_ADAMW_BLOCK)
-        step_elements<DT, GDT, SDT, MASTER, true>(t, r, grad_scale, scaled, at, CLPK_ADAMW_BLOCK);
+        step_elements<DT, GDT, SDT, MASTER, true>(t, r, grad_scale, at, CLPK_ADAMW_BLOCK);
     else
-        step_elements<DT, GDT, SDT, MASTER, false>(t, r, grad_scale, scaled, at, left < CLPK_ADAMW_BLOCK ? (uint32_t)left : CLPK_ADAMW_BLOCK);
+        step_elements<DT, GDT, SDT, MASTER, false>(t, r, grad_scale, at, left < CLPK_ADAMW_BLOCK ? (uint32_t)left : CLPK_ADAMW_BLOCK);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------
@@ -365,7 +470,7 @@ extern "C" int clpk_adamw(const clpk_adamw_args_t *args, void *stream)
     CLPK_REQUIRE(a.grad_dtype == a.dtype || a.grad_dtype == CLPK_DT_F32, "%s: grad_dtype %d is neither dtype nor F32", what, a.grad_dtype);
     CLPK_REQUIRE(a.state_dtype == CLPK_DT_F32 || a.state_dtype == CLPK_DT_I8, "%s: state_dtype %d is not F32 or I8", what, a.state_dtype);
     CLPK_REQUIRE(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0, "%s: beta1 %g, beta2 %g: both in [0, 1)", what, a.beta1, a.beta2);
-    CLPK_REQUIRE((float)a.eps > 0.0f && a.eps < 1e30, "%s: eps %g is not above 0 in fp32", what, a.eps);
+    CLPK_REQUIRE(a.eps >= 1.17549435e-38 && a.eps < 1e30, "%s: eps %g is not in [2^-126, 1e30)", what, a.eps);
     CLPK_REQUIRE(std::isfinite(a.weight_decay) && a.weight_decay >= 0.0 && (a.d_lr || (std::isfinite(a.lr) && a.lr >= 0.0)), "%s: lr %g, weight_decay %g", what, a.lr, a.weight_decay);
     CLPK_REQUIRE(a.d_step || a.step > 0, "%s: steps are counted from 1", what);
     CLPK_REQUIRE((uintptr_t)a.d_lr % 4 == 0 && (uintptr_t)a.d_step % 4 == 0 && (uintptr_t)a.d_grad_scale % 4 == 0, "%s: d_lr, d_step or d_grad_scale is not aligned to its elements", what);
@@ -383,6 +488,7 @@ extern "C" int clpk_adamw(const clpk_adamw_args_t *args, void *stream)
     c.rates.b2 = (float)a.beta2;
     c.rates.b2_rest = (float)(1.0 - a.beta2);
     c.rates.eps = (float)a.eps;
+    c.rates.none = -0.0f;
     if (!a.d_lr && !a.d_step)
         set_rates(c.rates, a.lr, a.beta1, a.beta2, a.weight_decay, (double)a.step);
     c.lr = a.lr;

@@ -622,7 +622,8 @@ typedef struct clpk_layer_norm_backward_args {
 CLPK_API int clpk_layer_norm_backward_workspace_bytes(uint32_t m, uint32_t d, size_t *bytes);
 CLPK_API int clpk_layer_norm_backward(const clpk_layer_norm_backward_args_t *args, void *stream);
 
-/* One step of Adam with decoupled weight decay over all tensors of a list, in fp32 whatever their types, each operation rounded:
+/* One step of Adam with decoupled weight decay over all tensors of a list, in fp32 whatever their types, each operation rounded (with
+ * moments in 8 bits the root and the quotient of p's line are up to 2^-23 of their value off before):
  *   g' = g * grad_scale
  *   m  = beta1 * m + (1 - beta1) * g'
  *   v  = beta2 * v + (1 - beta2) * g' * g'
@@ -656,7 +657,7 @@ typedef struct clpk_adamw_args {
     int           state_dtype;    /* CLPK_DT_F32 or CLPK_DT_I8                       */
     uint32_t      count;
     const clpk_adamw_tensor_t *h_tensors;   /* [count], read before the call returns */
-    double        lr, beta1, beta2, eps, weight_decay;
+    double        lr, beta1, beta2, eps, weight_decay;      /* betas in [0, 1), eps in [2^-126, 1e30) */
     uint64_t      step;           /* from 1; unused with d_step                      */
     const float  *d_lr;           /* NULL, or read by the step in place of lr        */
     const uint32_t *d_step;       /* NULL, or read by the step in place of step      */

@@ -164,6 +164,31 @@ def codes(size, steps):
     return scale, torch.where(finite[:, None], q, torch.zeros_like(q)).flatten()
 
 
+def step_off(p, update):
+    """What a parameter may be off in fp32 with moments in 8 bits.  A root that is 2^-23 off, a product and a sum (2^-24 each) make the
+    quotient's lower side 2^-22 off, its reciprocal 2^-23 more, the two products behind it 2^-24 each; the plain form has five
+    roundings of 2^-24 there: less than 2^-20 of the update in all.  The last sum is rounded on either side."""
+    return 2.0 ** -20 * update.double().abs() + 2 * U * p.double().abs() + 2.0 ** -149
+
+
+def same_step(got, want):
+    """Equal, bit for bit, and parameters with moments in 8 bits as near as step_off says; one of 16 bits besides by a place, where its
+    rounding falls to the other side."""
+    want = dict(want)
+    off = want.pop("off", None)
+    if off is not None:
+        for name in ("param", "master"):
+            if name not in want:
+                continue
+            a, b = got[name], want.pop(name)
+            assert a.dtype == b.dtype and a.shape == b.shape
+            assert torch.equal(torch.isfinite(a), torch.isfinite(b)) and torch.equal(torch.isnan(a), torch.isnan(b))
+            fine = torch.isfinite(b)
+            place = 0 if b.dtype == torch.float32 else 2 * F.rounded(b.double(), "bf16" if b.dtype == torch.bfloat16 else "f16")
+            F.check(torch.where(fine, a, torch.zeros_like(a)), torch.where(fine, b, torch.zeros_like(b)).double(), torch.nan_to_num(off + place, 0, 0, 0), name)
+    same(got, want)
+
+
 def adamw_plain(t, lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, step=3, grad_scale=None):
     """What one step makes of a Tensor: its values by name."""
     p = t.master.clone() if t.master is not None else t.param.float()
@@ -179,12 +204,14 @@ def adamw_plain(t, lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, s
     v = v * beta2 + (g * g) * (1 - beta2)
     root = torch.sqrt(v)
     c1, c2 = -math.expm1(step * math.log(beta1)) if beta1 else 1.0, -math.expm1(step * math.log(beta2)) if beta2 else 1.0
-    p = p * (1 - lr * weight_decay) - (m / (root * (1 / math.sqrt(c2)) + eps)) * (lr / c1)
+    update = (m / (root * (1 / math.sqrt(c2)) + eps)) * (lr / c1)
+    p = p * (1 - lr * weight_decay) - update
     out = {"param": p.to(t.param.dtype)}
     if t.master is not None:
         out["master"] = p
     if t.state == "f32":
         return dict(out, m=m, v=v)
+    out["off"] = step_off(p, update)
     out["m_scale"], q = codes(m.abs(), 127)
     out["m"] = (q[:t.n] * torch.sign(torch.nan_to_num(m))).to(torch.int8)
     out["v_scale"], q = codes(root, 255)
