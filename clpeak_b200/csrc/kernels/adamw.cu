@@ -88,6 +88,21 @@ __device__ __forceinline__ float2 step_add(float2 a, float2 b)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+__device__ __forceinline__ float2 step_sub(float2 a, float2 b)          // b * -1 + a
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %6};\n\tfma.rn.f32x2 a, b, c, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(-1.0f));
+    return d;
+}
+// the largest of three, NaN where one is NaN
+__device__ __forceinline__ float step_max(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float2 step_both(float x) { return make_float2(x, x); }
 
 constexpr uint32_t kByteFloat = 0x4B000000u;            // 2^23: a byte in its lowest place is added to it
@@ -114,7 +129,7 @@ __device__ __forceinline__ float rcp_near(float x)      // 2^-23 of the value of
 }
 
 // Codes of four elements, as numbers that have them in their lowest byte: rint(sqrt(size * inverse)) with the sign of m for m, whose
-// size is |m|, and of 1 at least for v above 0, whose size is sqrt(v).
+// size is |m|, and of 1 at least for v, whose size is sqrt(v).
 //
 // Roots are taken with 2^-23 of their value first.  The one or two of them and the rounding of the product leave the last one, which is 255 at
 // most, less than 2^-13 off, and that tells the code unless it lies so near to the middle between two; then the roots are
@@ -127,14 +142,7 @@ __device__ __forceinline__ void step_codes(float2 (&t)[2], const float2 (&of)[2]
         const float2 size = V ? make_float2(root_of(x.x, near), root_of(x.y, near)) : make_float2(fabsf(x.x), fabsf(x.y));
         const float2 y = step_mul(size, step_both(inverse), none);
         root = make_float2(root_of(y.x, near), root_of(y.y, near));
-        if (V) {
-            if (x.x > 0.0f)
-                root.x = fmaxf(root.x, 1.0f);
-            if (x.y > 0.0f)
-                root.y = fmaxf(root.y, 1.0f);
-        } else {
-            root = make_float2(copysignf(root.x, x.x), copysignf(root.y, x.y));
-        }
+        root = V ? make_float2(fmaxf(root.x, 1.0f), fmaxf(root.y, 1.0f)) : make_float2(copysignf(root.x, x.x), copysignf(root.y, x.y));
         return step_add(root, step_both(kRoundCode));
     };
     float far = 0.0f;
@@ -142,10 +150,10 @@ __device__ __forceinline__ void step_codes(float2 (&t)[2], const float2 (&of)[2]
     for (int i = 0; i < 2; i++) {
         float2 root;
         t[i] = codes(of[i], true, root);
-        const float2 c = step_add(t[i], step_both(-kRoundCode)), off = step_add(root, make_float2(-c.x, -c.y));
-        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+        const float2 off = step_sub(root, step_add(t[i], step_both(-kRoundCode)));
+        far = step_max(far, fabsf(off.x), fabsf(off.y));
     }
-    if (far > 0.5f - 1.0f / 8192 || exact) {
+    if (far > 0.5f - 1.0f / 8192 || exact) {            // not with a NaN, of whose block the codes are 0
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             float2 root;
@@ -292,15 +300,15 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
     }
 
     if constexpr (kSmall) {
-        uint32_t top_m = 0, top_v = 0;                  // zeros behind the last element are the largest of nothing
+        float most_m = 0.0f, most_v = 0.0f, least_v = v[0];
 #pragma unroll
-        for (int j = 0; j < N; j++)
-            if (FAST || mine(j) < left) {
-                top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-                top_v = max(top_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-            }
-        top_m = __reduce_max_sync(0xffffffffu, top_m);
-        top_v = __reduce_max_sync(0xffffffffu, top_v);
+        for (int j = 0; j < N; j += 2) {                // behind the last element m and v are what became of zeros: zeros, or NaN by a factor that is none
+            const bool a = FAST || mine(j) < left, b = FAST || mine(j + 1) < left;
+            most_m = step_max(most_m, a ? fabsf(m[j]) : 0.0f, b ? fabsf(m[j + 1]) : 0.0f);
+            most_v = step_max(most_v, a ? v[j] : 0.0f, b ? v[j + 1] : 0.0f);
+            least_v = fminf(least_v, fminf(v[j], v[j + 1]));
+        }
+        const uint32_t top_m = __reduce_max_sync(0xffffffffu, __float_as_uint(most_m)), top_v = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
         // the largest root is that of the largest v; where that is below 2^-90, roots that are near lose what lies below 2^-126
         const bool low = top_v < 0x12800000u;
         const float im = step_scale(top_m, 127.0f * 127.0f, sm), iv = step_scale(__float_as_uint(__fsqrt_rn(__uint_as_float(top_v))), 255.0f * 255.0f, sv);
@@ -318,6 +326,11 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
             qm[h] = word(im);
             step_codes<true>(c, v4, iv, r.none, low);
             qv[h] = word(iv);
+            if (least_v == 0.0f)                        // of a v of 0 the code is 0
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (v[4 * h + j] == 0.0f)
+                        qv[h] &= ~(0xFFu << (8 * j));
         }
         if (lane == 0 && (FAST || left > 0)) {
             t.m_scale[block / CLPK_ADAMW_BLOCK] = sm;
@@ -338,7 +351,7 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
 }
 
 template <int DT, int GDT, int SDT, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kStepThreads, 4) adamw_kernel(const __grid_constant__ StepTable<CAP> table)
+__global__ void __launch_bounds__(kStepThreads, SDT == CLPK_DT_I8 ? 6 : 4) adamw_kernel(const __grid_constant__ StepTable<CAP> table)
 {
     __shared__ StepRates told;
     griddep_wait();
