@@ -8,9 +8,13 @@
 // that share it, as the vectors it was loaded in, and the squares are summed about the mean: that is a second pass over registers,
 // and it keeps the digits that sum x^2 - d mean^2 loses where the mean is large.
 //
-// dw and db are sums down the columns.  A CTA takes every gridDim-th row; a thread has the same columns of each, so that its share
-// of both sums stays in registers, and one part for each CTA goes to the workspace, which a second kernel adds up: 8 bytes a column
-// and CTA beside 6 a column and row.  The order of the sums depends on the sizes alone.
+// CTAs stay, with the weights in registers, and take every gridDim-th row; a thread copies its pieces of the rows that come next into
+// shared memory of its own (cp.async) while it computes, so that an SM has 40 to 200 KB on their way whatever its threads wait for.
+//
+// dw and db are sums down the columns: a thread has the same columns of each of its rows, so that its share of both sums stays in
+// registers, and one part for each CTA goes to the workspace, which a second kernel adds up: 8 bytes a column and CTA beside 6 a
+// column and row.  The order of the sums depends on the sizes alone.
+#include "../clpk_activation.cuh"
 #include "../clpk_elements.cuh"
 #include "../clpk_internal.h"
 #include "../clpk_ptx.cuh"
@@ -18,6 +22,16 @@
 #include <algorithm>
 
 namespace clpk {
+
+// Two sums with one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 
 struct NormParams {
     const void *x, *weight, *bias;
@@ -70,77 +84,138 @@ __device__ __forceinline__ void load_weights(float (&w)[N], const void *base, ui
     raw.widen(w);
 }
 
-constexpr int kNormWarps = 4;                       // rows of a CTA whose rows are a warp's
+// ---- rows ahead ----------------------------------------------------------------------------------------------
+//
+// A thread's share of a row is asked for some rows ahead, into shared memory that is the thread's own: what it reads there it has copied
+// there itself, so that no thread waits for another, and no register holds what is on its way.
+
+__device__ __forceinline__ void ask_piece(void *to, const void *from, uint32_t bytes)       // 16, or fewer and zeros behind them
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void asked()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_asked()                    // all but the last N groups are there
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// the pieces of a row that fall to thread t of THREADS
+template <int DT, int THREADS, int PIECES>
+__device__ __forceinline__ void ask_row(uint4 *to, uint32_t stride, const typename Element<DT>::T *row, uint32_t t, uint32_t d)
+{
+    constexpr uint32_t N = kPiece<DT>, kBytes = 16 / N;
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+        const uint32_t at = (i * THREADS + t) * N, left = at < d ? d - at : 0;
+        if (left)
+            ask_piece(to + i * stride, row + at, left < N ? left * kBytes : 16);
+    }
+}
+
+constexpr int kNormWarps = 4;                       // rows that a CTA takes at once where a row is a warp's
+constexpr int kNormAhead = 2;                       // rows on their way behind the one that is computed
+
+// How many CTAs an SM holds: 128 registers a thread for 32 elements with their weights, 80 and 48 for 16 and 8.
+__host__ __device__ constexpr int norm_ctas(int threads, int elems) { return threads == 32 ? (elems == 32 ? 4 : elems == 16 ? 6 : 10) : 512 / threads; }
+template <int DT> constexpr uint32_t norm_bytes(int threads, int elems)
+{
+    return (kNormAhead + 1) * (threads == 32 ? 32 * kNormWarps : threads) * elems * (uint32_t)sizeof(typename Element<DT>::T);
+}
 
 // THREADS share a row of up to THREADS * ELEMS elements; rows and weights start on 16 bytes
 template <int DT, int WDT, int THREADS, int ELEMS>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS) layer_norm_kernel(NormParams p)
+__global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, norm_ctas(THREADS, ELEMS)) layer_norm_kernel(NormParams p)
 {
     using T = typename Element<DT>::T;
-    constexpr int N = kPiece<DT>, kPieces = ELEMS / N;
+    constexpr int N = kPiece<DT>, kPieces = ELEMS / N, kRows = THREADS == 32 ? kNormWarps : 1;
+    constexpr uint32_t kAll = THREADS == 32 ? 32 * kNormWarps : THREADS, kStage = kPieces * kAll;
+    extern __shared__ __align__(16) uint4 ring[];
     __shared__ float shared[2][THREADS / 32];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t row = THREADS == 32 ? blockIdx.x * kNormWarps + (threadIdx.x >> 5) : blockIdx.x, t = threadIdx.x % THREADS;
-    if (row >= p.m)                                 // whole warps, and THREADS == 32 alone: no barrier follows
-        return;
-    const T *x = static_cast<const T *>(p.x) + row * p.ldx;
-    Raw<DT, N> raw[kPieces];
-    float sum = 0.0f;
+    const uint32_t t = threadIdx.x % THREADS, step = gridDim.x * kRows;
+    const uint64_t first = blockIdx.x * kRows + (THREADS == 32 ? threadIdx.x >> 5 : 0);
+    uint4 *const mine = ring + threadIdx.x;
+    const auto ask = [&](uint64_t row, uint32_t stage) {
+        if (row < p.m)
+            ask_row<DT, THREADS, kPieces>(mine + stage * kStage, kAll, static_cast<const T *>(p.x) + row * p.ldx, t, p.d);
+        asked();
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kNormAhead; i++)
+        ask(first + (uint64_t)i * step, i);
+    float w[ELEMS], b[ELEMS];
 #pragma unroll
     for (int i = 0; i < kPieces; i++) {
         const uint32_t at = (i * THREADS + t) * N;
-        if (at + N <= p.d)
-            raw[i].load(x + at);
-        else
-            raw[i].load_some(x + at, at < p.d ? p.d - at : 0);
+        load_weights<WDT, N>(reinterpret_cast<float(&)[N]>(w[i * N]), p.weight, at, p.d, 1.0f);
+        load_weights<WDT, N>(reinterpret_cast<float(&)[N]>(b[i * N]), p.bias, at, p.d, 0.0f);
     }
+    uint32_t stage = 0;
+    for (uint64_t row = first; row < p.m; row += step) {
+        ask(row + (uint64_t)kNormAhead * step, stage == 0 ? kNormAhead : stage - 1);
+        wait_asked<kNormAhead>();
+        Raw<DT, N> raw[kPieces];
+        float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPieces; i++) {
-        float v[N];
-        raw[i].widen(v);
+        for (int i = 0; i < kPieces; i++) {
+            const uint32_t at = (i * THREADS + t) * N;
+            raw[i].v[0] = at < p.d ? mine[stage * kStage + i * kAll] : make_uint4(0, 0, 0, 0);
+            float v[N];
+            raw[i].widen(v);
 #pragma unroll
-        for (int j = 0; j < N; j++)
-            sum += v[j];
+            for (int j = 0; j < N; j++)
+                sum += v[j];
+        }
+        const float mean = row_sum<THREADS>(sum, shared[0]) / (float)p.d;
+        float squares = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const uint32_t at = (i * THREADS + t) * N;
+            float v[N];
+            raw[i].widen(v);
+            if (at + N <= p.d) {
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    squares = fmaf(v[j] - mean, v[j] - mean, squares);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (at + j < p.d)
+                        squares = fmaf(v[j] - mean, v[j] - mean, squares);
+            }
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<THREADS>(squares, shared[1]) / (float)p.d + p.eps);
+        if (t == 0) {
+            if (p.mean)
+                p.mean[row] = mean;
+            if (p.rstd)
+                p.rstd[row] = rstd;
+        }
+        T *y = static_cast<T *>(p.y) + row * p.ldy;
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const uint32_t at = (i * THREADS + t) * N;
+            if (at >= p.d)
+                break;
+            float v[N];
+            raw[i].widen(v);
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                v[j] = fmaf((v[j] - mean) * rstd, w[i * N + j], b[i * N + j]);
+            raw[i].round(v);
+            if (at + N <= p.d)
+                raw[i].store(y + at);
+            else
+                raw[i].store_some(y + at, p.d - at);
+        }
+        stage = stage == kNormAhead ? 0 : stage + 1;
     }
-    const float mean = row_sum<THREADS>(sum, shared[0]) / (float)p.d;
-    float squares = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPieces; i++) {
-        const uint32_t at = (i * THREADS + t) * N;
-        float v[N];
-        raw[i].widen(v);
-#pragma unroll
-        for (int j = 0; j < N; j++)
-            if (at + N <= p.d || at + j < p.d)
-                squares = fmaf(v[j] - mean, v[j] - mean, squares);
-    }
-    const float rstd = 1.0f / sqrtf(row_sum<THREADS>(squares, shared[1]) / (float)p.d + p.eps);
-    if (t == 0) {
-        if (p.mean)
-            p.mean[row] = mean;
-        if (p.rstd)
-            p.rstd[row] = rstd;
-    }
-    T *y = static_cast<T *>(p.y) + row * p.ldy;
-#pragma unroll
-    for (int i = 0; i < kPieces; i++) {
-        const uint32_t at = (i * THREADS + t) * N;
-        if (at >= p.d)
-            break;
-        float v[N], w[N], b[N];
-        raw[i].widen(v);
-        load_weights<WDT>(w, p.weight, at, p.d, 1.0f);
-        load_weights<WDT>(b, p.bias, at, p.d, 0.0f);
-#pragma unroll
-        for (int j = 0; j < N; j++)
-            v[j] = fmaf((v[j] - mean) * rstd, w[j], b[j]);
-        raw[i].round(v);
-        if (at + N <= p.d)
-            raw[i].store(y + at);
-        else
-            raw[i].store_some(y + at, p.d - at);
-    }
+    wait_asked<0>();
 }
 
 // Rows that do not start on 16 bytes, or longer than the registers hold: element by element, read three times
@@ -218,84 +293,138 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 *shared)
 
 constexpr int kNormGradWarps = 8;                   // of a CTA whose rows are a warp's
 
+// CTAs of an SM, and rows on their way behind the one that is computed: as many as registers (two sums for each element) and shared memory
+// (x and dy) hold, two rows at most.
+__host__ __device__ constexpr int norm_grad_threads(int threads) { return threads == 32 ? 32 * kNormGradWarps : threads; }
+__host__ __device__ constexpr uint32_t norm_grad_stage(int threads, int elems, uint32_t elem) { return 2 * norm_grad_threads(threads) * elems * elem; }
+__host__ __device__ constexpr int norm_grad_ctas(int threads, int elems, uint32_t elem)
+{
+    const int regs = elems == 8 ? 64 : elems == 16 ? 85 : 128, ctas = 65536 / (regs * norm_grad_threads(threads));
+    return ctas * 2 * norm_grad_stage(threads, elems, elem) <= 220 * 1024 ? ctas : 1;
+}
+__host__ __device__ constexpr int norm_grad_ahead(int threads, int elems, uint32_t elem)
+{
+    const int stages = 220 * 1024 / (norm_grad_ctas(threads, elems, elem) * norm_grad_stage(threads, elems, elem));
+    return stages >= 3 ? 2 : stages - 1;
+}
+
 template <int DT, int WDT, int THREADS, int ELEMS>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormGradWarps : THREADS) layer_norm_gradients_kernel(NormGradParams p)
+__global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THREADS, ELEMS, sizeof(typename Element<DT>::T))) layer_norm_gradients_kernel(NormGradParams p)
 {
     using T = typename Element<DT>::T;
-    constexpr int N = kPiece<DT>, kPieces = ELEMS / N, kRows = THREADS == 32 ? kNormGradWarps : 1;
+    constexpr int N = kPiece<DT>, kPieces = ELEMS / N, kRows = THREADS == 32 ? kNormGradWarps : 1, kAhead = norm_grad_ahead(THREADS, ELEMS, sizeof(T));
+    constexpr uint32_t kAll = norm_grad_threads(THREADS), kStage = 2 * kPieces * kAll;
+    extern __shared__ __align__(16) uint4 ring[];
     __shared__ float2 shared[2][THREADS / 32];
-    __shared__ float joined[THREADS == 32 ? 2 * 32 * ELEMS : 1];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t warp = threadIdx.x >> 5, t = threadIdx.x % THREADS;
-    float dw[ELEMS] = {}, db[ELEMS] = {};
-    uint32_t turn = 0;
-    Raw<DT, N> x[kPieces], dy[kPieces];
-    const uint32_t first = blockIdx.x * kRows + (kRows > 1 ? warp : 0), step = gridDim.x * kRows;
-    auto ask = [&](uint32_t row) {                  // a row ahead, so that its way lies under the sums of the one before
-        const T *from_x = static_cast<const T *>(p.x) + row * p.ldx, *from_dy = static_cast<const T *>(p.dy) + row * p.lddy;
-#pragma unroll
-        for (int i = 0; i < kPieces; i++) {
-            const uint32_t at = (i * THREADS + t) * N;
-            if (at + N <= p.d) {
-                x[i].load(from_x + at);
-                dy[i].load(from_dy + at);
-            } else {
-                x[i].load_some(from_x + at, at < p.d ? p.d - at : 0);
-                dy[i].load_some(from_dy + at, at < p.d ? p.d - at : 0);
-            }
+    const uint32_t warp = threadIdx.x >> 5, t = threadIdx.x % THREADS, step = gridDim.x * kRows;
+    const uint64_t first = blockIdx.x * kRows + (kRows > 1 ? warp : 0);
+    uint4 *const mine = ring + threadIdx.x;
+    const auto ask = [&](uint64_t row, uint32_t stage) {
+        if (row < p.m) {
+            ask_row<DT, THREADS, kPieces>(mine + stage * kStage, kAll, static_cast<const T *>(p.x) + row * p.ldx, t, p.d);
+            ask_row<DT, THREADS, kPieces>(mine + stage * kStage + kPieces * kAll, kAll, static_cast<const T *>(p.dy) + row * p.lddy, t, p.d);
         }
+        asked();
     };
-    if (first < p.m)
-        ask(first);
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; i++)
+        ask(first + (uint64_t)i * step, i);
+    float2 dw[ELEMS / 2] = {}, db[ELEMS / 2] = {}, w[ELEMS / 2];
+#pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+        float one[N];
+        load_weights<WDT, N>(one, p.weight, (i * THREADS + t) * N, p.d, 1.0f);
+#pragma unroll
+        for (int j = 0; j < N / 2; j++)
+            w[i * N / 2 + j] = make_float2(one[2 * j], one[2 * j + 1]);
+    }
+    uint32_t stage = 0, turn = 0;
+    float mean = first < p.m ? p.mean[first] : 0.0f, rstd = first < p.m ? p.rstd[first] : 0.0f;
     for (uint64_t row = first; row < p.m; row += step) {
-        const float mean = p.mean[row], rstd = p.rstd[row];
-        float hat[ELEMS], g[ELEMS];
-        float2 sum = make_float2(0.0f, 0.0f);
+        ask(row + (uint64_t)kAhead * step, stage == 0 ? kAhead : stage - 1);
+        const bool more = row + step < p.m;
+        const float next_mean = more ? p.mean[row + step] : 0.0f, next_rstd = more ? p.rstd[row + step] : 0.0f;
+        wait_asked<kAhead>();
+        // x - mean and dy of a piece, two numbers at a time; zeros behind the row, where a mean that is not finite must not come in
+        const auto values = [&](int i, float2 (&off)[N / 2], float2 (&dy)[N / 2]) {
+            const uint32_t at = (i * THREADS + t) * N;
+            Raw<DT, N> x, d;
+            float vx[N], vd[N];
+            x.v[0] = mine[stage * kStage + i * kAll];
+            d.v[0] = mine[stage * kStage + (kPieces + i) * kAll];
+            x.widen(vx);
+            d.widen(vd);
+            if (at + N > p.d) {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    vx[j] = at + j < p.d ? vx[j] : mean;
+                    vd[j] = at + j < p.d ? vd[j] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) {
+                off[j] = add2(make_float2(vx[2 * j], vx[2 * j + 1]), make_float2(-mean, -mean));
+                dy[j] = make_float2(vd[2 * j], vd[2 * j + 1]);
+            }
+            if (at + N > p.d) {
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (at + j >= p.d)
+                        (j % 2 ? off[j / 2].y : off[j / 2].x) = 0.0f;
+            }
+        };
+        const float2 scale = make_float2(rstd, rstd);
+        float2 sum_g = make_float2(0.0f, 0.0f), sum_go = sum_g;     // of g and of g * (x - mean)
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
-            const uint32_t at = (i * THREADS + t) * N;
-            float vx[N], vdy[N], w[N];
-            x[i].widen(vx);
-            dy[i].widen(vdy);
-            load_weights<WDT>(w, p.weight, at, p.d, 1.0f);
+            float2 off[N / 2], dy[N / 2];
+            values(i, off, dy);
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const int e = i * N + j;
-                // behind the row x and dy are zeros, and a mean or rstd that is not finite must not come back in
-                hat[e] = at + N <= p.d || at + j < p.d ? (vx[j] - mean) * rstd : 0.0f;
-                g[e] = vdy[j] * w[j];
-                dw[e] = fmaf(vdy[j], hat[e], dw[e]);
-                db[e] += vdy[j];
-                sum.x += g[e];
-                sum.y = fmaf(g[e], hat[e], sum.y);
+            for (int j = 0; j < N / 2; j++) {
+                const int e = i * N / 2 + j;
+                const float2 g = mul2(dy[j], w[e]);
+                dw[e] = fma2(dy[j], mul2(off[j], scale), dw[e]);
+                db[e] = add2(db[e], dy[j]);
+                sum_g = add2(sum_g, g);
+                sum_go = fma2(g, off[j], sum_go);
             }
         }
-        if (row + step < p.m)
-            ask((uint32_t)(row + step));
-        if (!p.dx)
-            continue;
-        sum = row_sums<THREADS>(sum, shared[turn]);
-        turn ^= 1;
-        const float c1 = sum.x / (float)p.d, c2 = sum.y / (float)p.d;
-        T *dx = static_cast<T *>(p.dx) + row * p.lddx;
+        if (p.dx) {
+            const float2 sum = row_sums<THREADS>(make_float2(sum_g.x + sum_g.y, sum_go.x + sum_go.y), shared[turn]);
+            turn ^= 1;
+            // dx = rstd g + (x - mean) by + also, by = -rstd^3 sum g (x - mean) / d, also = -rstd sum g / d
+            const float by = -rstd * (rstd * (rstd * (sum.y / (float)p.d))), also = -rstd * (sum.x / (float)p.d);
+            asm volatile("" ::: "memory");          // read again rather than kept in registers
+            T *dx = static_cast<T *>(p.dx) + row * p.lddx;
 #pragma unroll
-        for (int i = 0; i < kPieces; i++) {
-            const uint32_t at = (i * THREADS + t) * N;
-            if (at >= p.d)
-                break;
-            float v[N];
+            for (int i = 0; i < kPieces; i++) {
+                const uint32_t at = (i * THREADS + t) * N;
+                if (at >= p.d)
+                    break;
+                float2 off[N / 2], dy[N / 2];
+                float v[N];
+                values(i, off, dy);
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                v[j] = rstd * (g[i * N + j] - c1 - hat[i * N + j] * c2);
-            Raw<DT, N> out;
-            out.round(v);
-            if (at + N <= p.d)
-                out.store(dx + at);
-            else
-                out.store_some(dx + at, p.d - at);
+                for (int j = 0; j < N / 2; j++) {
+                    const float2 one = fma2(mul2(dy[j], w[i * N / 2 + j]), scale, fma2(off[j], make_float2(by, by), make_float2(also, also)));
+                    v[2 * j] = one.x;
+                    v[2 * j + 1] = one.y;
+                }
+                Raw<DT, N> out;
+                out.round(v);
+                if (at + N <= p.d)
+                    out.store(dx + at);
+                else
+                    out.store_some(dx + at, p.d - at);
+            }
         }
+        mean = next_mean;
+        rstd = next_rstd;
+        stage = stage == kAhead ? 0 : stage + 1;
     }
+    wait_asked<0>();
     if (!p.parts)
         return;
     float *part = p.parts + (uint64_t)blockIdx.x * 2 * p.d;
@@ -304,31 +433,31 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormGradWarps : THREADS)
         for (int i = 0; i < kPieces; i++)
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                const uint32_t at = (i * THREADS + t) * N + j;
+                const uint32_t at = (i * THREADS + t) * N + j, e = i * N + j;
                 if (at < p.d) {
-                    part[at] = dw[i * N + j];
-                    part[p.d + at] = db[i * N + j];
+                    part[at] = e % 2 ? dw[e / 2].y : dw[e / 2].x;
+                    part[p.d + at] = e % 2 ? db[e / 2].y : db[e / 2].x;
                 }
             }
     } else {
-        // the warps' shares, one warp after another
-        for (uint32_t w = 0; w < kNormGradWarps; w++) {
-            if (w == warp) {
+        // the warps' shares side by side where the rows were, then added in their order
+        float *const shares = reinterpret_cast<float *>(ring);
+        static_assert(kNormGradWarps * 2 * 32 * ELEMS * sizeof(float) <= (kAhead + 1) * norm_grad_stage(32, ELEMS, sizeof(T)), "room for all shares");
+        __syncthreads();
 #pragma unroll
-                for (int e = 0; e < ELEMS; e++) {
-                    const uint32_t at = e * 32 + t;
-                    joined[at] = w ? joined[at] + dw[e] : dw[e];
-                    joined[32 * ELEMS + at] = w ? joined[32 * ELEMS + at] + db[e] : db[e];
-                }
-            }
-            __syncthreads();
+        for (int e = 0; e < ELEMS; e++) {
+            shares[((warp * 2 + 0) * ELEMS + e) * 32 + t] = e % 2 ? dw[e / 2].y : dw[e / 2].x;
+            shares[((warp * 2 + 1) * ELEMS + e) * 32 + t] = e % 2 ? db[e / 2].y : db[e / 2].x;
         }
-        for (uint32_t e = warp; e < ELEMS; e += kNormGradWarps) {
-            const uint32_t at = (e / N * 32 + t) * N + e % N;
-            if (at < p.d) {
-                part[at] = joined[e * 32 + t];
-                part[p.d + at] = joined[32 * ELEMS + e * 32 + t];
-            }
+        __syncthreads();
+        for (uint32_t i = warp; i < 2 * ELEMS; i += kNormGradWarps) {
+            float sum = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kNormGradWarps; w++)
+                sum += shares[(w * 2 * ELEMS + i) * 32 + t];
+            const uint32_t e = i % ELEMS, at = (e / N * 32 + t) * N + e % N;
+            if (at < p.d)
+                part[i / ELEMS * p.d + at] = sum;
         }
     }
 }
@@ -395,11 +524,12 @@ struct NormJoinParams {
     uint32_t n_parts, d;
 };
 
-// The parts' sums, rounded: a lane has a column, the eight warps an eighth of the parts each
+// The parts' sums, rounded: a lane has a column, and each of 32 warps every 32nd part, so that all loads are on their way at once
+constexpr int kNormJoinWarps = 32;
 template <int WDT>
-__global__ void __launch_bounds__(256) layer_norm_join_kernel(NormJoinParams p)
+__global__ void __launch_bounds__(32 * kNormJoinWarps) layer_norm_join_kernel(NormJoinParams p)
 {
-    __shared__ float sums[8][32];
+    __shared__ float sums[kNormJoinWarps][32];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane, which = blockIdx.y;
@@ -408,8 +538,8 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(NormJoinParams p)
     float sum = 0.0f;
     if (col < p.d) {
         const float *from = p.parts + (uint64_t)which * p.d + col;
-#pragma unroll 8
-        for (uint32_t i = warp; i < p.n_parts; i += 8)
+#pragma unroll 16
+        for (uint32_t i = warp; i < p.n_parts; i += kNormJoinWarps)
             sum += from[(uint64_t)i * 2 * p.d];
     }
     sums[warp][lane] = sum;
@@ -417,43 +547,70 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(NormJoinParams p)
     if (warp > 0 || col >= p.d)
         return;
 #pragma unroll
-    for (uint32_t w = 1; w < 8; w++)
+    for (uint32_t w = 1; w < kNormJoinWarps; w++)
         sum += sums[w][lane];
     static_cast<typename Element<WDT>::T *>(p.out[which])[col] = Element<WDT>::round(sum);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------
 
-constexpr uint32_t kNormLongest = 32768, kNormGradLongest = 16384;      // elements of a row in registers
+constexpr uint32_t kNormLongest = 16384, kNormGradLongest = 16384;      // elements of a row in registers
+
+template <int DT, int WDT, int THREADS, int ELEMS>
+static int launch_norm_rows(const NormParams &p, cudaStream_t s)
+{
+    constexpr int kThreads = THREADS == 32 ? 32 * kNormWarps : THREADS;
+    constexpr uint32_t kBytes = norm_bytes<DT>(THREADS, ELEMS);
+    if (kBytes > 47 * 1024)
+        CLPK_CUDA(cudaFuncSetAttribute(layer_norm_kernel<DT, WDT, THREADS, ELEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes));
+    const uint32_t ctas = std::min<uint32_t>(THREADS == 32 ? (p.m - 1) / kNormWarps + 1 : p.m, norm_ctas(THREADS, ELEMS) * (uint32_t)num_sms());
+    return launch_behind(layer_norm_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm", ctas, kThreads, kBytes, s, p);
+}
 
 template <int DT, int WDT>
 static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
 {
     if (!aligned || p.d > kNormLongest)
         return launch_behind(layer_norm_plain_kernel<DT, WDT>, "layer_norm_plain", p.m, 256, 0, s, p);
-    const unsigned by_warps = (p.m - 1) / kNormWarps + 1;
     if (p.d <= 256)
-        return launch_behind(layer_norm_kernel<DT, WDT, 32, 8>, "layer_norm", by_warps, 32 * kNormWarps, 0, s, p);
+        return launch_norm_rows<DT, WDT, 32, 8>(p, s);
     if (p.d <= 512)
-        return launch_behind(layer_norm_kernel<DT, WDT, 32, 16>, "layer_norm", by_warps, 32 * kNormWarps, 0, s, p);
+        return launch_norm_rows<DT, WDT, 32, 16>(p, s);
     if (p.d <= 1024)
-        return launch_behind(layer_norm_kernel<DT, WDT, 32, 32>, "layer_norm", by_warps, 32 * kNormWarps, 0, s, p);
+        return launch_norm_rows<DT, WDT, 32, 32>(p, s);
     if (p.d <= 4096)
-        return launch_behind(layer_norm_kernel<DT, WDT, 128, 32>, "layer_norm", p.m, 128, 0, s, p);
+        return launch_norm_rows<DT, WDT, 128, 32>(p, s);
     if (p.d <= 8192)
-        return launch_behind(layer_norm_kernel<DT, WDT, 256, 32>, "layer_norm", p.m, 256, 0, s, p);
-    if (p.d <= 16384)
-        return launch_behind(layer_norm_kernel<DT, WDT, 512, 32>, "layer_norm", p.m, 512, 0, s, p);
-    return launch_behind(layer_norm_kernel<DT, WDT, 1024, 32>, "layer_norm", p.m, 1024, 0, s, p);
+        return launch_norm_rows<DT, WDT, 256, 32>(p, s);
+    return launch_norm_rows<DT, WDT, 512, 32>(p, s);
 }
 
-// Parts of dw and db: CTAs of layer_norm_gradients_kernel.  A whole B200's: the workspace's size may not depend on the card at hand.
-static uint32_t norm_parts(uint32_t m, uint32_t d)
+// Threads and elements of each that share a row in layer_norm_gradients_kernel
+struct NormGradShape {
+    int threads, elems;
+};
+constexpr NormGradShape norm_grad_shape(uint32_t d)
+{
+    return d <= 256 ? NormGradShape{32, 8} : d <= 512 ? NormGradShape{32, 16} : d <= 1024 ? NormGradShape{32, 32} : d <= 2048 ? NormGradShape{128, 16}
+         : d <= 4096 ? NormGradShape{256, 16} : d <= 8192 ? NormGradShape{256, 32} : NormGradShape{512, 32};
+}
+
+// Parts of dw and db: the CTAs that share the rows.  A whole B200's: the workspace's size may not depend on the card at hand.
+static uint32_t norm_parts(uint32_t m, uint32_t d, uint64_t elem)
 {
     constexpr uint32_t kSms = 148;
-    if (d <= 1024)
-        return std::min(m ? (m - 1) / kNormGradWarps + 1 : 1, 4 * kSms);
-    return std::min(std::max(m, 1u), (d <= 2048 ? 4 : d <= 4096 ? 2 : 1) * kSms);
+    const NormGradShape shape = norm_grad_shape(d);
+    const uint32_t rows = shape.threads == 32 ? kNormGradWarps : 1;
+    return std::min(m ? (m - 1) / rows + 1 : 1, (uint32_t)norm_grad_ctas(shape.threads, shape.elems, (uint32_t)elem) * kSms);
+}
+
+template <int DT, int WDT, int THREADS, int ELEMS>
+static int launch_norm_gradient_rows(const NormGradParams &p, uint32_t parts, cudaStream_t s)
+{
+    constexpr uint32_t kElem = sizeof(typename Element<DT>::T), kBytes = (norm_grad_ahead(THREADS, ELEMS, kElem) + 1) * norm_grad_stage(THREADS, ELEMS, kElem);
+    if (kBytes > 47 * 1024)
+        CLPK_CUDA(cudaFuncSetAttribute(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes));
+    return launch_behind(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm_gradients", parts, norm_grad_threads(THREADS), kBytes, s, p);
 }
 
 template <int DT, int WDT>
@@ -464,19 +621,14 @@ static int launch_norm_gradients(const NormGradParams &p, bool aligned, uint32_t
             CLPK_TRY(launch_behind(layer_norm_plain_dx_kernel<DT, WDT>, "layer_norm_plain_dx", p.m, 256, 0, s, p));
         return p.parts ? launch_behind(layer_norm_plain_columns_kernel<DT>, "layer_norm_plain_columns", dim3((p.d - 1) / 256 + 1, parts), 256, 0, s, p) : CLPK_OK;
     }
-    if (p.d <= 256)
-        return launch_behind(layer_norm_gradients_kernel<DT, WDT, 32, 8>, "layer_norm_gradients", parts, 32 * kNormGradWarps, 0, s, p);
-    if (p.d <= 512)
-        return launch_behind(layer_norm_gradients_kernel<DT, WDT, 32, 16>, "layer_norm_gradients", parts, 32 * kNormGradWarps, 0, s, p);
-    if (p.d <= 1024)
-        return launch_behind(layer_norm_gradients_kernel<DT, WDT, 32, 32>, "layer_norm_gradients", parts, 32 * kNormGradWarps, 0, s, p);
-    if (p.d <= 2048)
-        return launch_behind(layer_norm_gradients_kernel<DT, WDT, 128, 16>, "layer_norm_gradients", parts, 128, 0, s, p);
-    if (p.d <= 4096)
-        return launch_behind(layer_norm_gradients_kernel<DT, WDT, 256, 16>, "layer_norm_gradients", parts, 256, 0, s, p);
-    if (p.d <= 8192)
-        return launch_behind(layer_norm_gradients_kernel<DT, WDT, 512, 16>, "layer_norm_gradients", parts, 512, 0, s, p);
-    return launch_behind(layer_norm_gradients_kernel<DT, WDT, 512, 32>, "layer_norm_gradients", parts, 512, 0, s, p);
+    const NormGradShape shape = norm_grad_shape(p.d);
+    if (shape.threads == 32)
+        return shape.elems == 8    ? launch_norm_gradient_rows<DT, WDT, 32, 8>(p, parts, s)
+               : shape.elems == 16 ? launch_norm_gradient_rows<DT, WDT, 32, 16>(p, parts, s)
+                                   : launch_norm_gradient_rows<DT, WDT, 32, 32>(p, parts, s);
+    if (shape.elems == 16)
+        return shape.threads == 128 ? launch_norm_gradient_rows<DT, WDT, 128, 16>(p, parts, s) : launch_norm_gradient_rows<DT, WDT, 256, 16>(p, parts, s);
+    return shape.threads == 256 ? launch_norm_gradient_rows<DT, WDT, 256, 32>(p, parts, s) : launch_norm_gradient_rows<DT, WDT, 512, 32>(p, parts, s);
 }
 
 // calls f<DT, WDT>
@@ -517,8 +669,8 @@ static int check_array(const char *what, const char *name, const void *base, int
 
 static uint64_t norm_workspace(uint32_t m, uint32_t d)
 {
-    // fewer rows have no more parts
-    return (uint64_t)norm_parts(m, d) * 2 * d * sizeof(float);
+    // elements of 16 bits have more parts than those of 32, and fewer rows no more
+    return (uint64_t)norm_parts(m, d, 2) * 2 * d * sizeof(float);
 }
 
 } // namespace clpk
@@ -585,7 +737,7 @@ int clpk_layer_norm_backward(const clpk_layer_norm_backward_args_t *args, void *
     CLPK_TRY(check_array(what, "d_rstd", a.d_rstd, CLPK_DT_F32, &any));
     if (a.d_dx)
         CLPK_TRY(check_rows(what, "d_dx", a.d_dx, a.d, &a.lddx, a.dtype, &aligned));
-    const uint32_t parts = norm_parts(a.m, a.d);
+    const uint32_t parts = norm_parts(a.m, a.d, element_bytes(a.dtype));
     const uint64_t need = norm_workspace(a.m, a.d);
     CLPK_REQUIRE(!columns || (a.d_workspace && a.workspace_bytes >= need && (uintptr_t)a.d_workspace % 16 == 0), "%s: needs a 16-byte aligned workspace of %llu bytes",
                  what, (unsigned long long)need);
@@ -596,10 +748,11 @@ int clpk_layer_norm_backward(const clpk_layer_norm_backward_args_t *args, void *
         return rc;
     const NormJoinParams join = {p.parts, {a.d_dweight, a.d_dbias}, parts, a.d};
     const dim3 grid((a.d - 1) / 32 + 1, 2);
+    constexpr int kThreads = 32 * kNormJoinWarps;
     switch (a.weight_dtype) {
-    case CLPK_DT_F32: return launch_behind(layer_norm_join_kernel<CLPK_DT_F32>, "layer_norm_join", grid, 256, 0, s, join);
-    case CLPK_DT_F16: return launch_behind(layer_norm_join_kernel<CLPK_DT_F16>, "layer_norm_join", grid, 256, 0, s, join);
-    default:          return launch_behind(layer_norm_join_kernel<CLPK_DT_BF16>, "layer_norm_join", grid, 256, 0, s, join);
+    case CLPK_DT_F32: return launch_behind(layer_norm_join_kernel<CLPK_DT_F32>, "layer_norm_join", grid, kThreads, 0, s, join);
+    case CLPK_DT_F16: return launch_behind(layer_norm_join_kernel<CLPK_DT_F16>, "layer_norm_join", grid, kThreads, 0, s, join);
+    default:          return launch_behind(layer_norm_join_kernel<CLPK_DT_BF16>, "layer_norm_join", grid, kThreads, 0, s, join);
     }
 }
 
