@@ -115,6 +115,25 @@ template <int DT, int N> struct Raw {
             }
         }
     }
+    // two by two
+    __device__ __forceinline__ void widen(float2 (&f)[N / 2]) const
+    {
+#pragma unroll
+        for (int j = 0; j < N / 2; j++) {
+            if constexpr (DT == CLPK_DT_F32)
+                f[j] = make_float2(__uint_as_float(word(2 * j)), __uint_as_float(word(2 * j + 1)));
+            else
+                f[j] = Element<DT>::widen2(word(j));
+        }
+    }
+    __device__ __forceinline__ void round(const float2 (&f)[N / 2])
+    {
+        float one[N];
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            one[j] = j % 2 ? f[j / 2].y : f[j / 2].x;
+        round(one);
+    }
     __device__ __forceinline__ void round(const float (&f)[N])
     {
         if constexpr (DT == CLPK_DT_F32) {

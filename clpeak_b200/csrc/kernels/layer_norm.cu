@@ -39,7 +39,7 @@ struct NormParams {
     float *mean, *rstd;
     uint64_t ldx, ldy;
     uint32_t m, d;
-    float eps;
+    float eps, one_of_d;                            // 1 / d
 };
 
 // The sum over all threads of a row, the same in each.  `shared`: a word for each warp; not to be written again before all threads
@@ -65,14 +65,15 @@ __device__ __forceinline__ float row_sum(float v, float *shared)
 // Eight elements of a row, or as many as a vector has: what a thread loads at a time
 template <int DT> constexpr int kPiece = Element<DT>::kPerVector;
 
-// weights of a piece in fp32; `none` where there are none
-template <int WDT, int N>
-__device__ __forceinline__ void load_weights(float (&w)[N], const void *base, uint32_t at, uint32_t d, float none)
+// weights of a piece in fp32, two by two; `none` where there are none
+template <int WDT, int PAIRS>
+__device__ __forceinline__ void load_weights(float2 (&w)[PAIRS], const void *base, uint32_t at, uint32_t d, float none)
 {
+    constexpr int N = 2 * PAIRS;
     if (!base) {
 #pragma unroll
-        for (int j = 0; j < N; j++)
-            w[j] = none;
+        for (int j = 0; j < PAIRS; j++)
+            w[j] = make_float2(none, none);
         return;
     }
     const typename Element<WDT>::T *p = static_cast<const typename Element<WDT>::T *>(base) + at;
@@ -148,65 +149,69 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
 #pragma unroll
     for (uint32_t i = 0; i < kNormAhead; i++)
         ask(first + (uint64_t)i * step, i);
-    float w[ELEMS], b[ELEMS];
+    float2 w[ELEMS / 2], b[ELEMS / 2];
 #pragma unroll
     for (int i = 0; i < kPieces; i++) {
         const uint32_t at = (i * THREADS + t) * N;
-        load_weights<WDT, N>(reinterpret_cast<float(&)[N]>(w[i * N]), p.weight, at, p.d, 1.0f);
-        load_weights<WDT, N>(reinterpret_cast<float(&)[N]>(b[i * N]), p.bias, at, p.d, 0.0f);
+        load_weights<WDT>(reinterpret_cast<float2(&)[N / 2]>(w[i * N / 2]), p.weight, at, p.d, 1.0f);
+        load_weights<WDT>(reinterpret_cast<float2(&)[N / 2]>(b[i * N / 2]), p.bias, at, p.d, 0.0f);
     }
     uint32_t stage = 0;
     for (uint64_t row = first; row < p.m; row += step) {
         ask(row + (uint64_t)kNormAhead * step, stage == 0 ? kNormAhead : stage - 1);
         wait_asked<kNormAhead>();
         Raw<DT, N> raw[kPieces];
-        float sum = 0.0f;
+        float2 sum = make_float2(0.0f, 0.0f), squares = sum;
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
             const uint32_t at = (i * THREADS + t) * N;
             raw[i].v[0] = at < p.d ? mine[stage * kStage + i * kAll] : make_uint4(0, 0, 0, 0);
-            float v[N];
+            float2 v[N / 2];
             raw[i].widen(v);
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                sum += v[j];
+            for (int j = 0; j < N / 2; j++)
+                sum = add2(sum, v[j]);
         }
-        const float mean = row_sum<THREADS>(sum, shared[0]) / (float)p.d;
-        float squares = 0.0f;
+        const float mean = row_sum<THREADS>(sum.x + sum.y, shared[0]) * p.one_of_d;
+        const float2 minus = make_float2(-mean, -mean);
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
             const uint32_t at = (i * THREADS + t) * N;
-            float v[N];
+            float2 v[N / 2];
             raw[i].widen(v);
             if (at + N <= p.d) {
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    squares = fmaf(v[j] - mean, v[j] - mean, squares);
+                for (int j = 0; j < N / 2; j++) {
+                    const float2 off = add2(v[j], minus);
+                    squares = fma2(off, off, squares);
+                }
             } else {
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (at + j < p.d)
-                        squares = fmaf(v[j] - mean, v[j] - mean, squares);
+                for (int j = 0; j < N; j++) {
+                    const float off = (j % 2 ? v[j / 2].y : v[j / 2].x) - mean;
+                    squares.x = at + j < p.d ? fmaf(off, off, squares.x) : squares.x;
+                }
             }
         }
-        const float rstd = 1.0f / sqrtf(row_sum<THREADS>(squares, shared[1]) / (float)p.d + p.eps);
+        const float rstd = 1.0f / sqrtf(row_sum<THREADS>(squares.x + squares.y, shared[1]) * p.one_of_d + p.eps);
         if (t == 0) {
             if (p.mean)
                 p.mean[row] = mean;
             if (p.rstd)
                 p.rstd[row] = rstd;
         }
+        const float2 scale = make_float2(rstd, rstd);
         T *y = static_cast<T *>(p.y) + row * p.ldy;
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
             const uint32_t at = (i * THREADS + t) * N;
             if (at >= p.d)
                 break;
-            float v[N];
+            float2 v[N / 2];
             raw[i].widen(v);
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                v[j] = fmaf((v[j] - mean) * rstd, w[i * N + j], b[i * N + j]);
+            for (int j = 0; j < N / 2; j++)
+                v[j] = fma2(mul2(add2(v[j], minus), scale), w[i * N / 2 + j], b[i * N / 2 + j]);
             raw[i].round(v);
             if (at + N <= p.d)
                 raw[i].store(y + at);
@@ -264,11 +269,12 @@ struct NormGradParams {
     float *parts;                                   // [gridDim][2][d]: shares of dw and db; NULL: not asked for
     uint64_t ldx, lddy, lddx;
     uint32_t m, d;
+    float one_of_d;                                 // 1 / d
 };
 
-// both sums over all threads of a row; `shared` as in row_sum
+// both sums over all threads of a row, which are a CTA or group `group` of it; `shared` as in row_sum
 template <int THREADS>
-__device__ __forceinline__ float2 row_sums(float2 v, float2 *shared)
+__device__ __forceinline__ float2 row_sums(float2 v, float2 *shared, uint32_t group)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -276,10 +282,11 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 *shared)
         v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
     if constexpr (THREADS > 32) {
-        if ((threadIdx.x & 31) == 0)
-            shared[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = (threadIdx.x & 31) < THREADS / 32 ? shared[threadIdx.x & 31] : make_float2(0.0f, 0.0f);
+        const uint32_t warp = threadIdx.x % THREADS >> 5, lane = threadIdx.x & 31;
+        if (lane == 0)
+            shared[warp] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(THREADS) : "memory");
+        v = lane < THREADS / 32 ? shared[lane] : make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int o = THREADS / 64; o > 0; o >>= 1) {
             v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
@@ -291,35 +298,34 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 *shared)
     return v;
 }
 
-constexpr int kNormGradWarps = 8;                   // of a CTA whose rows are a warp's
-
-// CTAs of an SM, and rows on their way behind the one that is computed: as many as registers (two sums for each element) and shared memory
-// (x and dy) hold, two rows at most.
-__host__ __device__ constexpr int norm_grad_threads(int threads) { return threads == 32 ? 32 * kNormGradWarps : threads; }
-__host__ __device__ constexpr uint32_t norm_grad_stage(int threads, int elems, uint32_t elem) { return 2 * norm_grad_threads(threads) * elems * elem; }
-__host__ __device__ constexpr int norm_grad_ctas(int threads, int elems, uint32_t elem)
+// A CTA for each SM: groups of threads that have a row each, as many as registers (two sums for each element) and shared memory (two rows
+// of x and dy at least) hold, and rows on their way behind the one that is computed, two at most.
+__host__ __device__ constexpr uint32_t norm_grad_stage(int threads, int elems, uint32_t elem) { return 2 * threads * elems * elem; }
+__host__ __device__ constexpr int norm_grad_groups(int threads, int elems, uint32_t elem)
 {
-    const int regs = elems == 8 ? 64 : elems == 16 ? 85 : 128, ctas = 65536 / (regs * norm_grad_threads(threads));
-    return ctas * 2 * norm_grad_stage(threads, elems, elem) <= 220 * 1024 ? ctas : 1;
+    int groups = (elems == 8 ? 1024 : elems == 16 ? 768 : 512) / threads;
+    while (groups > 1 && groups * 2 * norm_grad_stage(threads, elems, elem) > 220 * 1024)
+        groups /= 2;
+    return groups;
 }
 __host__ __device__ constexpr int norm_grad_ahead(int threads, int elems, uint32_t elem)
 {
-    const int stages = 220 * 1024 / (norm_grad_ctas(threads, elems, elem) * norm_grad_stage(threads, elems, elem));
+    const int stages = 220 * 1024 / (norm_grad_groups(threads, elems, elem) * norm_grad_stage(threads, elems, elem));
     return stages >= 3 ? 2 : stages - 1;
 }
 
 template <int DT, int WDT, int THREADS, int ELEMS>
-__global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THREADS, ELEMS, sizeof(typename Element<DT>::T))) layer_norm_gradients_kernel(NormGradParams p)
+__global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, sizeof(typename Element<DT>::T)), 1) layer_norm_gradients_kernel(NormGradParams p)
 {
     using T = typename Element<DT>::T;
-    constexpr int N = kPiece<DT>, kPieces = ELEMS / N, kRows = THREADS == 32 ? kNormGradWarps : 1, kAhead = norm_grad_ahead(THREADS, ELEMS, sizeof(T));
-    constexpr uint32_t kAll = norm_grad_threads(THREADS), kStage = 2 * kPieces * kAll;
+    constexpr int N = kPiece<DT>, kPieces = ELEMS / N, kGroups = norm_grad_groups(THREADS, ELEMS, sizeof(T)), kAhead = norm_grad_ahead(THREADS, ELEMS, sizeof(T));
     extern __shared__ __align__(16) uint4 ring[];
-    __shared__ float2 shared[2][THREADS / 32];
+    __shared__ float2 shared[2][kGroups][THREADS / 32];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t warp = threadIdx.x >> 5, t = threadIdx.x % THREADS, step = gridDim.x * kRows;
-    const uint64_t first = blockIdx.x * kRows + (kRows > 1 ? warp : 0);
+    const uint32_t group = threadIdx.x / THREADS, t = threadIdx.x % THREADS, groups = blockDim.x / THREADS, step = gridDim.x * groups;
+    const uint32_t kAll = blockDim.x, kStage = 2 * kPieces * kAll;
+    const uint64_t first = blockIdx.x * groups + group;
     uint4 *const mine = ring + threadIdx.x;
     const auto ask = [&](uint64_t row, uint32_t stage) {
         if (row < p.m) {
@@ -328,18 +334,20 @@ __global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THR
         }
         asked();
     };
+    // Behind the row x and dy are zeros, here and as the copies fill them up: what they bring to a sum is zero, but for a row that is NaN
+    // in any case.
+#pragma unroll
+    for (int i = 0; i < kPieces; i++)
+        if ((i * THREADS + t) * N >= p.d)
+            for (uint32_t stage = 0; stage <= kAhead; stage++)
+                mine[stage * kStage + i * kAll] = mine[stage * kStage + (kPieces + i) * kAll] = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; i++)
         ask(first + (uint64_t)i * step, i);
     float2 dw[ELEMS / 2] = {}, db[ELEMS / 2] = {}, w[ELEMS / 2];
 #pragma unroll
-    for (int i = 0; i < kPieces; i++) {
-        float one[N];
-        load_weights<WDT, N>(one, p.weight, (i * THREADS + t) * N, p.d, 1.0f);
-#pragma unroll
-        for (int j = 0; j < N / 2; j++)
-            w[i * N / 2 + j] = make_float2(one[2 * j], one[2 * j + 1]);
-    }
+    for (int i = 0; i < kPieces; i++)
+        load_weights<WDT>(reinterpret_cast<float2(&)[N / 2]>(w[i * N / 2]), p.weight, (i * THREADS + t) * N, p.d, 1.0f);
     uint32_t stage = 0, turn = 0;
     float mean = first < p.m ? p.mean[first] : 0.0f, rstd = first < p.m ? p.rstd[first] : 0.0f;
     for (uint64_t row = first; row < p.m; row += step) {
@@ -347,33 +355,16 @@ __global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THR
         const bool more = row + step < p.m;
         const float next_mean = more ? p.mean[row + step] : 0.0f, next_rstd = more ? p.rstd[row + step] : 0.0f;
         wait_asked<kAhead>();
-        // x - mean and dy of a piece, two numbers at a time; zeros behind the row, where a mean that is not finite must not come in
+        // x - mean and dy of a piece, two numbers at a time
         const auto values = [&](int i, float2 (&off)[N / 2], float2 (&dy)[N / 2]) {
-            const uint32_t at = (i * THREADS + t) * N;
             Raw<DT, N> x, d;
-            float vx[N], vd[N];
             x.v[0] = mine[stage * kStage + i * kAll];
             d.v[0] = mine[stage * kStage + (kPieces + i) * kAll];
-            x.widen(vx);
-            d.widen(vd);
-            if (at + N > p.d) {
+            x.widen(off);
+            d.widen(dy);
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    vx[j] = at + j < p.d ? vx[j] : mean;
-                    vd[j] = at + j < p.d ? vd[j] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < N / 2; j++) {
-                off[j] = add2(make_float2(vx[2 * j], vx[2 * j + 1]), make_float2(-mean, -mean));
-                dy[j] = make_float2(vd[2 * j], vd[2 * j + 1]);
-            }
-            if (at + N > p.d) {
-#pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (at + j >= p.d)
-                        (j % 2 ? off[j / 2].y : off[j / 2].x) = 0.0f;
-            }
+            for (int j = 0; j < N / 2; j++)
+                off[j] = add2(off[j], make_float2(-mean, -mean));
         };
         const float2 scale = make_float2(rstd, rstd);
         float2 sum_g = make_float2(0.0f, 0.0f), sum_go = sum_g;     // of g and of g * (x - mean)
@@ -392,10 +383,10 @@ __global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THR
             }
         }
         if (p.dx) {
-            const float2 sum = row_sums<THREADS>(make_float2(sum_g.x + sum_g.y, sum_go.x + sum_go.y), shared[turn]);
+            const float2 sum = row_sums<THREADS>(make_float2(sum_g.x + sum_g.y, sum_go.x + sum_go.y), shared[turn][group], group);
             turn ^= 1;
             // dx = rstd g + (x - mean) by + also, by = -rstd^3 sum g (x - mean) / d, also = -rstd sum g / d
-            const float by = -rstd * (rstd * (rstd * (sum.y / (float)p.d))), also = -rstd * (sum.x / (float)p.d);
+            const float by = -rstd * (rstd * (rstd * (sum.y * p.one_of_d))), also = -rstd * (sum.x * p.one_of_d);
             asm volatile("" ::: "memory");          // read again rather than kept in registers
             T *dx = static_cast<T *>(p.dx) + row * p.lddx;
 #pragma unroll
@@ -404,16 +395,12 @@ __global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THR
                 if (at >= p.d)
                     break;
                 float2 off[N / 2], dy[N / 2];
-                float v[N];
                 values(i, off, dy);
 #pragma unroll
-                for (int j = 0; j < N / 2; j++) {
-                    const float2 one = fma2(mul2(dy[j], w[i * N / 2 + j]), scale, fma2(off[j], make_float2(by, by), make_float2(also, also)));
-                    v[2 * j] = one.x;
-                    v[2 * j + 1] = one.y;
-                }
+                for (int j = 0; j < N / 2; j++)
+                    off[j] = fma2(mul2(dy[j], w[i * N / 2 + j]), scale, fma2(off[j], make_float2(by, by), make_float2(also, also)));
                 Raw<DT, N> out;
-                out.round(v);
+                out.round(off);
                 if (at + N <= p.d)
                     out.store(dx + at);
                 else
@@ -427,38 +414,25 @@ __global__ void __launch_bounds__(norm_grad_threads(THREADS), norm_grad_ctas(THR
     wait_asked<0>();
     if (!p.parts)
         return;
+    // the groups' shares side by side where the rows were, a row for each element of a thread, then added in their order
+    float *const shares = reinterpret_cast<float *>(ring);
+    static_assert(sizeof(float) <= (kAhead + 1) * sizeof(T), "room for all shares");
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < ELEMS; e++) {
+        shares[((group * 2 + 0) * ELEMS + e) * THREADS + t] = e % 2 ? dw[e / 2].y : dw[e / 2].x;
+        shares[((group * 2 + 1) * ELEMS + e) * THREADS + t] = e % 2 ? db[e / 2].y : db[e / 2].x;
+    }
+    __syncthreads();
     float *part = p.parts + (uint64_t)blockIdx.x * 2 * p.d;
-    if constexpr (THREADS > 32) {
-#pragma unroll
-        for (int i = 0; i < kPieces; i++)
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const uint32_t at = (i * THREADS + t) * N + j, e = i * N + j;
-                if (at < p.d) {
-                    part[at] = e % 2 ? dw[e / 2].y : dw[e / 2].x;
-                    part[p.d + at] = e % 2 ? db[e / 2].y : db[e / 2].x;
-                }
-            }
-    } else {
-        // the warps' shares side by side where the rows were, then added in their order
-        float *const shares = reinterpret_cast<float *>(ring);
-        static_assert(kNormGradWarps * 2 * 32 * ELEMS * sizeof(float) <= (kAhead + 1) * norm_grad_stage(32, ELEMS, sizeof(T)), "room for all shares");
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < ELEMS; e++) {
-            shares[((warp * 2 + 0) * ELEMS + e) * 32 + t] = e % 2 ? dw[e / 2].y : dw[e / 2].x;
-            shares[((warp * 2 + 1) * ELEMS + e) * 32 + t] = e % 2 ? db[e / 2].y : db[e / 2].x;
-        }
-        __syncthreads();
-        for (uint32_t i = warp; i < 2 * ELEMS; i += kNormGradWarps) {
-            float sum = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < kNormGradWarps; w++)
-                sum += shares[(w * 2 * ELEMS + i) * 32 + t];
-            const uint32_t e = i % ELEMS, at = (e / N * 32 + t) * N + e % N;
-            if (at < p.d)
-                part[i / ELEMS * p.d + at] = sum;
-        }
+    for (uint32_t i = group; i < 2 * ELEMS; i += groups) {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (uint32_t g = 0; g < groups; g++)
+            sum += shares[(g * 2 * ELEMS + i) * THREADS + t];
+        const uint32_t e = i % ELEMS, at = (e / N * THREADS + t) * N + e % N;
+        if (at < p.d)
+            part[i / ELEMS * p.d + at] = sum;
     }
 }
 
@@ -487,7 +461,7 @@ __global__ void __launch_bounds__(256) layer_norm_plain_dx_kernel(NormGradParams
         sum.x += g;
         sum.y = fmaf(g, hat, sum.y);
     }
-    sum = row_sums<256>(sum, shared);
+    sum = row_sums<256>(sum, shared, 0);
     const float c1 = sum.x / (float)p.d, c2 = sum.y / (float)p.d;
 #pragma unroll 4
     for (uint64_t at = threadIdx.x; at < p.d; at += 256) {
@@ -585,6 +559,8 @@ static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
     return launch_norm_rows<DT, WDT, 512, 32>(p, s);
 }
 
+constexpr uint32_t kNormParts = 148;                // at most
+
 // Threads and elements of each that share a row in layer_norm_gradients_kernel
 struct NormGradShape {
     int threads, elems;
@@ -595,22 +571,27 @@ constexpr NormGradShape norm_grad_shape(uint32_t d)
          : d <= 4096 ? NormGradShape{256, 16} : d <= 8192 ? NormGradShape{256, 32} : NormGradShape{512, 32};
 }
 
-// Parts of dw and db: the CTAs that share the rows.  A whole B200's: the workspace's size may not depend on the card at hand.
+// Groups of a CTA, and the CTAs that share the rows, each with a part of dw and db.  Few rows are spread over the SMs.  A whole B200's SMs:
+// the workspace's size may not depend on the card at hand.
+static uint32_t norm_groups(uint32_t m, uint32_t d, uint64_t elem)
+{
+    const NormGradShape shape = norm_grad_shape(d);
+    return std::min((uint32_t)norm_grad_groups(shape.threads, shape.elems, (uint32_t)elem), m ? (m - 1) / kNormParts + 1 : 1);
+}
 static uint32_t norm_parts(uint32_t m, uint32_t d, uint64_t elem)
 {
-    constexpr uint32_t kSms = 148;
-    const NormGradShape shape = norm_grad_shape(d);
-    const uint32_t rows = shape.threads == 32 ? kNormGradWarps : 1;
-    return std::min(m ? (m - 1) / rows + 1 : 1, (uint32_t)norm_grad_ctas(shape.threads, shape.elems, (uint32_t)elem) * kSms);
+    return std::min(m ? (m - 1) / norm_groups(m, d, elem) + 1 : 1, kNormParts);
 }
 
 template <int DT, int WDT, int THREADS, int ELEMS>
 static int launch_norm_gradient_rows(const NormGradParams &p, uint32_t parts, cudaStream_t s)
 {
-    constexpr uint32_t kElem = sizeof(typename Element<DT>::T), kBytes = (norm_grad_ahead(THREADS, ELEMS, kElem) + 1) * norm_grad_stage(THREADS, ELEMS, kElem);
-    if (kBytes > 47 * 1024)
-        CLPK_CUDA(cudaFuncSetAttribute(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes));
-    return launch_behind(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm_gradients", parts, norm_grad_threads(THREADS), kBytes, s, p);
+    constexpr uint32_t kElem = sizeof(typename Element<DT>::T), kEach = (norm_grad_ahead(THREADS, ELEMS, kElem) + 1) * norm_grad_stage(THREADS, ELEMS, kElem);
+    constexpr uint32_t kMost = norm_grad_groups(THREADS, ELEMS, kElem) * kEach;
+    if (kMost > 40 * 1024)
+        CLPK_CUDA(cudaFuncSetAttribute(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost));
+    const uint32_t groups = norm_groups(p.m, p.d, kElem);
+    return launch_behind(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm_gradients", parts, groups * THREADS, groups * kEach, s, p);
 }
 
 template <int DT, int WDT>
@@ -669,8 +650,7 @@ static int check_array(const char *what, const char *name, const void *base, int
 
 static uint64_t norm_workspace(uint32_t m, uint32_t d)
 {
-    // elements of 16 bits have more parts than those of 32, and fewer rows no more
-    return (uint64_t)norm_parts(m, d, 2) * 2 * d * sizeof(float);
+    return (uint64_t)std::min(std::max(m, 1u), kNormParts) * 2 * d * sizeof(float);
 }
 
 } // namespace clpk
@@ -696,7 +676,7 @@ int clpk_layer_norm(const clpk_layer_norm_args_t *args, void *stream)
     CLPK_TRY(check_array(what, "d_bias", a.d_bias, a.weight_dtype, &aligned));
     CLPK_TRY(check_array(what, "d_mean", a.d_mean, CLPK_DT_F32, &any));
     CLPK_TRY(check_array(what, "d_rstd", a.d_rstd, CLPK_DT_F32, &any));
-    const NormParams p = {a.d_x, a.d_weight, a.d_bias, a.d_y, a.d_mean, a.d_rstd, a.ldx, a.ldy, a.m, a.d, a.eps};
+    const NormParams p = {a.d_x, a.d_weight, a.d_bias, a.d_y, a.d_mean, a.d_rstd, a.ldx, a.ldy, a.m, a.d, a.eps, (float)(1.0 / a.d)};
     return CLPK_BY_TYPES(a.dtype, a.weight_dtype, launch_norm, p, aligned, as_stream(stream));
 }
 
@@ -742,7 +722,7 @@ int clpk_layer_norm_backward(const clpk_layer_norm_backward_args_t *args, void *
     CLPK_REQUIRE(!columns || (a.d_workspace && a.workspace_bytes >= need && (uintptr_t)a.d_workspace % 16 == 0), "%s: needs a 16-byte aligned workspace of %llu bytes",
                  what, (unsigned long long)need);
     const NormGradParams p = {a.d_x, a.d_weight, a.d_dy, a.d_mean, a.d_rstd, a.d_dx, columns ? static_cast<float *>(a.d_workspace) : nullptr,
-                              a.ldx, a.lddy, a.lddx, a.m, a.d};
+                              a.ldx, a.lddy, a.lddx, a.m, a.d, (float)(1.0 / a.d)};
     const int rc = CLPK_BY_TYPES(a.dtype, a.weight_dtype, launch_norm_gradients, p, aligned, parts, s);
     if (rc != CLPK_OK || !columns)
         return rc;

@@ -44,7 +44,7 @@ def test_workspace_of_the_norms_gradients(K):
     for _ in range(300):
         m, d = round((1 << 20) ** rng.random()), round((1 << 16) ** rng.random())
         need = norm_need(K, m, d)
-        assert need % (8 * d) == 0 and 1 <= need // (8 * d) <= min(m, 888)
+        assert need % (8 * d) == 0 and 1 <= need // (8 * d) <= min(m, 148)
         assert norm_need(K, max(1, m - rng.randint(0, m)), d) <= need
     assert norm_need(K, 0, 8) > 0
     for m, d in ((2 ** 31, 8), (8, 2 ** 30 + 1), (8, 0)):
