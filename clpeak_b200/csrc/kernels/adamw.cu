@@ -58,8 +58,8 @@ template <int CAP> struct StepTable {
     uint32_t first[CAP];                                // chunk of the launch; `aligned` in the top bit
 };
 constexpr uint32_t kStepAligned = 0x80000000u;
-constexpr int kStepFew = 48, kStepMany = 440;
-static_assert(sizeof(StepTable<kStepFew>) <= 4096 && sizeof(StepTable<kStepMany>) <= 32764, "parameters of a kernel");
+constexpr int kStepFew = 48, kStepSome = 144, kStepMany = 440;
+static_assert(sizeof(StepTable<kStepMany>) <= 32764, "parameters of a kernel");
 
 __host__ __device__ __forceinline__ void set_rates(StepRates &r, double lr, double beta1, double beta2, double decay, double step)
 {
@@ -423,14 +423,14 @@ static int launch_step(StepTable<CAP> &table, const clpk_adamw_tensor_t *tensors
 template <int DT, int GDT, int SDT, bool MASTER>
 static int run_step(const StepCommon &c, const clpk_adamw_tensor_t *tensors, uint32_t count, cudaStream_t s)
 {
-    if (count <= kStepFew) {                            // less to send along with the launch
-        StepTable<kStepFew> table;
+    const auto with = [&](auto &table) {
         table.c = c;
         return launch_step<DT, GDT, SDT, MASTER>(table, tensors, count, s);
-    }
-    StepTable<kStepMany> table;
-    table.c = c;
-    return launch_step<DT, GDT, SDT, MASTER>(table, tensors, count, s);
+    };
+    StepTable<kStepFew> few;                            // the less to send along with the launch: 64 tensors 5.7 us with room for 440
+    StepTable<kStepSome> some;
+    StepTable<kStepMany> many;
+    return count <= kStepFew ? with(few) : count <= kStepSome ? with(some) : with(many);
 }
 
 template <int DT, int GDT>

@@ -104,18 +104,32 @@ __device__ __forceinline__ void wait_asked()                    // all but the l
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// the pieces of a row that fall to thread t of THREADS
-template <int DT, int THREADS, int PIECES>
-__device__ __forceinline__ void ask_row(uint4 *to, uint32_t stride, const typename Element<DT>::T *row, uint32_t t, uint32_t d)
-{
-    constexpr uint32_t N = kPiece<DT>, kBytes = 16 / N;
+// The pieces of rows that fall to a thread, one row after another: `at`, the thread's first piece of the next row, and how many bytes of each
+// piece there are.
+template <int DT, int THREADS, int PIECES> struct RowsAhead {
+    static constexpr uint32_t N = kPiece<DT>;
+    const typename Element<DT>::T *at;
+    uint64_t step;                                              // elements to the next row
+    uint32_t bytes[PIECES];
+
+    __device__ __forceinline__ RowsAhead(const void *base, uint64_t ld, uint64_t first, uint64_t rows, uint32_t t, uint32_t d)
+        : at(static_cast<const typename Element<DT>::T *>(base) + first * ld + t * N), step(rows * ld)
+    {
 #pragma unroll
-    for (int i = 0; i < PIECES; i++) {
-        const uint32_t at = (i * THREADS + t) * N, left = at < d ? d - at : 0;
-        if (left)
-            ask_piece(to + i * stride, row + at, left < N ? left * kBytes : 16);
+        for (int i = 0; i < PIECES; i++) {
+            const uint32_t from = (i * THREADS + t) * N;
+            bytes[i] = from >= d ? 0 : min(d - from, N) * (16 / N);
+        }
     }
-}
+    template <uint32_t STRIDE> __device__ __forceinline__ void ask(uint4 *to)
+    {
+#pragma unroll
+        for (int i = 0; i < PIECES; i++)
+            if (bytes[i])
+                ask_piece(to + i * STRIDE, at + i * THREADS * N, bytes[i]);
+        at += step;
+    }
+};
 
 constexpr int kNormWarps = 4;                       // rows that a CTA takes at once where a row is a warp's
 constexpr int kNormAhead = 2;                       // rows on their way behind the one that is computed
@@ -141,9 +155,10 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
     const uint32_t t = threadIdx.x % THREADS, step = gridDim.x * kRows;
     const uint64_t first = blockIdx.x * kRows + (THREADS == 32 ? threadIdx.x >> 5 : 0);
     uint4 *const mine = ring + threadIdx.x;
+    RowsAhead<DT, THREADS, kPieces> ahead(p.x, p.ldx, first, step, t, p.d);
     const auto ask = [&](uint64_t row, uint32_t stage) {
         if (row < p.m)
-            ask_row<DT, THREADS, kPieces>(mine + stage * kStage, kAll, static_cast<const T *>(p.x) + row * p.ldx, t, p.d);
+            ahead.template ask<kAll>(mine + stage * kStage);
         asked();
     };
 #pragma unroll
@@ -156,6 +171,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
         load_weights<WDT>(reinterpret_cast<float2(&)[N / 2]>(w[i * N / 2]), p.weight, at, p.d, 1.0f);
         load_weights<WDT>(reinterpret_cast<float2(&)[N / 2]>(b[i * N / 2]), p.bias, at, p.d, 0.0f);
     }
+    T *y = static_cast<T *>(p.y) + first * p.ldy + t * N;
     uint32_t stage = 0;
     for (uint64_t row = first; row < p.m; row += step) {
         ask(row + (uint64_t)kNormAhead * step, stage == 0 ? kNormAhead : stage - 1);
@@ -201,7 +217,6 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
                 p.rstd[row] = rstd;
         }
         const float2 scale = make_float2(rstd, rstd);
-        T *y = static_cast<T *>(p.y) + row * p.ldy;
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
             const uint32_t at = (i * THREADS + t) * N;
@@ -214,10 +229,11 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
                 v[j] = fma2(mul2(add2(v[j], minus), scale), w[i * N / 2 + j], b[i * N / 2 + j]);
             raw[i].round(v);
             if (at + N <= p.d)
-                raw[i].store(y + at);
+                raw[i].store(y + i * THREADS * N);
             else
-                raw[i].store_some(y + at, p.d - at);
+                raw[i].store_some(y + i * THREADS * N, p.d - at);
         }
+        y += step * p.ldy;
         stage = stage == kNormAhead ? 0 : stage + 1;
     }
     wait_asked<0>();
@@ -272,46 +288,66 @@ struct NormGradParams {
     float one_of_d;                                 // 1 / d
 };
 
-// both sums over all threads of a row, which are a CTA or group `group` of it; `shared` as in row_sum
-template <int THREADS>
-__device__ __forceinline__ float2 row_sums(float2 v, float2 *shared, uint32_t group)
+// Sums of V values each over all threads of a row, which are a CTA or group `group` of it.  Lanes halve what they add: each sends the values
+// that the other half of a warp goes on with, so that V values take little more than one.  `shared`: V words for each warp, not to be
+// written again before all threads have come to the next barrier.
+template <int THREADS, int V>
+__device__ __forceinline__ void row_sums(float (&v)[V], float *shared, uint32_t group)
 {
+    const uint32_t lane = threadIdx.x & 31;
+    int o = 16;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-    }
-    if constexpr (THREADS > 32) {
-        const uint32_t warp = threadIdx.x % THREADS >> 5, lane = threadIdx.x & 31;
-        if (lane == 0)
-            shared[warp] = v;
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(THREADS) : "memory");
-        v = lane < THREADS / 32 ? shared[lane] : make_float2(0.0f, 0.0f);
+    for (int left = V / 2; left > 0; left /= 2, o /= 2) {
+        const bool upper = lane & o;
 #pragma unroll
-        for (int o = THREADS / 64; o > 0; o >>= 1) {
-            v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-            v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        for (int i = 0; i < left; i++) {
+            const float keep = upper ? v[left + i] : v[i], give = upper ? v[i] : v[left + i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
         }
-        v.x = __shfl_sync(0xffffffffu, v.x, 0);
-        v.y = __shfl_sync(0xffffffffu, v.y, 0);
     }
-    return v;
+    constexpr uint32_t kEach = 32 / V;                          // lanes that have the same value now, value i from lane i * kEach on
+#pragma unroll
+    for (uint32_t x = kEach / 2; x > 0; x /= 2)
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], x);
+    if constexpr (THREADS == 32) {
+#pragma unroll
+        for (int i = V - 1; i >= 0; i--)
+            v[i] = __shfl_sync(0xffffffffu, v[0], i * kEach);
+    } else {
+        constexpr uint32_t kWarps = THREADS / 32;
+        if (lane % kEach == 0)
+            shared[threadIdx.x % THREADS / 32 * V + lane / kEach] = v[0];
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(THREADS) : "memory");
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; w += 32 / V)
+            if (w + lane / V < kWarps)
+                sum += shared[(w + lane / V) * V + lane % V];
+#pragma unroll
+        for (uint32_t x = V; x < 32 && x < kWarps * V; x *= 2)
+            sum += __shfl_xor_sync(0xffffffffu, sum, x);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            v[i] = __shfl_sync(0xffffffffu, sum, i);
+    }
 }
 
-// A CTA for each SM: groups of threads that have a row each, as many as registers (two sums for each element) and shared memory (two rows
-// of x and dy at least) hold, and rows on their way behind the one that is computed, two at most.
-__host__ __device__ constexpr uint32_t norm_grad_stage(int threads, int elems, uint32_t elem) { return 2 * threads * elems * elem; }
+// A CTA for each SM: groups of threads that share a row each, as many as registers (two sums for each element) and shared memory (two rows
+// of x and dy at least, and the weights) hold, and rows on their way behind the one that is computed, two at most.
+constexpr uint32_t kNormGradBytes = 216 * 1024;
+__host__ __device__ constexpr uint32_t norm_grad_row(int threads, int elems, uint32_t elem) { return 2 * threads * elems * elem; }
+__host__ __device__ constexpr uint32_t norm_grad_room(int threads, int elems) { return kNormGradBytes - threads * elems * 4; }
 __host__ __device__ constexpr int norm_grad_groups(int threads, int elems, uint32_t elem)
 {
-    int groups = (elems == 8 ? 1024 : elems == 16 ? 768 : 512) / threads;
-    while (groups > 1 && groups * 2 * norm_grad_stage(threads, elems, elem) > 220 * 1024)
+    int groups = (elems == 8 ? 1024 : elems == 32 ? 512 : threads == 32 ? 640 : 768) / threads;        // 64, 128, 102 and 85 registers
+    while (groups > 1 && groups * 2 * norm_grad_row(threads, elems, elem) > norm_grad_room(threads, elems))
         groups /= 2;
     return groups;
 }
 __host__ __device__ constexpr int norm_grad_ahead(int threads, int elems, uint32_t elem)
 {
-    const int stages = 220 * 1024 / (norm_grad_groups(threads, elems, elem) * norm_grad_stage(threads, elems, elem));
-    return stages >= 3 ? 2 : stages - 1;
+    const int rows = norm_grad_room(threads, elems) / (norm_grad_groups(threads, elems, elem) * norm_grad_row(threads, elems, elem));
+    return rows >= 3 ? 2 : rows - 1;
 }
 
 template <int DT, int WDT, int THREADS, int ELEMS>
@@ -319,47 +355,66 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
 {
     using T = typename Element<DT>::T;
     constexpr int N = kPiece<DT>, kPieces = ELEMS / N, kGroups = norm_grad_groups(THREADS, ELEMS, sizeof(T)), kAhead = norm_grad_ahead(THREADS, ELEMS, sizeof(T));
+    constexpr uint32_t kAll = THREADS * kGroups, kRow = 2 * kPieces * kAll;     // also where fewer groups run
     extern __shared__ __align__(16) uint4 ring[];
-    __shared__ float2 shared[2][kGroups][THREADS / 32];
+    __shared__ float shared[2][kGroups][THREADS / 32 * 2];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t group = threadIdx.x / THREADS, t = threadIdx.x % THREADS, groups = blockDim.x / THREADS, step = gridDim.x * groups;
-    const uint32_t kAll = blockDim.x, kStage = 2 * kPieces * kAll;
     const uint64_t first = blockIdx.x * groups + group;
     uint4 *const mine = ring + threadIdx.x;
-    const auto ask = [&](uint64_t row, uint32_t stage) {
+    RowsAhead<DT, THREADS, kPieces> ahead_x(p.x, p.ldx, first, step, t, p.d), ahead_dy(p.dy, p.lddy, first, step, t, p.d);
+    const auto ask = [&](uint64_t row, uint32_t turn) {
         if (row < p.m) {
-            ask_row<DT, THREADS, kPieces>(mine + stage * kStage, kAll, static_cast<const T *>(p.x) + row * p.ldx, t, p.d);
-            ask_row<DT, THREADS, kPieces>(mine + stage * kStage + kPieces * kAll, kAll, static_cast<const T *>(p.dy) + row * p.lddy, t, p.d);
+            ahead_x.template ask<kAll>(mine + turn * kRow);
+            ahead_dy.template ask<kAll>(mine + turn * kRow + kPieces * kAll);
         }
         asked();
     };
-    // Behind the row x and dy are zeros, here and as the copies fill them up: what they bring to a sum is zero, but for a row that is NaN
-    // in any case.
+    // Behind a row x and dy are zeros, here and as the copies fill them up: what they bring to a sum is zero, but for a row that is NaN in
+    // any case.
 #pragma unroll
     for (int i = 0; i < kPieces; i++)
-        if ((i * THREADS + t) * N >= p.d)
-            for (uint32_t stage = 0; stage <= kAhead; stage++)
-                mine[stage * kStage + i * kAll] = mine[stage * kStage + (kPieces + i) * kAll] = make_uint4(0, 0, 0, 0);
+        if (ahead_x.bytes[i] == 0)
+            for (uint32_t turn = 0; turn <= kAhead; turn++)
+                mine[turn * kRow + i * kAll] = mine[turn * kRow + (kPieces + i) * kAll] = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; i++)
         ask(first + (uint64_t)i * step, i);
-    float2 dw[ELEMS / 2] = {}, db[ELEMS / 2] = {}, w[ELEMS / 2];
+    // the weights of a thread's elements, four by four: in shared memory, where they take no registers from the sums (8192 x 4096 bf16 56
+    // and so 50 us)
+    float4 *const weights = reinterpret_cast<float4 *>(ring + (kAhead + 1) * kRow) + t;
+    if (group == 0) {
 #pragma unroll
-    for (int i = 0; i < kPieces; i++)
-        load_weights<WDT>(reinterpret_cast<float2(&)[N / 2]>(w[i * N / 2]), p.weight, (i * THREADS + t) * N, p.d, 1.0f);
-    uint32_t stage = 0, turn = 0;
+        for (int i = 0; i < kPieces; i++) {
+            float2 w[N / 2];
+            load_weights<WDT>(w, p.weight, (i * THREADS + t) * N, p.d, 1.0f);
+#pragma unroll
+            for (int j = 0; j < N / 4; j++)
+                weights[(i * N / 4 + j) * THREADS] = make_float4(w[2 * j].x, w[2 * j].y, w[2 * j + 1].x, w[2 * j + 1].y);
+        }
+    }
+    __syncthreads();
+    float2 dw[ELEMS / 2] = {}, db[ELEMS / 2] = {};
+    T *dx = static_cast<T *>(p.dx) + first * p.lddx + t * N;
+    uint32_t turn = 0, flip = 0;
     float mean = first < p.m ? p.mean[first] : 0.0f, rstd = first < p.m ? p.rstd[first] : 0.0f;
     for (uint64_t row = first; row < p.m; row += step) {
-        ask(row + (uint64_t)kAhead * step, stage == 0 ? kAhead : stage - 1);
+        ask(row + (uint64_t)kAhead * step, turn == 0 ? kAhead : turn - 1);
         const bool more = row + step < p.m;
         const float next_mean = more ? p.mean[row + step] : 0.0f, next_rstd = more ? p.rstd[row + step] : 0.0f;
         wait_asked<kAhead>();
-        // x - mean and dy of a piece, two numbers at a time
-        const auto values = [&](int i, float2 (&off)[N / 2], float2 (&dy)[N / 2]) {
+        // x - mean, dy and the weights of a piece, two numbers at a time
+        const auto values = [&](int i, float2 (&off)[N / 2], float2 (&dy)[N / 2], float2 (&w)[N / 2]) {
             Raw<DT, N> x, d;
-            x.v[0] = mine[stage * kStage + i * kAll];
-            d.v[0] = mine[stage * kStage + (kPieces + i) * kAll];
+            x.v[0] = mine[turn * kRow + i * kAll];
+            d.v[0] = mine[turn * kRow + (kPieces + i) * kAll];
+#pragma unroll
+            for (int j = 0; j < N / 4; j++) {
+                const float4 f = weights[(i * N / 4 + j) * THREADS];
+                w[2 * j] = make_float2(f.x, f.y);
+                w[2 * j + 1] = make_float2(f.z, f.w);
+            }
             x.widen(off);
             d.widen(dy);
 #pragma unroll
@@ -367,15 +422,15 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
                 off[j] = add2(off[j], make_float2(-mean, -mean));
         };
         const float2 scale = make_float2(rstd, rstd);
-        float2 sum_g = make_float2(0.0f, 0.0f), sum_go = sum_g;     // of g and of g * (x - mean)
+        float2 sum_g = make_float2(0.0f, 0.0f), sum_go = sum_g;         // of g and of g * (x - mean)
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
-            float2 off[N / 2], dy[N / 2];
-            values(i, off, dy);
+            float2 off[N / 2], dy[N / 2], w[N / 2];
+            values(i, off, dy, w);
 #pragma unroll
             for (int j = 0; j < N / 2; j++) {
                 const int e = i * N / 2 + j;
-                const float2 g = mul2(dy[j], w[e]);
+                const float2 g = mul2(dy[j], w[j]);
                 dw[e] = fma2(dy[j], mul2(off[j], scale), dw[e]);
                 db[e] = add2(db[e], dy[j]);
                 sum_g = add2(sum_g, g);
@@ -383,33 +438,33 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
             }
         }
         if (p.dx) {
-            const float2 sum = row_sums<THREADS>(make_float2(sum_g.x + sum_g.y, sum_go.x + sum_go.y), shared[turn][group], group);
-            turn ^= 1;
-            // dx = rstd g + (x - mean) by + also, by = -rstd^3 sum g (x - mean) / d, also = -rstd sum g / d
-            const float by = -rstd * (rstd * (rstd * (sum.y * p.one_of_d))), also = -rstd * (sum.x * p.one_of_d);
-            asm volatile("" ::: "memory");          // read again rather than kept in registers
-            T *dx = static_cast<T *>(p.dx) + row * p.lddx;
+            float sums[2] = {sum_g.x + sum_g.y, sum_go.x + sum_go.y};
+            row_sums<THREADS, 2>(sums, shared[flip][group], group);
+            flip ^= 1;
+            // dx = rstd g + xhat by + also, by = -rstd * mean(g xhat), also = -rstd * mean(g)
+            const float by = -rstd * (rstd * (sums[1] * p.one_of_d)), also = -rstd * (sums[0] * p.one_of_d);
+            asm volatile("" ::: "memory");                      // all is read again rather than kept in registers
 #pragma unroll
             for (int i = 0; i < kPieces; i++) {
-                const uint32_t at = (i * THREADS + t) * N;
-                if (at >= p.d)
+                if (ahead_x.bytes[i] == 0)
                     break;
-                float2 off[N / 2], dy[N / 2];
-                values(i, off, dy);
+                float2 off[N / 2], dy[N / 2], w[N / 2];
+                values(i, off, dy, w);
 #pragma unroll
                 for (int j = 0; j < N / 2; j++)
-                    off[j] = fma2(mul2(dy[j], w[i * N / 2 + j]), scale, fma2(off[j], make_float2(by, by), make_float2(also, also)));
+                    off[j] = fma2(mul2(dy[j], w[j]), scale, fma2(mul2(off[j], scale), make_float2(by, by), make_float2(also, also)));
                 Raw<DT, N> out;
                 out.round(off);
-                if (at + N <= p.d)
-                    out.store(dx + at);
+                if (ahead_x.bytes[i] == 16)
+                    out.store(dx + i * THREADS * N);
                 else
-                    out.store_some(dx + at, p.d - at);
+                    out.store_some(dx + i * THREADS * N, ahead_x.bytes[i] / (16 / N));
             }
+            dx += step * p.lddx;
         }
         mean = next_mean;
         rstd = next_rstd;
-        stage = stage == kAhead ? 0 : stage + 1;
+        turn = turn == kAhead ? 0 : turn + 1;
     }
     wait_asked<0>();
     if (!p.parts)
@@ -442,7 +497,7 @@ __global__ void __launch_bounds__(256) layer_norm_plain_dx_kernel(NormGradParams
 {
     using E = Element<DT>;
     using W = Element<WDT>;
-    __shared__ float2 shared[8];
+    __shared__ float shared[16];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t row = blockIdx.x;
@@ -453,16 +508,15 @@ __global__ void __launch_bounds__(256) layer_norm_plain_dx_kernel(NormGradParams
         hat = (E::widen(x[at]) - mean) * rstd;
         g = E::widen(dy[at]) * (p.weight ? W::widen(static_cast<const typename W::T *>(p.weight)[at]) : 1.0f);
     };
-    float2 sum = make_float2(0.0f, 0.0f);
-    float hat, g;
+    float sums[2] = {}, hat, g;
 #pragma unroll 4
     for (uint64_t at = threadIdx.x; at < p.d; at += 256) {
         values(at, hat, g);
-        sum.x += g;
-        sum.y = fmaf(g, hat, sum.y);
+        sums[0] += g;
+        sums[1] = fmaf(g, hat, sums[1]);
     }
-    sum = row_sums<256>(sum, shared, 0);
-    const float c1 = sum.x / (float)p.d, c2 = sum.y / (float)p.d;
+    row_sums<256, 2>(sums, shared, 0);
+    const float c1 = sums[0] * p.one_of_d, c2 = sums[1] * p.one_of_d;
 #pragma unroll 4
     for (uint64_t at = threadIdx.x; at < p.d; at += 256) {
         values(at, hat, g);
@@ -567,7 +621,7 @@ struct NormGradShape {
 };
 constexpr NormGradShape norm_grad_shape(uint32_t d)
 {
-    return d <= 256 ? NormGradShape{32, 8} : d <= 512 ? NormGradShape{32, 16} : d <= 1024 ? NormGradShape{32, 32} : d <= 2048 ? NormGradShape{128, 16}
+    return d <= 256 ? NormGradShape{32, 8} : d <= 512 ? NormGradShape{32, 16} : d <= 1024 ? NormGradShape{64, 16} : d <= 2048 ? NormGradShape{128, 16}
          : d <= 4096 ? NormGradShape{256, 16} : d <= 8192 ? NormGradShape{256, 32} : NormGradShape{512, 32};
 }
 
@@ -586,12 +640,12 @@ static uint32_t norm_parts(uint32_t m, uint32_t d, uint64_t elem)
 template <int DT, int WDT, int THREADS, int ELEMS>
 static int launch_norm_gradient_rows(const NormGradParams &p, uint32_t parts, cudaStream_t s)
 {
-    constexpr uint32_t kElem = sizeof(typename Element<DT>::T), kEach = (norm_grad_ahead(THREADS, ELEMS, kElem) + 1) * norm_grad_stage(THREADS, ELEMS, kElem);
-    constexpr uint32_t kMost = norm_grad_groups(THREADS, ELEMS, kElem) * kEach;
+    constexpr uint32_t kElem = sizeof(typename Element<DT>::T), kEach = (norm_grad_ahead(THREADS, ELEMS, kElem) + 1) * norm_grad_row(THREADS, ELEMS, kElem);
+    constexpr uint32_t kMost = norm_grad_groups(THREADS, ELEMS, kElem) * kEach + THREADS * ELEMS * 4;
     if (kMost > 40 * 1024)
         CLPK_CUDA(cudaFuncSetAttribute(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost));
     const uint32_t groups = norm_groups(p.m, p.d, kElem);
-    return launch_behind(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm_gradients", parts, groups * THREADS, groups * kEach, s, p);
+    return launch_behind(layer_norm_gradients_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm_gradients", parts, groups * THREADS, kMost, s, p);
 }
 
 template <int DT, int WDT>
@@ -603,12 +657,13 @@ static int launch_norm_gradients(const NormGradParams &p, bool aligned, uint32_t
         return p.parts ? launch_behind(layer_norm_plain_columns_kernel<DT>, "layer_norm_plain_columns", dim3((p.d - 1) / 256 + 1, parts), 256, 0, s, p) : CLPK_OK;
     }
     const NormGradShape shape = norm_grad_shape(p.d);
-    if (shape.threads == 32)
-        return shape.elems == 8    ? launch_norm_gradient_rows<DT, WDT, 32, 8>(p, parts, s)
-               : shape.elems == 16 ? launch_norm_gradient_rows<DT, WDT, 32, 16>(p, parts, s)
-                                   : launch_norm_gradient_rows<DT, WDT, 32, 32>(p, parts, s);
+    if (shape.elems == 8)
+        return launch_norm_gradient_rows<DT, WDT, 32, 8>(p, parts, s);
     if (shape.elems == 16)
-        return shape.threads == 128 ? launch_norm_gradient_rows<DT, WDT, 128, 16>(p, parts, s) : launch_norm_gradient_rows<DT, WDT, 256, 16>(p, parts, s);
+        return shape.threads == 32    ? launch_norm_gradient_rows<DT, WDT, 32, 16>(p, parts, s)
+               : shape.threads == 64  ? launch_norm_gradient_rows<DT, WDT, 64, 16>(p, parts, s)
+               : shape.threads == 128 ? launch_norm_gradient_rows<DT, WDT, 128, 16>(p, parts, s)
+                                      : launch_norm_gradient_rows<DT, WDT, 256, 16>(p, parts, s);
     return shape.threads == 256 ? launch_norm_gradient_rows<DT, WDT, 256, 32>(p, parts, s) : launch_norm_gradient_rows<DT, WDT, 512, 32>(p, parts, s);
 }
 
