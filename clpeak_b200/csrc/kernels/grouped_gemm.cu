@@ -783,10 +783,14 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
                 uses ^= 1u << s;
                 const uint32_t rows = t.k_rows - (t.k_blocks - 1) * kGroupedK;      // of none: zeros all
                 uint8_t *const st = smem + (size_t)s * kGroupedStageBytes;
-                const uint32_t boxes = 2 + t.width / 128, each = (kGroupedK - rows) * (kRowBytesK / 16);
-                for (uint32_t i = lane; i < boxes * each; i += 32) {
-                    const uint32_t box = i / each, at = i - box * each;
-                    *reinterpret_cast<uint4 *>(st + box * kMnLead + rows * kRowBytesK + at * 16) = make_uint4(0, 0, 0, 0);
+                // a row is 128 bytes of a box: eight lanes, four rows at a time
+                uint8_t *const from = st + (rows + (lane >> 3)) * kRowBytesK + (lane & 7) * 16;
+                for (uint32_t row = rows + (lane >> 3), at = 0; row < kGroupedK; row += 4, at += 4 * kRowBytesK) {
+                    *reinterpret_cast<uint4 *>(from + at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(from + at + kMnLead) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(from + at + 2 * kMnLead) = make_uint4(0, 0, 0, 0);
+                    if (t.width > 128)
+                        *reinterpret_cast<uint4 *>(from + at + 3 * kMnLead) = make_uint4(0, 0, 0, 0);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
