@@ -225,6 +225,8 @@ def main() -> None:
         end.synchronize()
         served.check()
         print(f"served in 8 bits, {m} tokens: {float(off):.4f} off the layer in bf16, {begin.elapsed_time(end) / 50 * 1e3:.1f} us a call")
+    from . import block                     # the layer behind a norm, trained by AdamW
+    block.main()
 
 
 if __name__ == "__main__":

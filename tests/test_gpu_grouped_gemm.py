@@ -264,3 +264,21 @@ def test_refusals(K, cuda):
     refused(K.clpk_grouped_gemm_backward, backward(), "pitch of d_dw", lddw=62)
     refused(K.clpk_grouped_gemm_backward, backward(), "stride_dw", stride_dw=8)
     assert bool((c == F.SENTINEL).all()) and bool((da == F.SENTINEL).all()) and bool((dw == F.SENTINEL).all())
+
+
+def test_sizes_drawn_over_the_whole_range(K, cuda):
+    """Sums that are cut and that are not, groups of any size, odd sizes: each element of both passes."""
+    import random
+    rng = random.Random(11)
+    spread = lambda lo, hi: round(lo * (hi / lo) ** rng.random())       # noqa: E731
+    for i in range(30):
+        groups = spread(1, 60)
+        rows = [rng.choice((0, 1, 2, spread(1, 4000 // groups + 1), spread(1, 8000 // groups + 1))) for _ in range(groups)]
+        if not sum(rows):
+            rows[0] = 3
+        n, k = spread(1, 3000), spread(1, 3000)
+        if sum(rows) * n * k > 2e10 or groups * n * k > 2e8:
+            n, k = n // 8 + 1, k // 8 + 1
+        case = Case(rows, n, k, rng.choice(("bf16", "f16")), first=rng.choice((0, 3)), spare=rng.choice((0, 70)), pad=i % 2, seed=i)
+        case.check_forward(K, rng.choice((case.dtype, "f32")))
+        case.check_backward(K, rng.choice((case.dtype, "f32")))
