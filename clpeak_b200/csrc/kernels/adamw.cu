@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kStepThreads, SDT == CLPK_DT_I8 ? 6 : 4) adamw
     if (table.c.d_lr || table.c.d_step) {
         if (threadIdx.x == 0) {
             const double lr = table.c.d_lr ? (double)*table.c.d_lr : table.c.lr;
-            set_rates(told, lr, table.c.beta1, table.c.beta2, table.c.decay, table.c.d_step ? (double)*table.c.d_step : (double)table.c.step);
+            set_rates(told, lr, table.c.beta1, table.c.beta2, table.c.decay, table.c.d_step ? (double)max(*table.c.d_step, 1u) : (double)table.c.step);
         }
         __syncthreads();
         r.keep = told.keep;

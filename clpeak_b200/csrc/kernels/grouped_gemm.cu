@@ -737,6 +737,7 @@ __global__ void __launch_bounds__(kGroupedThreads) grouped_kernel(const __grid_c
             } else if (lane == 0) {
                 *reinterpret_cast<volatile unsigned long long *>(done) = 0;
             }
+            __syncwarp();                                       // what lane 0 has seen, the others read behind it
             __threadfence();
             uint32_t begin = pair;
             while (sh->start[begin].tile == t.tile && sh->start[begin].kb > 0)
@@ -837,7 +838,7 @@ static int run_grouped(const GroupedMaps &maps, GroupedParams &p, int dtype, boo
     p.offsets = offsets;
     p.done = static_cast<unsigned long long *>(workspace);
     p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kGroupedPartsAt);
-    p.shape.pairs = std::min(kGroupedPairs, (uint32_t)num_sms() / 2);
+    p.shape.pairs = std::max(1u, std::min(kGroupedPairs, (uint32_t)num_sms() / 2));
     const uint32_t ctas = 2 * p.shape.pairs;
     if (backward)
         return dtype == CLPK_DT_F16 ? launch_clusters(grouped_kernel<CLPK_DT_F16, true>, "grouped (gradients)", ctas, kGroupedThreads, kGroupedSmemBytes, 2, s, maps, p)

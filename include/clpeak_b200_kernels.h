@@ -660,7 +660,7 @@ typedef struct clpk_adamw_args {
     double        lr, beta1, beta2, eps, weight_decay;      /* betas in [0, 1), eps in [2^-126, 1e30) */
     uint64_t      step;           /* from 1; unused with d_step                      */
     const float  *d_lr;           /* NULL, or read by the step in place of lr        */
-    const uint32_t *d_step;       /* NULL, or read by the step in place of step      */
+    const uint32_t *d_step;       /* NULL, or read by the step in place of step; 0: 1 */
     const float  *d_grad_scale;   /* NULL: 1                                         */
 } clpk_adamw_args_t;
 
@@ -676,7 +676,8 @@ CLPK_API int clpk_adamw(const clpk_adamw_args_t *args, void *stream);
  * Matrices are row-major with pitches as those of the feed-forward layers: multiples of 16 bytes, 0: rows one behind another, and what
  * lies between rows is neither read into a result nor written.  stride_* elements lie between one group's weights and the next, a
  * multiple of 16 bytes; 0: one behind another.  Outputs do not overlap inputs.  *d_status is cleared by the call and set where a
- * device-side wait expired.  The workspace belongs to one call at a time. */
+ * device-side wait expired.  The workspace belongs to one call at a time and need not be cleared, but for a captured call that is
+ * replayed after a wait of it has expired. */
 typedef struct clpk_grouped_gemm_args {
     int            dtype;         /* CLPK_DT_BF16 or F16: of A and W                 */
     int            out_dtype;     /* of C: `dtype` or CLPK_DT_F32                    */

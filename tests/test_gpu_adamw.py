@@ -118,6 +118,16 @@ def test_rate_and_step_from_the_device_in_a_graph(K, cuda):
             B.same_step(got, w)
 
 
+def test_a_step_of_none_is_the_first(K, cuda):
+    t, u = (B.Tensor(gen(15), 700, "f32", "f32", "f32", False) for _ in range(2))
+    count = torch.zeros(1, dtype=torch.int32, device="cuda")
+    step(K, [t], "f32", "f32", "f32", d_step=count.data_ptr())
+    count.fill_(1)
+    step(K, [u], "f32", "f32", "f32", d_step=count.data_ptr())
+    B.same(t.values(), u.values())
+    assert bool(torch.isfinite(t.param).all())
+
+
 def test_blocks_of_nothing_and_of_what_is_not_finite(K, cuda):
     g = gen(8)
     t = B.Tensor(g, 256 * 6 + 10, "f32", "f32", "i8", False)
