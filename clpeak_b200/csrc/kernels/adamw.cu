@@ -162,14 +162,19 @@ __device__ __forceinline__ void step_codes(float2 (&t)[2], const float2 (&of)[2]
     }
 }
 
-// the scale of a block from its largest size, whose bits order like the values; 1 / scale, or 0 where there is none
-__device__ __forceinline__ float step_scale(uint32_t top, float squared_steps, float &scale)
+// The scale of a block from its largest size, whose bits order like the values; 1 / scale, or 0 where there is none.  The quotient by a
+// constant is a product with the reciprocal and one correction by its remainder (Markstein 1990), rounded as a division is for every
+// positive number: all of them were compared.
+template <int STEPS>
+__device__ __forceinline__ float step_scale(uint32_t top, float &scale)
 {
+    constexpr float kSquared = (float)(STEPS * STEPS), kReciprocal = (float)(1.0 / (STEPS * STEPS));
     if (top >= 0x7F800000u) {
         scale = __uint_as_float(0x7FC00000u);
         return 0.0f;
     }
-    scale = __fdiv_rn(__uint_as_float(top), squared_steps);
+    const float size = __uint_as_float(top), near = __fmul_rn(size, kReciprocal);
+    scale = __fmaf_rn(__fmaf_rn(-near, kSquared, size), kReciprocal, near);
     if (scale < 1.17549435e-38f) {
         scale = 0.0f;
         return 0.0f;
@@ -311,7 +316,7 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
         const uint32_t top_m = __reduce_max_sync(0xffffffffu, __float_as_uint(most_m)), top_v = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
         // the largest root is that of the largest v; where that is below 2^-90, roots that are near lose what lies below 2^-126
         const bool low = top_v < 0x12800000u;
-        const float im = step_scale(top_m, 127.0f * 127.0f, sm), iv = step_scale(__float_as_uint(__fsqrt_rn(__uint_as_float(top_v))), 255.0f * 255.0f, sv);
+        const float im = step_scale<127>(top_m, sm), iv = step_scale<255>(__float_as_uint(__fsqrt_rn(__uint_as_float(top_v))), sv);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             float2 c[2] = {};

@@ -430,11 +430,11 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
 #pragma unroll
             for (int j = 0; j < N / 2; j++) {
                 const int e = i * N / 2 + j;
-                const float2 g = mul2(dy[j], w[j]);
-                dw[e] = fma2(dy[j], mul2(off[j], scale), dw[e]);
+                const float2 both = mul2(dy[j], off[j]);
+                dw[e] = fma2(both, scale, dw[e]);
                 db[e] = add2(db[e], dy[j]);
-                sum_g = add2(sum_g, g);
-                sum_go = fma2(g, off[j], sum_go);
+                sum_g = fma2(dy[j], w[j], sum_g);
+                sum_go = fma2(both, w[j], sum_go);
             }
         }
         if (p.dx) {
