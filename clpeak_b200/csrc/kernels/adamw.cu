@@ -163,8 +163,8 @@ __device__ __forceinline__ void step_codes(float2 (&t)[2], const float2 (&of)[2]
 }
 
 // The scale of a block from its largest size, whose bits order like the values; 1 / scale, or 0 where there is none.  The quotient by a
-// constant is a product with the reciprocal and one correction by its remainder (Markstein 1990), rounded as a division is for every
-// positive number: all of them were compared.
+// constant is a product with the reciprocal and one correction by its remainder, the reciprocal a near one and a correction likewise (Markstein
+// 1990): rounded as a division is, for every positive number and every scale that there is; all of them were compared.
 template <int STEPS>
 __device__ __forceinline__ float step_scale(uint32_t top, float &scale)
 {
@@ -179,7 +179,8 @@ __device__ __forceinline__ float step_scale(uint32_t top, float &scale)
         scale = 0.0f;
         return 0.0f;
     }
-    return __frcp_rn(scale);
+    const float r = rcp_near(scale);
+    return __fmaf_rn(r, __fmaf_rn(-scale, r, 1.0f), r);
 }
 
 // Eight elements of a thread, in pairs.  FAST: neighbours, in whole vectors; otherwise 32 apart, one at a time, those below `left` only.
