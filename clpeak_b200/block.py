@@ -35,6 +35,19 @@ def _check_rows(name: str, x: torch.Tensor, dtype: torch.dtype, most: int, cols:
     return x.contiguous() if x.shape[0] > 1 and x.stride(0) < cols else x
 
 
+def _span(x: torch.Tensor) -> tuple[int, int]:
+    """The bytes from x's first element to behind its last."""
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size() if x.numel() else x.data_ptr()
+
+
+def _check_apart(name: str, x: torch.Tensor, other: str, out: torch.Tensor) -> None:
+    """What a call reads may not lie where it writes."""
+    (a, b), (c, d) = _span(x), _span(out)
+    if a < d and c < b:
+        raise ValueError(f"{name} lies in the object's own {other}")
+
+
 def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
@@ -58,6 +71,8 @@ class Norm:
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x = _check_rows("x", x, self.dtype, self.rows, self.d, self.device)
+        for name, out in (("y", self.y), ("dx", self.dx)):
+            _check_apart("x", x, name, out)
         m = x.shape[0]
         self.x = None
         args = N.LayerNormArgs(dtype=DTYPES[self.dtype], weight_dtype=N.DT_F32, m=m, d=self.d, d_x=x.data_ptr(), d_weight=self.weight.data_ptr(),
@@ -75,6 +90,7 @@ class Norm:
         dy = _check_rows("dy", dy, self.dtype, self.rows, self.d, self.device)
         if dy.shape[0] != m:
             raise ValueError(f"dy must have {m} rows")
+        _check_apart("dy", dy, "dx", self.dx)
         args = N.LayerNormBackwardArgs(dtype=DTYPES[self.dtype], weight_dtype=N.DT_F32, m=m, d=self.d, d_x=x.data_ptr(), d_weight=self.weight.data_ptr(),
                                        d_dy=dy.data_ptr(), d_mean=self.mean.data_ptr(), d_rstd=self.rstd.data_ptr(), d_dx=self.dx.data_ptr(),
                                        d_dweight=self.dweight.data_ptr(), d_dbias=self.dbias.data_ptr(), ldx=_pitch(x), lddy=_pitch(dy),
@@ -110,6 +126,8 @@ class Experts:
 
     def forward(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
         x = _check_rows("x", x, torch.bfloat16, self.rows, self.k, self.device)
+        for name, out in (("y", self.y), ("dx", self.dx)):
+            _check_apart("x", x, name, out)
         if offsets.dtype != torch.int32 or tuple(offsets.shape) != (self.groups + 1,) or not offsets.is_contiguous():
             raise ValueError(f"offsets must be contiguous int32 [{self.groups + 1}]")
         _check_device("offsets", offsets, self.device)
@@ -127,6 +145,7 @@ class Experts:
         dy = _check_rows("dy", dy, torch.bfloat16, self.rows, self.n, self.device)
         if dy.shape[0] != self.x.shape[0]:
             raise ValueError(f"dy must have {self.x.shape[0]} rows")
+        _check_apart("dy", dy, "dx", self.dx)
         dx = self.dx[:self.x.shape[0]].zero_()
         args = N.GroupedGemmBackwardArgs(dw_dtype=N.DT_BF16, d_dc=dy.data_ptr(), lddc=_pitch(dy), d_da=dx.data_ptr(), d_dw=self.dw.data_ptr(), **self._common(self.x, 1))
         self.K.clpk_grouped_gemm_backward(C.byref(args), _stream(self.device))
@@ -142,7 +161,8 @@ class Experts:
 class AdamW:
     """Steps of Adam with decoupled weight decay on tensors of one type, whose gradients lie in tensors of that type or in fp32.  `state`:
     moments in "f32" or "i8"; `master`: 16-bit parameters have a copy in fp32, on which the step is taken.  The tensors are contiguous
-    and keep their places; parameters that are changed by others need load() where there are master copies."""
+    and keep their places, which do not overlap: a parameter that two layers share is given once; parameters that are changed by others
+    need load() where there are master copies."""
 
     def __init__(self, params: list[torch.Tensor], grads: list[torch.Tensor], state: str = "f32", master: bool = False, beta1: float = 0.9, beta2: float = 0.95,
                  eps: float = 1e-8, weight_decay: float = 0.0):
@@ -158,6 +178,9 @@ class AdamW:
                 raise ValueError(f"tensor {i}: parameter and gradient must be contiguous and as large as one another")
             _check_device(f"parameter {i}", p, self.device)
             _check_device(f"gradient {i}", g, self.device)
+        spans = sorted(_span(t) for t in [*params, *grads] if t.numel())
+        if any(begin < end for (_, end), (begin, _) in zip(spans, spans[1:])):
+            raise ValueError("parameters and gradients overlap")
         if master and params[0].dtype == torch.float32:
             raise ValueError("parameters in fp32 have no master copies")
         self.params, self.grads, self.K, self.count = params, grads, N.kernels(), 0
@@ -179,16 +202,21 @@ class AdamW:
     def load(self) -> None:
         """The master copies from the parameters."""
         for p, c in zip(self.params, self.master or ()):
-            c.copy_(p.flatten())
+            c.copy_(p.detach().flatten())
 
-    def step(self, rate: float, grad_scale: torch.Tensor | None = None) -> None:
-        """One step; `grad_scale`: a factor of all gradients, fp32 on the GPU."""
-        if grad_scale is not None:
-            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
-                raise ValueError("grad_scale must be one number in fp32")
-            _check_device("grad_scale", grad_scale, self.device)
-        self.args.lr, self.args.step = rate, self.count + 1
-        self.args.d_grad_scale = grad_scale.data_ptr() if grad_scale is not None else None
+    def step(self, rate: float | torch.Tensor, grad_scale: torch.Tensor | None = None, number: torch.Tensor | None = None) -> None:
+        """One step; `grad_scale`: a factor of all gradients, fp32 on the GPU.  A captured step repeats its rate and its number, which are
+        part of the launch, unless both are tensors on the GPU: a rate in fp32 and the number of the step, from 1, in int32."""
+        told = {}
+        for name, t, dtype in (("rate", rate, torch.float32), ("grad_scale", grad_scale, torch.float32), ("number", number, torch.int32)):
+            told[name] = None
+            if isinstance(t, torch.Tensor):
+                if t.dtype != dtype or t.numel() != 1:
+                    raise ValueError(f"{name} must be one number in {dtype}")
+                _check_device(name, t, self.device)
+                told[name] = t.data_ptr()
+        self.args.lr, self.args.step = 0.0 if told["rate"] else rate, self.count + 1
+        self.args.d_lr, self.args.d_grad_scale, self.args.d_step = told["rate"], told["grad_scale"], told["number"]
         self.K.clpk_adamw(C.byref(self.args), _stream(self.device))
         self.count += 1
 

@@ -600,7 +600,7 @@ CLPK_API int clpk_layer_norm(const clpk_layer_norm_args_t *args, void *stream);
 /* Gradients of clpk_layer_norm, from that of y and the mean and rstd that it kept: with xhat = (x - mean) * rstd, g = dy * weight
  *   dx = rstd * (g - sum g / d - xhat * sum (g * xhat) / d),   dweight = sum over rows of dy * xhat,   dbias = sum over rows of dy
  * in fp32 and rounded once.  Any of d_dx, d_dweight and d_dbias may be NULL: what is not asked for is not computed.  Sums are formed
- * in the same order in every call.  m = 0: dweight and dbias are zeros. */
+ * in the same order in every call.  m = 0: dweight and dbias are zeros.  Outputs do not overlap inputs or the workspace. */
 typedef struct clpk_layer_norm_backward_args {
     int           dtype;          /* of x, dy and dx                                 */
     int           weight_dtype;   /* of weight, dweight and dbias                    */
@@ -676,7 +676,7 @@ CLPK_API int clpk_adamw(const clpk_adamw_args_t *args, void *stream);
  * Matrices are row-major with pitches as those of the feed-forward layers: multiples of 16 bytes, 0: rows one behind another, and what
  * lies between rows is neither read into a result nor written.  stride_* elements lie between one group's weights and the next, a
  * multiple of 16 bytes; 0: one behind another.  Outputs do not overlap inputs.  *d_status is cleared by the call and set where a
- * device-side wait expired.  The workspace belongs to one call at a time and need not be cleared, but for a captured call that is
+ * device-side wait expired.  With m = 0 the offsets are not looked at.  The workspace belongs to one call at a time and need not be cleared, but for a captured call that is
  * replayed after a wait of it has expired. */
 typedef struct clpk_grouped_gemm_args {
     int            dtype;         /* CLPK_DT_BF16 or F16: of A and W                 */

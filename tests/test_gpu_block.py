@@ -152,3 +152,58 @@ def test_refusals(K, cuda):
     with pytest.raises(N.ClpkError, match="lr"):
         step.step(-1.0)
     assert step.count == 0
+
+
+def test_results_as_arguments(K, cuda):
+    """An object's own results lie where its next call writes; a copy, or another object's, will do."""
+    norm, other, experts = block.Norm(16, 9), block.Norm(16, 9), block.Experts(3, 16, 16, 9)
+    offsets = torch.tensor([0, 4, 4, 9], dtype=torch.int32, device="cuda")
+    x = randn(9, 16, seed=10)
+    y, z = norm.forward(x), experts.forward(x, offsets)
+    for call, name in ((lambda: norm.forward(y), "x lies in .* y"), (lambda: norm.forward(norm.dx[:4]), "x lies in .* dx"), (lambda: norm.backward(norm.dx), "dy lies"),
+                       (lambda: experts.forward(z, offsets), "x lies in .* y"), (lambda: experts.forward(experts.dx, offsets), "x lies in .* dx"),
+                       (lambda: experts.backward(experts.dx), "dy lies")):
+        with pytest.raises(ValueError, match=name):
+            call()
+    assert torch.equal(other.forward(y), other.forward(y.clone())) and torch.equal(norm.y, y)
+    want = other.forward(y).clone()
+    assert torch.equal(norm.forward(y.clone()), want)
+    want = experts.forward(z.clone(), offsets).clone()
+    assert torch.equal(experts.forward(x, offsets), z) and torch.equal(experts.forward(z.clone(), offsets), want)
+
+
+def test_tensors_that_overlap_and_parameters_with_gradients(K, cuda):
+    p, g = torch.randn(40, device="cuda"), torch.randn(40, device="cuda")
+    for params, grads in (([p, p], [g, g.clone()]), ([p[:8], p[7:]], [g[:8], g[7:].clone()]), ([p, p.clone()], [g, g]), ([p], [p])):
+        with pytest.raises(ValueError, match="overlap"):
+            block.AdamW(params, grads)
+    halves = block.AdamW([p[:8], p[8:], p[:0]], [g[:8], g[8:], g[:0]])
+    whole = torch.nn.Parameter(p.clone())
+    all_of = block.AdamW([whole], [g.clone()])
+    halves.step(1e-2)
+    all_of.step(1e-2)
+    assert torch.equal(p, whole.detach())
+    weight = torch.nn.Parameter(torch.randn(300, device="cuda").half())
+    step = block.AdamW([weight], [torch.randn(300, device="cuda")], master=True)
+    step.step(1e-2)
+    assert not step.master[0].requires_grad and torch.equal(step.master[0].half(), weight.detach())
+
+
+@pytest.mark.parametrize("state", ["f32", "i8"])
+def test_a_captured_step_that_counts(K, cuda, state):
+    """Rate and number in tensors are those of each replay: as steps one by one."""
+    p, g = randn(700, seed=11, dtype=torch.float32), randn(700, seed=12, dtype=torch.float32)
+    one, two = (block.AdamW([p.clone()], [g.clone()], state) for _ in range(2))
+    rate, number = torch.zeros((), device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two.step(rate, number=number)
+        number += 1
+    for i in range(4):
+        rate.fill_(0.5 ** (i + 4))
+        graph.replay()
+        one.step(0.5 ** (i + 4))
+        assert torch.equal(one.params[0], two.params[0]), i
+    for bad in ({"rate": torch.zeros(2, device="cuda")}, {"rate": rate.half()}, {"rate": rate, "number": number.long()}, {"rate": rate, "number": number.cpu()}):
+        with pytest.raises(ValueError):
+            two.step(**bad)
