@@ -48,6 +48,7 @@ constexpr int kGroupedThreads = 32 * (kGroupedZeroWarp + 1);
 constexpr uint32_t kGroupedChunk = 32;                          // columns of an accumulator that a warp takes at a time
 constexpr uint32_t kGroupedUnits = 2 * kGroupedEpilogueWarps;   // of a tile: what a warp has of it
 constexpr uint32_t kGroupedCutTiles = 2 * kGroupedPairs;        // tiles that may be cut, at most
+constexpr uint32_t kGroupedCutWarps = (kGroupedCutTiles + 31) / 32;
 constexpr uint32_t kGroupedSlotFloats = kGroupedM * kGroupedN;
 constexpr uint32_t kGroupedLeast = 6;                           // K blocks of a part; fewer stay with the pair before or behind
 constexpr uint32_t kGroupedTileCost = 6;                        // what a tile takes besides its K blocks, in K blocks
@@ -137,8 +138,8 @@ struct GroupedSmem {
     unsigned long long load[kGroupedPairs];                     // cost of what has been dealt to a pair
     unsigned long long rest[kGroupedCutTiles + 1];              // of the tiles that may be cut, one behind another
     unsigned long long begins[kGroupedPairs];
-    unsigned long long warp_cost[(kGroupedCutTiles + 31) / 32], most;
-    uint32_t join;
+    unsigned long long warp_cost[kGroupedCutWarps], warp_most[kGroupedCutWarps];
+    uint32_t warp_join[kGroupedCutWarps];
 };
 constexpr uint32_t kGroupedSmemBytes = kGroupedStages * kGroupedStageBytes + (uint32_t)sizeof(GroupedSmem);
 static_assert(kGroupedSmemBytes <= kSmemMax, "ring, barriers and the list of groups");
@@ -198,10 +199,6 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
     }
     if (t < kGroupedPairs)
         sh->load[t] = 0;
-    if (t == 0) {
-        sh->most = 0;
-        sh->join = 0;
-    }
     if (__syncthreads_or(bad)) {                                // nothing to walk
         if (t == 0)
             sh->n_tiles = sh->dealt = 0;
@@ -215,23 +212,20 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
 #pragma unroll 1
     for (uint32_t i = i0; i < i1; i++) {
         const GroupTiles g = entry_tiles(sh, p, i, kind, group);
+        sh->first[i] = g.cols * g.features;
         own += g.cols * g.features;
     }
     uint32_t at = warp_before(own);
     if (lane == 31)
         sh->warps[warp] = at + own;
     __syncthreads();
-    uint32_t n_tiles = 0;
-#pragma unroll 1
-    for (uint32_t w = 0; w < kGroupedThreads / 32; w++) {
-        at += w < warp ? sh->warps[w] : 0;
-        n_tiles += sh->warps[w];
-    }
+    const uint32_t told = lane < kGroupedThreads / 32 ? sh->warps[lane] : 0, n_tiles = __reduce_add_sync(0xffffffffu, told);
+    at += __reduce_add_sync(0xffffffffu, lane < warp ? told : 0);
 #pragma unroll 1
     for (uint32_t i = i0; i < i1; i++) {
+        const uint32_t tiles = sh->first[i];
         sh->first[i] = at;
-        const GroupTiles g = entry_tiles(sh, p, i, kind, group);
-        at += g.cols * g.features;
+        at += tiles;
     }
     if (t == 0)
         sh->first[entries] = n_tiles;
@@ -240,35 +234,37 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
     // What may be cut: half a round to one and a half, a thread for each of its tiles.
     const uint32_t whole = n_tiles >= P + P / 2 ? (n_tiles - P / 2) / P * P : 0, rest = n_tiles - whole;
     unsigned long long cost = 0;
-    if (warp < (kGroupedCutTiles + 31) / 32) {
+    if (warp < kGroupedCutWarps) {
         uint32_t join = 0;
         if (t < rest) {
             const GroupTiles g = entry_tiles(sh, p, entry_of(sh, entries, whole + t), kind, group);
             cost = tile_cost(g);
             join = kGroupedJoinCost * block_cost(g.width);
         }
-        unsigned long long sum = cost, most = cost;
-#pragma unroll 1
-        for (int o = 16; o > 0; o /= 2) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        }
+        // in halves of 24 and up to 32 bits, for the instructions that reduce a warp's
+        const uint32_t low = (uint32_t)cost & 0xFFFFFFu, high = (uint32_t)(cost >> 24), top = __reduce_max_sync(0xffffffffu, high);
+        const unsigned long long sum = ((unsigned long long)__reduce_add_sync(0xffffffffu, high) << 24) + __reduce_add_sync(0xffffffffu, low);
+        const unsigned long long most = ((unsigned long long)top << 24) + __reduce_max_sync(0xffffffffu, high == top ? low : 0);
         join = __reduce_max_sync(0xffffffffu, join);
         if (lane == 0) {
             sh->warp_cost[warp] = sum;
-            atomicMax(&sh->most, most);
-            atomicMax(&sh->join, join);
+            sh->warp_most[warp] = most;
+            sh->warp_join[warp] = join;
         }
     }
     __syncthreads();
-    unsigned long long total = 0, from = 0;
-#pragma unroll 1
-    for (uint32_t w = 0; w < (kGroupedCutTiles + 31) / 32; w++) {
-        from += w < warp ? sh->warp_cost[w] : 0;
-        total += sh->warp_cost[w];
+    unsigned long long total = 0, from = 0, most = 0;
+    uint32_t join = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kGroupedCutWarps; w++) {
+        const unsigned long long c = sh->warp_cost[w];
+        from += w < warp ? c : 0;
+        total += c;
+        most = max(most, sh->warp_most[w]);
+        join = max(join, sh->warp_join[w]);
     }
     // dealt out: as many as a pair gets of the longest; cut: an equal share and the joining
-    const bool cut = ((rest + P - 1) / P) * sh->most > total / P + sh->join;
+    const bool cut = (rest + P - 1) / P * P * most > total + (unsigned long long)join * P;
     if (t == 0) {
         sh->n_tiles = n_tiles;
         sh->dealt = cut ? whole : n_tiles;
@@ -279,7 +275,7 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
         __syncthreads();
         return true;
     }
-    if (warp < (kGroupedCutTiles + 31) / 32) {
+    if (warp < kGroupedCutWarps) {
         from += warp_before(cost);
         if (t <= rest)
             sh->rest[t] = from;                                 // and the total behind the last
@@ -303,37 +299,45 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
     if (warp == 0) {                                            // where the pairs begin: each fills up to one level what it has
         constexpr uint32_t kPairsEach = (kGroupedPairs + 31) / 32;
         const float all_cost = (float)total;
+        unsigned long long has[kPairsEach];
         float level = 3e38f;
-#pragma unroll 1
-        for (int round = 0; round < 5; round++) {
-            float sum = 0, count = 0;
-#pragma unroll 1
-            for (uint32_t c = lane * kPairsEach; c < min(P, (lane + 1) * kPairsEach); c++)
-                if ((float)sh->load[c] < level) {
-                    sum += (float)sh->load[c];
-                    count += 1;
-                }
 #pragma unroll
-            for (int o = 16; o > 0; o /= 2) {
+        for (uint32_t j = 0; j < kPairsEach; j++)
+            has[j] = lane * kPairsEach + j < P ? sh->load[lane * kPairsEach + j] : ~0ull;
+        uint32_t count = 0;
+#pragma unroll 1
+        for (int round = 0; round < 8; round++) {               // mostly two: all have about as much
+            float sum = 0;
+            uint32_t below = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kPairsEach; j++)
+                if (has[j] != ~0ull && (float)has[j] < level) {
+                    sum += (float)has[j];
+                    below++;
+                }
+            below = __reduce_add_sync(0xffffffffu, below);
+            if (below == count)
+                break;
+            count = below;
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2)
                 sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                count += __shfl_xor_sync(0xffffffffu, count, o);
-            }
-            level = (all_cost + sum) / fmaxf(count, 1.0f);
+            level = (all_cost + sum) / (float)max(count, 1u);
         }
         // in whole numbers, so that no pair begins in front of the one before it
         const unsigned long long full = (unsigned long long)level;
-        const auto room = [&](uint32_t c) { return full > sh->load[c] ? full - sh->load[c] : 0ull; };
         unsigned long long own_room = 0;
-#pragma unroll 1
-        for (uint32_t c = lane * kPairsEach; c < min(P, (lane + 1) * kPairsEach); c++)
-            own_room += room(c);
+#pragma unroll
+        for (uint32_t j = 0; j < kPairsEach; j++)
+            own_room += full > has[j] ? full - has[j] : 0;
         unsigned long long before = warp_before(own_room);
         const float all = fmaxf((float)__shfl_sync(0xffffffffu, before + own_room, 31), 1.0f);
-#pragma unroll 1
-        for (uint32_t c = lane * kPairsEach; c < min(P, (lane + 1) * kPairsEach); c++) {
-            sh->begins[c] = (unsigned long long)(all_cost * ((float)before / all));
-            before += room(c);
-        }
+#pragma unroll
+        for (uint32_t j = 0; j < kPairsEach; j++)
+            if (lane * kPairsEach + j < P) {
+                sh->begins[lane * kPairsEach + j] = (unsigned long long)(all_cost * ((float)before / all));
+                before += full > has[j] ? full - has[j] : 0;
+            }
     }
     __syncthreads();
     if (t <= P) {
@@ -471,21 +475,24 @@ __device__ __forceinline__ void store_rows(const float (&v)[kGroupedChunk], cons
         const uint32_t odd = lane & 1, f = feature + (lane & ~1), give = odd ? 0x5410 : 0x7632, one = odd ? 0x3254 : 0x5410, two = odd ? 0x3276 : 0x7610;
         uint16_t *to = static_cast<uint16_t *>(out.base) + (row0 + odd) * out.ld + f;
         const uint64_t step = 2 * out.ld;
-        auto put = [&](uint32_t j, uint32_t w) {
-            if (WHOLE || j + odd < rows) {
-                if (WHOLE || f + 1 < out.features)
-                    *reinterpret_cast<uint32_t *>(to) = w;
-                else if (f < out.features)
-                    *to = (uint16_t)w;
-            }
-            to += step;
-        };
+        uint32_t w[kGroupedChunk / 2];                          // all before the first store, so that what is left out costs no waits
 #pragma unroll
         for (uint32_t j = 0; j < kGroupedChunk; j += 4) {
             const uint32_t a = E::round2(v[j], v[j + 1]), b = E::round2(v[j + 2], v[j + 3]);
             const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(a, b, give), 1);
-            put(j, __byte_perm(a, got, one));
-            put(j + 2, __byte_perm(b, got, two));
+            w[j / 2] = __byte_perm(a, got, one);
+            w[j / 2 + 1] = __byte_perm(b, got, two);
+        }
+        if (WHOLE || f + 1 < out.features) {
+#pragma unroll
+            for (uint32_t j = 0; j < kGroupedChunk / 2; j++, to += step)
+                if (WHOLE || 2 * j + odd < rows)
+                    *reinterpret_cast<uint32_t *>(to) = w[j];
+        } else if (f < out.features) {
+#pragma unroll
+            for (uint32_t j = 0; j < kGroupedChunk / 2; j++, to += step)
+                if (2 * j + odd < rows)
+                    *to = (uint16_t)w[j];
         }
     }
 }
@@ -494,7 +501,7 @@ template <int DT>
 __device__ __forceinline__ void store_tile_rows(const float (&v)[kGroupedChunk], const GroupedParams &p, const GroupedTile &t, uint32_t col, uint32_t lane_feature, int lane)
 {
     const GroupedResult &out = p.out[t.kind];
-    if (col >= t.rows)
+    if (col >= t.rows || t.feature + lane_feature >= out.features)
         return;
     const uint32_t rows = t.rows - col;
     const uint64_t row = t.row + col;
