@@ -129,7 +129,7 @@ struct GroupedSmem {
     uint64_t tmem_full[2];
     uint64_t tmem_empty[2];
     uint32_t tmem_base;
-    uint32_t n_tiles, dealt;                                    // tiles in front of `dealt` are dealt in turn, the others cut
+    uint32_t dealt;                                             // tiles in front of it are dealt in turn, the others cut
     GroupedPlace start[kGroupedPairs + 1];                      // of each pair among the others
     uint32_t offsets[kGroupedMost + 1];
     uint32_t first[2 * kGroupedMost + 1];                       // tile of each entry
@@ -158,6 +158,17 @@ __device__ __forceinline__ T warp_before(T own)                 // exclusive sum
             sum += v;
     }
     return sum - own;
+}
+
+// Sum and maximum over the lanes of numbers below 2^51, in halves of 24 and 27 bits, for the instructions that reduce a warp's
+__device__ __forceinline__ unsigned long long warp_total(unsigned long long v)
+{
+    return ((unsigned long long)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 24)) << 24) + __reduce_add_sync(0xffffffffu, (uint32_t)v & 0xFFFFFFu);
+}
+__device__ __forceinline__ unsigned long long warp_most(unsigned long long v)
+{
+    const uint32_t high = (uint32_t)(v >> 24), top = __reduce_max_sync(0xffffffffu, high);
+    return ((unsigned long long)top << 24) + __reduce_max_sync(0xffffffffu, high == top ? (uint32_t)v & 0xFFFFFFu : 0);
 }
 
 __device__ __forceinline__ uint32_t entry_of(const GroupedSmem *sh, uint32_t entries, uint32_t tile)     // the last one that does not begin behind it
@@ -201,7 +212,7 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
         sh->load[t] = 0;
     if (__syncthreads_or(bad)) {                                // nothing to walk
         if (t == 0)
-            sh->n_tiles = sh->dealt = 0;
+            sh->dealt = 0;
         if (t <= P)
             sh->start[t] = {0, 0};
         __syncthreads();
@@ -241,10 +252,7 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
             cost = tile_cost(g);
             join = kGroupedJoinCost * block_cost(g.width);
         }
-        // in halves of 24 and up to 32 bits, for the instructions that reduce a warp's
-        const uint32_t low = (uint32_t)cost & 0xFFFFFFu, high = (uint32_t)(cost >> 24), top = __reduce_max_sync(0xffffffffu, high);
-        const unsigned long long sum = ((unsigned long long)__reduce_add_sync(0xffffffffu, high) << 24) + __reduce_add_sync(0xffffffffu, low);
-        const unsigned long long most = ((unsigned long long)top << 24) + __reduce_max_sync(0xffffffffu, high == top ? low : 0);
+        const unsigned long long sum = warp_total(cost), most = warp_most(cost);
         join = __reduce_max_sync(0xffffffffu, join);
         if (lane == 0) {
             sh->warp_cost[warp] = sum;
@@ -253,22 +261,13 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
         }
     }
     __syncthreads();
-    unsigned long long total = 0, from = 0, most = 0;
-    uint32_t join = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kGroupedCutWarps; w++) {
-        const unsigned long long c = sh->warp_cost[w];
-        from += w < warp ? c : 0;
-        total += c;
-        most = max(most, sh->warp_most[w]);
-        join = max(join, sh->warp_join[w]);
-    }
+    const bool told_cut = lane < kGroupedCutWarps;
+    const unsigned long long told_cost = told_cut ? sh->warp_cost[lane] : 0, total = warp_total(told_cost), most = warp_most(told_cut ? sh->warp_most[lane] : 0);
+    const uint32_t join = __reduce_max_sync(0xffffffffu, told_cut ? sh->warp_join[lane] : 0);
     // dealt out: as many as a pair gets of the longest; cut: an equal share and the joining
     const bool cut = (rest + P - 1) / P * P * most > total + (unsigned long long)join * P;
-    if (t == 0) {
-        sh->n_tiles = n_tiles;
+    if (t == 0)
         sh->dealt = cut ? whole : n_tiles;
-    }
     if (!cut) {
         if (t <= P)
             sh->start[t] = {n_tiles, 0};
@@ -276,7 +275,7 @@ __device__ __forceinline__ bool list_tiles(GroupedSmem *sh, const GroupedParams 
         return true;
     }
     if (warp < kGroupedCutWarps) {
-        from += warp_before(cost);
+        const unsigned long long from = warp_total(lane < warp ? told_cost : 0) + warp_before(cost);
         if (t <= rest)
             sh->rest[t] = from;                                 // and the total behind the last
     }
@@ -377,7 +376,7 @@ struct GroupedTile {
     uint32_t k_row, k_rows;                                     // dW: the group's rows
 };
 
-// The tiles of a pair, one after another; every role walks the same list.
+// The tiles of a pair, one after another; every role walks the same list, as a whole warp.
 struct GroupedWalk {
     const GroupedParams &p;
     const GroupedSmem *sh;
@@ -401,8 +400,13 @@ struct GroupedWalk {
         } else {
             i++;
         }
-        while (sh->first[entry + 1] <= tile)
-            entry++;
+        // the last entry that does not begin behind the tile; a round of tiles may lie many groups on
+        uint32_t behind;
+        do {
+            const uint32_t at = entry + 1 + (threadIdx.x & 31);
+            behind = __popc(__ballot_sync(0xffffffffu, at < s.lists * s.groups && sh->first[at] <= tile));
+            entry += behind;
+        } while (behind == 32);
         const GroupTiles g = entry_tiles(sh, s, entry, t.kind, t.group);
         const uint32_t begin = sh->offsets[t.group], rows = sh->offsets[t.group + 1] - begin;
         t.tile = tile;
