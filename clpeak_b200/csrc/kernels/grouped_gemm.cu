@@ -77,7 +77,7 @@ __host__ __device__ __forceinline__ GroupTiles group_tiles(const GroupedShape &p
     if (kind == kWeightGrad)
         return {p.dw_cols, p.dw_width, p.feature_tiles[kind], rows ? (rows + kGroupedK - 1) / kGroupedK : 1};   // of none: zeros
     const uint32_t cols = (rows + kGroupedN - 1) / kGroupedN;
-    return {cols, cols ? ((rows + cols - 1) / cols + 31) / 32 * 32 : 32, p.feature_tiles[kind], p.k_blocks[kind]};
+    return {cols, ((cols > 1 ? (rows + cols - 1) / cols : max(rows, 1u)) + 31) / 32 * 32, p.feature_tiles[kind], p.k_blocks[kind]};
 }
 
 // What a K block takes, in units of a column: loading and multiplying 256 features and `width` rows
@@ -411,9 +411,14 @@ struct GroupedWalk {
         const uint32_t begin = sh->offsets[t.group], rows = sh->offsets[t.group + 1] - begin;
         t.tile = tile;
         // strips of eight tiles along N, those fastest: neighbours share what they read
-        const uint32_t at = tile - sh->first[entry], strip = at / (8 * g.features), in = at - strip * 8 * g.features, wide = min(8u, g.cols - strip * 8);
-        const uint32_t col = strip * 8 + in % wide;
-        t.feature = in / wide * kGroupedM;
+        uint32_t in = tile - sh->first[entry], before = 0, wide = g.cols;
+        if (g.cols > 8) {                                       // a division takes longer than a small group's tile has
+            before = in / (8 * g.features) * 8;
+            in -= before * g.features;
+            wide = min(8u, g.cols - before);
+        }
+        const uint32_t feature = wide > 1 ? in / wide : in, col = before + in - feature * wide;
+        t.feature = feature * kGroupedM;
         t.width = g.width;
         t.k_blocks = g.k_blocks;
         t.kb0 = kb0;
