@@ -350,6 +350,36 @@ __host__ __device__ constexpr int norm_grad_ahead(int threads, int elems, uint32
     return rows >= 3 ? 2 : rows - 1;
 }
 
+// The groups' shares of dw and db, one group's behind the other's, to the CTA's part.  Not inlined: beside it the loop over rows gets
+// registers with which it takes 6 % longer (8192 x 4096).
+template <uint32_t COLUMNS>
+__device__ __noinline__ void add_shares(const float *shares, float *part, uint32_t groups, uint32_t d)
+{
+    const bool whole = d % 4 == 0;
+#pragma unroll 2
+    for (uint32_t i = 4 * threadIdx.x; i < 2 * COLUMNS; i += 4 * blockDim.x) {
+        const uint32_t at = i % COLUMNS;
+        if (at >= d)
+            continue;
+        float4 sum = *reinterpret_cast<const float4 *>(shares + i);
+#pragma unroll 4
+        for (uint32_t g = 1; g < groups; g++) {
+            const float4 f = *reinterpret_cast<const float4 *>(shares + g * 2 * COLUMNS + i);
+            sum = make_float4(sum.x + f.x, sum.y + f.y, sum.z + f.z, sum.w + f.w);
+        }
+        float *const to = part + i / COLUMNS * d + at;
+        if (whole) {
+            *reinterpret_cast<float4 *>(to) = sum;
+        } else {
+            const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++)
+                if (at + j < d)
+                    to[j] = v[j];
+        }
+    }
+}
+
 template <int DT, int WDT, int THREADS, int ELEMS>
 __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, sizeof(typename Element<DT>::T)), 1) layer_norm_gradients_kernel(NormGradParams p)
 {
@@ -469,26 +499,22 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
     wait_asked<0>();
     if (!p.parts)
         return;
-    // the groups' shares side by side where the rows were, a row for each element of a thread, then added in their order
+    // the groups' shares side by side where the rows were, each in the order of its columns, then added in their order
+    constexpr uint32_t kColumns = THREADS * ELEMS;
     float *const shares = reinterpret_cast<float *>(ring);
     static_assert(sizeof(float) <= (kAhead + 1) * sizeof(T), "room for all shares");
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < ELEMS; e++) {
-        shares[((group * 2 + 0) * ELEMS + e) * THREADS + t] = e % 2 ? dw[e / 2].y : dw[e / 2].x;
-        shares[((group * 2 + 1) * ELEMS + e) * THREADS + t] = e % 2 ? db[e / 2].y : db[e / 2].x;
-    }
+    for (int i = 0; i < kPieces; i++)
+#pragma unroll
+        for (int j = 0; j < N / 4; j++) {
+            const int e = i * N / 2 + 2 * j;
+            float4 *const to = reinterpret_cast<float4 *>(shares + group * 2 * kColumns + (i * THREADS + t) * N) + j;
+            to[0] = make_float4(dw[e].x, dw[e].y, dw[e + 1].x, dw[e + 1].y);
+            to[kColumns / 4] = make_float4(db[e].x, db[e].y, db[e + 1].x, db[e + 1].y);
+        }
     __syncthreads();
-    float *part = p.parts + (uint64_t)blockIdx.x * 2 * p.d;
-    for (uint32_t i = group; i < 2 * ELEMS; i += groups) {
-        float sum = 0.0f;
-#pragma unroll 4
-        for (uint32_t g = 0; g < groups; g++)
-            sum += shares[(g * 2 * ELEMS + i) * THREADS + t];
-        const uint32_t e = i % ELEMS, at = (e / N * THREADS + t) * N + e % N;
-        if (at < p.d)
-            part[i / ELEMS * p.d + at] = sum;
-    }
+    add_shares<kColumns>(shares, p.parts + (uint64_t)blockIdx.x * 2 * p.d, groups, p.d);
 }
 
 // Rows that do not start on 16 bytes, or are too long for registers: dx of a row by a CTA, element by element, read twice
@@ -554,6 +580,7 @@ struct NormJoinParams {
 
 // The parts' sums, rounded: a lane has a column, and each of 32 warps every 32nd part, so that all loads are on their way at once
 constexpr int kNormJoinWarps = 32;
+constexpr uint32_t kNormParts = 148;                // at most
 template <int WDT>
 __global__ void __launch_bounds__(32 * kNormJoinWarps) layer_norm_join_kernel(NormJoinParams p)
 {
@@ -566,9 +593,14 @@ __global__ void __launch_bounds__(32 * kNormJoinWarps) layer_norm_join_kernel(No
     float sum = 0.0f;
     if (col < p.d) {
         const float *from = p.parts + (uint64_t)which * p.d + col;
-#pragma unroll 16
-        for (uint32_t i = warp; i < p.n_parts; i += kNormJoinWarps)
-            sum += from[(uint64_t)i * 2 * p.d];
+        constexpr uint32_t kEach = (kNormParts + kNormJoinWarps - 1) / kNormJoinWarps;
+        float part[kEach];
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++)
+            part[j] = warp + j * kNormJoinWarps < p.n_parts ? from[(uint64_t)(warp + j * kNormJoinWarps) * 2 * p.d] : 0.0f;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++)
+            sum += part[j];
     }
     sums[warp][lane] = sum;
     __syncthreads();
@@ -612,8 +644,6 @@ static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
         return launch_norm_rows<DT, WDT, 256, 32>(p, s);
     return launch_norm_rows<DT, WDT, 512, 32>(p, s);
 }
-
-constexpr uint32_t kNormParts = 148;                // at most
 
 // Threads and elements of each that share a row in layer_norm_gradients_kernel
 struct NormGradShape {
