@@ -135,7 +135,10 @@ constexpr int kNormWarps = 4;                       // rows that a CTA takes at 
 constexpr int kNormAhead = 2;                       // rows on their way behind the one that is computed
 
 // How many CTAs an SM holds: 128 registers a thread for 32 elements with their weights, 80 and 48 for 16 and 8.
-__host__ __device__ constexpr int norm_ctas(int threads, int elems) { return threads == 32 ? (elems == 32 ? 4 : elems == 16 ? 6 : 10) : 512 / threads; }
+__host__ __device__ constexpr int norm_ctas(int threads, int elems)
+{
+    return threads == 32 ? (elems == 32 ? 4 : elems == 16 ? 6 : 10) : (elems == 32 ? 512 : 768) / threads;
+}
 template <int DT> constexpr uint32_t norm_bytes(int threads, int elems)
 {
     return (kNormAhead + 1) * (threads == 32 ? 32 * kNormWarps : threads) * elems * (uint32_t)sizeof(typename Element<DT>::T);
@@ -339,7 +342,7 @@ __host__ __device__ constexpr uint32_t norm_grad_row(int threads, int elems, uin
 __host__ __device__ constexpr uint32_t norm_grad_room(int threads, int elems) { return kNormGradBytes - threads * elems * 4; }
 __host__ __device__ constexpr int norm_grad_groups(int threads, int elems, uint32_t elem)
 {
-    int groups = (elems == 8 ? 1024 : elems == 32 ? 512 : threads == 32 ? 640 : 768) / threads;        // 64, 128, 102 and 85 registers
+    int groups = (elems == 8 ? 640 : elems == 32 || threads <= 64 ? 512 : 768) / threads;        // 102, 128 and 85 registers
     while (groups > 1 && groups * 2 * norm_grad_row(threads, elems, elem) > norm_grad_room(threads, elems))
         groups /= 2;
     return groups;
@@ -503,6 +506,7 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
     constexpr uint32_t kColumns = THREADS * ELEMS;
     float *const shares = reinterpret_cast<float *>(ring);
     static_assert(sizeof(float) <= (kAhead + 1) * sizeof(T), "room for all shares");
+    static_assert(THREADS == 32 || kGroups < 16, "barriers of a CTA");
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPieces; i++)
@@ -627,9 +631,14 @@ static int launch_norm_rows(const NormParams &p, cudaStream_t s)
     return launch_behind(layer_norm_kernel<DT, WDT, THREADS, ELEMS>, "layer_norm", ctas, kThreads, kBytes, s, p);
 }
 
+// Threads that share a row, and elements of each: what leaves few threads without a part of the row, 16 elements rather than 32 while two
+// rows at least fit an SM.  bf16, against 128 and 256 threads of 32 for all: 8192 rows of 2048 12.3 and 20.3 us, of 2560 18.0 and 21.2, of 4096
+// 25.0 and 25.1, of 5120 35.1 and 40.4, of 6144 37.8 and 42.0.  Where the SMs take all rows at once a row is for more threads: one of 1024 1.9
+// and 2.7 us, but 16384 of 768 12.5 and 11.0.
 template <int DT, int WDT>
 static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
 {
+    const auto few = [&](int threads, int elems) { return p.m <= norm_ctas(threads, elems) * (uint32_t)num_sms(); };
     if (!aligned || p.d > kNormLongest)
         return launch_behind(layer_norm_plain_kernel<DT, WDT>, "layer_norm_plain", p.m, 256, 0, s, p);
     if (p.d <= 256)
@@ -637,22 +646,32 @@ static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
     if (p.d <= 512)
         return launch_norm_rows<DT, WDT, 32, 16>(p, s);
     if (p.d <= 1024)
-        return launch_norm_rows<DT, WDT, 32, 32>(p, s);
+        return few(64, 16) ? launch_norm_rows<DT, WDT, 64, 16>(p, s) : launch_norm_rows<DT, WDT, 32, 32>(p, s);
+    if (p.d <= 2048)
+        return launch_norm_rows<DT, WDT, 128, 16>(p, s);
+    if (p.d <= 2560)
+        return launch_norm_rows<DT, WDT, 160, 16>(p, s);
     if (p.d <= 4096)
-        return launch_norm_rows<DT, WDT, 128, 32>(p, s);
+        return launch_norm_rows<DT, WDT, 256, 16>(p, s);
+    if (p.d <= 5120)
+        return launch_norm_rows<DT, WDT, 320, 16>(p, s);
+    if (p.d <= 6144)
+        return launch_norm_rows<DT, WDT, 384, 16>(p, s);
     if (p.d <= 8192)
-        return launch_norm_rows<DT, WDT, 256, 32>(p, s);
+        return few(512, 16) ? launch_norm_rows<DT, WDT, 512, 16>(p, s) : launch_norm_rows<DT, WDT, 256, 32>(p, s);
     return launch_norm_rows<DT, WDT, 512, 32>(p, s);
 }
 
-// Threads and elements of each that share a row in layer_norm_gradients_kernel
+// Threads and elements of each that share a row in layer_norm_gradients_kernel: as above (8192 rows of 2560 31.2 us, with 256 threads 34.9; of
+// 6144 57.1, with 256 of 32 elements 71.7)
 struct NormGradShape {
     int threads, elems;
 };
 constexpr NormGradShape norm_grad_shape(uint32_t d)
 {
     return d <= 256 ? NormGradShape{32, 8} : d <= 512 ? NormGradShape{32, 16} : d <= 1024 ? NormGradShape{64, 16} : d <= 2048 ? NormGradShape{128, 16}
-         : d <= 4096 ? NormGradShape{256, 16} : d <= 8192 ? NormGradShape{256, 32} : NormGradShape{512, 32};
+         : d <= 2560 ? NormGradShape{160, 16} : d <= 4096 ? NormGradShape{256, 16} : d <= 5120 ? NormGradShape{320, 16} : d <= 6144 ? NormGradShape{384, 16}
+         : d <= 8192 ? NormGradShape{256, 32} : NormGradShape{512, 32};
 }
 
 // Groups of a CTA, and the CTAs that share the rows, each with a part of dw and db.  Few rows are spread over the SMs.  A whole B200's SMs:
@@ -689,12 +708,17 @@ static int launch_norm_gradients(const NormGradParams &p, bool aligned, uint32_t
     const NormGradShape shape = norm_grad_shape(p.d);
     if (shape.elems == 8)
         return launch_norm_gradient_rows<DT, WDT, 32, 8>(p, parts, s);
-    if (shape.elems == 16)
-        return shape.threads == 32    ? launch_norm_gradient_rows<DT, WDT, 32, 16>(p, parts, s)
-               : shape.threads == 64  ? launch_norm_gradient_rows<DT, WDT, 64, 16>(p, parts, s)
-               : shape.threads == 128 ? launch_norm_gradient_rows<DT, WDT, 128, 16>(p, parts, s)
-                                      : launch_norm_gradient_rows<DT, WDT, 256, 16>(p, parts, s);
-    return shape.threads == 256 ? launch_norm_gradient_rows<DT, WDT, 256, 32>(p, parts, s) : launch_norm_gradient_rows<DT, WDT, 512, 32>(p, parts, s);
+    if (shape.elems == 32)
+        return shape.threads == 256 ? launch_norm_gradient_rows<DT, WDT, 256, 32>(p, parts, s) : launch_norm_gradient_rows<DT, WDT, 512, 32>(p, parts, s);
+    switch (shape.threads) {
+    case 32:  return launch_norm_gradient_rows<DT, WDT, 32, 16>(p, parts, s);
+    case 64:  return launch_norm_gradient_rows<DT, WDT, 64, 16>(p, parts, s);
+    case 128: return launch_norm_gradient_rows<DT, WDT, 128, 16>(p, parts, s);
+    case 160: return launch_norm_gradient_rows<DT, WDT, 160, 16>(p, parts, s);
+    case 256: return launch_norm_gradient_rows<DT, WDT, 256, 16>(p, parts, s);
+    case 320: return launch_norm_gradient_rows<DT, WDT, 320, 16>(p, parts, s);
+    default:  return launch_norm_gradient_rows<DT, WDT, 384, 16>(p, parts, s);
+    }
 }
 
 // calls f<DT, WDT>

@@ -238,3 +238,12 @@ def test_refusals(K, cuda):
         refused(b, back_args(), "workspace of", **change)
     K.clpk_layer_norm_backward(C.byref(back_args()), F.stream())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,d", [(11, 2056), (9, 2560), (7, 2561), (5, 4104), (9, 5120), (7, 5121), (6, 6144), (5, 6145), (149, 8192), (300, 6152), (1777, 600), (1776, 1000), (2000, 1024)])
+def test_shapes_of_a_row(K, cuda, m, d):
+    """Widths and numbers of rows where the threads that share a row change, the last threads with nothing, a piece of a vector, or all of it."""
+    for dtype, wdtype in (("bf16", "f32"), ("f32", "f32"), ("f16", "f16")):
+        x, dy = F.filled(values(m, d, d), dtype, pad=8), F.filled(values(m, d, d + 1), dtype, pad=16)
+        weight, bias = weights(d, wdtype, d)
+        check_all(K, x, dy, weight, bias, dtype, wdtype, pad=8)
