@@ -592,7 +592,7 @@ typedef struct clpk_layer_norm_args {
     float        *d_mean;         /* [m], or NULL: for the backward pass             */
     float        *d_rstd;         /* [m], or NULL                                    */
     uint64_t      ldx, ldy;
-    float         eps;            /* >= 0; with 0 a row of equal elements is NaN     */
+    float         eps;            /* >= 0; with 0 a row whose squares are 0 is NaN   */
 } clpk_layer_norm_args_t;
 
 CLPK_API int clpk_layer_norm(const clpk_layer_norm_args_t *args, void *stream);
