@@ -22,6 +22,12 @@
 // the end for longer than it costs to put sums together, the last half to one and a half rounds are cut by cost instead, also inside their
 // sums, so that all pairs finish together.  A tile that several pairs have summed is finished by the one that comes last, in
 // the order of K: the sums are the same in every call.
+//
+// Bound by tensor cores and their power where groups are long: 8 groups of 2048 rows x 8192 x 4096 bf16 690-710 us alone (1.55-1.6 PFLOPS) and
+// 860 at the power limit.  By memory where they are short: 64 rows of 64 groups x 1408 x 2048 67 us, 5.5 TB/s with the launch.  Weight
+// gradients of 512 rows a group have eight K blocks a tile of 256 KB: the epilogue's stores (16 groups x 4096 x 2048, both gradients, 264 us
+// alone with the tensor pipe at 64 %).  The smallest call takes 5.4 us: 1 to set up, 1.3 for the list, the rest a launch, one block's way from
+// memory and the result's.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -52,7 +58,10 @@ constexpr uint32_t kGroupedCutWarps = (kGroupedCutTiles + 31) / 32;
 constexpr uint32_t kGroupedSlotFloats = kGroupedM * kGroupedN;
 constexpr uint32_t kGroupedLeast = 6;                           // K blocks of a part; fewer stay with the pair before or behind
 constexpr uint32_t kGroupedTileCost = 6;                        // what a tile takes besides its K blocks, in K blocks
-constexpr uint32_t kGroupedJoinCost = 48;                       // and to put one together, in its K blocks
+// And to put one together, in its K blocks.  Cut at this estimate: one row x 4096 x 4096 16.8 us, uncut 24.4.  Uncut, and so with 16 here: 64
+// groups of a row x 1408 x 2048 66.5 and 71.2 us, 8 of a row x 4096 x 4096 49.4 and 55.2, rows' gradients of 16 x 512 x 4096 x 2048 113 and
+// 124.  With 24 or 32 two rows x 4096 x 4096 would gain (19.3 -> 18.3), the 16 groups lose.
+constexpr uint32_t kGroupedJoinCost = 48;
 
 constexpr uint32_t kMnLead = 64 * kRowBytesK;                   // as in clpk_linear_grad.cuh: from one box of 64 elements along M or N to the next
 constexpr uint32_t kMnStep = 16 * kRowBytesK / 16;              // 16 rows of K, in the descriptor's units of 16 bytes
@@ -400,7 +409,8 @@ struct GroupedWalk {
         } else {
             i++;
         }
-        // the last entry that does not begin behind the tile; a round of tiles may lie many groups on
+        // the last entry that does not begin behind the tile; a round of tiles may lie many groups on (1000 groups of two rows x 256 x 256:
+        // 31 us, one group after another 60)
         uint32_t behind;
         do {
             const uint32_t at = entry + 1 + (threadIdx.x & 31);
@@ -484,7 +494,7 @@ __device__ __forceinline__ void store_rows(const float (&v)[kGroupedChunk], cons
         const uint32_t odd = lane & 1, f = feature + (lane & ~1), give = odd ? 0x5410 : 0x7632, one = odd ? 0x3254 : 0x5410, two = odd ? 0x3276 : 0x7610;
         uint16_t *to = static_cast<uint16_t *>(out.base) + (row0 + odd) * out.ld + f;
         const uint64_t step = 2 * out.ld;
-        uint32_t w[kGroupedChunk / 2];                          // all before the first store, so that what is left out costs no waits
+        uint32_t w[kGroupedChunk / 2];                          // all before the first store: exchanges between stores that may be left out wait one by one
 #pragma unroll
         for (uint32_t j = 0; j < kGroupedChunk; j += 4) {
             const uint32_t a = E::round2(v[j], v[j + 1]), b = E::round2(v[j + 2], v[j + 3]);
