@@ -109,6 +109,16 @@ def test_as_many_groups_as_there_may_be(K, cuda):
     case.check_backward(K, "f32")
 
 
+def test_groups_far_apart(K, cuda):
+    """Hundreds of groups without rows between a pair's tiles, and hundreds of tiles of a group each."""
+    rows = [0] * 1024
+    for at, n in ((0, 40), (31, 1), (32, 3), (64, 2), (399, 300), (400, 5), (1000, 33), (1023, 2)):
+        rows[at] = n
+    for case in (Case(rows, 264, 136, "bf16"), Case([2] * 777 + [0] * 64 + [1] * 96, 72, 264, "f16")):
+        case.check_forward(K, "f32")
+        case.check_backward(K, "f32")
+
+
 def test_one_gradient_at_a_time(K, cuda):
     case = Case([70, 0, 333], 520, 264, "f16", spare=2)
     da, dw, _ = case.backward(K, "f16")
