@@ -65,6 +65,10 @@ __device__ __forceinline__ float row_sum(float v, float *shared)
     return v;
 }
 
+// 1 / sqrt of the variance and eps.  There is none where the squares have gone beyond fp32, and the row is NaN (inf * 0): with the 0 that
+// 1 / sqrt(inf) is, it would come out as its bias.
+__device__ __forceinline__ float row_rstd(float variance) { return 1.0f / sqrtf(fmaf(variance, 0.0f, variance)); }
+
 // Eight elements of a row, or as many as a vector has: what a thread loads at a time
 template <int DT> constexpr int kPiece = Element<DT>::kPerVector;
 
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
                 }
             }
         }
-        const float rstd = 1.0f / sqrtf(row_sum<THREADS>(squares.x + squares.y, shared[1]) * p.one_of_d + p.eps);
+        const float rstd = row_rstd(row_sum<THREADS>(squares.x + squares.y, shared[1]) * p.one_of_d + p.eps);
         if (t == 0) {
             if (p.mean)
                 p.mean[row] = mean;
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(256) layer_norm_plain_kernel(NormParams p)
         const float off = E::widen(x[at]) - mean;
         squares = fmaf(off, off, squares);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<256>(squares, shared[1]) / (float)p.d + p.eps);
+    const float rstd = row_rstd(row_sum<256>(squares, shared[1]) / (float)p.d + p.eps);
     if (threadIdx.x == 0) {
         if (p.mean)
             p.mean[row] = mean;

@@ -580,7 +580,8 @@ CLPK_API int clpk_gated_ffn_backward(const clpk_gated_ffn_backward_args_t *args,
  * in fp32 and rounded once.  dtype: CLPK_DT_F32, F16 or BF16, of x and y; weight_dtype: `dtype` or CLPK_DT_F32.  Rows lie ld*
  * elements apart, 0: one behind another; any alignment, pitch and length will do (rows that start on 16 bytes and have up to
  * 16384 elements are faster).  What lies between rows is neither read into a result nor written; y does not overlap x.  A row
- * with an infinity or a NaN is NaN, and so is an fp32 row whose sum or sum of squares goes beyond fp32. */
+ * with an infinity or a NaN is NaN, and so is one of fp32 or bf16 whose sum, or sum of squares about the mean, goes beyond fp32:
+ * y and rstd are, and with them its dx and its share of dweight. */
 typedef struct clpk_layer_norm_args {
     int           dtype;
     int           weight_dtype;

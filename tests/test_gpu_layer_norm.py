@@ -247,3 +247,40 @@ def test_shapes_of_a_row(K, cuda, m, d):
         x, dy = F.filled(values(m, d, d), dtype, pad=8), F.filled(values(m, d, d + 1), dtype, pad=16)
         weight, bias = weights(d, wdtype, d)
         check_all(K, x, dy, weight, bias, dtype, wdtype, pad=8)
+
+
+def slices(x, dtype, fill=77):
+    """The values as rows that do not start on 16 bytes."""
+    wide = torch.full((x.shape[0], x.shape[1] + 3), fill, dtype=F.TORCH[dtype], device="cuda")
+    wide[:, 1:x.shape[1] + 1] = x.to(F.TORCH[dtype])
+    return wide[:, 1:x.shape[1] + 1]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d,aligned", [(4, True), (96, True), (300, True), (1000, True), (4096, True), (8200, True), (16391, True), (40000, True), (4, False), (1000, False)])
+def test_rows_whose_squares_leave_fp32(K, cuda, dtype, d, aligned):
+    """Finite elements with a finite sum, whose squares or the sum of them are beyond fp32: the row is NaN with its rstd and its gradients, and
+    no other row is."""
+    place = F.filled if aligned else slices
+    x = values(7, d, 40)
+    sign = 1 - 2 * (torch.arange(d, device="cuda") % 2).float()
+    bad = [1, 3, 4]
+    x[1], x[3] = 1e20 * sign, 1e25 * sign
+    x[4] = (3e38 / d) ** 0.5 * 1.25 * sign                      # each square fits, their sum does not
+    x = place(x, dtype)
+    weight, bias = weights(d, "f32", 41)
+    y, mean, rstd = forward(K, x, dtype, "f32", weight, bias)
+    good = [0, 2, 5, 6]
+    assert bool(torch.isfinite(mean).all()) and bool(torch.isnan(rstd[bad]).all()) and bool(torch.isnan(y[bad]).all())
+    for got, (want, allowed) in zip((y, mean, rstd), B.norm64(x[good], weight, bias, 1e-5, dtype)):
+        F.check(got[good], want, allowed)
+    dy = place(values(7, d, 42), dtype)
+    dx, dweight, dbias = backward(K, x, dy, mean, rstd, weight, dtype, "f32")
+    assert bool(torch.isnan(dx[bad]).all()) and bool(torch.isnan(dweight).all()) and bool(torch.isfinite(dbias).all())
+    (want, allowed), _, _ = B.norm_backward64(x[good], dy[good], mean[good], rstd[good], weight, dtype, "f32")
+    F.check(dx[good], want, allowed, "dx")
+    # the largest squares that fit
+    x = place(0.5 * (3e38 / d) ** 0.5 * sign.expand(2, d), dtype)
+    y, mean, rstd = forward(K, x, dtype, "f32", weight, bias)
+    for got, (want, allowed) in zip((y, mean, rstd), B.norm64(x, weight, bias, 1e-5, dtype)):
+        F.check(got, want, allowed)
