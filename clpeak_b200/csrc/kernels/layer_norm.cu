@@ -23,6 +23,7 @@
 #include "../clpk_ptx.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace clpk {
 
@@ -43,6 +44,9 @@ struct NormParams {
     uint64_t ldx, ldy;
     uint32_t m, d;
     float eps, one_of_d;                            // 1 / d
+    // 1 / d in two parts, for the mean: a quotient to 2^-46, so that the mean of equal elements is one of them wherever their sum is exact.
+    // The first is rounded down and the second above 0, for an infinite sum to stay infinite.
+    float one_of_d_low, one_of_d_rest;
 };
 
 // The sum over all threads of a row, the same in each.  `shared`: a word for each warp; not to be written again before all threads
@@ -141,10 +145,11 @@ template <int DT, int THREADS, int PIECES> struct RowsAhead {
 constexpr int kNormWarps = 4;                       // rows that a CTA takes at once where a row is a warp's
 constexpr int kNormAhead = 2;                       // rows on their way behind the one that is computed
 
-// How many CTAs an SM holds: 128 registers a thread for 32 elements with their weights, 80 and 48 for 16 and 8.
+// How many CTAs an SM holds: 128 registers a thread for 32 elements with their weights, 80 and 56 for 16 and 8 (with 48, for ten, some are
+// spilled: 65536 x 256 bf16 16.3 us, so 15.0).
 __host__ __device__ constexpr int norm_ctas(int threads, int elems)
 {
-    return threads == 32 ? (elems == 32 ? 4 : elems == 16 ? 6 : 10) : (elems == 32 ? 512 : 768) / threads;
+    return threads == 32 ? (elems == 32 ? 4 : elems == 16 ? 6 : 9) : (elems == 32 ? 512 : 768) / threads;
 }
 template <int DT> constexpr uint32_t norm_bytes(int threads, int elems)
 {
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kNormWarps : THREADS, nor
             for (int j = 0; j < N / 2; j++)
                 sum = add2(sum, v[j]);
         }
-        const float mean = row_sum<THREADS>(sum.x + sum.y, shared[0]) * p.one_of_d;
+        const float all = row_sum<THREADS>(sum.x + sum.y, shared[0]), mean = fmaf(all, p.one_of_d_low, all * p.one_of_d_rest);
         const float2 minus = make_float2(-mean, -mean);
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
@@ -791,7 +796,8 @@ int clpk_layer_norm(const clpk_layer_norm_args_t *args, void *stream)
     CLPK_TRY(check_array(what, "d_bias", a.d_bias, a.weight_dtype, &aligned));
     CLPK_TRY(check_array(what, "d_mean", a.d_mean, CLPK_DT_F32, &any));
     CLPK_TRY(check_array(what, "d_rstd", a.d_rstd, CLPK_DT_F32, &any));
-    const NormParams p = {a.d_x, a.d_weight, a.d_bias, a.d_y, a.d_mean, a.d_rstd, a.ldx, a.ldy, a.m, a.d, a.eps, (float)(1.0 / a.d)};
+    const float near = (float)(1.0 / a.d), low = (double)near > 1.0 / a.d ? std::nextafterf(near, 0.0f) : near;
+    const NormParams p = {a.d_x, a.d_weight, a.d_bias, a.d_y, a.d_mean, a.d_rstd, a.ldx, a.ldy, a.m, a.d, a.eps, near, low, std::max((float)(1.0 / a.d - low), 1e-37f)};
     return CLPK_BY_TYPES(a.dtype, a.weight_dtype, launch_norm, p, aligned, as_stream(stream));
 }
 

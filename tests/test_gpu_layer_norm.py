@@ -284,3 +284,18 @@ def test_rows_whose_squares_leave_fp32(K, cuda, dtype, d, aligned):
     y, mean, rstd = forward(K, x, dtype, "f32", weight, bias)
     for got, (want, allowed) in zip((y, mean, rstd), B.norm64(x, weight, bias, 1e-5, dtype)):
         F.check(got, want, allowed)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [7, 56, 100, 1000, 1001, 2056, 5000, 9000, 16376, 20000])
+def test_the_mean_of_equal_elements_is_one_of_them(K, cuda, dtype, d):
+    """Sums of equal elements with few bits are exact, and a sum over the number of its terms is the element again: nothing is left of the
+    row but the bias, and nothing at all without eps."""
+    equal = (3.0, 1000.0, -0.375, 56.0)
+    x = F.filled(torch.tensor(equal, device="cuda")[:, None].expand(4, d), dtype)
+    weight, bias = weights(d, "f32", 43)
+    y, mean, rstd = forward(K, x, dtype, "f32", weight, bias)
+    assert mean.tolist() == list(equal) and bool((abs(rstd - 1e-5 ** -0.5) < 1e-3).all())
+    assert torch.equal(y, bias.to(F.TORCH[dtype]).expand(4, d))
+    y, _, _ = forward(K, x, dtype, "f32", weight, bias, eps=0.0)
+    assert bool(torch.isnan(y).all())
