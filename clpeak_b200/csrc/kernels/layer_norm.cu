@@ -448,8 +448,11 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
         const bool more = row + step < p.m;
         const float next_mean = more ? p.mean[row + step] : 0.0f, next_rstd = more ? p.rstd[row + step] : 0.0f;
         wait_asked<kAhead>();
-        // x - mean, dy and the weights of a piece, two numbers at a time
-        const auto values = [&](int i, float2 (&off)[N / 2], float2 (&dy)[N / 2], float2 (&w)[N / 2]) {
+        // |mean| * rstd beyond fp32 is a row of equal elements, whose xhat is 0: so is what stands for it behind the row's end, -mean * 0
+        const float by_hat = fabsf(mean * rstd) > 3.402823466e38f && rstd <= 3.402823466e38f ? 0.0f : rstd;
+        const float2 scale = make_float2(by_hat, by_hat);
+        // xhat, dy and the weights of a piece, two numbers at a time.  xhat first: dy times x - mean may leave fp32 where dy times xhat does not.
+        const auto values = [&](int i, float2 (&hat)[N / 2], float2 (&dy)[N / 2], float2 (&w)[N / 2]) {
             Raw<DT, N> x, d;
             x.v[0] = mine[turn * kRow + i * kAll];
             d.v[0] = mine[turn * kRow + (kPieces + i) * kAll];
@@ -459,46 +462,45 @@ __global__ void __launch_bounds__(THREADS * norm_grad_groups(THREADS, ELEMS, siz
                 w[2 * j] = make_float2(f.x, f.y);
                 w[2 * j + 1] = make_float2(f.z, f.w);
             }
-            x.widen(off);
+            x.widen(hat);
             d.widen(dy);
 #pragma unroll
             for (int j = 0; j < N / 2; j++)
-                off[j] = add2(off[j], make_float2(-mean, -mean));
+                hat[j] = mul2(add2(hat[j], make_float2(-mean, -mean)), scale);
         };
-        const float2 scale = make_float2(rstd, rstd);
-        float2 sum_g = make_float2(0.0f, 0.0f), sum_go = sum_g;         // of g and of g * (x - mean)
+        float2 sum_g = make_float2(0.0f, 0.0f), sum_gh = sum_g;         // of g and of g * xhat
 #pragma unroll
         for (int i = 0; i < kPieces; i++) {
-            float2 off[N / 2], dy[N / 2], w[N / 2];
-            values(i, off, dy, w);
+            float2 hat[N / 2], dy[N / 2], w[N / 2];
+            values(i, hat, dy, w);
 #pragma unroll
             for (int j = 0; j < N / 2; j++) {
                 const int e = i * N / 2 + j;
-                const float2 both = mul2(dy[j], off[j]);
-                dw[e] = fma2(both, scale, dw[e]);
+                const float2 both = mul2(dy[j], hat[j]);
+                dw[e] = add2(dw[e], both);
                 db[e] = add2(db[e], dy[j]);
                 sum_g = fma2(dy[j], w[j], sum_g);
-                sum_go = fma2(both, w[j], sum_go);
+                sum_gh = fma2(both, w[j], sum_gh);
             }
         }
         if (p.dx) {
-            float sums[2] = {sum_g.x + sum_g.y, sum_go.x + sum_go.y};
+            float sums[2] = {sum_g.x + sum_g.y, sum_gh.x + sum_gh.y};
             row_sums<THREADS, 2>(sums, shared[flip][group], group);
             flip ^= 1;
             // dx = rstd g + xhat by + also, by = -rstd * mean(g xhat), also = -rstd * mean(g)
-            const float by = -rstd * (rstd * (sums[1] * p.one_of_d)), also = -rstd * (sums[0] * p.one_of_d);
+            const float by = -rstd * (sums[1] * p.one_of_d), also = -rstd * (sums[0] * p.one_of_d);
             asm volatile("" ::: "memory");                      // all is read again rather than kept in registers
 #pragma unroll
             for (int i = 0; i < kPieces; i++) {
                 if (ahead_x.bytes[i] == 0)
                     break;
-                float2 off[N / 2], dy[N / 2], w[N / 2];
-                values(i, off, dy, w);
+                float2 hat[N / 2], dy[N / 2], w[N / 2];
+                values(i, hat, dy, w);
 #pragma unroll
                 for (int j = 0; j < N / 2; j++)
-                    off[j] = fma2(mul2(dy[j], w[j]), scale, fma2(mul2(off[j], scale), make_float2(by, by), make_float2(also, also)));
+                    hat[j] = fma2(mul2(dy[j], w[j]), make_float2(rstd, rstd), fma2(hat[j], make_float2(by, by), make_float2(also, also)));
                 Raw<DT, N> out;
-                out.round(off);
+                out.round(hat);
                 if (ahead_x.bytes[i] == 16)
                     out.store(dx + i * THREADS * N);
                 else

@@ -299,3 +299,28 @@ def test_the_mean_of_equal_elements_is_one_of_them(K, cuda, dtype, d):
     assert torch.equal(y, bias.to(F.TORCH[dtype]).expand(4, d))
     y, _, _ = forward(K, x, dtype, "f32", weight, bias, eps=0.0)
     assert bool(torch.isnan(y).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [40, 250, 1000, 1001, 4096, 6150, 9001, 16391])
+def test_gradients_of_very_small_and_very_large_rows(K, cuda, dtype, d):
+    """dy times what is left of x without its mean may be no number of fp32 where dy times xhat is one."""
+    weight, bias = weights(d, "f32", 44)
+    for size, gradient in ((1e-17, 1e-26), (1e-14, 1e-30), (1e15, 1e25), (1e13, 1e30)):
+        x, dy = F.filled(values(9, d, 45) * size, dtype), F.filled(values(9, d, 46) * gradient, dtype)
+        _, mean, rstd = forward(K, x, dtype, "f32", weight, bias, eps=0.0)
+        for t, (want, allowed), name in zip(backward(K, x, dy, mean, rstd, weight, dtype, "f32"), B.norm_backward64(x, dy, mean, rstd, weight, dtype, "f32"),
+                                            ("dx", "dweight", "dbias")):
+            F.check(t, want, allowed, f"{name}, {size} and {gradient}")
+
+
+@pytest.mark.parametrize("d", [37, 1001, 4094, 16381])
+def test_gradients_of_equal_elements_far_from_zero(K, cuda, d):
+    """What lies behind a row in its last vector is no part of it, however large the mean and rstd are."""
+    x, dy = F.filled(torch.full((3, d), 2.0 ** 83, device="cuda"), "f32"), F.filled(values(3, d, 47) * 1e-3, "f32")
+    weight, bias = weights(d, "f32", 48)
+    _, mean, rstd = forward(K, x, "f32", "f32", weight, bias, eps=2e-38)
+    assert mean.tolist() == [2.0 ** 83] * 3
+    for t, (want, allowed), name in zip(backward(K, x, dy, mean, rstd, weight, "f32", "f32"), B.norm_backward64(x, dy, mean, rstd, weight, "f32", "f32"),
+                                        ("dx", "dweight", "dbias")):
+        F.check(t, want, allowed, name)
