@@ -183,7 +183,7 @@ class AdamW:
             raise ValueError("parameters and gradients overlap")
         if master and params[0].dtype == torch.float32:
             raise ValueError("parameters in fp32 have no master copies")
-        self.params, self.grads, self.K, self.count = params, grads, N.kernels(), 0
+        self.params, self.grads, self.K, self.count = list(params), list(grads), N.kernels(), 0       # the table points to them
         new = lambda p, t, n: torch.zeros(n, dtype=t, device=p.device)          # noqa: E731
         blocks = lambda p: -(-p.numel() // N.ADAMW_BLOCK)                        # noqa: E731
         small = state == "i8"

@@ -77,3 +77,17 @@ def test_the_same_answer_as_through_ctypes(K, name, struct):
     for args in [(C.byref(struct()), 0), (C.byref(struct()), None), (C.byref(array[1]), 0), (struct(), 0), (None, 0), (C.byref(N.GemmArgs()), 0), (C.byref(struct()),),
                  (C.byref(array[0], C.sizeof(struct)), 0), (C.byref(struct()), -1)]:
         assert outcome(getattr(K, name), args) == outcome(lambda *a: K.call(name, *a), args)
+
+
+def test_adamw_keeps_what_its_table_points_to():
+    """The lists that a program gives are its own to change; the tensors behind the table's addresses stay."""
+    import torch
+
+    from clpeak_b200 import block
+    params, grads = [torch.ones(8), torch.ones(3)], [torch.zeros(8), torch.zeros(3)]
+    kept = [t.data_ptr() for t in params + grads]
+    step = block.AdamW(params, grads, "i8")
+    params.clear()
+    grads[0] = torch.zeros(8)
+    assert [t.data_ptr() for t in [*step.params, *step.grads]] == kept
+    assert [(t.d_param, t.d_grad) for t in step.table] == list(zip(kept[:2], kept[2:]))
