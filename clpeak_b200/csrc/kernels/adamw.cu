@@ -165,7 +165,8 @@ __device__ __forceinline__ void step_codes(float2 (&t)[2], const float2 (&of)[2]
 
 // The scale of a block from its largest size, whose bits order like the values; 1 / scale, or 0 where there is none.  The quotient by a
 // constant is a product with the reciprocal and one correction by its remainder, the reciprocal a near one and a correction likewise (Markstein
-// 1990): rounded as a division is, for every positive number and every scale that there is; all of them were compared.
+// 1990): rounded as a division is.  The tests compare the quotients of all numbers between two powers of two, at 1, at both ends of fp32
+// and about the least scale; the reciprocals were compared with __frcp_rn's, of every number from 2^-126 to 1e36.
 template <int STEPS>
 __device__ __forceinline__ float step_scale(uint32_t top, float &scale)
 {
@@ -250,8 +251,9 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
         qm[1] ^= 0x80808080u;
     }
     const auto mul = [&](float2 a, float2 b) { return step_mul(a, b, r.none); };
-    // With moments in 8 bits the instructions are the bound: root and quotient come with 2^-23 of their value.  A near root is 0 where v is
-    // below 2^-126, so eps has to hide what is lost there, 2^-63: by 2^-22.
+    // With moments in 8 bits the instructions are the bound: root and reciprocal come with 2^-23 of their value.  A near root is 0 where v is
+    // below 2^-126, so eps has to hide what is lost there, 2^-63: by 2^-22.  So the quotient's lower side is 2^-22 off, its reciprocal 2^-23
+    // more, and the quotient less than 2^-21 beside what its roundings are in any case.
     const bool near = kSmall && r.eps >= r.root_scale * 4.547473508864641e-13f;
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
@@ -357,7 +359,8 @@ __device__ __forceinline__ void step_elements(const StepTensor &t, const StepRat
     }
 }
 
-// CTAs an SM: what the registers allow.  With moments in 8 bits six, 40 registers a thread, were 683 us where four took 770 (12 bytes an element).
+// CTAs an SM: what the registers allow.  With moments in 8 bits six, 40 registers a thread, were 683 us where four took 770 (12 bytes an element),
+// although 36 to 56 bytes a thread are spilled with 40.
 template <int DT, int GDT, int SDT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kStepThreads, SDT == CLPK_DT_I8 ? 6 : 4) adamw_kernel(const __grid_constant__ StepTable<CAP> table)
 {

@@ -624,7 +624,7 @@ CLPK_API int clpk_layer_norm_backward_workspace_bytes(uint32_t m, uint32_t d, si
 CLPK_API int clpk_layer_norm_backward(const clpk_layer_norm_backward_args_t *args, void *stream);
 
 /* One step of Adam with decoupled weight decay over all tensors of a list, in fp32 whatever their types, each operation rounded (with
- * moments in 8 bits the root and the quotient of p's line are up to 2^-23 of their value off before):
+ * moments in 8 bits the quotient in p's line is up to 2^-21 of its value off before, roots of v below 2^-126 that are taken as 0 counted):
  *   g' = g * grad_scale
  *   m  = beta1 * m + (1 - beta1) * g'
  *   v  = beta2 * v + (1 - beta2) * g' * g'

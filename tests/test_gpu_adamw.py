@@ -267,3 +267,58 @@ def test_refusals(K, cuda):
     refused("has", tensor={"n": 2 ** 41})
     with pytest.raises(N.ClpkError, match="args is NULL"):
         K.clpk_adamw(None, F.stream())
+
+
+@pytest.mark.parametrize("power", [0, -113, -112, 127])
+def test_the_scale_of_every_number(K, cuda, power):
+    """Of all 2^23 numbers between two powers of two: the scale is the quotient by a constant, rounded once, and 0 below 2^-126."""
+    count = 1 << 19
+    t = B.Tensor.__new__(B.Tensor)
+    t.n, t.state, t.master = 256 * count, "i8", None
+    t.param, t.grad = (torch.zeros(t.n, device="cuda") for _ in range(2))
+    t.m, t.v = torch.zeros(t.n, dtype=torch.int8, device="cuda"), torch.zeros(t.n, dtype=torch.uint8, device="cuda")
+    t.m_scale, t.v_scale = (torch.zeros(count, device="cuda") for _ in range(2))
+    for part in range(16):
+        bits = torch.arange(part * count, (part + 1) * count, device="cuda", dtype=torch.int32) + ((power + 127) << 23)
+        size = bits.view(torch.float32)
+        t.grad.view(-1, 256)[:, 37] = size
+        # beta1 = beta2 = 0: m is the gradient, and the root of its square is its size
+        step(K, [t], "f32", "f32", "i8", beta1=0.0, beta2=0.0, lr=0.0)
+        for scale, steps in ((t.m_scale, 127), (t.v_scale, 255) if power == 0 else (t.m_scale, 127)):
+            want = (size.double() / steps ** 2).float()         # 53 bits are enough for one rounding to 24 behind another
+            want = torch.where(want < 2.0 ** -126, torch.zeros_like(want), want)
+            assert torch.equal(scale, want)
+            codes = (t.m if steps == 127 else t.v).view(-1, 256)[:, 37]
+            assert torch.equal(codes, torch.where(want > 0, steps, 0).to(codes.dtype))
+
+
+def test_steps_side_by_side(K, cuda):
+    """Two streams with tensors of their own: as one behind the other."""
+    make = lambda: [[B.Tensor(gen(20 + i), n, "bf16", "f32", "i8", True) for n in (70000, 5, 300001)] for i in range(2)]      # noqa: E731
+    one, two, streams = make(), make(), [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(5):
+        for tensors in one:
+            step(K, tensors, "bf16", "f32", "i8", step=i + 1)
+    torch.cuda.synchronize()
+    for i in range(5):
+        for tensors, s in zip(two, streams):
+            with torch.cuda.stream(s):
+                step(K, tensors, "bf16", "f32", "i8", step=i + 1)
+    torch.cuda.synchronize()
+    for a, b in zip(one, two):
+        for x, y in zip(a, b):
+            B.same(x.values(), y.values())
+
+
+@pytest.mark.parametrize("above", [0.9, 1.01, 16.0])
+def test_roots_that_eps_hides(K, cuda, above):
+    """Moments whose v lies about 2^-126, where a near root is 0, with eps about the least that makes up for it: 2^-41 of the root's factor."""
+    root_scale = 1 / math.sqrt(-math.expm1(3 * math.log(0.95)))
+    t = B.Tensor(gen(16), 256 * 8, "f32", "f32", "i8", False)
+    for x in (t.m, t.v, t.param):
+        x.zero_()
+    spread = 2 ** torch.linspace(-4, 1, t.n, device="cuda", dtype=torch.float64)
+    t.grad.copy_((2.0 ** -126 * spread / 0.05).sqrt())
+    check(K, [t], "f32", "f32", "i8", step=3, eps=above * root_scale * 2.0 ** -41)
+    assert bool((t.param < 0).all())
