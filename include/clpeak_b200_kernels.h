@@ -600,7 +600,7 @@ CLPK_API int clpk_layer_norm(const clpk_layer_norm_args_t *args, void *stream);
 
 /* Gradients of clpk_layer_norm, from that of y and the mean and rstd that it kept: with xhat = (x - mean) * rstd, g = dy * weight
  *   dx = rstd * (g - sum g / d - xhat * sum (g * xhat) / d),   dweight = sum over rows of dy * xhat,   dbias = sum over rows of dy
- * in fp32 and rounded once.  Any of d_dx, d_dweight and d_dbias may be NULL: what is not asked for is not computed.  Sums are formed
+ * in fp32 and rounded once.  Any of d_dx, d_dweight and d_dbias may be NULL: what is not asked for is not written.  Sums are formed
  * in the same order in every call.  m = 0: dweight and dbias are zeros.  Outputs do not overlap inputs or the workspace. */
 typedef struct clpk_layer_norm_backward_args {
     int           dtype;          /* of x, dy and dx                                 */
@@ -670,7 +670,7 @@ CLPK_API int clpk_adamw(const clpk_adamw_args_t *args, void *stream);
 /* ---- products of experts ------------------------------------------------------------------------
  * Rows of A lie sorted by group (tokens by expert); group e has the rows from d_offsets[e] up to d_offsets[e + 1] and weights W[e] of
  * its own:
- *   C[r] = A[r] W[e]^T          sums in fp32, rounded once
+ *   C[r] = A[r] W[e]^T          sums in fp32 as the tensor cores form them, rounded once
  * d_offsets: 32-bit integers on the device, read by the kernels; they do not decrease and lie in [0, m].  Where they do, *d_status
  * becomes 0x401 and no result is written.  Groups may be empty; rows in front of the first group and behind the last stay as they are
  * in C.  Up to 1024 groups.
@@ -698,7 +698,7 @@ CLPK_API int clpk_grouped_gemm_workspace_bytes(uint32_t groups, size_t *bytes);
 CLPK_API int clpk_grouped_gemm(const clpk_grouped_gemm_args_t *args, void *stream);
 
 /* Gradients of clpk_grouped_gemm from that of C:
- *   dA[r] = dC[r] W[e],   dW[e] = sum over the group's rows of dC[r]^T A[r]      sums in fp32, rounded once
+ *   dA[r] = dC[r] W[e],   dW[e] = sum over the group's rows of dC[r]^T A[r]      sums and rounding as above
  * dA and its rows of no group as C; dW[e] of an empty group is zeros.  Rows of A and dC that are no group's are not read into a
  * result.  d_da or d_dw may be NULL: what is not asked for is not computed.  Sums are formed in the same order in every call with the
  * same offsets. */
