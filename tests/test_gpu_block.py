@@ -207,3 +207,35 @@ def test_a_captured_step_that_counts(K, cuda, state):
     for bad in ({"rate": torch.zeros(2, device="cuda")}, {"rate": rate.half()}, {"rate": rate, "number": number.long()}, {"rate": rate, "number": number.cpu()}):
         with pytest.raises(ValueError):
             two.step(**bad)
+
+
+@pytest.mark.parametrize("state", ["f32", "i8"])
+def test_gradients_of_a_training_step(K, cuda, state):
+    """One step of train(): its loss and all its gradients against autograd in 64 bits, and each parameter goes against its own."""
+    d, f, tokens = 64, 128, 256
+    target, norm, layer = (block.Norm(d, tokens), FeedForward(d, f, tokens, seed=1)), block.Norm(d, tokens), FeedForward(d, f, tokens, seed=2)
+    layer.wd.copy_(target[1].wd)
+    layer.wd_t.copy_(target[1].wd_t)
+    for i, t in enumerate((target[0].weight, norm.weight)):
+        t.add_(randn(d, seed=30 + i, std=0.3, dtype=torch.float32))
+    for i, t in enumerate((target[0].bias, norm.bias)):
+        t.add_(randn(d, seed=40 + i, std=0.3, dtype=torch.float32))
+    trained = {"weight": norm.weight, "bias": norm.bias, "wg": layer.wg, "wu": layer.wu}
+    before = {name: t.clone() for name, t in trained.items()}
+    x = randn(tokens, d, seed=1)                            # train()'s own, of the same seed
+
+    def run(norm, layer, weight, bias, wg, wu):
+        x64 = x.double()
+        off = x64 - x64.mean(1, keepdim=True)
+        h = off / torch.sqrt((off * off).mean(1, keepdim=True) + norm.eps) * weight + bias
+        return (F.act64("silu", h @ wg.T) * (h @ wu.T)) @ layer.wd.double().T
+    leaves = [t.double().clone().requires_grad_() for t in before.values()]
+    loss = (run(norm, layer, *leaves) - run(*target, *(t.double() for t in (target[0].weight, target[0].bias, target[1].wg, target[1].wu)))).square().mean()
+    want = torch.autograd.grad(loss * 1024, leaves)         # train() scales by it
+    losses = block.train(norm, layer, target, steps=1, rate=1e-3, state=state)
+    # bf16 rounds the norm's rows, h and y on both sides of the difference: as near() counts
+    assert len(losses) == 1 and abs(losses[0] - float(loss.detach())) < 2.0 ** -6 * float(loss.detach())
+    for (name, t), got, w in zip(trained.items(), (norm.dweight, norm.dbias, layer.dwg, layer.dwu), want):
+        near(got, w, name)
+        moved = t.double() - before[name].double()
+        assert float((moved * w).sum()) < 0 and float(moved.abs().max()) > 0, name

@@ -324,3 +324,23 @@ def test_gradients_of_equal_elements_far_from_zero(K, cuda, d):
     for t, (want, allowed), name in zip(backward(K, x, dy, mean, rstd, weight, "f32", "f32"), B.norm_backward64(x, dy, mean, rstd, weight, "f32", "f32"),
                                         ("dx", "dweight", "dbias")):
         F.check(t, want, allowed, name)
+
+
+def test_gradients_side_by_side(K, cuda):
+    """Two streams with workspaces of their own: as one behind the other."""
+    cases = []
+    for m, d, seed in ((3000, 1200, 50), (901, 4096, 60)):
+        x, dy = F.filled(values(m, d, seed), "bf16"), F.filled(values(m, d, seed + 1), "bf16")
+        weight, bias = weights(d, "f32", seed + 2)
+        _, mean, rstd = forward(K, x, "bf16", "f32", weight, bias)
+        cases.append(((K, x, dy, mean, rstd, weight, "bf16", "f32"), B.norm_workspace(K, m, d)))
+    want = [backward(*args, workspace=space) for args, space in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for (args, space), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(backward(*args, workspace=space))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
