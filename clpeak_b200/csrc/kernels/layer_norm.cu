@@ -10,13 +10,13 @@
 //
 // CTAs stay, with the weights in registers, and take every gridDim-th row; a thread copies its pieces of the rows that come next into
 // shared memory of its own (cp.async) while it computes, so that an SM has 40 to 200 KB on their way whatever its threads wait for.
-// 16384 x 8192 bf16: 90 to 96 us, 5.6 to 6.0 TB/s, 86 to 91 % of a copy's rate (149 without rows ahead); what is missing is the wait for
+// 16384 x 8192 bf16: 90 to 96 us, 5.6 to 6.0 TB/s, 85 to 91 % of a copy's rate (149 without rows ahead); what is missing is the wait for
 // a row's two sums with two rows an SM.  One row: 2 us, launch to launch.
 //
 // dw and db are sums down the columns: a thread has the same columns of each of its rows, so that its share of both sums stays in
 // registers, and one part for each CTA goes to the workspace, which a second kernel adds up: 8 bytes a column and CTA beside 6 a
-// column and row.  The order of the sums depends on the sizes alone.  8192 x 4096 bf16: 41 to 43 us, 4.7 to 4.9 TB/s; 40 of them are the
-// first kernel's, at 2.5 instructions a cycle and 52 % of the memory's peak, with three rows an SM.
+// column and row.  The order of the sums depends on the sizes alone.  8192 x 4096 bf16: 41 to 44 us, 4.5 to 4.9 TB/s; 41 of them are the
+// first kernel's, at 2.5 instructions a cycle and 51 % of the memory's peak, with three rows an SM.
 #include "../clpk_activation.cuh"
 #include "../clpk_elements.cuh"
 #include "../clpk_internal.h"
@@ -366,7 +366,8 @@ __host__ __device__ constexpr int norm_grad_ahead(int threads, int elems, uint32
 }
 
 // The groups' shares of dw and db, one group's behind the other's, to the CTA's part.  Not inlined: beside it the loop over rows gets
-// other registers, and takes longer (8192 x 4096 bf16: 48.9 us, so 40.9).
+// other registers, and mostly takes longer (bf16 8192 x 5120: 60.9 us, so 50.0; 4096 x 8192 49.4 and 40.5; 8192 x 4096 41.1 and 40.7; one row
+// of 4096 4.95 and 5.15).
 template <uint32_t COLUMNS>
 __device__ __noinline__ void add_shares(const float *shares, float *part, uint32_t groups, uint32_t d)
 {
@@ -645,8 +646,8 @@ static int launch_norm_rows(const NormParams &p, cudaStream_t s)
 }
 
 // Threads that share a row, and elements of each: what leaves few threads without a part of the row, 16 elements rather than 32 while two
-// rows at least fit an SM.  bf16, against 128 and 256 threads of 32 for all: 8192 rows of 2048 12.3 and 20.3 us, of 2560 18.0 and 21.2, of 4096
-// 25.0 and 25.1, of 5120 35.1 and 40.4, of 6144 37.8 and 42.0.  Where the SMs take all rows at once a row is for more threads: one of 1024 1.9
+// rows at least fit an SM.  bf16, against 128 and 256 threads of 32 for all: 8192 rows of 2048 12.8 and 20.3 us, of 2560 18.2 and 21.2, of 4096
+// 25.0 and 25.1, of 5120 35.5 and 40.4, of 6144 37.9 and 42.0.  Where the SMs take all rows at once a row is for more threads: one of 1024 1.9
 // and 2.7 us, but 16384 of 768 12.5 and 11.0.
 template <int DT, int WDT>
 static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
@@ -675,8 +676,9 @@ static int launch_norm(const NormParams &p, bool aligned, cudaStream_t s)
     return launch_norm_rows<DT, WDT, 512, 32>(p, s);
 }
 
-// Threads and elements of each that share a row in layer_norm_gradients_kernel: as above (8192 rows of 2560 31.2 us, with 256 threads 34.9; of
-// 6144 57.1, with 256 of 32 elements 71.7)
+// Threads and elements of each that share a row in layer_norm_gradients_kernel: as above.  bf16, 8192 rows: of 2560 27.8 us, with 256 threads
+// 35.9; of 5120 50.0, with 384 54.4; of 5128 57.2, with 256 of 32 elements 59.2, of 6144 58.6 and 57.9 (fp32 93.3 and 93.2, 110 and 100; 20 rows
+// of 6144 7.8 and 8.1).
 struct NormGradShape {
     int threads, elems;
 };
