@@ -126,7 +126,7 @@ class Experts:
 
     def forward(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
         x = _check_rows("x", x, torch.bfloat16, self.rows, self.k, self.device)
-        for name, out in (("y", self.y), ("dx", self.dx)):
+        for name, out in (("y", self.y), ("dx", self.dx), ("dw", self.dw)):
             _check_apart("x", x, name, out)
         if offsets.dtype != torch.int32 or tuple(offsets.shape) != (self.groups + 1,) or not offsets.is_contiguous():
             raise ValueError(f"offsets must be contiguous int32 [{self.groups + 1}]")
@@ -145,7 +145,8 @@ class Experts:
         dy = _check_rows("dy", dy, torch.bfloat16, self.rows, self.n, self.device)
         if dy.shape[0] != self.x.shape[0]:
             raise ValueError(f"dy must have {self.x.shape[0]} rows")
-        _check_apart("dy", dy, "dx", self.dx)
+        for name, out in (("dx", self.dx), ("dw", self.dw)):
+            _check_apart("dy", dy, name, out)
         dx = self.dx[:self.x.shape[0]].zero_()
         args = N.GroupedGemmBackwardArgs(dw_dtype=N.DT_BF16, d_dc=dy.data_ptr(), lddc=_pitch(dy), d_da=dx.data_ptr(), d_dw=self.dw.data_ptr(), **self._common(self.x, 1))
         self.K.clpk_grouped_gemm_backward(C.byref(args), _stream(self.device))

@@ -239,3 +239,16 @@ def test_gradients_of_a_training_step(K, cuda, state):
         near(got, w, name)
         moved = t.double() - before[name].double()
         assert float((moved * w).sum()) < 0 and float(moved.abs().max()) > 0, name
+
+
+def test_weights_gradients_as_arguments(K, cuda):
+    """Experts' dw has rows as long as x's, and as dy's where n is k; the backward pass writes it while it reads both."""
+    experts, other = block.Experts(3, 16, 16, 9), block.Experts(3, 16, 16, 9)
+    offsets = torch.tensor([0, 4, 4, 9], dtype=torch.int32, device="cuda")
+    x, dy = randn(9, 16, seed=13), randn(9, 16, seed=14)
+    experts.forward(x, offsets)
+    dw = experts.backward(dy)[1]
+    for call, name in ((lambda: experts.forward(dw[1, :9], offsets), "x lies in .* dw"), (lambda: experts.backward(dw[2, 2:11]), "dy lies in .* dw")):
+        with pytest.raises(ValueError, match=name):
+            call()
+    assert torch.equal(other.forward(dw[0, :9], offsets), other.forward(dw[0, :9].clone(), offsets))
